@@ -61,6 +61,17 @@ SIGNATURES = {
     "detllm_qkv_attn_decode_ext": [P, I, L, I, I, I, P, P, P, P, L, P, L, P, L, P, L, P, L, P,
                                    L, P, P, P, P, P, P, P, P, L, P, P, P, I, P, L, P, L, I, P,
                                    P, P, P, P, P, S],
+    "detllm_attn_window_prefill": [P, P, P, P, P, I, P, L, I, I, I, I, I, I, I, P, S],
+    "detllm_attn_window_decode_work": [I, I, I, I, I, I, P],
+    "detllm_attn_window_decode": [P, P, P, P, P, I, P, L, I, I, I, I, P, I, I, P, L, P, P, S],
+    "detllm_attn_prefill_acc": [P, P, P, P, P, I, P, L, I, I, I, I, I, P, L, P, S],
+    "detllm_attn_decode_acc_work": [I, I, I, I, P],
+    "detllm_attn_decode_acc": [P, P, P, P, P, I, P, L, I, I, I, I, P, P, L, P, L, P, P, S],
+    "detllm_kv_select_work": [I, I, P],
+    "detllm_kv_select": [P, L, P, L, I, I, I, I, I, I, P, P, P, L, S],
+    "detllm_kv_compact": [P, P, I, P, I, P, I, P, I, I, I, S],
+    "detllm_attn_decode_shared_work": [I, I, I, I, I, P],
+    "detllm_attn_decode_shared": [P, P, P, P, P, I, P, L, I, I, I, I, P, I, P, L, P, P, S],
     "detllm_decode_prologue": [P, L, I, L, P, P, P, P, L, S],
     "detllm_op_quant_i8_pertoken": [P, P, P, I, I, P, P, P, S],
     "detllm_op_requant_i32_common": [P, P, P, I, L, I, I, I, P, P, S],
@@ -76,7 +87,9 @@ SIGNATURES = {
 }
 
 # host-only entry points (no device work, so no stream argument)
-HOST_ONLY = frozenset({"detllm_igemv_plan", "detllm_attn_split_plan"})
+HOST_ONLY = frozenset({"detllm_igemv_plan", "detllm_attn_split_plan",
+                       "detllm_attn_window_decode_work", "detllm_attn_decode_acc_work",
+                       "detllm_kv_select_work", "detllm_attn_decode_shared_work"})
 
 _CT = {P: ctypes.c_void_p, I: ctypes.c_int, L: ctypes.c_int64, S: ctypes.c_void_p}
 

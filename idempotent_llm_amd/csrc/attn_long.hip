@@ -1,0 +1,381 @@
+// Attention forms for long caches (gfx950): windowed attention with sinks and
+// attention that accumulates each slot's weight. No counterpart in the
+// reference; the integers of a query are those of attention.hip's kernels over
+// the slots it sees.
+//
+// Windowed (attn_window.h has the rule): the kernels are attention.hip's over
+// a shorter list of pages, those of the sinks and those from the window's
+// first slot on, so their work follows the window and not the cache. The
+// range is found on the device, per query tile in prefill and per row in
+// decode, because it depends on the row's validity flags: a launch is sized
+// for rows without gaps, and a row whose window spans more slots takes more
+// steps in the same blocks.
+//
+// Accumulating: the p of a slot, summed over the query heads of a kv head (and
+// over a tile's queries), is added to acc [B][n_kv][slots]. p is an integer, so
+// the order of the additions does not change the sum. A decode block owns its
+// (row, kv head, slots) and adds without atomics; prefill tiles share slots
+// and add with 64-bit atomics.
+
+#include "attn_decode.h"
+#include "attn_prefill.h"
+#include "../../include/detllm_hip.h"
+
+namespace {
+
+__global__ __launch_bounds__(256, 2) void k_window_prefill(PrefillArgs a) {
+  keep_hidden_args();
+  prefill_body<true, false>(a);
+}
+__global__ __launch_bounds__(256, 2) void k_acc_prefill(PrefillArgs a) {
+  keep_hidden_args();
+  prefill_body<false, true>(a);
+}
+
+// The pages a row's newest query sees, numbered without the gap.
+struct WinView {
+  static constexpr bool kWhole = false;
+  int n;      // slots of the list
+  int pre;    // slots before the gap
+  int skip;   // slots left out
+  int sink_end, lo;
+  __device__ __forceinline__ int slot(int s) const { return s < pre ? s : s + skip; }
+  __device__ __forceinline__ bool sees(int s) const { return s < sink_end || s >= lo; }
+};
+__device__ __forceinline__ WinView win_view(const WinRange& r, int S) {
+  return WinView{S - r.skip * DI_PAGE, r.pre * DI_PAGE, r.skip * DI_PAGE, r.sink_end, r.lo};
+}
+
+struct WindowArgs {
+  SplitArgs s;
+  int window, sinks;
+  int zs;          // blocks per (row, kv head)
+  int lds_slots;   // one block: slots whose scores its LDS holds
+  WinRange* range; // [B] (split form)
+};
+
+// One block per (row, kv head). Scores in LDS; a row whose window spans more
+// slots than that holds keeps them in the scratch.
+template <int G>
+__global__ __launch_bounds__(256) void k_window_decode(WindowArgs w) {
+  keep_hidden_args();
+  extern __shared__ __attribute__((aligned(16))) int32_t sh_scores[];
+  __shared__ int32_t pg_lds[DEC_MAX_PAGES];
+  DecodeArgs a = w.s.d;
+  const int kvh = blockIdx.x, b = blockIdx.y;
+  const i64 q0 = (i64)b * a.n_q + kvh * G;
+  bool over;
+  const int S = scanned_slots(a, a.tpos, &over);
+  const WinView v = win_view(
+      window_range<256>(a.valid + (i64)b * a.valid_stride, S, S, w.window, w.sinks), S);
+  const int npages = (v.n + DI_PAGE - 1) / DI_PAGE;
+  for (int i = threadIdx.x; i < npages; i += 256) pg_lds[i] = a.kv.page(b, v.slot(i * DI_PAGE));
+  if (npages == 0 && threadIdx.x == 0) pg_lds[0] = -1;  // S = 0: loads read page 0
+  __syncthreads();
+  if (v.n <= w.lds_slots) {
+    a.S = v.n;  // (the scores' row stride)
+    decode_body<G, VPRE, false, false, 4, false, WinView>(
+        a, v.n, kvh, b, a.q8 + q0 * 128, a.tpos + q0, sh_scores, pg_lds, KPre<2>{}, OmPre<G, 2>{}, v);
+  } else {
+    decode_body<G, VPRE, true, false, 4, false, WinView>(
+        a, v.n, kvh, b, a.q8 + q0 * 128, a.tpos + q0, sh_scores, pg_lds, KPre<2>{}, OmPre<G, 2>{}, v);
+  }
+  report_slots(a, over, kvh == 0);
+}
+
+template <int G>
+__global__ __launch_bounds__(256) void k_window_scores(WindowArgs w) {
+  keep_hidden_args();
+  const DecodeArgs& a = w.s.d;
+  const int kvh = blockIdx.x, b = blockIdx.y, z = blockIdx.z;
+  bool over;
+  const int S = scanned_slots(a, a.tpos, &over);
+  const WinRange r = window_range<256>(a.valid + (i64)b * a.valid_stride, S, S, w.window, w.sinks);
+  if (kvh == 0 && z == 0 && threadIdx.x == 0) w.range[b] = r;
+  const WinView v = win_view(r, S);
+  int c = z;
+  do {
+    split_scores_chunk<G, WinView>(w.s, kvh, b, c, v);
+    __syncthreads();  // (the chunk's LDS is reused)
+    c += w.zs;
+  } while (c * w.s.chunk < v.n);
+  report_slots(a, over, kvh == 0 && z == 0);
+}
+
+template <int G>
+__global__ __launch_bounds__(256) void k_window_pv(WindowArgs w) {
+  keep_hidden_args();
+  const DecodeArgs& a = w.s.d;
+  const int kvh = blockIdx.x, b = blockIdx.y;
+  bool over;
+  const int S = scanned_slots(a, a.tpos, &over);
+  const WinView v = win_view(w.range[b], S);
+  int c = blockIdx.z;
+  do {
+    split_pv_chunk<G, WinView>(w.s, kvh, b, c, v);
+    __syncthreads();
+    c += w.zs;
+  } while (c * w.s.chunk < v.n);
+}
+
+template <int G, bool SCR>
+__global__ __launch_bounds__(256) void k_acc_decode(DecodeArgs a) {
+  keep_hidden_args();
+  extern __shared__ __attribute__((aligned(16))) int32_t sh_scores[];
+  __shared__ int32_t pg_lds[DEC_MAX_PAGES];
+  const int kvh = blockIdx.x, b = blockIdx.y;
+  const i64 q0 = (i64)b * a.n_q + kvh * G;
+  bool over;
+  const int S = scanned_slots(a, a.tpos, &over);
+  const int npages = (a.S + DI_PAGE - 1) / DI_PAGE;
+  for (int i = threadIdx.x; i < npages; i += 256) pg_lds[i] = a.kv.page(b, (i64)i * DI_PAGE);
+  if (npages == 0 && threadIdx.x == 0) pg_lds[0] = -1;
+  __syncthreads();
+  decode_body<G, VPRE, SCR, false, 4, false, WholeRow, true>(
+      a, S, kvh, b, a.q8 + q0 * 128, a.tpos + q0, sh_scores, pg_lds);
+  report_slots(a, over, kvh == 0);
+}
+
+template <int G>
+__global__ __launch_bounds__(256) void k_acc_scores(SplitArgs sa) {
+  keep_hidden_args();
+  split_scores_chunk<G>(sa, blockIdx.x, blockIdx.y, blockIdx.z);
+}
+template <int G>
+__global__ __launch_bounds__(256) void k_acc_pv(SplitArgs sa) {
+  keep_hidden_args();
+  split_pv_chunk<G, WholeRow, true>(sa, blockIdx.x, blockIdx.y, blockIdx.z);
+}
+
+// How a decode over about n slots per row runs: chunk slots per block (a
+// multiple of the page; 0: one block per (row, kv head)).
+int decode_chunk(int B, int n, int n_q, int n_kv) {
+  const int G = n_q / n_kv;
+  const i64 pairs = (i64)B * n_kv;
+  const int from = pairs > 128 ? INT32_MAX : G > 4 ? 1537 : G > 2 ? (pairs <= 64 ? 896 : 1536) : pairs <= 64 ? 768 : 1152;
+  if (n < from) return 0;
+  int chunk = 0, ns = 0;
+  if (detllm_attn_split_plan(B, n, n_q, n_kv, &chunk, &ns) != 0 || ns <= 1) return 0;
+  return chunk;
+}
+
+// Bytes of the split form's scores and chunk maxima: [B][n_q][ns * chunk] and
+// [B][n_q][ns] int32 with ns = ceil(S / chunk), 16-byte sizes.
+i64 split_bytes(int B, int S, int n_q, int chunk, i64* cmax_at) {
+  const i64 ns = ((i64)S + chunk - 1) / chunk, rows = (i64)B * n_q;
+  *cmax_at = rows * ns * chunk * 4;
+  return *cmax_at + (rows * ns * 4 + 15) / 16 * 16;
+}
+i64 one_block_bytes(int B, int S, int n_q, int G) {
+  const i64 spad = ((i64)S + 15) / 16 * 16;
+  return (i64)G * spad * 4 > DECODE_LDS_BYTES ? (i64)B * n_q * spad * 4 : 0;
+}
+int heads_ok(int n_q, int n_kv) {
+  if (n_q <= 0 || n_kv <= 0 || n_q % n_kv) return DI_EINVAL;
+  const int G = n_q / n_kv;
+  return G == 1 || G == 2 || G == 4 || G == 8 ? DI_OK : DI_ENOSYS;
+}
+// Slots a windowed query sees in a row without gaps, with the partial pages at
+// the ends of the two ranges.
+int window_slots(int S, int window, int sinks) {
+  return (int)imin(S, (i64)window + sinks + 2 * DI_PAGE);
+}
+SplitArgs split_args(const DecodeArgs& d, int B, int chunk, void* work) {
+  SplitArgs sa{};
+  sa.d = d;
+  i64 cmax_at = 0;
+  split_bytes(B, d.S, d.n_q, chunk, &cmax_at);
+  sa.d.scratch = (int32_t*)work;
+  sa.cmax = (int32_t*)((char*)work + cmax_at);
+  sa.chunk = chunk;
+  sa.ns = (d.S + chunk - 1) / chunk;
+  sa.spad = (i64)sa.ns * chunk;
+  sa.out_stride = (i64)B * d.n_q * 128;
+  sa.add = 1;
+  return sa;
+}
+
+}  // namespace
+
+extern "C" {
+
+int detllm_attn_window_prefill(const int8_t* q8, const int64_t* tpos, const int8_t* kpool,
+                               const int8_t* vpool, const int32_t* table, int width,
+                               const uint8_t* valid, int64_t valid_stride, int B, int T,
+                               int S_past, int n_q, int n_kv, int window, int sinks, int64_t* out,
+                               hipStream_t s) {
+  if (window < 1 || sinks < 0) return DI_EINVAL;
+  if (B <= 0 || T <= 0) return DI_OK;
+  const i64 S = (i64)S_past + T;
+  if (n_q <= 0 || n_kv <= 0 || n_q % n_kv || S_past < 0 || !kv_ok(kpool, vpool, table, width) ||
+      S > (i64)width * DI_PAGE || valid_stride < S || !q8 || !tpos || !valid || !out)
+    return DI_EINVAL;
+  if (S > DEC_MAX_S) return DI_ERANGE;  // int32 MFMA accumulators of P.V
+  PrefillArgs a{q8, tpos, KVPages{(int8_t*)kpool, (int8_t*)vpool, table, width, n_kv}, valid, out,
+                T, (int)S, S_past, n_q, n_kv, B, valid_stride, window, sinks};
+  const i64 pairs = (i64)(((T + 63) / 64 + 1) / 2) * n_q * B;
+  if (2 * pairs > 0x7fffffff) return DI_ERANGE;
+  hipLaunchKernelGGL(k_window_prefill, dim3((unsigned)(2 * pairs)), dim3(256), prefill_lds(S), s, a);
+  DI_LAUNCH_CHECK();
+  return DI_OK;
+}
+
+int detllm_attn_prefill_acc(const int8_t* q8, const int64_t* tpos, const int8_t* kpool,
+                            const int8_t* vpool, const int32_t* table, int width,
+                            const uint8_t* valid, int64_t valid_stride, int B, int T, int S_past,
+                            int n_q, int n_kv, int64_t* acc, int64_t acc_stride, int64_t* out,
+                            hipStream_t s) {
+  if (B <= 0 || T <= 0) return DI_OK;
+  const i64 S = (i64)S_past + T;
+  if (n_q <= 0 || n_kv <= 0 || n_q % n_kv || S_past < 0 || !kv_ok(kpool, vpool, table, width) ||
+      S > (i64)width * DI_PAGE || valid_stride < S || acc_stride < S || !q8 || !tpos || !valid ||
+      !acc || !out)
+    return DI_EINVAL;
+  if (S > DEC_MAX_S) return DI_ERANGE;
+  PrefillArgs a{q8, tpos, KVPages{(int8_t*)kpool, (int8_t*)vpool, table, width, n_kv}, valid, out,
+                T, (int)S, S_past, n_q, n_kv, B, valid_stride, 0, 0, acc, acc_stride};
+  const i64 pairs = (i64)(((T + 63) / 64 + 1) / 2) * n_q * B;
+  if (2 * pairs > 0x7fffffff) return DI_ERANGE;
+  hipLaunchKernelGGL(k_acc_prefill, dim3((unsigned)(2 * pairs)), dim3(256), prefill_lds(S), s, a);
+  DI_LAUNCH_CHECK();
+  return DI_OK;
+}
+
+int detllm_attn_window_decode_work(int B, int S, int n_q, int n_kv, int window, int sinks,
+                                   int64_t* bytes) {
+  if (!bytes || B < 0 || S < 0 || window < 1 || sinks < 0) return DI_EINVAL;
+  if (const int rc = heads_ok(n_q, n_kv)) return rc;
+  if (S > DEC_MAX_S) return DI_ERANGE;
+  *bytes = 0;
+  if (B == 0 || S == 0) return DI_OK;
+  const int chunk = decode_chunk(B, window_slots(S, window, sinks), n_q, n_kv);
+  i64 at;
+  *bytes = chunk ? split_bytes(B, S, n_q, chunk, &at) + (i64)B * sizeof(WinRange)
+                 : one_block_bytes(B, S, n_q, n_q / n_kv);
+  return DI_OK;
+}
+
+int detllm_attn_window_decode(const int8_t* q8, const int64_t* tpos, const int8_t* kpool,
+                              const int8_t* vpool, const int32_t* table, int width,
+                              const uint8_t* valid, int64_t valid_stride, int B, int S, int n_q,
+                              int n_kv, const int64_t* s_dev, int window, int sinks, void* work,
+                              int64_t work_bytes, int64_t* out, int32_t* err, hipStream_t s) {
+  i64 need = 0;
+  if (const int rc = detllm_attn_window_decode_work(B < 0 ? 0 : B, S, n_q, n_kv, window, sinks, &need))
+    return rc;
+  if (B <= 0) return DI_OK;
+  if (!kv_ok(kpool, vpool, table, width) || S > (i64)width * DI_PAGE || valid_stride < S || !q8 ||
+      !tpos || !valid || !out)
+    return DI_EINVAL;
+  if (need > 0 && (!work || work_bytes < need)) return DI_ERANGE;
+  const int G = n_q / n_kv, slots = window_slots(S, window, sinks);
+  const int chunk = S > 0 ? decode_chunk(B, slots, n_q, n_kv) : 0;
+  WindowArgs w{};
+  const DecodeArgs d{q8, tpos, KVPages{(int8_t*)kpool, (int8_t*)vpool, table, width, n_kv}, valid,
+                     out, (int32_t*)work, s_dev, S, n_q, n_kv, valid_stride, err};
+  w.window = window;
+  w.sinks = sinks;
+  if (chunk) {
+    w.s = split_args(d, B, chunk, work);
+    i64 at;
+    w.range = (WinRange*)((char*)work + split_bytes(B, S, n_q, chunk, &at));
+    w.zs = (slots + chunk - 1) / chunk;
+    const dim3 grid(n_kv, B, w.zs);
+    const size_t dyn = (size_t)G * chunk * 4;
+    switch (G) {
+#define DI_WIN_SPLIT(G_)                                                     \
+  case G_:                                                                   \
+    hipLaunchKernelGGL(k_window_scores<G_>, grid, dim3(256), 0, s, w);       \
+    hipLaunchKernelGGL(k_window_pv<G_>, grid, dim3(256), dyn, s, w);         \
+    break
+      DI_WIN_SPLIT(1);
+      DI_WIN_SPLIT(2);
+      DI_WIN_SPLIT(4);
+      DI_WIN_SPLIT(8);
+#undef DI_WIN_SPLIT
+    }
+  } else {
+    w.s.d = d;
+    const i64 fit = DECODE_LDS_BYTES / (4 * G) / 16 * 16;
+    w.lds_slots = (int)imin(((i64)slots + 15) / 16 * 16, fit);
+    if (one_block_bytes(B, S, n_q, G) == 0) w.lds_slots = (S + 15) / 16 * 16;  // no scratch
+    const dim3 grid(n_kv, B);
+    const size_t dyn = (size_t)G * w.lds_slots * 4;
+    switch (G) {
+      case 1: hipLaunchKernelGGL(k_window_decode<1>, grid, dim3(256), dyn, s, w); break;
+      case 2: hipLaunchKernelGGL(k_window_decode<2>, grid, dim3(256), dyn, s, w); break;
+      case 4: hipLaunchKernelGGL(k_window_decode<4>, grid, dim3(256), dyn, s, w); break;
+      case 8: hipLaunchKernelGGL(k_window_decode<8>, grid, dim3(256), dyn, s, w); break;
+    }
+  }
+  DI_LAUNCH_CHECK();
+  return DI_OK;
+}
+
+int detllm_attn_decode_acc_work(int B, int S, int n_q, int n_kv, int64_t* bytes) {
+  if (!bytes || B < 0 || S < 0) return DI_EINVAL;
+  if (const int rc = heads_ok(n_q, n_kv)) return rc;
+  if (S > DEC_MAX_S) return DI_ERANGE;
+  *bytes = 0;
+  if (B == 0 || S == 0) return DI_OK;
+  const int chunk = decode_chunk(B, S, n_q, n_kv);
+  i64 at;
+  *bytes = chunk ? split_bytes(B, S, n_q, chunk, &at) : one_block_bytes(B, S, n_q, n_q / n_kv);
+  return DI_OK;
+}
+
+int detllm_attn_decode_acc(const int8_t* q8, const int64_t* tpos, const int8_t* kpool,
+                           const int8_t* vpool, const int32_t* table, int width,
+                           const uint8_t* valid, int64_t valid_stride, int B, int S, int n_q,
+                           int n_kv, const int64_t* s_dev, int64_t* acc, int64_t acc_stride,
+                           void* work, int64_t work_bytes, int64_t* out, int32_t* err,
+                           hipStream_t s) {
+  i64 need = 0;
+  if (const int rc = detllm_attn_decode_acc_work(B < 0 ? 0 : B, S, n_q, n_kv, &need)) return rc;
+  if (B <= 0) return DI_OK;
+  if (!kv_ok(kpool, vpool, table, width) || S > (i64)width * DI_PAGE || valid_stride < S ||
+      acc_stride < S || !q8 || !tpos || !valid || !acc || !out)
+    return DI_EINVAL;
+  if (need > 0 && (!work || work_bytes < need)) return DI_ERANGE;
+  const int G = n_q / n_kv;
+  const int chunk = S > 0 ? decode_chunk(B, S, n_q, n_kv) : 0;
+  DecodeArgs d{q8, tpos, KVPages{(int8_t*)kpool, (int8_t*)vpool, table, width, n_kv}, valid,
+               out, need > 0 ? (int32_t*)work : nullptr, s_dev, S, n_q, n_kv, valid_stride, err,
+               nullptr, nullptr, acc, acc_stride};
+  if (chunk) {
+    const SplitArgs sa = split_args(d, B, chunk, work);
+    const dim3 grid(n_kv, B, sa.ns);
+    const size_t dyn = (size_t)G * chunk * 4;
+    switch (G) {
+#define DI_ACC_SPLIT(G_)                                                  \
+  case G_:                                                                \
+    hipLaunchKernelGGL(k_acc_scores<G_>, grid, dim3(256), 0, s, sa);      \
+    hipLaunchKernelGGL(k_acc_pv<G_>, grid, dim3(256), dyn, s, sa);        \
+    break
+      DI_ACC_SPLIT(1);
+      DI_ACC_SPLIT(2);
+      DI_ACC_SPLIT(4);
+      DI_ACC_SPLIT(8);
+#undef DI_ACC_SPLIT
+    }
+  } else {
+    const dim3 grid(n_kv, B);
+    const size_t dyn = d.scratch ? 0 : (size_t)G * (((i64)S + 15) / 16 * 16) * 4;
+    switch (G) {
+#define DI_ACC_ONE(G_)                                                                        \
+  case G_:                                                                                    \
+    if (d.scratch) hipLaunchKernelGGL((k_acc_decode<G_, true>), grid, dim3(256), dyn, s, d);  \
+    else hipLaunchKernelGGL((k_acc_decode<G_, false>), grid, dim3(256), dyn, s, d);           \
+    break
+      DI_ACC_ONE(1);
+      DI_ACC_ONE(2);
+      DI_ACC_ONE(4);
+      DI_ACC_ONE(8);
+#undef DI_ACC_ONE
+    }
+  }
+  DI_LAUNCH_CHECK();
+  return DI_OK;
+}
+
+}  // extern "C"

@@ -20,13 +20,16 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/library.h>
 
+#include <algorithm>
 #include <string>
 #include <tuple>
 #include <utility>
+#include <vector>
 
 #include "../../include/detllm_hip.h"
 
@@ -137,7 +140,12 @@ const Entry ENTRIES[] = {
     DI_ENTRY(detllm_op_requant_i8_rowcol), DI_ENTRY(detllm_op_requant_i8_static),
     DI_ENTRY(detllm_op_residual), DI_ENTRY(detllm_op_rmsnorm), DI_ENTRY(detllm_op_softmax),
     DI_ENTRY(detllm_op_di_exp), DI_ENTRY(detllm_op_swiglu), DI_ENTRY(detllm_op_rope),
-    DI_ENTRY(detllm_op_scalar),
+    DI_ENTRY(detllm_op_scalar), DI_ENTRY(detllm_attn_window_prefill),
+    DI_ENTRY(detllm_attn_window_decode_work), DI_ENTRY(detllm_attn_window_decode),
+    DI_ENTRY(detllm_attn_prefill_acc), DI_ENTRY(detllm_attn_decode_acc_work),
+    DI_ENTRY(detllm_attn_decode_acc), DI_ENTRY(detllm_kv_select_work),
+    DI_ENTRY(detllm_kv_select), DI_ENTRY(detllm_kv_compact),
+    DI_ENTRY(detllm_attn_decode_shared_work), DI_ENTRY(detllm_attn_decode_shared),
 };
 #undef DI_ENTRY
 
@@ -462,9 +470,237 @@ Tensor op_attn_decode(const Tensor& q8, const Tensor& tpos, const Tensor& kpool,
   return out;
 }
 
+// ------------------------------------------------------------- long caches
+
+#define DI_CHECK(cond, op, ...) TORCH_CHECK_VALUE(cond, op, ": ", __VA_ARGS__)
+
+// What the kernels index by the shapes of q8 and of the cache alone. T: the
+// chunk's queries (0: one query per row, q8 [B, n_q, 128]); S: the last slot
+// they reach. n_kv: K's and V's heads.
+struct Cache {
+  int B, n_q, n_kv, width;
+};
+Cache check_cache(const char* op, const Tensor& q8, const Tensor& tpos, const Tensor& kpool,
+                  const Tensor& vpool, const Tensor& table, const Tensor& valid, bool chunk,
+                  int64_t S) {
+  const int64_t lead = chunk ? 4 : 3;
+  rank(q8, lead, op);
+  rank(kpool, 4, op);
+  rank(table, 2, op);
+  rank(valid, 2, op);
+  DI_CHECK(q8.scalar_type() == at::kChar && kpool.scalar_type() == at::kChar &&
+               vpool.scalar_type() == at::kChar,
+           op, "expected int8 queries and pools");
+  DI_CHECK(tpos.scalar_type() == at::kLong && table.scalar_type() == at::kInt &&
+               (valid.scalar_type() == at::kBool || valid.scalar_type() == at::kByte),
+           op, "expected int64 tpos, an int32 table and a bool mask");
+  DI_CHECK(q8.size(-1) == 128 && tpos.sizes() == q8.sizes().slice(0, lead - 1), op,
+           "expected queries of 128 channels with a constant each, got ", q8.sizes(), " and ",
+           tpos.sizes());
+  DI_CHECK(kpool.size(0) > 0 && kpool.size(1) > 0 && kpool.size(2) == 128 &&
+               kpool.size(3) == 128 && vpool.sizes() == kpool.sizes(),
+           op, "expected pools [pages, n_kv, 128, 128], got ", kpool.sizes(), " and ",
+           vpool.sizes());
+  const int64_t B = q8.size(0), n_q = q8.size(1), n_kv = kpool.size(1);
+  DI_CHECK(n_q > 0 && n_q % n_kv == 0, op, n_q, " query heads over ", n_kv, " kv heads");
+  DI_CHECK(table.size(0) == B && valid.size(0) == B, op, "a table of ", table.size(0),
+           " rows and a mask of ", valid.size(0), " for ", B);
+  DI_CHECK(S >= 0 && S <= 131071 && S <= table.size(1) * 128 && S <= valid.size(1), op, S,
+           " slots over a table of ", table.size(1), " pages and a mask of ", valid.size(1));
+  DI_CHECK(kpool.is_contiguous() && vpool.is_contiguous() && table.is_contiguous() &&
+               valid.stride(1) == 1,
+           op, "expected contiguous pools, table and mask rows");
+  for (const Tensor* t : {&tpos, &kpool, &vpool, &table, &valid})
+    DI_CHECK(t->device() == q8.device(), op, "operands on ", q8.device(), " and ", t->device());
+  return {(int)B, (int)n_q, (int)n_kv, (int)table.size(1)};
+}
+int as_i32(int64_t v) { return (int)std::min<int64_t>(v, INT32_MAX); }
+
+// acc [B, n_kv, slots]: what a kernel adds to in place
+void check_acc(const char* op, const Tensor& acc, int64_t B, int64_t n_kv, int64_t S,
+               const Tensor& like) {
+  rank(acc, 3, op);
+  DI_CHECK(acc.scalar_type() == at::kLong && acc.is_contiguous() &&
+               acc.device() == like.device(),
+           op, "expected contiguous int64 accumulators on ", like.device());
+  DI_CHECK(acc.size(0) == B && acc.size(1) == n_kv && acc.size(2) >= S, op, "accumulators ",
+           acc.sizes(), " for ", B, " rows, ", n_kv, " kv heads and ", S, " slots");
+}
+
+// The arguments that every attention entry begins with (B and n_q behind them)
+#define DI_CACHE_ARGS                                                                         \
+  ptr<int8_t>(qc), i64(tc), ptr<int8_t>(kpool), ptr<int8_t>(vpool), ptr<int32_t>(table),      \
+      c.width, ptr<uint8_t>(v), valid.stride(0)
+
+Tensor op_attn_window_prefill(const Tensor& q8, const Tensor& tpos, const Tensor& kpool,
+                              const Tensor& vpool, const Tensor& table, const Tensor& valid,
+                              int64_t S_past, int64_t window, int64_t sinks) {
+  constexpr const char* op = "attn_window_prefill";
+  rank(q8, 4, op);
+  const int64_t T = q8.size(2);
+  DI_CHECK(S_past >= 0 && window >= 1 && sinks >= 0, op, "S_past ", S_past, ", window ", window,
+           ", sinks ", sinks);
+  const Cache c = check_cache(op, q8, tpos, kpool, vpool, table, valid, true, S_past + T);
+  const c10::DeviceGuard guard(q8.device());
+  Tensor out = empty({c.B, T, c.n_q * 128}, at::kLong, q8);
+  const Tensor qc = q8.contiguous(), tc = tpos.contiguous(), v = valid.view(at::kByte);
+  DI_RUN(detllm_attn_window_prefill, DI_CACHE_ARGS, c.B, (int)T, (int)S_past, c.n_q, c.n_kv,
+         as_i32(window), as_i32(sinks), ptr<int64_t>(out));
+  return out;
+}
+
+Tensor op_attn_prefill_acc(const Tensor& q8, const Tensor& tpos, const Tensor& kpool,
+                           const Tensor& vpool, const Tensor& table, const Tensor& valid,
+                           int64_t S_past, const Tensor& acc) {
+  constexpr const char* op = "attn_prefill_acc";
+  rank(q8, 4, op);
+  const int64_t T = q8.size(2);
+  DI_CHECK(S_past >= 0, op, "S_past ", S_past);
+  const Cache c = check_cache(op, q8, tpos, kpool, vpool, table, valid, true, S_past + T);
+  check_acc(op, acc, c.B, c.n_kv, S_past + T, q8);
+  const c10::DeviceGuard guard(q8.device());
+  Tensor out = empty({c.B, T, c.n_q * 128}, at::kLong, q8);
+  const Tensor qc = q8.contiguous(), tc = tpos.contiguous(), v = valid.view(at::kByte);
+  DI_RUN(detllm_attn_prefill_acc, DI_CACHE_ARGS, c.B, (int)T, (int)S_past, c.n_q, c.n_kv,
+         ptr<int64_t>(acc), acc.size(2), ptr<int64_t>(out));
+  mutated(acc);
+  return out;
+}
+
+// Scratch of one call (torch's allocator orders its reuse by stream)
+Tensor scratch(int64_t bytes, const Tensor& like) { return empty({bytes}, at::kByte, like); }
+
+Tensor op_attn_window_decode(const Tensor& q8, const Tensor& tpos, const Tensor& kpool,
+                             const Tensor& vpool, const Tensor& table, const Tensor& valid,
+                             int64_t S, int64_t window, int64_t sinks) {
+  constexpr const char* op = "attn_window_decode";
+  DI_CHECK(window >= 1 && sinks >= 0, op, "window ", window, ", sinks ", sinks);
+  const Cache c = check_cache(op, q8, tpos, kpool, vpool, table, valid, false, S);
+  const int win = as_i32(window), sk = as_i32(sinks);
+  int64_t bytes = 0;
+  check(detllm_attn_window_decode_work(c.B, (int)S, c.n_q, c.n_kv, win, sk, &bytes),
+        "detllm_attn_window_decode_work");
+  const c10::DeviceGuard guard(q8.device());
+  Tensor out = empty({c.B, c.n_q * 128}, at::kLong, q8);
+  const Tensor work = scratch(bytes, q8);
+  const Tensor qc = q8.contiguous(), tc = tpos.contiguous(), v = valid.view(at::kByte);
+  DI_RUN(detllm_attn_window_decode, DI_CACHE_ARGS, c.B, (int)S, c.n_q, c.n_kv, nullptr, win, sk,
+         work.data_ptr(), bytes, ptr<int64_t>(out), nullptr);
+  return out;
+}
+
+Tensor op_attn_decode_acc(const Tensor& q8, const Tensor& tpos, const Tensor& kpool,
+                          const Tensor& vpool, const Tensor& table, const Tensor& valid,
+                          int64_t S, const Tensor& acc) {
+  constexpr const char* op = "attn_decode_acc";
+  const Cache c = check_cache(op, q8, tpos, kpool, vpool, table, valid, false, S);
+  check_acc(op, acc, c.B, c.n_kv, S, q8);
+  int64_t bytes = 0;
+  check(detllm_attn_decode_acc_work(c.B, (int)S, c.n_q, c.n_kv, &bytes),
+        "detllm_attn_decode_acc_work");
+  const c10::DeviceGuard guard(q8.device());
+  Tensor out = empty({c.B, c.n_q * 128}, at::kLong, q8);
+  const Tensor work = scratch(bytes, q8);
+  const Tensor qc = q8.contiguous(), tc = tpos.contiguous(), v = valid.view(at::kByte);
+  DI_RUN(detllm_attn_decode_acc, DI_CACHE_ARGS, c.B, (int)S, c.n_q, c.n_kv, nullptr,
+         ptr<int64_t>(acc), acc.size(2), work.data_ptr(), bytes, ptr<int64_t>(out), nullptr);
+  mutated(acc);
+  return out;
+}
+
+Tensor op_attn_decode_shared(const Tensor& q8, const Tensor& tpos, const Tensor& kpool,
+                             const Tensor& vpool, const Tensor& table, const Tensor& valid,
+                             int64_t S, int64_t shared) {
+  constexpr const char* op = "attn_decode_shared";
+  DI_CHECK(shared >= 0 && shared <= S && shared % 128 == 0, op, shared, " of ", S,
+           " slots shared (whole pages of 128)");
+  const Cache c = check_cache(op, q8, tpos, kpool, vpool, table, valid, false, S);
+  int64_t bytes = 0;
+  check(detllm_attn_decode_shared_work(c.B, (int)S, c.n_q, c.n_kv, (int)shared, &bytes),
+        "detllm_attn_decode_shared_work");
+  const c10::DeviceGuard guard(q8.device());
+  Tensor out = empty({c.B, c.n_q * 128}, at::kLong, q8);
+  const Tensor work = scratch(bytes, q8);
+  const Tensor qc = q8.contiguous(), tc = tpos.contiguous(), v = valid.view(at::kByte);
+  DI_RUN(detllm_attn_decode_shared, DI_CACHE_ARGS, c.B, (int)S, c.n_q, c.n_kv, nullptr,
+         (int)shared, work.data_ptr(), bytes, ptr<int64_t>(out), nullptr);
+  return out;
+}
+
+T2 op_kv_select(const Tensor& acc, const Tensor& valid, int64_t S, int64_t budget, int64_t recent,
+                int64_t sinks) {
+  constexpr const char* op = "kv_select";
+  rank(acc, 3, op);
+  rank(valid, 2, op);
+  const int64_t B = acc.size(0), n_kv = acc.size(1);
+  DI_CHECK(acc.scalar_type() == at::kLong && acc.is_contiguous(), op,
+           "expected contiguous int64 accumulators");
+  DI_CHECK((valid.scalar_type() == at::kBool || valid.scalar_type() == at::kByte) &&
+               valid.stride(1) == 1 && valid.device() == acc.device() && valid.size(0) == B,
+           op, "expected a bool mask of ", B, " rows on ", acc.device());
+  DI_CHECK(n_kv > 0 && S >= 0 && S <= acc.size(2) && S <= valid.size(1) && S < INT32_MAX, op, S,
+           " slots of accumulators ", acc.sizes(), " and a mask ", valid.sizes());
+  DI_CHECK(budget >= 1 && budget < INT32_MAX && recent >= 0 && sinks >= 0 &&
+               recent <= budget - sinks,
+           op, "recent ", recent, " and sinks ", sinks, " of a budget of ", budget);
+  int64_t bytes = 0;
+  check(detllm_kv_select_work((int)B, (int)S, &bytes), "detllm_kv_select_work");
+  const c10::DeviceGuard guard(acc.device());
+  Tensor keep = empty({B, budget}, at::kInt, acc), kept = empty({B, n_kv, budget}, at::kLong, acc);
+  const Tensor work = scratch(bytes, acc), v = valid.view(at::kByte);
+  DI_RUN(detllm_kv_select, i64(acc), acc.size(2), ptr<uint8_t>(v), valid.stride(0), (int)B, (int)S,
+         (int)n_kv, (int)budget, (int)recent, (int)sinks, ptr<int32_t>(keep), ptr<int64_t>(kept),
+         work.data_ptr(), bytes);
+  return {keep, kept};
+}
+
+void op_kv_compact(at::TensorList kpools, at::TensorList vpools, const Tensor& table,
+                   const Tensor& dst, const Tensor& keep) {
+  constexpr const char* op = "kv_compact";
+  rank(table, 2, op);
+  rank(dst, 2, op);
+  rank(keep, 2, op);
+  const int64_t B = table.size(0);
+  DI_CHECK(!kpools.empty() && kpools.size() == vpools.size(), op, kpools.size(), " K pools and ",
+           vpools.size(), " V pools");
+  for (const Tensor* t : {&table, &dst, &keep})
+    DI_CHECK(t->scalar_type() == at::kInt && t->is_contiguous() && t->size(0) == B &&
+                 t->device() == table.device(),
+             op, "expected contiguous int32 table, dst and keep of ", B, " rows on ",
+             table.device());
+  std::vector<int8_t*> k, v;
+  rank(kpools[0], 4, op);
+  for (size_t i = 0; i < kpools.size(); ++i)
+    for (const Tensor* t : {&kpools[i], &vpools[i]}) {
+      rank(*t, 4, op);
+      DI_CHECK(t->scalar_type() == at::kChar && t->is_contiguous() && t->size(0) > 0 &&
+                   t->size(1) > 0 && t->size(2) == 128 && t->size(3) == 128 &&
+                   t->sizes() == kpools[0].sizes() && t->device() == table.device(),
+               op, "expected contiguous int8 pools [pages, n_kv, 128, 128] on ", table.device());
+      (t == &kpools[i] ? k : v).push_back(ptr<int8_t>(*t));
+    }
+  DI_CHECK(table.size(1) > 0 && dst.size(1) * 128 >= keep.size(1), op, keep.size(1),
+           " slots for ", dst.size(1), " pages");
+  const c10::DeviceGuard guard(table.device());
+  DI_RUN(detllm_kv_compact, k.data(), v.data(), (int)k.size(), ptr<int32_t>(table),
+         (int)table.size(1), ptr<int32_t>(dst), (int)dst.size(1), ptr<int32_t>(keep), (int)B,
+         (int)keep.size(1), (int)kpools[0].size(1));
+  for (size_t i = 0; i < kpools.size(); ++i) {
+    mutated(kpools[i]);
+    mutated(vpools[i]);
+  }
+}
+
 }  // namespace
 
 TORCH_LIBRARY_IMPL(detllm_rocm, CUDA, m) {
+  m.impl("attn_window_prefill", &op_attn_window_prefill);
+  m.impl("attn_window_decode", &op_attn_window_decode);
+  m.impl("attn_prefill_acc", &op_attn_prefill_acc);
+  m.impl("attn_decode_acc", &op_attn_decode_acc);
+  m.impl("attn_decode_shared", &op_attn_decode_shared);
+  m.impl("kv_select", &op_kv_select);
+  m.impl("kv_compact", &op_kv_compact);
   m.impl("int_gemm", &op_int_gemm);
   m.impl("isqrt_i64", &op_isqrt);
   m.impl("ilog2_i64", &op_ilog2);

@@ -35,12 +35,16 @@ OPS = ("int_gemm", "isqrt_i64", "ilog2_i64", "greedy_pick", "embed_normq", "norm
        "residual_normq", "swiglu_quant", "merge_rowcol", "qkv_epilogue", "attn_prefill",
        "attn_decode")
 
+# The operators for long caches (no counterpart in the reference)
+LONG_OPS = ("attn_window_prefill", "attn_window_decode", "attn_prefill_acc", "attn_decode_acc",
+            "attn_decode_shared", "kv_select", "kv_compact")
+
 
 def _op(schema):
     """Define one operator; the decorated function is its fake (shapes and
     integer dtypes), the result the operator itself."""
     name = schema.split("(", 1)[0]
-    assert name in OPS
+    assert name in OPS + LONG_OPS
     torch.library.define(f"{NS}::{name}", schema[len(name):], tags=(torch.Tag.pt2_compliant_tag,))
 
     def wrap(fake):
@@ -169,6 +173,79 @@ def attn_decode(q8, tpos, kpool, vpool, table, valid, S, err):
     return q8.new_empty(q8.shape[0], q8.shape[1] * 128, dtype=I64)
 
 
+# ----------------------------------------------------------- long caches
+#
+# Operands that do not fit raise ValueError before any launch. Slots are at
+# most 131071 per row, n_q / n_kv is 1, 2, 4 or 8 in the decode forms.
+
+@_op("attn_window_prefill(Tensor q8, Tensor tpos, Tensor kpool, Tensor vpool, Tensor table, "
+     "Tensor valid, SymInt S_past, SymInt window, SymInt sinks) -> Tensor")
+def attn_window_prefill(q8, tpos, kpool, vpool, table, valid, S_past, window, sinks):
+    """attn_prefill with a sliding window and sinks: the query at slot t sees
+    the last ``window`` (at least 1) valid slots up to t and the row's first
+    ``sinks`` valid slots. Padding does not count: a row sees the same tokens
+    in every batch."""
+    B, n_q, T, _ = q8.shape
+    return q8.new_empty(B, T, n_q * 128, dtype=I64)
+
+
+@_op("attn_window_decode(Tensor q8, Tensor tpos, Tensor kpool, Tensor vpool, Tensor table, "
+     "Tensor valid, SymInt S, SymInt window, SymInt sinks) -> Tensor")
+def attn_window_decode(q8, tpos, kpool, vpool, table, valid, S, window, sinks):
+    """attn_decode with a sliding window and sinks (attn_window_prefill's
+    rule), the rows' queries at slot S - 1."""
+    return q8.new_empty(q8.shape[0], q8.shape[1] * 128, dtype=I64)
+
+
+@_op("attn_prefill_acc(Tensor q8, Tensor tpos, Tensor kpool, Tensor vpool, Tensor table, "
+     "Tensor valid, SymInt S_past, Tensor(a7!) acc) -> Tensor")
+def attn_prefill_acc(q8, tpos, kpool, vpool, table, valid, S_past, acc):
+    """attn_prefill, and acc [B, n_kv, slots] int64 += each slot's weight
+    (probabilities in [0, 2^14]) over the kv head's query heads and the
+    chunk's queries at valid slots. Calls that add to one acc must follow
+    each other."""
+    B, n_q, T, _ = q8.shape
+    return q8.new_empty(B, T, n_q * 128, dtype=I64)
+
+
+@_op("attn_decode_acc(Tensor q8, Tensor tpos, Tensor kpool, Tensor vpool, Tensor table, "
+     "Tensor valid, SymInt S, Tensor(a7!) acc) -> Tensor")
+def attn_decode_acc(q8, tpos, kpool, vpool, table, valid, S, acc):
+    """attn_decode, and acc [B, n_kv, slots] int64 += each slot's weight over
+    the kv head's query heads, for the rows whose slot S - 1 is valid."""
+    return q8.new_empty(q8.shape[0], q8.shape[1] * 128, dtype=I64)
+
+
+@_op("attn_decode_shared(Tensor q8, Tensor tpos, Tensor kpool, Tensor vpool, Tensor table, "
+     "Tensor valid, SymInt S, SymInt shared) -> Tensor")
+def attn_decode_shared(q8, tpos, kpool, vpool, table, valid, S, shared):
+    """attn_decode of rows that share their first ``shared`` slots (a multiple
+    of 128): row 0's pages stand for every row's there and are read once for
+    the batch; valid stays each row's own."""
+    return q8.new_empty(q8.shape[0], q8.shape[1] * 128, dtype=I64)
+
+
+@_op("kv_select(Tensor acc, Tensor valid, SymInt S, SymInt budget, SymInt recent, SymInt sinks) "
+     "-> (Tensor, Tensor)")
+def kv_select(acc, valid, S, budget, recent, sinks):
+    """Which of the rows' slots [0, S) stay when at most ``budget`` may: all
+    valid ones where they fit, else the first ``sinks``, the last ``recent``
+    and the heaviest others by acc summed over the kv heads, ties to the
+    lower slot. -> (keep [B, budget] int32 ascending, -1 behind; their
+    accumulators [B, n_kv, budget], 0 behind)."""
+    return (acc.new_empty(acc.shape[0], budget, dtype=torch.int32),
+            acc.new_empty(acc.shape[0], acc.shape[1], budget))
+
+
+@_op("kv_compact(Tensor(a0!)[] kpools, Tensor(a1!)[] vpools, Tensor table, Tensor dst, "
+     "Tensor keep) -> ()")
+def kv_compact(kpools, vpools, table, dst, keep):
+    """Every layer's K and V of the slots keep [B, budget] (kv_select's) copied
+    in order to the pages dst [B, pages] (-1: not written), zeros behind
+    them. dst[b, j] is one of table[b, :j + 1], or in no row's table; no page
+    is in dst twice."""
+
+
 # Loading the native binding registers the kernels. Where it cannot be loaded
 # (not built, or built for another torch), the import goes on and a call of an
 # operator raises, as the other entries do; a call after it has been built
@@ -194,7 +271,7 @@ def _load_kernels():
 def _register_stand_ins():
     global _stand_ins
     _stand_ins = torch.library.Library(NS, "IMPL")
-    for name in OPS:
+    for name in OPS + LONG_OPS:
         def call_again(keyset, *args, _op=getattr(torch.ops.detllm_rocm, name).default, **kwargs):
             _load_kernels()
             return _op.redispatch(keyset, *args, **kwargs)

@@ -377,6 +377,83 @@ int detllm_attn_decode_split_sum(const int8_t* q8, const int64_t* tpos, const in
  * (or detllm_qkv_attn_decode) is the faster call. Writes *chunk, *nsplit. */
 int detllm_attn_split_plan(int B, int S, int n_q, int n_kv, int* chunk, int* nsplit);
 
+/* ---- long caches: no counterpart in the reference. The integers of a query
+ * are those of detllm_attn_prefill / detllm_attn_decode over the slots it sees;
+ * arguments with those names mean the same. The entries named *_work write the
+ * bytes of device scratch (`work`, 16-byte aligned) that the call of the same
+ * sizes needs (host only); less returns -34. n_q / n_kv is 1, 2, 4 or 8 in the
+ * decode forms, S (or S_past + T) at most 131071. */
+
+/* Windowed attention with sinks: the query at slot t sees the valid slots
+ * s <= t with fewer than `window` valid slots in (s, t] or fewer than `sinks`
+ * valid slots in [0, s), its last `window` tokens and the row's first `sinks`,
+ * whatever the padding between them. window >= 1, sinks >= 0. Prefill: queries
+ * at slots S_past + t; decode: one query per row, at the last scanned slot. */
+int detllm_attn_window_prefill(const int8_t* q8, const int64_t* tpos, const int8_t* kpool,
+                               const int8_t* vpool, const int32_t* table, int width,
+                               const uint8_t* valid, int64_t valid_stride, int B, int T,
+                               int S_past, int n_q, int n_kv, int window, int sinks, int64_t* out,
+                               hipStream_t s);
+int detllm_attn_window_decode_work(int B, int S, int n_q, int n_kv, int window, int sinks,
+                                   int64_t* bytes);
+int detllm_attn_window_decode(const int8_t* q8, const int64_t* tpos, const int8_t* kpool,
+                              const int8_t* vpool, const int32_t* table, int width,
+                              const uint8_t* valid, int64_t valid_stride, int B, int S, int n_q,
+                              int n_kv, const int64_t* s_dev, int window, int sinks, void* work,
+                              int64_t work_bytes, int64_t* out, int32_t* err, hipStream_t s);
+
+/* Attention that accumulates its weights: detllm_attn_prefill /
+ * detllm_attn_decode, and acc [B][n_kv][acc_stride] int64 (acc_stride >= the
+ * slots) += for each slot the p of the kv head's query heads, over the chunk's
+ * queries that sit at valid slots (decode: if the last scanned slot is valid).
+ * Calls that add to one acc follow each other (one stream, or events). */
+int detllm_attn_prefill_acc(const int8_t* q8, const int64_t* tpos, const int8_t* kpool,
+                            const int8_t* vpool, const int32_t* table, int width,
+                            const uint8_t* valid, int64_t valid_stride, int B, int T, int S_past,
+                            int n_q, int n_kv, int64_t* acc, int64_t acc_stride, int64_t* out,
+                            hipStream_t s);
+int detllm_attn_decode_acc_work(int B, int S, int n_q, int n_kv, int64_t* bytes);
+int detllm_attn_decode_acc(const int8_t* q8, const int64_t* tpos, const int8_t* kpool,
+                           const int8_t* vpool, const int32_t* table, int width,
+                           const uint8_t* valid, int64_t valid_stride, int B, int S, int n_q,
+                           int n_kv, const int64_t* s_dev, int64_t* acc, int64_t acc_stride,
+                           void* work, int64_t work_bytes, int64_t* out, int32_t* err,
+                           hipStream_t s);
+
+/* Eviction by accumulated weight. detllm_kv_select: of row b's slots [0, S)
+ * those that stay, keep [B][budget] ascending (-1 behind them), and their
+ * accumulators, kept [B][n_kv][budget] (0 behind them). A row of at most
+ * `budget` valid slots keeps them all; else its first `sinks` and last `recent`
+ * valid slots and, of the valid slots between, the budget - sinks - recent with
+ * the largest acc summed over the kv heads (int64, wrapping), ties to the lower
+ * slot. recent + sinks <= budget. */
+int detllm_kv_select_work(int B, int S, int64_t* bytes);
+int detllm_kv_select(const int64_t* acc, int64_t acc_stride, const uint8_t* valid,
+                     int64_t valid_stride, int B, int S, int n_kv, int budget, int recent,
+                     int sinks, int32_t* keep, int64_t* kept, void* work, int64_t work_bytes,
+                     hipStream_t s);
+
+/* detllm_kv_compact: slot keep[b][i] of every layer's K and V copied to slot i
+ * of the pages dst [B][dst_width] (-1: not written); the slots of these pages
+ * past row b's last kept one, and those of kept slots whose page is not mapped,
+ * become 0. kpools / vpools: HOST arrays of n_layers device pointers. keep as
+ * detllm_kv_select writes it. The page dst[b][j] may be one of row b's pages
+ * table[b][0..j]; otherwise no page of dst is in table, and none is in dst
+ * twice. */
+int detllm_kv_compact(int8_t* const* kpools, int8_t* const* vpools, int n_layers,
+                      const int32_t* table, int width, const int32_t* dst, int dst_width,
+                      const int32_t* keep, int B, int budget, int n_kv, hipStream_t s);
+
+/* detllm_attn_decode of a batch whose rows share their first `shared` slots (a
+ * multiple of 128, at most S): row 0's pages stand for those of every row
+ * there, and are read once for the batch. valid is each row's own. */
+int detllm_attn_decode_shared_work(int B, int S, int n_q, int n_kv, int shared, int64_t* bytes);
+int detllm_attn_decode_shared(const int8_t* q8, const int64_t* tpos, const int8_t* kpool,
+                              const int8_t* vpool, const int32_t* table, int width,
+                              const uint8_t* valid, int64_t valid_stride, int B, int S, int n_q,
+                              int n_kv, const int64_t* s_dev, int shared, void* work,
+                              int64_t work_bytes, int64_t* out, int32_t* err, hipStream_t s);
+
 /* Per-step bookkeeping of the graph-captured decode (src/detllm/graphed.py:
  * 112-131: the validity flag of the step's slot, the device scalars holding
  * the write slot and the scanned-slot count, the positions), one launch
