@@ -32,18 +32,21 @@ __global__ __launch_bounds__(256, 2) void k_acc_prefill(PrefillArgs a) {
   prefill_body<false, true>(a);
 }
 
-// The pages a row's newest query sees, numbered without the gap.
+// The listed pages of a row's newest query (window_pages), numbered 0, 1, ...
 struct WinView {
   static constexpr bool kWhole = false;
-  int n;      // slots of the list
-  int pre;    // slots before the gap
-  int skip;   // slots left out
+  const uint16_t* list;
+  int n;  // slots of the list
   int sink_end, lo;
-  __device__ __forceinline__ int slot(int s) const { return s < pre ? s : s + skip; }
+  __device__ __forceinline__ int slot(int s) const {
+    return (int)list[s >> 7] * DI_PAGE + (s & (DI_PAGE - 1));
+  }
   __device__ __forceinline__ bool sees(int s) const { return s < sink_end || s >= lo; }
 };
-__device__ __forceinline__ WinView win_view(const WinRange& r, int S) {
-  return WinView{S - r.skip * DI_PAGE, r.pre * DI_PAGE, r.skip * DI_PAGE, r.sink_end, r.lo};
+__device__ __forceinline__ WinView win_view(const WinRange& r, const uint16_t* list, int S) {
+  int n = r.pages * DI_PAGE;
+  if (r.pages > 0) n -= ::max(((int)list[r.pages - 1] + 1) * DI_PAGE - S, 0);
+  return WinView{list, n, r.sink_end, r.lo};
 }
 
 struct WindowArgs {
@@ -51,7 +54,9 @@ struct WindowArgs {
   int window, sinks;
   int zs;          // blocks per (row, kv head)
   int lds_slots;   // one block: slots whose scores its LDS holds
-  WinRange* range; // [B] (split form)
+  WinRange* range; // [B], and the lists [B][pages] (split form: made by the
+  uint16_t* lists; // scores launch for the second)
+  int pages;
 };
 
 // One block per (row, kv head). Scores in LDS; a row whose window spans more
@@ -61,13 +66,14 @@ __global__ __launch_bounds__(256) void k_window_decode(WindowArgs w) {
   keep_hidden_args();
   extern __shared__ __attribute__((aligned(16))) int32_t sh_scores[];
   __shared__ int32_t pg_lds[DEC_MAX_PAGES];
+  __shared__ uint16_t list[DEC_MAX_PAGES];
   DecodeArgs a = w.s.d;
   const int kvh = blockIdx.x, b = blockIdx.y;
   const i64 q0 = (i64)b * a.n_q + kvh * G;
   bool over;
   const int S = scanned_slots(a, a.tpos, &over);
   const WinView v = win_view(
-      window_range<256>(a.valid + (i64)b * a.valid_stride, S, S, w.window, w.sinks), S);
+      window_pages<256>(a.valid + (i64)b * a.valid_stride, S, S, w.window, w.sinks, list), list, S);
   const int npages = (v.n + DI_PAGE - 1) / DI_PAGE;
   for (int i = threadIdx.x; i < npages; i += 256) pg_lds[i] = a.kv.page(b, v.slot(i * DI_PAGE));
   if (npages == 0 && threadIdx.x == 0) pg_lds[0] = -1;  // S = 0: loads read page 0
@@ -90,9 +96,14 @@ __global__ __launch_bounds__(256) void k_window_scores(WindowArgs w) {
   const int kvh = blockIdx.x, b = blockIdx.y, z = blockIdx.z;
   bool over;
   const int S = scanned_slots(a, a.tpos, &over);
-  const WinRange r = window_range<256>(a.valid + (i64)b * a.valid_stride, S, S, w.window, w.sinks);
-  if (kvh == 0 && z == 0 && threadIdx.x == 0) w.range[b] = r;
-  const WinView v = win_view(r, S);
+  __shared__ uint16_t list[DEC_MAX_PAGES];
+  const WinRange r =
+      window_pages<256>(a.valid + (i64)b * a.valid_stride, S, S, w.window, w.sinks, list);
+  if (kvh == 0 && z == 0) {
+    if (threadIdx.x == 0) w.range[b] = r;
+    for (int i = threadIdx.x; i < r.pages; i += 256) w.lists[(i64)b * w.pages + i] = list[i];
+  }
+  const WinView v = win_view(r, list, S);
   int c = z;
   do {
     split_scores_chunk<G, WinView>(w.s, kvh, b, c, v);
@@ -109,7 +120,7 @@ __global__ __launch_bounds__(256) void k_window_pv(WindowArgs w) {
   const int kvh = blockIdx.x, b = blockIdx.y;
   bool over;
   const int S = scanned_slots(a, a.tpos, &over);
-  const WinView v = win_view(w.range[b], S);
+  const WinView v = win_view(w.range[b], w.lists + (i64)b * w.pages, S);
   int c = blockIdx.z;
   do {
     split_pv_chunk<G, WinView>(w.s, kvh, b, c, v);
@@ -166,6 +177,7 @@ i64 split_bytes(int B, int S, int n_q, int chunk, i64* cmax_at) {
   *cmax_at = rows * ns * chunk * 4;
   return *cmax_at + (rows * ns * 4 + 15) / 16 * 16;
 }
+int pages_of(int S) { return (S + DI_PAGE - 1) / DI_PAGE; }
 i64 one_block_bytes(int B, int S, int n_q, int G) {
   const i64 spad = ((i64)S + 15) / 16 * 16;
   return (i64)G * spad * 4 > DECODE_LDS_BYTES ? (i64)B * n_q * spad * 4 : 0;
@@ -175,10 +187,10 @@ int heads_ok(int n_q, int n_kv) {
   const int G = n_q / n_kv;
   return G == 1 || G == 2 || G == 4 || G == 8 ? DI_OK : DI_ENOSYS;
 }
-// Slots a windowed query sees in a row without gaps, with the partial pages at
-// the ends of the two ranges.
+// Slots that a launch is sized for: what a query sees, and the rest of the
+// pages at the ends of the two ranges and around two stretches of padding.
 int window_slots(int S, int window, int sinks) {
-  return (int)imin(S, (i64)window + sinks + 2 * DI_PAGE);
+  return (int)imin(S, (i64)window + sinks + 6 * DI_PAGE);
 }
 SplitArgs split_args(const DecodeArgs& d, int B, int chunk, void* work) {
   SplitArgs sa{};
@@ -215,7 +227,8 @@ int detllm_attn_window_prefill(const int8_t* q8, const int64_t* tpos, const int8
                 T, (int)S, S_past, n_q, n_kv, B, valid_stride, window, sinks};
   const i64 pairs = (i64)(((T + 63) / 64 + 1) / 2) * n_q * B;
   if (2 * pairs > 0x7fffffff) return DI_ERANGE;
-  hipLaunchKernelGGL(k_window_prefill, dim3((unsigned)(2 * pairs)), dim3(256), prefill_lds(S), s, a);
+  hipLaunchKernelGGL(k_window_prefill, dim3((unsigned)(2 * pairs)), dim3(256),
+                     prefill_lds(S, true), s, a);
   DI_LAUNCH_CHECK();
   return DI_OK;
 }
@@ -250,7 +263,7 @@ int detllm_attn_window_decode_work(int B, int S, int n_q, int n_kv, int window, 
   if (B == 0 || S == 0) return DI_OK;
   const int chunk = decode_chunk(B, window_slots(S, window, sinks), n_q, n_kv);
   i64 at;
-  *bytes = chunk ? split_bytes(B, S, n_q, chunk, &at) + (i64)B * sizeof(WinRange)
+  *bytes = chunk ? split_bytes(B, S, n_q, chunk, &at) + (i64)B * (sizeof(WinRange) + 2 * pages_of(S))
                  : one_block_bytes(B, S, n_q, n_q / n_kv);
   return DI_OK;
 }
@@ -279,6 +292,8 @@ int detllm_attn_window_decode(const int8_t* q8, const int64_t* tpos, const int8_
     w.s = split_args(d, B, chunk, work);
     i64 at;
     w.range = (WinRange*)((char*)work + split_bytes(B, S, n_q, chunk, &at));
+    w.lists = (uint16_t*)(w.range + B);
+    w.pages = pages_of(S);
     w.zs = (slots + chunk - 1) / chunk;
     const dim3 grid(n_kv, B, w.zs);
     const size_t dyn = (size_t)G * chunk * 4;

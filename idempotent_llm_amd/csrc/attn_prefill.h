@@ -66,9 +66,10 @@ __device__ __forceinline__ void pf_pack(const uint32_t (&p)[4], int& whi, int& w
   wlo = (int)((l01 | l23) & 0x7f7f7f7fu);
 }
 
-// Dynamic LDS of a launch over S slots: column sums, tile masks, page ids
-inline size_t prefill_lds(i64 S) {
-  return PF_CSUM + 8 * (size_t)((S + 63) / 64) + 4 * (size_t)((S + 127) / 128);
+// Dynamic LDS of a launch over S slots: column sums, tile masks, page ids (and
+// the windowed form's page numbers)
+inline size_t prefill_lds(i64 S, bool win = false) {
+  return PF_CSUM + 8 * (size_t)((S + 63) / 64) + (win ? 6 : 4) * (size_t)((S + 127) / 128);
 }
 
 // v[i] of each lane summed over its aligned row of 16 lanes: lane i of the row
@@ -147,16 +148,25 @@ __device__ __forceinline__ void prefill_body(const PrefillArgs& a) {
   const int wlim = a.S_past + qt * 64 + wave * 16;  // the smallest limit in the wave
   const int kend = min(a.S, a.S_past + qt * 64 + 64);
   const uint8_t* vrow = a.valid + (i64)b * a.valid_stride;
-  // The windowed form walks the pages of the sinks and those from the first
-  // query's window on; tile and page numbers below count that list, and
-  // slot64 / slot_page give their first slots.
+  // The windowed form walks the pages that its queries see (window_pages);
+  // tile and page numbers below count that list.
+  uint16_t* const list = (uint16_t*)(pages + (a.S + 127) / 128);  // WIN: the pages' numbers
   WinRange wr{};
-  if constexpr (WIN) wr = window_range<256>(vrow, a.S_past + qt * 64 + 1, kend, a.window, a.sinks);
-  const int ntiles = (kend + 63) / 64 - 2 * wr.skip;
+  int ntiles = (kend + 63) / 64;
+  if constexpr (WIN) {
+    wr = window_pages<256>(vrow, a.S_past + qt * 64 + 1, kend, a.window, a.sinks, list);
+    ntiles = 2 * wr.pages;
+    if (wr.pages > 0 && listed_slot64(list, ntiles - 1) >= kend) --ntiles;
+    ntiles = __builtin_amdgcn_readfirstlane(ntiles);
+  }
   const int ntiles2 = (ntiles + 1) / 2;  // 128-slot tiles = pages
-  auto slot64 = [&](int it) { return (it < 2 * wr.pre ? it : it + 2 * wr.skip) * 64; };
+  auto slot64 = [&](int it) {
+    if constexpr (WIN) return __builtin_amdgcn_readfirstlane(listed_slot64(list, it));
+    return it * 64;
+  };
   auto page_of = [&](int i) {
-    return a.kv.page(b, (i64)(i < wr.pre ? i : i + wr.skip) * DI_PAGE);
+    if constexpr (WIN) return a.kv.page(b, (int)list[i] * DI_PAGE);
+    return a.kv.page(b, (i64)i * DI_PAGE);
   };
 
   // Key tiles of 128 slots reach LDS by direct-to-LDS loads; each tile is
@@ -214,7 +224,7 @@ __device__ __forceinline__ void prefill_body(const PrefillArgs& a) {
     uint32_t f[4];
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      const int s = slot64(i0 + 4 * u) + lane;
+      const int s = (!WIN || i0 + 4 * u < ntiles ? slot64(i0 + 4 * u) : 0) + lane;
       const uint32_t v = vrow[s < a.S ? s : 0];  // (the guard below still waits for each)
       f[u] = (i0 + 4 * u < ntiles && s < a.S) ? v : 0u;
     }
@@ -304,7 +314,7 @@ __device__ __forceinline__ void prefill_body(const PrefillArgs& a) {
   // that over the wave
   int wlo = 0, wlo_min = 0, wlo_max = 0;
   if constexpr (WIN) {
-    wlo = window_begin(vmask, wr, a.S_past + (tok ? t : a.T - 1), a.window);
+    wlo = window_begin(vmask, list, wr, ntiles, a.S_past + (tok ? t : a.T - 1), a.window);
     wlo_min = __builtin_amdgcn_readfirstlane(wlo);
     wlo_max = __builtin_amdgcn_readlane(wlo, 15);
   }

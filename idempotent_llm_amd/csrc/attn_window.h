@@ -8,7 +8,11 @@
 // s >= lo(t) or s < e: lo(t) the window-th valid slot from t backward (0 if
 // there are fewer), e one past the sinks-th valid slot. A block finds both by
 // counting the row's validity flags, from its query backward and from slot 0
-// forward, 16 flags per thread and step: as many as it is going to scan.
+// forward, 16 flags per thread and step: as many as it is going to scan. The
+// pages it scans are then those of the two ranges that hold a valid slot: a row
+// whose window reaches back over padding does not scan the padding's pages (32
+// rows of 8000 slots, a window of 2048 behind prompts padded by up to 3000
+// slots: 110 -> @@ us).
 #pragma once
 
 #include "common.h"
@@ -73,78 +77,140 @@ __device__ __forceinline__ int block_count_before(int c, int* red, int* total) {
   return before;
 }
 
+// The n-th valid slot is found in steps of 16 NT flags; the first step of both
+// directions is loaded and counted together (one round trip and one count where
+// the window and the sinks lie in it).
+template <int NT>
+struct ValidScan {
+  int* red;    // shared: NT / 64 words
+  int* found;  // shared: 2 words
+
+  // one past the n-th valid slot of [0, end) after `seen` in [0, base): `end` if
+  // there are fewer. All of these are block-uniform.
+  __device__ __forceinline__ int forward(const uint8_t* vrow, int end, int n, int base, int seen) {
+    for (; base < end; base += 16 * NT) {
+      const int s0 = base + 16 * (int)threadIdx.x;
+      const uint32_t m = valid16(vrow, s0, end);
+      int total;
+      const int before = seen + block_count_before<NT>(__popc(m), red, &total);
+      if (seen + total >= n) {
+        if (before < n && before + __popc(m) >= n) found[0] = s0 + nth_bit(m, n - 1 - before) + 1;
+        __syncthreads();
+        return found[0];
+      }
+      seen += total;
+    }
+    return end;
+  }
+  // the n-th valid slot from end - 1 backward after `seen` in [top, end): 0 if
+  // there are fewer
+  __device__ __forceinline__ int backward(const uint8_t* vrow, int end, int n, int top, int seen) {
+    for (; top > 0; top -= 16 * NT) {
+      const int s0 = top - 16 * NT + 16 * (int)threadIdx.x;
+      const uint32_t m = s0 >= 0 ? valid16(vrow, s0, end) : 0u;
+      const int c = __popc(m);
+      int total;
+      const int before = block_count_before<NT>(c, red, &total);
+      const int after = seen + total - before - c;
+      if (seen + total >= n) {
+        if (after < n && after + c >= n) found[1] = s0 + nth_bit(m, c - (n - after));
+        __syncthreads();
+        return found[1];
+      }
+      seen += total;
+    }
+    return 0;
+  }
+};
+
 // One past the n-th valid slot of [0, end) (`end` if there are fewer; 0 for
-// n <= 0). Every thread of the block calls it and gets the result.
+// n <= 0), and the n-th valid slot from end - 1 backward (0 if there are fewer;
+// n >= 1). Every thread of the block calls them and gets the result.
 template <int NT>
 __device__ __forceinline__ int nth_valid_end(const uint8_t* vrow, int end, int n) {
-  __shared__ int red[NT / 64], found;
-  if (n <= 0) return 0;
-  int seen = 0;
-  for (int base = 0; base < end; base += 16 * NT) {
-    const int s0 = base + 16 * (int)threadIdx.x;
-    const uint32_t m = valid16(vrow, s0, end);
-    int total;
-    const int before = seen + block_count_before<NT>(__popc(m), red, &total);
-    if (seen + total >= n) {  // block-uniform
-      if (before < n && before + __popc(m) >= n) found = s0 + nth_bit(m, n - 1 - before) + 1;
-      __syncthreads();
-      return found;
-    }
-    seen += total;
-  }
-  return end;
+  __shared__ int red[NT / 64], found[2];
+  return n <= 0 ? 0 : ValidScan<NT>{red, found}.forward(vrow, end, n, 0, 0);
 }
-
-// The n-th valid slot from end - 1 backward (0 if there are fewer; n >= 1).
 template <int NT>
 __device__ __forceinline__ int nth_valid_back(const uint8_t* vrow, int end, int n) {
-  __shared__ int red[NT / 64], found;
-  int seen = 0;
-  for (int top = (end + 15) & ~15; top > 0; top -= 16 * NT) {
-    // the step's slots [top - 16 NT, top), none below 0
-    const int s0 = top - 16 * NT + 16 * (int)threadIdx.x;
-    const uint32_t m = s0 >= 0 ? valid16(vrow, s0, end) : 0u;
-    const int c = __popc(m);
-    int total;
-    const int before = block_count_before<NT>(c, red, &total);
-    const int after = seen + total - before - c;
-    if (seen + total >= n) {  // block-uniform
-      if (after < n && after + c >= n) found = s0 + nth_bit(m, c - (n - after));
-      __syncthreads();
-      return found;
-    }
-    seen += total;
-  }
-  return 0;
+  __shared__ int red[NT / 64], found[2];
+  return ValidScan<NT>{red, found}.backward(vrow, end, n, (end + 15) & ~15, 0);
 }
 
-// The pages that queries see from the one at slot end1 - 1 on (its window
-// begins lowest), below slot `end`: pages [0, pre) and those from pre + skip.
+// What queries see from the one at slot end1 - 1 on (its window begins lowest),
+// below slot `end`.
 struct WinRange {
   int sink_end;  // e
   int lo;        // lo(end1 - 1)
-  int pre;       // pages before the gap (0 when there is none)
-  int skip;      // pages left out
+  int pre;       // listed pages before the gap between sinks and window (0: no gap)
+  int pages;     // listed pages
 };
+
+// The pages that hold a valid slot of either range, ascending, to list (shared
+// memory, room for all pages below `end`), ready for the whole block.
 template <int NT>
-__device__ __forceinline__ WinRange window_range(const uint8_t* vrow, int end1, int end, int window,
-                                                 int sinks) {
+__device__ __forceinline__ WinRange window_pages(const uint8_t* vrow, int end1, int end, int window,
+                                                 int sinks, uint16_t* list) {
+  __shared__ int red[NT / 64], found[2];
+  ValidScan<NT> scan{red, found};
   WinRange r;
-  r.sink_end = nth_valid_end<NT>(vrow, end, sinks);
-  r.lo = nth_valid_back<NT>(vrow, end1, window);
+  {
+    const int top = (end1 + 15) & ~15;
+    const int f0 = 16 * (int)threadIdx.x, b0 = top - 16 * NT + f0;
+    const uint32_t mf = sinks > 0 ? valid16(vrow, f0, end) : 0u;
+    const uint32_t mb = b0 >= 0 ? valid16(vrow, b0, end1) : 0u;
+    const int cf = __popc(mf), cb = __popc(mb);
+    int total;  // (a step's count is at most 16 NT < 2^16)
+    const int before = block_count_before<NT>(cf | cb << 16, red, &total);
+    const int tf = total & 0xFFFF, tb = total >> 16;
+    const int bf = before & 0xFFFF, after = tb - (before >> 16) - cb;
+    if (sinks > 0 && bf < sinks && bf + cf >= sinks) found[0] = f0 + nth_bit(mf, sinks - 1 - bf) + 1;
+    if (after < window && after + cb >= window) found[1] = b0 + nth_bit(mb, cb - (window - after));
+    __syncthreads();
+    const int fe = found[0], fl = found[1];
+    r.sink_end = sinks <= 0 ? 0 : tf >= sinks ? fe : scan.forward(vrow, end, sinks, 16 * NT, tf);
+    r.lo = tb >= window ? fl : scan.backward(vrow, end1, window, top - 16 * NT, tb);
+  }
   const int np = (r.sink_end + DI_PAGE - 1) / DI_PAGE, pw = r.lo / DI_PAGE;
-  r.pre = pw > np ? np : 0;
-  r.skip = pw > np ? pw - np : 0;
+  const int skip = pw > np ? pw - np : 0, first = pw > np ? np : 0;
+  const int cand = (end + DI_PAGE - 1) / DI_PAGE - skip;  // the ranges' pages
+  int n = 0;
+  r.pre = 0;
+  for (int i0 = 0; i0 < cand; i0 += NT / 8) {  // 8 threads a page
+    const int i = i0 + (int)threadIdx.x / 8;
+    const int page = i < first ? i : i + skip;
+    const uint32_t m = i < cand ? valid16(vrow, page * DI_PAGE + 16 * ((int)threadIdx.x & 7), end) : 0u;
+    const u64 any = __ballot(m != 0);
+    const bool in = ((any >> (threadIdx.x & 56)) & 0xFF) != 0;
+    const bool lead = (threadIdx.x & 7) == 0;
+    int total;
+    const int before = block_count_before<NT>(in && lead ? (i < first ? 0x10001 : 1) : 0, red, &total);
+    if (in && lead) list[n + (before & 0xFFFF)] = (uint16_t)page;
+    n += total & 0xFFFF;
+    r.pre += total >> 16;
+  }
+  r.pages = n;
+  __syncthreads();
   return r;
 }
 
-// lo(t) from the validity masks of the listed 64-slot tiles (window_range's
-// pages in order): the window-th valid slot from t backward.
-__device__ __forceinline__ int window_begin(const u64* vmask, const WinRange& r, int t, int window) {
-  const int first = 2 * r.pre, last = (t >> 6) - 2 * r.skip;
-  int c = __popcll(vmask[last] & (~0ull >> (63 - (t & 63))));
-  for (int it = first; it < last; ++it) c += __popcll(vmask[it]);
-  int k = c - window;  // valid slots of the tiles before the window
+// First slot of the listed 64-slot tile `it`
+__device__ __forceinline__ int listed_slot64(const uint16_t* list, int it) {
+  return (int)list[it >> 1] * DI_PAGE + (it & 1) * 64;
+}
+
+// lo(t) from the validity masks of the listed tiles: the window-th valid slot
+// from t backward.
+__device__ __forceinline__ int window_begin(const u64* vmask, const uint16_t* list,
+                                            const WinRange& r, int ntiles, int t, int window) {
+  const int first = 2 * r.pre;
+  int c = 0;  // valid slots from the window's first page to t
+  for (int it = first; it < ntiles; ++it) {
+    const int d = t - listed_slot64(list, it);
+    if (d < 0) break;
+    c += __popcll(d >= 63 ? vmask[it] : vmask[it] & (~0ull >> (63 - d)));
+  }
+  int k = c - window;  // those before the window
   if (k < 0) return 0;
   int it = first;
   u64 m = vmask[it];
@@ -152,7 +218,7 @@ __device__ __forceinline__ int window_begin(const u64* vmask, const WinRange& r,
     k -= n;
     m = vmask[++it];
   }
-  return (it + 2 * r.skip) * 64 + nth_bit(m, k);
+  return listed_slot64(list, it) + nth_bit(m, k);
 }
 
 }  // namespace
