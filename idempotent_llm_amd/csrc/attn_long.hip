@@ -61,8 +61,8 @@ struct WindowArgs {
 
 // One block per (row, kv head). Scores in LDS; a row whose window spans more
 // slots than that holds keeps them in the scratch.
-template <int G>
-__global__ __launch_bounds__(256) void k_window_decode(WindowArgs w) {
+template <int G, int NW>
+__global__ __launch_bounds__(64 * NW) void k_window_decode(WindowArgs w) {
   keep_hidden_args();
   extern __shared__ __attribute__((aligned(16))) int32_t sh_scores[];
   __shared__ int32_t pg_lds[DEC_MAX_PAGES];
@@ -73,18 +73,20 @@ __global__ __launch_bounds__(256) void k_window_decode(WindowArgs w) {
   bool over;
   const int S = scanned_slots(a, a.tpos, &over);
   const WinView v = win_view(
-      window_pages<256>(a.valid + (i64)b * a.valid_stride, S, S, w.window, w.sinks, list), list, S);
+      window_pages<64 * NW>(a.valid + (i64)b * a.valid_stride, S, S, w.window, w.sinks, list), list, S);
   const int npages = (v.n + DI_PAGE - 1) / DI_PAGE;
-  for (int i = threadIdx.x; i < npages; i += 256) pg_lds[i] = a.kv.page(b, v.slot(i * DI_PAGE));
+  for (int i = threadIdx.x; i < npages; i += 64 * NW) pg_lds[i] = a.kv.page(b, v.slot(i * DI_PAGE));
   if (npages == 0 && threadIdx.x == 0) pg_lds[0] = -1;  // S = 0: loads read page 0
   __syncthreads();
   if (v.n <= w.lds_slots) {
     a.S = v.n;  // (the scores' row stride)
-    decode_body<G, VPRE, false, false, 4, false, WinView>(
-        a, v.n, kvh, b, a.q8 + q0 * 128, a.tpos + q0, sh_scores, pg_lds, KPre<2>{}, OmPre<G, 2>{}, v);
+    decode_body<G, VPRE, false, false, NW, false, WinView>(
+        a, v.n, kvh, b, a.q8 + q0 * 128, a.tpos + q0, sh_scores, pg_lds, KPre<8 / NW>{},
+        OmPre<G, 8 / NW>{}, v);
   } else {
-    decode_body<G, VPRE, true, false, 4, false, WinView>(
-        a, v.n, kvh, b, a.q8 + q0 * 128, a.tpos + q0, sh_scores, pg_lds, KPre<2>{}, OmPre<G, 2>{}, v);
+    decode_body<G, VPRE, true, false, NW, false, WinView>(
+        a, v.n, kvh, b, a.q8 + q0 * 128, a.tpos + q0, sh_scores, pg_lds, KPre<8 / NW>{},
+        OmPre<G, 8 / NW>{}, v);
   }
   report_slots(a, over, kvh == 0);
 }
@@ -129,8 +131,8 @@ __global__ __launch_bounds__(256) void k_window_pv(WindowArgs w) {
   } while (c * w.s.chunk < v.n);
 }
 
-template <int G, bool SCR>
-__global__ __launch_bounds__(256) void k_acc_decode(DecodeArgs a) {
+template <int G, bool SCR, int NW>
+__global__ __launch_bounds__(64 * NW) void k_acc_decode(DecodeArgs a) {
   keep_hidden_args();
   extern __shared__ __attribute__((aligned(16))) int32_t sh_scores[];
   __shared__ int32_t pg_lds[DEC_MAX_PAGES];
@@ -139,10 +141,10 @@ __global__ __launch_bounds__(256) void k_acc_decode(DecodeArgs a) {
   bool over;
   const int S = scanned_slots(a, a.tpos, &over);
   const int npages = (a.S + DI_PAGE - 1) / DI_PAGE;
-  for (int i = threadIdx.x; i < npages; i += 256) pg_lds[i] = a.kv.page(b, (i64)i * DI_PAGE);
+  for (int i = threadIdx.x; i < npages; i += 64 * NW) pg_lds[i] = a.kv.page(b, (i64)i * DI_PAGE);
   if (npages == 0 && threadIdx.x == 0) pg_lds[0] = -1;
   __syncthreads();
-  decode_body<G, VPRE, SCR, false, 4, false, WholeRow, true>(
+  decode_body<G, VPRE, SCR, false, NW, false, WholeRow, true>(
       a, S, kvh, b, a.q8 + q0 * 128, a.tpos + q0, sh_scores, pg_lds);
   report_slots(a, over, kvh == 0);
 }
@@ -317,10 +319,10 @@ int detllm_attn_window_decode(const int8_t* q8, const int64_t* tpos, const int8_
     const dim3 grid(n_kv, B);
     const size_t dyn = (size_t)G * w.lds_slots * 4;
     switch (G) {
-      case 1: hipLaunchKernelGGL(k_window_decode<1>, grid, dim3(256), dyn, s, w); break;
-      case 2: hipLaunchKernelGGL(k_window_decode<2>, grid, dim3(256), dyn, s, w); break;
-      case 4: hipLaunchKernelGGL(k_window_decode<4>, grid, dim3(256), dyn, s, w); break;
-      case 8: hipLaunchKernelGGL(k_window_decode<8>, grid, dim3(256), dyn, s, w); break;
+      case 1: hipLaunchKernelGGL((k_window_decode<1, 8>), grid, dim3(512), dyn, s, w); break;
+      case 2: hipLaunchKernelGGL((k_window_decode<2, 8>), grid, dim3(512), dyn, s, w); break;
+      case 4: hipLaunchKernelGGL((k_window_decode<4, 8>), grid, dim3(512), dyn, s, w); break;
+      case 8: hipLaunchKernelGGL((k_window_decode<8, 8>), grid, dim3(512), dyn, s, w); break;
     }
   }
   DI_LAUNCH_CHECK();
@@ -379,8 +381,8 @@ int detllm_attn_decode_acc(const int8_t* q8, const int64_t* tpos, const int8_t* 
     switch (G) {
 #define DI_ACC_ONE(G_)                                                                        \
   case G_:                                                                                    \
-    if (d.scratch) hipLaunchKernelGGL((k_acc_decode<G_, true>), grid, dim3(256), dyn, s, d);  \
-    else hipLaunchKernelGGL((k_acc_decode<G_, false>), grid, dim3(256), dyn, s, d);           \
+    if (d.scratch) hipLaunchKernelGGL((k_acc_decode<G_, true, 8>), grid, dim3(512), dyn, s, d);  \
+    else hipLaunchKernelGGL((k_acc_decode<G_, false, 8>), grid, dim3(512), dyn, s, d);           \
     break
       DI_ACC_ONE(1);
       DI_ACC_ONE(2);
