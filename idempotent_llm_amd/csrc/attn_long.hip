@@ -32,6 +32,8 @@ __global__ __launch_bounds__(256, 2) void k_acc_prefill(PrefillArgs a) {
   prefill_body<false, true>(a);
 }
 
+__host__ __device__ constexpr int pages_of(int S) { return (S + DI_PAGE - 1) / DI_PAGE; }
+
 // The listed pages of a row's newest query (window_pages), numbered 0, 1, ...
 struct WinView {
   static constexpr bool kWhole = false;
@@ -72,10 +74,14 @@ __global__ __launch_bounds__(64 * NW) void k_window_decode(WindowArgs w) {
   const i64 q0 = (i64)b * a.n_q + kvh * G;
   bool over;
   const int S = scanned_slots(a, a.tpos, &over);
+  // the row's page ids load beside the flags
+  __shared__ int32_t row_pages[DEC_MAX_PAGES];
+  for (int i = threadIdx.x; i < pages_of(a.S); i += 64 * NW)
+    row_pages[i] = a.kv.page(b, (i64)i * DI_PAGE);
   const WinView v = win_view(
       window_pages<64 * NW>(a.valid + (i64)b * a.valid_stride, S, S, w.window, w.sinks, list), list, S);
-  const int npages = (v.n + DI_PAGE - 1) / DI_PAGE;
-  for (int i = threadIdx.x; i < npages; i += 64 * NW) pg_lds[i] = a.kv.page(b, v.slot(i * DI_PAGE));
+  const int npages = pages_of(v.n);
+  for (int i = threadIdx.x; i < npages; i += 64 * NW) pg_lds[i] = row_pages[list[i]];
   if (npages == 0 && threadIdx.x == 0) pg_lds[0] = -1;  // S = 0: loads read page 0
   __syncthreads();
   if (v.n <= w.lds_slots) {
@@ -179,7 +185,6 @@ i64 split_bytes(int B, int S, int n_q, int chunk, i64* cmax_at) {
   *cmax_at = rows * ns * chunk * 4;
   return *cmax_at + (rows * ns * 4 + 15) / 16 * 16;
 }
-int pages_of(int S) { return (S + DI_PAGE - 1) / DI_PAGE; }
 i64 one_block_bytes(int B, int S, int n_q, int G) {
   const i64 spad = ((i64)S + 15) / 16 * 16;
   return (i64)G * spad * 4 > DECODE_LDS_BYTES ? (i64)B * n_q * spad * 4 : 0;

@@ -58,12 +58,13 @@ __device__ __forceinline__ int nth_bit(u64 m, int k) {
 template <int NT>
 __device__ __forceinline__ int block_count_before(int c, int* red, int* total) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int incl = c;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int o = __shfl_up(incl, d, 64);
-    if (lane >= d) incl += o;
-  }
+  int incl = c;  // inclusive over the wave: DPP shifts within rows of 16, then row ends
+  incl += __builtin_amdgcn_update_dpp(0, incl, 0x111, 0xF, 0xF, false);
+  incl += __builtin_amdgcn_update_dpp(0, incl, 0x112, 0xF, 0xF, false);
+  incl += __builtin_amdgcn_update_dpp(0, incl, 0x114, 0xF, 0xF, false);
+  incl += __builtin_amdgcn_update_dpp(0, incl, 0x118, 0xF, 0xF, false);
+  incl += __builtin_amdgcn_update_dpp(0, incl, 0x142, 0xA, 0xF, false);
+  incl += __builtin_amdgcn_update_dpp(0, incl, 0x143, 0xC, 0xF, false);
   __syncthreads();  // (the words may still be read from the last call)
   if (lane == 63) red[wave] = incl;
   __syncthreads();
@@ -142,54 +143,69 @@ __device__ __forceinline__ int nth_valid_back(const uint8_t* vrow, int end, int 
 struct WinRange {
   int sink_end;  // e
   int lo;        // lo(end1 - 1)
-  int pre;       // listed pages before the gap between sinks and window (0: no gap)
+  int pre;       // listed pages before the window's first page
   int pages;     // listed pages
 };
 
 // The pages that hold a valid slot of either range, ascending, to list (shared
-// memory, room for all pages below `end`), ready for the whole block.
+// memory, room for all pages below `end`), ready for the whole block. Sinks and
+// window that lie in the first step (NT / 8 pages from either end) are listed
+// from that step's flags; else the ranges' flags are read again.
 template <int NT>
 __device__ __forceinline__ WinRange window_pages(const uint8_t* vrow, int end1, int end, int window,
                                                  int sinks, uint16_t* list) {
   __shared__ int red[NT / 64], found[2];
   ValidScan<NT> scan{red, found};
   WinRange r;
-  {
-    const int top = (end1 + 15) & ~15;
-    const int f0 = 16 * (int)threadIdx.x, b0 = top - 16 * NT + f0;
-    const uint32_t mf = sinks > 0 ? valid16(vrow, f0, end) : 0u;
-    const uint32_t mb = b0 >= 0 ? valid16(vrow, b0, end1) : 0u;
-    const int cf = __popc(mf), cb = __popc(mb);
-    int total;  // (a step's count is at most 16 NT < 2^16)
-    const int before = block_count_before<NT>(cf | cb << 16, red, &total);
-    const int tf = total & 0xFFFF, tb = total >> 16;
-    const int bf = before & 0xFFFF, after = tb - (before >> 16) - cb;
-    if (sinks > 0 && bf < sinks && bf + cf >= sinks) found[0] = f0 + nth_bit(mf, sinks - 1 - bf) + 1;
-    if (after < window && after + cb >= window) found[1] = b0 + nth_bit(mb, cb - (window - after));
-    __syncthreads();
-    const int fe = found[0], fl = found[1];
-    r.sink_end = sinks <= 0 ? 0 : tf >= sinks ? fe : scan.forward(vrow, end, sinks, 16 * NT, tf);
-    r.lo = tb >= window ? fl : scan.backward(vrow, end1, window, top - 16 * NT, tb);
+  // forward from slot 0, and backward from the end of the last query's page
+  const int top = (end + DI_PAGE - 1) / DI_PAGE * DI_PAGE;
+  const int f0 = 16 * (int)threadIdx.x, b0 = top - 16 * NT + f0;
+  const uint32_t mf = sinks > 0 ? valid16(vrow, f0, end) : 0u;
+  const uint32_t mb = b0 >= 0 ? valid16(vrow, b0, end) : 0u;
+  // (the window counts from the first query on)
+  const int cut = end1 - b0;
+  const uint32_t m1 = cut >= 16 ? mb : cut <= 0 ? 0u : mb & ((1u << cut) - 1);
+  const int cf = __popc(mf), cb = __popc(m1);
+  int total;  // (a step's count is at most 16 NT < 2^16)
+  int before = block_count_before<NT>(cf | cb << 16, red, &total);
+  const int tf = total & 0xFFFF, tb = total >> 16;
+  const int bf = before & 0xFFFF, after = tb - (before >> 16) - cb;
+  if (sinks > 0 && bf < sinks && bf + cf >= sinks) found[0] = f0 + nth_bit(mf, sinks - 1 - bf) + 1;
+  if (after < window && after + cb >= window) found[1] = b0 + nth_bit(m1, cb - (window - after));
+  __syncthreads();
+  const int fe = found[0], fl = found[1];
+  const bool once = (sinks <= 0 || tf >= sinks || end <= 16 * NT) && (tb >= window || top <= 16 * NT);
+  r.sink_end = sinks <= 0 ? 0 : tf >= sinks ? fe : scan.forward(vrow, end, sinks, 16 * NT, tf);
+  r.lo = tb >= window ? fl : scan.backward(vrow, end1, window, top - 16 * NT, tb);
+  // the sinks' pages below the window's first page, then those from there on
+  const int pw = r.lo / DI_PAGE, np = ::min((r.sink_end + DI_PAGE - 1) / DI_PAGE, pw);
+  const int sh = threadIdx.x & 56;  // 8 threads a page
+  const bool lead = (threadIdx.x & 7) == 0;
+  if (once) {
+    const int pf = f0 / DI_PAGE, pb = b0 / DI_PAGE;
+    const bool inf = ((__ballot(mf != 0) >> sh) & 0xFF) != 0 && lead && pf < np;
+    const bool inb = ((__ballot(mb != 0) >> sh) & 0xFF) != 0 && lead && b0 >= 0 && pb >= pw;
+    before = block_count_before<NT>((inf ? 1 : 0) | (inb ? 0x10000 : 0), red, &total);
+    r.pre = total & 0xFFFF;
+    r.pages = r.pre + (total >> 16);
+    if (inf) list[before & 0xFFFF] = (uint16_t)pf;
+    if (inb) list[r.pre + (before >> 16)] = (uint16_t)pb;
+  } else {
+    const int cand = np + top / DI_PAGE - pw;
+    int n = 0;
+    r.pre = 0;
+    for (int i0 = 0; i0 < cand; i0 += NT / 8) {
+      const int i = i0 + (int)threadIdx.x / 8;
+      const int page = i < np ? i : i - np + pw;
+      const uint32_t m = i < cand ? valid16(vrow, page * DI_PAGE + 16 * ((int)threadIdx.x & 7), end) : 0u;
+      const bool in = ((__ballot(m != 0) >> sh) & 0xFF) != 0 && lead;
+      before = block_count_before<NT>(in ? (i < np ? 0x10001 : 1) : 0, red, &total);
+      if (in) list[n + (before & 0xFFFF)] = (uint16_t)page;
+      n += total & 0xFFFF;
+      r.pre += total >> 16;
+    }
+    r.pages = n;
   }
-  const int np = (r.sink_end + DI_PAGE - 1) / DI_PAGE, pw = r.lo / DI_PAGE;
-  const int skip = pw > np ? pw - np : 0, first = pw > np ? np : 0;
-  const int cand = (end + DI_PAGE - 1) / DI_PAGE - skip;  // the ranges' pages
-  int n = 0;
-  r.pre = 0;
-  for (int i0 = 0; i0 < cand; i0 += NT / 8) {  // 8 threads a page
-    const int i = i0 + (int)threadIdx.x / 8;
-    const int page = i < first ? i : i + skip;
-    const uint32_t m = i < cand ? valid16(vrow, page * DI_PAGE + 16 * ((int)threadIdx.x & 7), end) : 0u;
-    const u64 any = __ballot(m != 0);
-    const bool in = ((any >> (threadIdx.x & 56)) & 0xFF) != 0;
-    const bool lead = (threadIdx.x & 7) == 0;
-    int total;
-    const int before = block_count_before<NT>(in && lead ? (i < first ? 0x10001 : 1) : 0, red, &total);
-    if (in && lead) list[n + (before & 0xFFFF)] = (uint16_t)page;
-    n += total & 0xFFFF;
-    r.pre += total >> 16;
-  }
-  r.pages = n;
   __syncthreads();
   return r;
 }
