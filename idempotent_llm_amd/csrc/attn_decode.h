@@ -60,6 +60,7 @@ __device__ __forceinline__ int32_t row16_max(int32_t v) {
 struct WholeRow {
   static constexpr bool kWhole = true;
   __device__ __forceinline__ int slot(int s) const { return s; }
+  __device__ __forceinline__ int page(const KVPages& kv, int b, int s) const { return kv.page(b, s); }
   __device__ __forceinline__ bool sees(int) const { return true; }
 };
 
@@ -609,7 +610,7 @@ __device__ __forceinline__ void split_scores_chunk(const SplitArgs& sa, int kvh,
   int bound = a.S;
   if constexpr (!View::kWhole) bound = view.n;
   const int npg = (::min(sa.chunk, bound - lo) + DI_PAGE - 1) / DI_PAGE;
-  const int pgv = tid < npg ? a.kv.page(b, view.slot(lo + tid * DI_PAGE)) : -1;
+  const int pgv = tid < npg ? view.page(a.kv, b, lo + tid * DI_PAGE) : -1;
   v4i qa0 = v4i{0, 0, 0, 0}, qa1 = v4i{0, 0, 0, 0};
   if (l16 < G) {
     const int8_t* qsrc = a.q8 + q0 * 128;
@@ -698,7 +699,7 @@ __device__ __forceinline__ void split_pv_chunk(const SplitArgs& sa, int kvh, int
   int bound = a.S;
   if constexpr (!View::kWhole) bound = view.n;
   const int npg = (::min(sa.chunk, bound - lo) + DI_PAGE - 1) / DI_PAGE;
-  const int pgv = tid < npg ? a.kv.page(b, view.slot(lo + tid * DI_PAGE)) : -1;
+  const int pgv = tid < npg ? view.page(a.kv, b, lo + tid * DI_PAGE) : -1;
   i64 tph[G], hmax[G];
 #pragma unroll
   for (int hh = 0; hh < G; ++hh) {

@@ -17,9 +17,8 @@
 // (row, kv head, slots) and adds without atomics; prefill tiles share slots
 // and add with 64-bit atomics.
 
-#include "attn_decode.h"
+#include "attn_plan.h"
 #include "attn_prefill.h"
-#include "../../include/detllm_hip.h"
 
 namespace {
 
@@ -42,6 +41,9 @@ struct WinView {
   int sink_end, lo;
   __device__ __forceinline__ int slot(int s) const {
     return (int)list[s >> 7] * DI_PAGE + (s & (DI_PAGE - 1));
+  }
+  __device__ __forceinline__ int page(const KVPages& kv, int b, int s) const {
+    return kv.page(b, slot(s));
   }
   __device__ __forceinline__ bool sees(int s) const { return s < sink_end || s >= lo; }
 };
@@ -166,54 +168,11 @@ __global__ __launch_bounds__(256) void k_acc_pv(SplitArgs sa) {
   split_pv_chunk<G, WholeRow, true>(sa, blockIdx.x, blockIdx.y, blockIdx.z);
 }
 
-// How a decode over about n slots per row runs: chunk slots per block (a
-// multiple of the page; 0: one block per (row, kv head)).
-int decode_chunk(int B, int n, int n_q, int n_kv) {
-  const int G = n_q / n_kv;
-  const i64 pairs = (i64)B * n_kv;
-  const int from = pairs > 128 ? INT32_MAX : G > 4 ? 1537 : G > 2 ? (pairs <= 64 ? 896 : 1536) : pairs <= 64 ? 768 : 1152;
-  if (n < from) return 0;
-  int chunk = 0, ns = 0;
-  if (detllm_attn_split_plan(B, n, n_q, n_kv, &chunk, &ns) != 0 || ns <= 1) return 0;
-  return chunk;
-}
-
-// Bytes of the split form's scores and chunk maxima: [B][n_q][ns * chunk] and
-// [B][n_q][ns] int32 with ns = ceil(S / chunk), 16-byte sizes.
-i64 split_bytes(int B, int S, int n_q, int chunk, i64* cmax_at) {
-  const i64 ns = ((i64)S + chunk - 1) / chunk, rows = (i64)B * n_q;
-  *cmax_at = rows * ns * chunk * 4;
-  return *cmax_at + (rows * ns * 4 + 15) / 16 * 16;
-}
-i64 one_block_bytes(int B, int S, int n_q, int G) {
-  const i64 spad = ((i64)S + 15) / 16 * 16;
-  return (i64)G * spad * 4 > DECODE_LDS_BYTES ? (i64)B * n_q * spad * 4 : 0;
-}
-int heads_ok(int n_q, int n_kv) {
-  if (n_q <= 0 || n_kv <= 0 || n_q % n_kv) return DI_EINVAL;
-  const int G = n_q / n_kv;
-  return G == 1 || G == 2 || G == 4 || G == 8 ? DI_OK : DI_ENOSYS;
-}
 // Slots that a launch is sized for: what a query sees, and the rest of the
 // pages at the ends of the two ranges and around two stretches of padding.
 int window_slots(int S, int window, int sinks) {
   return (int)imin(S, (i64)window + sinks + 6 * DI_PAGE);
 }
-SplitArgs split_args(const DecodeArgs& d, int B, int chunk, void* work) {
-  SplitArgs sa{};
-  sa.d = d;
-  i64 cmax_at = 0;
-  split_bytes(B, d.S, d.n_q, chunk, &cmax_at);
-  sa.d.scratch = (int32_t*)work;
-  sa.cmax = (int32_t*)((char*)work + cmax_at);
-  sa.chunk = chunk;
-  sa.ns = (d.S + chunk - 1) / chunk;
-  sa.spad = (i64)sa.ns * chunk;
-  sa.out_stride = (i64)B * d.n_q * 128;
-  sa.add = 1;
-  return sa;
-}
-
 }  // namespace
 
 extern "C" {

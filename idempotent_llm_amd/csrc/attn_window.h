@@ -21,21 +21,28 @@ using namespace di;
 
 namespace {
 
+// The nonzero bytes of 16 flags, as bits.
+__device__ __forceinline__ uint32_t flag_bits(const uint32_t (&x)[4]) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t u = ((((x[i] & 0x7f7f7f7fu) + 0x7f7f7f7fu) | x[i]) & 0x80808080u) >> 7;
+    m |= ((u | u >> 7 | u >> 14 | u >> 21) & 0xFu) << (4 * i);
+  }
+  return m;
+}
+
 // The nonzero flags of slots s0 .. s0 + 15 below `end`, as bits.
 __device__ __forceinline__ uint32_t valid16(const uint8_t* vrow, int s0, int end) {
   if (s0 >= end) return 0;
-  uint32_t m = 0;
-  if (s0 + 16 <= end) {
+  if (end >= 16) {  // (16 flags that end at `end` where the group would pass it)
+    const int s1 = ::min(s0, end - 16);
     uint32_t x[4];
-    __builtin_memcpy(x, vrow + s0, 16);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t u = ((((x[i] & 0x7f7f7f7fu) + 0x7f7f7f7fu) | x[i]) & 0x80808080u) >> 7;
-      m |= ((u | u >> 7 | u >> 14 | u >> 21) & 0xFu) << (4 * i);
-    }
-  } else {
-    for (int i = 0; i < end - s0; ++i) m |= (vrow[s0 + i] != 0 ? 1u : 0u) << i;
+    __builtin_memcpy(x, vrow + s1, 16);
+    return flag_bits(x) >> (s0 - s1);
   }
+  uint32_t m = 0;
+  for (int i = 0; i < end - s0; ++i) m |= (vrow[s0 + i] != 0 ? 1u : 0u) << i;
   return m;
 }
 

@@ -367,6 +367,18 @@ SHARED = {
     "odd_rows": (9, 4, 2, 640, 65, dict(p_valid=0.9)),
     "two_blocks": (70, 4, 2, 384, 10, {}),
     "long": (5, 4, 2, 2048, 130, dict(p_valid=0.95)),
+    "one_group": (8, 2, 1, 1280, 40, dict(p_valid=0.9)),
+    "two_groups": (13, 4, 2, 896, 70, dict(p_valid=0.9)),
+    "one_group_8": (2, 16, 2, 8320, 200, dict(p_valid=0.9)),
+    "four_groups_1": (50, 2, 2, 384, 1, dict(p_valid=0.9)),
+    "no_suffix_joint": (40, 4, 2, 256, 0, dict(p_valid=0.9)),
+    "long_suffix": (10, 4, 2, 1024, 1000, dict(p_valid=0.9)),
+    "many_chunks": (5, 8, 1, 20000 // 128 * 128, 3, dict(p_valid=0.9)),
+    "dead_joint": (40, 4, 2, 256, 20, dict(gaps=((0, 0, 276), (39, 0, 256), (1, 250, 276)))),
+    "wide_tpos_joint": (33, 4, 2, 384, 40, dict(tpos=(0, 62), p_valid=0.8)),
+    "mixed_tpos_joint": (33, 4, 2, 384, 40, dict(tpos=(30, 48), p_valid=0.8)),
+    "flat_joint": (5, 4, 2, 2560, 20, dict(flat_heads=(0, 1), tpos=(38, 39))),
+    "extreme_joint": (33, 2, 2, 384, 70, dict(extreme=(0,), tpos=(28, 40))),
     "dead_prefix": (3, 4, 2, 256, 50, dict(gaps=((1, 0, 256),))),
     "dead_row": (3, 4, 2, 256, 50, dict(dead_rows=(1,))),
     "wide_tpos": (3, 4, 2, 256, 100, dict(tpos=(0, 62), p_valid=0.8)),
