@@ -9,9 +9,8 @@
 
 namespace {
 
-// ---- the weights of a row's valid slots, over all kv heads: w [B][S]
-__global__ __launch_bounds__(256) void k_kv_weight(const int64_t* acc, i64 acc_stride,
-                                                   const uint8_t* valid, i64 valid_stride, int S,
+// ---- the weights of a row's slots over all kv heads: w [B][S]
+__global__ __launch_bounds__(256) void k_kv_weight(const int64_t* acc, i64 acc_stride, int S,
                                                    int n_kv, int64_t* w) {
   keep_hidden_args();
   const int s = blockIdx.x * 256 + threadIdx.x, b = blockIdx.y;
@@ -22,101 +21,220 @@ __global__ __launch_bounds__(256) void k_kv_weight(const int64_t* acc, i64 acc_s
   w[(i64)b * S + s] = sum;
 }
 
-// ---- the slots that stay, a block per row. Of the valid slots the first
-// `sinks` and the last `recent` stay; between them, the `need` heaviest: their
-// least weight comes from a radix selection over the weights' 8 bytes (as
-// unsigned keys, the largest first), then one pass in slot order takes every
-// slot above it and the first ones that equal it.
+// ---- the slots that stay, a block per row. A thread owns `per` consecutive
+// slots, so one scan of the valid counts gives every slot its rank among the
+// valid ones (the first `sinks` and the last `recent` stay by rank) and one scan
+// of the kept counts its place. Between them the `need` heaviest stay. Their
+// least weight is found by digits of 8 bits from the highest bit in which the
+// weights differ (keys: the weight as unsigned, larger first), until the digit
+// that holds the need-th largest has few slots left; these are ranked one
+// against the other, by key and then by slot.
+// E > 0: a thread's keys stay in registers, summed here over the kv heads (rows
+// of at most 1024 E slots); E = 0: k_kv_weight has summed them to w.
 constexpr int SEL_NT = 1024;
+constexpr int SEL_RANK = SEL_NT / 8;  // slots ranked one against the other, 8 threads each
 
-__device__ __forceinline__ u64 weight_key(i64 w) { return (u64)w ^ (1ull << 63); }
+struct SelectArgs {
+  const int64_t* acc;
+  i64 acc_stride;
+  const uint8_t* valid;
+  i64 valid_stride;
+  const int64_t* w;
+  int S, n_kv, budget, recent, sinks;
+  int32_t* keep;
+  int64_t* kept;
+};
 
-__global__ __launch_bounds__(SEL_NT) void k_kv_select(const int64_t* acc, i64 acc_stride,
-                                                      const uint8_t* valid, i64 valid_stride,
-                                                      const int64_t* w, int S, int n_kv, int budget,
-                                                      int recent, int sinks, int32_t* keep,
-                                                      int64_t* kept) {
+template <int E>
+__global__ __launch_bounds__(SEL_NT) void k_kv_select(SelectArgs a) {
   keep_hidden_args();
-  __shared__ int hist[256], red[SEL_NT / 64], pick[2];
+  __shared__ int hist[256], red[SEL_NT / 64], pick[3], nlist;
+  __shared__ u64 diff, keys[SEL_RANK];
+  __shared__ int slots[SEL_RANK];
   const int b = blockIdx.x, tid = threadIdx.x;
-  const uint8_t* vrow = valid + (i64)b * valid_stride;
-  const int64_t* wrow = w + (i64)b * S;
-  int32_t* krow = keep + (i64)b * budget;
-  int count = 0;
-  for (int s0 = 16 * tid; s0 < S; s0 += 16 * SEL_NT) count += __popc(valid16(vrow, s0, S));
-  int n;
-  block_count_before<SEL_NT>(count, red, &n);
-  // valid slots in [lo, hi) compete for `need` places
-  int lo = S, hi = S, need = 0;
-  if (n > budget) {
-    lo = nth_valid_end<SEL_NT>(vrow, S, sinks);
-    hi = recent > 0 ? nth_valid_back<SEL_NT>(vrow, S, recent) : S;
-    need = budget - sinks - recent;
+  const uint8_t* vrow = a.valid + (i64)b * a.valid_stride;
+  int32_t* krow = a.keep + (i64)b * a.budget;
+  const int per = E > 0 ? E : (a.S + SEL_NT - 1) / SEL_NT;
+  const int s0 = tid * per;
+  auto key_of = [](i64 w) { return (u64)w ^ (1ull << 63); };
+  u64 reg[E > 0 ? E : 1];
+  if constexpr (E > 0) {
+    i64 sum[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) sum[e] = 0;
+    for (int h = 0; h < a.n_kv; ++h) {
+      const int64_t* row = a.acc + ((i64)b * a.n_kv + h) * a.acc_stride;
+#pragma unroll
+      for (int e = 0; e < E; ++e) sum[e] = wadd(sum[e], s0 + e < a.S ? row[s0 + e] : 0);
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) reg[e] = key_of(sum[e]);
   }
-  u64 least = 0;  // the need-th largest key
-  int ties = 0;   // places left for slots of that key
+  // each(f): f(slot, key, valid) of the thread's slots below S, in order
+  uint32_t vbits = 0;
+  if constexpr (E > 0) {
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      vbits |= (s0 + e < a.S && vrow[s0 + e < a.S ? s0 + e : 0] != 0 ? 1u : 0u) << e;
+  }
+  auto each = [&](auto&& f) {
+    if constexpr (E > 0) {
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        if ((vbits >> e) & 1u) f(s0 + e, reg[e]);
+    } else {
+      for (int e = 0; e < per; ++e)
+        if (s0 + e < a.S && vrow[s0 + e] != 0) f(s0 + e, key_of(a.w[(i64)b * a.S + s0 + e]));
+    }
+  };
+  int mine = 0, n;
+  each([&](int, u64) { ++mine; });
+  if (tid == 0) {
+    diff = 0;
+    nlist = 0;
+  }
+  const int rank0 = block_count_before<SEL_NT>(mine, red, &n);
+  // the valid slots of rank [lo, hi) compete for `need` places
+  const bool all = n <= a.budget;
+  const int lo = a.sinks, hi = n - a.recent, need = all ? 0 : a.budget - a.sinks - a.recent;
+  // each competing slot of this thread
+  auto compete = [&](auto&& f) {
+    int r = rank0;
+    each([&](int s, u64 k) {
+      if (r >= lo && r < hi) f(s, k);
+      ++r;
+    });
+  };
+  u64 least = 0;     // the digits found so far of the need-th largest key
+  u64 known = 0;     // their mask
+  int left = need;   // places for keys whose known digits are `least`
+  bool ranked = false;
   if (need > 0) {
-    u64 known = 0;
-    int left = need;
-    for (int sh = 56; sh >= 0; sh -= 8) {
-      const u64 mask = sh == 56 ? 0ull : ~0ull << (sh + 8);
+    // the bits in which the competing keys differ from the first of them
+    u64 base = 0, d = 0;
+    bool any = false;
+    compete([&](int, u64 k) {
+      if (!any) base = k;
+      any = true;
+      d |= k ^ base;
+    });
+    if (any && atomicAdd(&nlist, 1) == 0) keys[0] = base;
+    __syncthreads();
+    d |= any ? base ^ keys[0] : 0;
+    if (d) atomicOr((unsigned long long*)&diff, d);
+    __syncthreads();
+    const u64 all_diff = diff, first = keys[0];
+    int top = 64 - clz64(all_diff);  // bits [0, top) differ (0: all keys are equal)
+    known = top == 64 ? 0 : ~0ull << top;
+    least = first & known;
+    int count = hi - lo;  // keys whose known digits are `least`
+    while (top > 0 && left < count) {
+      if (count <= SEL_RANK) {  // block-uniform
+        ranked = true;
+        break;
+      }
+      const int sh = top > 8 ? top - 8 : 0;
+      const u64 digits = (1ull << (top - sh)) - 1;
       if (tid < 256) hist[tid] = 0;
       __syncthreads();
-      for (int s = lo + tid; s < hi; s += SEL_NT)
-        if (vrow[s] != 0) {
-          const u64 k = weight_key(wrow[s]);
-          if ((k & mask) == known) atomicAdd(&hist[(k >> sh) & 255], 1);
-        }
+      compete([&](int, u64 k) {
+        if ((k & known) == least) atomicAdd(&hist[(k >> sh) & digits], 1);
+      });
       __syncthreads();
-      // the digit that holds the left-th largest: keys above digit d number
-      // fewer than left, with d's at least left
-      const int d = 255 - tid;
-      const int c = tid < 256 ? hist[d] : 0;
+      // the digit that holds the left-th largest: keys of the digits above
+      // number fewer than left, with its own at least left
+      const int dg = 255 - tid, c = tid < 256 ? hist[dg] : 0;
       int total;
       const int above = block_count_before<SEL_NT>(c, red, &total);
       if (tid < 256 && above < left && above + c >= left) {
-        pick[0] = d;
+        pick[0] = dg;
         pick[1] = left - above;
+        pick[2] = c;
       }
       __syncthreads();
-      known |= (u64)pick[0] << sh;
+      least |= (u64)pick[0] << sh;
+      known |= digits << sh;
       left = pick[1];
+      count = pick[2];
+      top = sh;
     }
-    least = known;
-    ties = left;
-  }
-  // the kept slots in order
-  int at = 0, tied = 0;
-  for (int base = 0; base < S; base += SEL_NT) {
-    const int s = base + tid;
-    const bool v = s < S && vrow[s < S ? s : 0] != 0;
-    bool in = v && (n <= budget || s < lo || s >= hi);
-    bool tie = false;
-    if (v && !in && need > 0) {
-      const u64 k = weight_key(wrow[s]);
-      in = k > least;
-      tie = k == least;
+    if (ranked) {
+      // the key of the left-th largest, and the slots at or before which equal
+      // keys stay: every listed slot counts those ahead of it
+      __syncthreads();
+      if (tid == 0) nlist = 0;
+      __syncthreads();
+      compete([&](int s, u64 k) {
+        if ((k & known) == least) {
+          const int i = atomicAdd(&nlist, 1);
+          keys[i] = k;
+          slots[i] = s;
+        }
+      });
+      __syncthreads();
+      const int c = nlist, at = tid >> 3;
+      const u64 k = keys[at < c ? at : 0];
+      const int s = slots[at < c ? at : 0];
+      int ahead = 0;
+#pragma unroll 4
+      for (int i = tid & 7; i < c; i += 8)
+        ahead += keys[i] > k || (keys[i] == k && slots[i] < s) ? 1 : 0;
+      ahead = sum8_i32(ahead);
+      if (at < c && (tid & 7) == 0 && ahead == left - 1) {
+        diff = k;
+        pick[0] = s;
+      }
+      __syncthreads();
+      least = diff;
+      known = ~0ull;
     }
-    int total;
-    const int before = block_count_before<SEL_NT>(tie ? 1 : 0, red, &total);
-    in = in || (tie && tied + before < ties);
-    tied += total;
-    const int place = at + block_count_before<SEL_NT>(in ? 1 : 0, red, &total);
-    if (in) krow[place] = s;
-    at += total;
   }
-  for (int i = at + tid; i < budget; i += SEL_NT) krow[i] = -1;
+  // A competing slot stays if its known digits are above `least`, or equal it
+  // and: all of those stay (left covers them), or it lies at or before the last
+  // one that does (ranked), or its place among them is below left.
+  const int upto = ranked ? pick[0] : 0;
+  int tied = 0;
+  if (need > 0 && !ranked) {
+    int c = 0, total;
+    compete([&](int, u64 k) { c += (k & known) == least ? 1 : 0; });
+    tied = block_count_before<SEL_NT>(c, red, &total);
+  }
+  auto kept_each = [&](auto&& f) {
+    int r = rank0, t = tied;
+    each([&](int s, u64 k) {
+      bool in = all || r < lo || r >= hi;
+      if (!in && need > 0) {
+        const u64 kk = k & known;
+        in = kk > least;
+        if (kk == least) {
+          in = ranked ? s <= upto : t < left;
+          ++t;
+        }
+      }
+      ++r;
+      if (in) f(s);
+    });
+  };
+  int c = 0, total;
+  kept_each([&](int) { ++c; });
+  int place = block_count_before<SEL_NT>(c, red, &total);
+  kept_each([&](int s) { krow[place++] = s; });
+  for (int i = total + tid; i < a.budget; i += SEL_NT) krow[i] = -1;
   __syncthreads();
-  for (i64 i = tid; i < (i64)n_kv * budget; i += SEL_NT) {
-    const int h = (int)(i / budget), p = (int)(i % budget);
-    kept[((i64)b * n_kv + h) * budget + p] =
-        p < at ? acc[((i64)b * n_kv + h) * acc_stride + krow[p]] : 0;
+  for (int p = tid; p < a.budget; p += SEL_NT) {
+    const int s = p < total ? krow[p] : 0;
+    const int64_t* from = a.acc + (i64)b * a.n_kv * a.acc_stride + s;
+    int64_t* to = a.kept + (i64)b * a.n_kv * a.budget + p;
+#pragma unroll 8
+    for (int h = 0; h < a.n_kv; ++h)
+      to[(i64)h * a.budget] = p < total ? from[(i64)h * a.acc_stride] : 0;
   }
 }
 
 // ---- the kept slots' K and V moved to the pages of dst, in slot order
 constexpr int KVC_LAYERS = 32;  // layers per launch (pool pointers by value)
 constexpr int KVC_PAGES = 4;    // source pages of V in LDS at once
+constexpr int KVC_MAXP = 1024;  // pages of V listed at once
 
 struct CompactArgs {
   int8_t* k[KVC_LAYERS];
@@ -127,88 +245,158 @@ struct CompactArgs {
   int width, dst_width, budget, n_kv;
 };
 
-// Block = (kv head and K or V, row, layer), page after page of dst: slot i
-// comes from slot keep[i] >= i, so a page of dst may be the table's page of the
-// same place or an earlier one (everything it held has been read by then), and
-// the reads of a page end before its writes begin.
-__global__ __launch_bounds__(256) void k_kv_compact(CompactArgs a) {
-  keep_hidden_args();
-  __shared__ __attribute__((aligned(16))) int8_t src[KVC_PAGES][128 * DI_PAGE];
-  __shared__ int32_t slot[DI_PAGE];  // the page's source slots
-  const int h = blockIdx.x >> 1, b = blockIdx.y, tid = threadIdx.x;
-  const bool is_v = blockIdx.x & 1;
-  const KVPages kv{a.k[blockIdx.z], a.v[blockIdx.z], a.table, a.width, a.n_kv};
+// K: page after page of dst, 8 lanes a row of 128 bytes. Slot i comes from slot
+// keep[i] >= i, so a page of dst may be the table's page of the same place or an
+// earlier one: everything it held for later pages has been read, because the
+// reads of a page end before its writes begin (the barrier) and those of the
+// page after it come from places behind it.
+__device__ __forceinline__ void compact_k(const CompactArgs& a, const KVPages& kv, int h, int b) {
+  const int tid = threadIdx.x, npages = (a.budget + DI_PAGE - 1) / DI_PAGE;
   const int32_t* krow = a.keep + (i64)b * a.budget;
-  const int npages = min(a.dst_width, (a.budget + DI_PAGE - 1) / DI_PAGE);
-  for (int j = 0; j < npages; ++j) {
-    const int to = a.dst[(i64)b * a.dst_width + j];
-    __syncthreads();  // (the last page's reads of slot)
-    if (tid < DI_PAGE) {
-      const int i = j * DI_PAGE + tid;
-      slot[tid] = i < a.budget ? krow[i] : -1;
-    }
-    __syncthreads();
-    if (to < 0) continue;  // block-uniform
-    if (!is_v) {
-      v4i x[4];
+  const int32_t* drow = a.dst + (i64)b * a.dst_width;
+  int s[4];  // the next page's source slots of this thread's rows
+  auto load_slots = [&](int j) {
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const int s = slot[u * 32 + (tid >> 3)];
-        const int pg = kv.page(b, s);
-        x[u] = v4i{0, 0, 0, 0};
-        if (pg >= 0) x[u] = *(const v4i*)(kv.krow(pg, h, s & (DI_PAGE - 1)) + (tid & 7) * 16);
-      }
-      __syncthreads();
+    for (int u = 0; u < 4; ++u) {
+      const int i = j * DI_PAGE + u * 32 + (tid >> 3);
+      s[u] = i < a.budget ? krow[i] : -1;
+    }
+  };
+  v4i x[4], y[4];
+  auto load_rows = [&](v4i (&r)[4]) {
+    int pg[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) pg[u] = kv.page(b, s[u]);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      r[u] = v4i{0, 0, 0, 0};
+      if (pg[u] >= 0) r[u] = *(const v4i*)(kv.krow(pg[u], h, s[u] & (DI_PAGE - 1)) + (tid & 7) * 16);
+    }
+  };
+  load_slots(0);
+  load_rows(x);
+  if (npages > 1) load_slots(1);
+  for (int j = 0; j < npages; ++j) {
+    const int to = j < a.dst_width ? drow[j] : -1;
+    if (j + 1 < npages) load_rows(y);
+    if (j + 2 < npages) load_slots(j + 2);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) asm volatile("" ::"v"(x[u]));  // (this page's reads have ended)
+    __syncthreads();
+    if (to >= 0) {
 #pragma unroll
       for (int u = 0; u < 4; ++u)
         *(v4i*)(kv.krow(to, h, u * 32 + (tid >> 3)) + (tid & 7) * 16) = x[u];
-      continue;
     }
-    // V^T: thread (tid / 32, tid % 32) makes slots 4 (tid % 32) .. + 3 of
-    // channels tid / 32 + 8 u
-    uint32_t x[16];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) x[u] = y[u];
+  }
+}
+
+// V^T: a kept slot is a byte of each of 128 channel rows, so whole source pages
+// are read, each once, KVC_PAGES at a time: the next ones load to registers
+// while bytes are taken from those in LDS. Thread (tid / 32, tid % 32) makes
+// slots 4 (tid % 32) .. + 3 of channels tid / 32 + 8 u of a page of dst in
+// registers and writes them when every source page of that page has passed. The
+// same order as in compact_k: a page is written when its last source page, and
+// all before it, are in LDS or behind.
+__device__ __forceinline__ void compact_v(const CompactArgs& a, const KVPages& kv, int h, int b) {
+  __shared__ __attribute__((aligned(16))) int8_t src[KVC_PAGES][128 * DI_PAGE];
+  __shared__ uint16_t list[KVC_MAXP];    // source pages with kept slots, ascending
+  __shared__ int32_t start[KVC_MAXP + 1];  // the first kept slot from each
+  __shared__ int red[4];
+  const int tid = threadIdx.x;
+  const int32_t* krow = a.keep + (i64)b * a.budget;
+  const int32_t* drow = a.dst + (i64)b * a.dst_width;
+  int np = 0, n = 0;  // listed pages, kept slots
+  for (int i0 = 0; i0 < a.budget; i0 += 256) {
+    const int i = i0 + tid;
+    const int s = i < a.budget ? krow[i] : -1;
+    const int before_s = i > 0 && i < a.budget ? krow[i - 1] : -1;
+    const bool lead = s >= 0 && (i == 0 || s / DI_PAGE != before_s / DI_PAGE);
+    int total;
+    const int before = block_count_before<256>((lead ? 1 : 0) | (s >= 0 ? 0x10000 : 0), red, &total);
+    const int at = np + (before & 0xFFFF);
+    if (lead && at < KVC_MAXP) {  // (an ascending keep within the table has no more)
+      list[at] = (uint16_t)(s / DI_PAGE);
+      start[at] = i;
+    }
+    np = ::min(np + (total & 0xFFFF), KVC_MAXP);
+    n += total >> 16;
+  }
+  if (tid == 0) start[np] = n;
+  __syncthreads();
+  v4i pre[KVC_PAGES][4];
+  auto load = [&](int p0) {
+#pragma unroll
+    for (int q = 0; q < KVC_PAGES; ++q) {
+      const int pg = p0 + q < np ? kv.page(b, (i64)list[p0 + q] * DI_PAGE) : -1;
+      const int8_t* from = kv.vchan(pg < 0 ? 0 : pg, h, 0);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        pre[q][u] = v4i{0, 0, 0, 0};
+        if (pg >= 0) pre[q][u] = *(const v4i*)(from + (u * 256 + tid) * 16);
+      }
+    }
+  };
+  const int ch = tid >> 5, i4 = 4 * (tid & 31);
+  uint32_t x[16];
+#pragma unroll
+  for (int u = 0; u < 16; ++u) x[u] = 0;
+  const int npages = (a.budget + DI_PAGE - 1) / DI_PAGE;
+  int j = 0;  // the page of dst being made
+  auto flush = [&] {
+    const int to = j < a.dst_width ? drow[j] : -1;
+    if (to >= 0) {
+#pragma unroll
+      for (int u = 0; u < 16; ++u) *(uint32_t*)(kv.vchan(to, h, ch + 8 * u) + i4) = x[u];
+    }
 #pragma unroll
     for (int u = 0; u < 16; ++u) x[u] = 0;
-    int s4[4], first = -1, last = -1;
+    ++j;
+  };
+  if (np > 0) load(0);
+  for (int p0 = 0; p0 < np; p0 += KVC_PAGES) {
+    __syncthreads();  // the last pages have been read
 #pragma unroll
-    for (int r = 0; r < 4; ++r) s4[r] = slot[4 * (tid & 31) + r];
-    for (int i = 0; i < DI_PAGE; ++i) {
-      const int s = slot[i];
-      if (s >= 0) {
-        first = first < 0 ? s / DI_PAGE : first;
-        last = s / DI_PAGE;
-      }
-    }
-    for (int p0 = first; first >= 0 && p0 <= last; p0 += KVC_PAGES) {
-      __syncthreads();  // (the last pages' reads)
-      for (int q = 0; q < KVC_PAGES; ++q) {
-        const int pg = p0 + q <= last ? kv.page(b, (i64)(p0 + q) * DI_PAGE) : -1;
-        const int8_t* from = kv.vchan(pg < 0 ? 0 : pg, h, 0);
+    for (int q = 0; q < KVC_PAGES; ++q)
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          v4i y = v4i{0, 0, 0, 0};
-          if (pg >= 0) y = *(const v4i*)(from + (u * 256 + tid) * 16);
-          *(v4i*)(src[q] + (u * 256 + tid) * 16) = y;
-        }
-      }
-      __syncthreads();
+      for (int u = 0; u < 4; ++u) *(v4i*)(src[q] + (u * 256 + tid) * 16) = pre[q][u];
+    __syncthreads();
+    if (p0 + KVC_PAGES < np) load(p0 + KVC_PAGES);
+    const int end = start[::min(p0 + KVC_PAGES, np)];
+    for (;;) {
+      // bytes of page j from these source pages
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const int q = s4[r] / DI_PAGE - p0;
-        if (s4[r] >= 0 && q >= 0 && q < KVC_PAGES) {
-          const int8_t* from = src[q] + (tid >> 5) * DI_PAGE + (s4[r] & (DI_PAGE - 1));
+        const int i = j * DI_PAGE + i4 + r;
+        if (i >= start[p0] && i < end) {
+          const int s = krow[i], pg = s / DI_PAGE;
+          int q = 0;
+#pragma unroll
+          for (int t = 1; t < KVC_PAGES; ++t) q = p0 + t < np && (int)list[p0 + t] <= pg ? t : q;
+          const int8_t* from = src[q] + ch * DI_PAGE + (s & (DI_PAGE - 1));
 #pragma unroll
           for (int u = 0; u < 16; ++u)
             x[u] |= (uint32_t)(uint8_t)from[u * 8 * DI_PAGE] << (8 * r);
         }
       }
+      if (end < (j + 1) * DI_PAGE) break;  // block-uniform
+      flush();
     }
-    __syncthreads();
-#pragma unroll
-    for (int u = 0; u < 16; ++u)
-      *(uint32_t*)(kv.vchan(to, h, (tid >> 5) + 8 * u) + 4 * (tid & 31)) = x[u];
   }
+  while (j < npages) flush();
 }
+
+__global__ __launch_bounds__(256) void k_kv_compact(CompactArgs a) {
+  keep_hidden_args();
+  const int h = blockIdx.x >> 1, b = blockIdx.y;
+  const KVPages kv{a.k[blockIdx.z], a.v[blockIdx.z], a.table, a.width, a.n_kv};
+  if (blockIdx.x & 1) compact_v(a, kv, h, b);
+  else compact_k(a, kv, h, b);
+}
+
+constexpr int SEL_FUSED = 16 * SEL_NT;  // slots per row whose keys fit registers
 
 }  // namespace
 
@@ -216,7 +404,7 @@ extern "C" {
 
 int detllm_kv_select_work(int B, int S, int64_t* bytes) {
   if (!bytes || B < 0 || S < 0) return DI_EINVAL;
-  *bytes = (i64)B * S * 8;
+  *bytes = S > SEL_FUSED ? (i64)B * S * 8 : 0;
   return DI_OK;
 }
 
@@ -229,13 +417,22 @@ int detllm_kv_select(const int64_t* acc, int64_t acc_stride, const uint8_t* vali
     return DI_EINVAL;
   if (B <= 0) return DI_OK;
   if (!keep || !kept || (S > 0 && (!acc || !valid))) return DI_EINVAL;
-  if (B > 65535) return DI_ERANGE;
-  if (S > 0 && (!work || work_bytes < (i64)B * S * 8)) return DI_ERANGE;
-  if (S > 0)
-    hipLaunchKernelGGL(k_kv_weight, dim3((S + 255) / 256, B), dim3(256), 0, s, acc, acc_stride,
-                       valid, valid_stride, S, n_kv, (int64_t*)work);
-  hipLaunchKernelGGL(k_kv_select, dim3(B), dim3(SEL_NT), 0, s, acc, acc_stride, valid, valid_stride,
-                     (const int64_t*)work, S, n_kv, budget, recent, sinks, keep, kept);
+  if (B > 65535 || S > 131071) return DI_ERANGE;
+  const SelectArgs a{acc, acc_stride, valid, valid_stride, (const int64_t*)work, S, n_kv, budget,
+                     recent, sinks, keep, kept};
+  const dim3 grid(B), block(SEL_NT);
+  if (S <= SEL_NT) {
+    hipLaunchKernelGGL(k_kv_select<1>, grid, block, 0, s, a);
+  } else if (S <= 4 * SEL_NT) {
+    hipLaunchKernelGGL(k_kv_select<4>, grid, block, 0, s, a);
+  } else if (S <= SEL_FUSED) {
+    hipLaunchKernelGGL(k_kv_select<16>, grid, block, 0, s, a);
+  } else {
+    if (!work || work_bytes < (i64)B * S * 8) return DI_ERANGE;
+    hipLaunchKernelGGL(k_kv_weight, dim3((S + 255) / 256, B), dim3(256), 0, s, acc, acc_stride, S,
+                       n_kv, (int64_t*)work);
+    hipLaunchKernelGGL(k_kv_select<0>, grid, block, 0, s, a);
+  }
   DI_LAUNCH_CHECK();
   return DI_OK;
 }
@@ -246,7 +443,7 @@ int detllm_kv_compact(int8_t* const* kpools, int8_t* const* vpools, int n_layers
   if (n_layers < 0 || width < 1 || dst_width < 0 || budget < 0 || n_kv < 1) return DI_EINVAL;
   if (B <= 0 || n_layers == 0 || dst_width == 0 || budget == 0) return DI_OK;
   if (!kpools || !vpools || !table || !dst || !keep) return DI_EINVAL;
-  if (B > 65535 || n_kv > (1 << 20)) return DI_ERANGE;
+  if (B > 65535 || n_kv > (1 << 20) || width > KVC_MAXP) return DI_ERANGE;
   for (int l = 0; l < n_layers; ++l)
     if (!kpools[l] || !vpools[l]) return DI_EINVAL;
   for (int l0 = 0; l0 < n_layers; l0 += KVC_LAYERS) {

@@ -638,7 +638,7 @@ T2 op_kv_select(const Tensor& acc, const Tensor& valid, int64_t S, int64_t budge
   DI_CHECK((valid.scalar_type() == at::kBool || valid.scalar_type() == at::kByte) &&
                valid.stride(1) == 1 && valid.device() == acc.device() && valid.size(0) == B,
            op, "expected a bool mask of ", B, " rows on ", acc.device());
-  DI_CHECK(n_kv > 0 && S >= 0 && S <= acc.size(2) && S <= valid.size(1) && S < INT32_MAX, op, S,
+  DI_CHECK(n_kv > 0 && S >= 0 && S <= acc.size(2) && S <= valid.size(1) && S <= 131071, op, S,
            " slots of accumulators ", acc.sizes(), " and a mask ", valid.sizes());
   DI_CHECK(budget >= 1 && budget < INT32_MAX && recent >= 0 && sinks >= 0 &&
                recent <= budget - sinks,

@@ -426,7 +426,7 @@ int detllm_attn_decode_acc(const int8_t* q8, const int64_t* tpos, const int8_t* 
  * `budget` valid slots keeps them all; else its first `sinks` and last `recent`
  * valid slots and, of the valid slots between, the budget - sinks - recent with
  * the largest acc summed over the kv heads (int64, wrapping), ties to the lower
- * slot. recent + sinks <= budget. */
+ * slot. recent + sinks <= budget, S <= 131071. */
 int detllm_kv_select_work(int B, int S, int64_t* bytes);
 int detllm_kv_select(const int64_t* acc, int64_t acc_stride, const uint8_t* valid,
                      int64_t valid_stride, int B, int S, int n_kv, int budget, int recent,
@@ -436,7 +436,8 @@ int detllm_kv_select(const int64_t* acc, int64_t acc_stride, const uint8_t* vali
 /* detllm_kv_compact: slot keep[b][i] of every layer's K and V copied to slot i
  * of the pages dst [B][dst_width] (-1: not written); the slots of these pages
  * past row b's last kept one, and those of kept slots whose page is not mapped,
- * become 0. kpools / vpools: HOST arrays of n_layers device pointers. keep as
+ * become 0. kpools / vpools: HOST arrays of n_layers device pointers; width at
+ * most 1024. keep as
  * detllm_kv_select writes it. The page dst[b][j] may be one of row b's pages
  * table[b][0..j]; otherwise no page of dst is in table, and none is in dst
  * twice. */

@@ -239,6 +239,10 @@ SELECT = {
     "all_equal": (2, 8, 3000, 333, 16, 4, 1.0, "zero"),
     "typical": (4, 8, 4000, 1024, 256, 4, 0.95, "random"),
     "long": (1, 8, 20000, 5000, 100, 4, 0.9, "random"),
+    "mid": (2, 8, 9000, 2000, 100, 4, 0.9, "random"),
+    "ranked_ties": (2, 1, 900, 300, 5, 2, 1.0, "few"),
+    "one_heavy": (2, 2, 3000, 8, 4, 3, 1.0, "one"),
+    "long_ties": (1, 1, 17000, 3000, 10, 4, 0.9, "ties"),
     "wide": (3, 8, 2500, 600, 50, 4, 0.9, "wide"),
     "sparse": (3, 4, 3000, 100, 20, 4, 0.06, "random"),
     "dead": (2, 4, 300, 100, 20, 4, 0.0, "random"),
@@ -249,6 +253,12 @@ SELECT = {
 def _weights(kind, B, n_kv, S, rng):
     if kind == "ties":
         return rng.integers(0, 5, (B, n_kv, S), dtype=np.int64)
+    if kind == "few":      # groups of equal weights of about a hundred slots
+        return rng.integers(0, 9, (B, n_kv, S), dtype=np.int64) << 30
+    if kind == "one":      # one slot holds nearly everything
+        w = np.ones((B, n_kv, S), dtype=np.int64)
+        w[..., S // 3] = 1 << 50
+        return w
     if kind == "zero":
         return np.zeros((B, n_kv, S), dtype=np.int64)
     if kind == "wide":     # sums that wrap, negative ones among them
