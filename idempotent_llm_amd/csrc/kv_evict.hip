@@ -62,10 +62,19 @@ __global__ __launch_bounds__(SEL_NT) void k_kv_select(SelectArgs a) {
     i64 sum[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) sum[e] = 0;
-    for (int h = 0; h < a.n_kv; ++h) {
-      const int64_t* row = a.acc + ((i64)b * a.n_kv + h) * a.acc_stride;
+    constexpr int HU = E > 4 ? 2 : 8;  // heads in flight
+    for (int h = 0; h < (a.S > 0 ? a.n_kv : 0); h += HU) {
+      i64 x[HU][E];
 #pragma unroll
-      for (int e = 0; e < E; ++e) sum[e] = wadd(sum[e], s0 + e < a.S ? row[s0 + e] : 0);
+      for (int q = 0; q < HU; ++q) {
+        const int64_t* row = a.acc + ((i64)b * a.n_kv + ::min(h + q, a.n_kv - 1)) * a.acc_stride;
+#pragma unroll
+        for (int e = 0; e < E; ++e) x[q][e] = row[::min(s0 + e, a.S - 1)];
+      }
+#pragma unroll
+      for (int q = 0; q < HU; ++q)
+#pragma unroll
+        for (int e = 0; e < E; ++e) sum[e] = wadd(sum[e], h + q < a.n_kv ? x[q][e] : 0);
     }
 #pragma unroll
     for (int e = 0; e < E; ++e) reg[e] = key_of(sum[e]);
@@ -233,7 +242,7 @@ __global__ __launch_bounds__(SEL_NT) void k_kv_select(SelectArgs a) {
 
 // ---- the kept slots' K and V moved to the pages of dst, in slot order
 constexpr int KVC_LAYERS = 32;  // layers per launch (pool pointers by value)
-constexpr int KVC_PAGES = 4;    // source pages of V in LDS at once
+constexpr int KVC_PAGES = 2;    // source pages of V in LDS at once
 constexpr int KVC_MAXP = 1024;  // pages of V listed at once
 
 struct CompactArgs {
