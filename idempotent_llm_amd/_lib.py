@@ -70,7 +70,7 @@ SIGNATURES = {
     "detllm_kv_select_work": [I, I, P],
     "detllm_kv_select": [P, L, P, L, I, I, I, I, I, I, P, P, P, L, S],
     "detllm_kv_compact": [P, P, I, P, I, P, I, P, I, I, I, S],
-    "detllm_attn_decode_shared_work": [I, I, I, I, I, P],
+    "detllm_attn_decode_shared_work": [I, I, I, I, I, P, P],
     "detllm_attn_decode_shared": [P, P, P, P, P, I, P, L, I, I, I, I, P, I, P, L, P, P, S],
     "detllm_decode_prologue": [P, L, I, L, P, P, P, P, L, S],
     "detllm_op_quant_i8_pertoken": [P, P, P, I, I, P, P, P, S],
@@ -157,6 +157,26 @@ def attn_split_plan(B: int, S: int, n_q: int, n_kv: int):
     if rc != 0:
         raise RuntimeError(f"detllm_attn_split_plan failed (code {rc})")
     return ch.value, ns.value
+
+
+def attn_acc_work(B: int, S: int, n_q: int, n_kv: int) -> int:
+    """Bytes of scratch of detllm_attn_decode_acc at this shape."""
+    out = ctypes.c_int64(0)
+    rc = load().detllm_attn_decode_acc_work(int(B), int(S), int(n_q), int(n_kv), ctypes.byref(out))
+    if rc != 0:
+        raise RuntimeError(f"detllm_attn_decode_acc_work failed (code {rc})")
+    return out.value
+
+
+def attn_shared_work(B: int, S: int, n_q: int, n_kv: int, shared: int):
+    """(bytes of scratch, whether the prefix is read once for the batch) of
+    detllm_attn_decode_shared at this shape."""
+    out, joint = ctypes.c_int64(0), ctypes.c_int(0)
+    rc = load().detllm_attn_decode_shared_work(int(B), int(S), int(n_q), int(n_kv), int(shared),
+                                               ctypes.byref(out), ctypes.byref(joint))
+    if rc != 0:
+        raise RuntimeError(f"detllm_attn_decode_shared_work failed (code {rc})")
+    return out.value, bool(joint.value)
 
 
 def pro_fits(K: int, ksplit: int) -> bool:

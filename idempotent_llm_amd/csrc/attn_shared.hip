@@ -695,10 +695,13 @@ int shared_args_ok(int B, int S, int n_q, int n_kv, int shared) {
 
 extern "C" {
 
-int detllm_attn_decode_shared_work(int B, int S, int n_q, int n_kv, int shared, int64_t* bytes) {
+int detllm_attn_decode_shared_work(int B, int S, int n_q, int n_kv, int shared, int64_t* bytes,
+                                   int* joint) {
   if (!bytes) return DI_EINVAL;
   if (const int rc = shared_args_ok(B, S, n_q, n_kv, shared)) return rc;
-  *bytes = shared_plan(B, S, shared, n_q, n_kv).bytes;
+  const SharedPlan p = shared_plan(B, S, shared, n_q, n_kv);
+  *bytes = p.bytes;
+  if (joint) *joint = p.joint;
   return DI_OK;
 }
 

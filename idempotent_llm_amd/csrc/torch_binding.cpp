@@ -616,7 +616,8 @@ Tensor op_attn_decode_shared(const Tensor& q8, const Tensor& tpos, const Tensor&
            " slots shared (whole pages of 128)");
   const Cache c = check_cache(op, q8, tpos, kpool, vpool, table, valid, false, S);
   int64_t bytes = 0;
-  check(detllm_attn_decode_shared_work(c.B, (int)S, c.n_q, c.n_kv, (int)shared, &bytes),
+  check(detllm_attn_decode_shared_work(c.B, (int)S, c.n_q, c.n_kv, (int)shared, &bytes,
+                                       nullptr),
         "detllm_attn_decode_shared_work");
   const c10::DeviceGuard guard(q8.device());
   Tensor out = empty({c.B, c.n_q * 128}, at::kLong, q8);

@@ -114,22 +114,27 @@ class GraphedDecode:
         logits, _, _, _ = self.model.forward(self.ids_buf, self.pos_buf, self.cache)
         return logits
 
-    def _capture(self):
-        # warm-up: one real execution of this same step (idempotent: it writes
-        # the same K/V bytes to the same slot), so that every kernel of the
-        # step is loaded before the capture
+    def _warm_up(self):
+        """One real execution of this same step (idempotent: it writes the
+        same K/V bytes to the same slot; weights it adds are taken back), so
+        that every kernel of the step is loaded before the capture."""
+        acc = None if self.cache.acc is None else self.cache.acc.clone()
         self._run()
+        if acc is not None:
+            self.cache.acc.copy_(acc)
         torch.cuda.synchronize()
+
+    def _capture(self):
+        self._warm_up()
         g = torch.cuda.CUDAGraph()
         with torch.cuda.graph(g):
             self.out = self._run()
         self.graph = g
 
     def _capture_pick(self):
-        # warm-up as in _capture (the forward only: the pick would overwrite
-        # this step's input ids), then one graph of the forward and the pick
-        self._run()
-        torch.cuda.synchronize()
+        # (the forward only: the pick would overwrite this step's input ids),
+        # then one graph of the forward and the pick
+        self._warm_up()
         g = torch.cuda.CUDAGraph()
         with torch.cuda.graph(g):
             self.out_pick = self._run()

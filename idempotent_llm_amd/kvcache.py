@@ -20,6 +20,16 @@ Slot semantics are the reference's: slot order is call order for every row,
 ``valid`` marks real tokens, ``length`` counts filled slots. Slots that are
 not valid are never read as data by the kernels (their K/V bytes are
 unspecified), which is why pools are not zero-filled.
+
+For long contexts (no counterpart in the reference):
+
+* ``track_weights()`` makes the model's attention add each slot's weight, over
+  all layers, to ``acc`` [B, n_kv, slots], and ``evict(budget, recent, sinks)``
+  keeps the slots that kv_select picks by it, moves them together in every
+  layer and returns the other pages. Positions are the caller's, so decoding
+  goes on where it was;
+* ``fork(rows)`` makes a one-row cache one of ``rows`` rows that share its full
+  pages (``shared`` slots); decode attention reads these once for the batch.
 """
 
 from __future__ import annotations
@@ -52,6 +62,10 @@ class KVCache:
         self.nslots = None          # [1] int64 device: slots visible to a graphed step
         self.pool_generation = 0
         self._dims = None           # (n_layers, n_kv, hd, device)
+        self._free: list = []       # page ids handed back by evict
+        self.tracking = False
+        self.acc = None             # [B, n_kv, width * PAGE] int64 (track_weights)
+        self.shared = 0             # slots whose pages all rows share (fork)
 
     # -- reference-compatible surface ------------------------------------------
     @property
@@ -125,6 +139,11 @@ class KVCache:
         if self.table is not None:
             host[:, :self.width] = self._table_host
             valid[:, :self.valid_buf.shape[1]] = self.valid_buf
+        if self.tracking:
+            acc = torch.zeros(B, self._dims[1], width * PAGE, dtype=torch.int64, device=dev)
+            if self.acc is not None:
+                acc[:, :, :self.acc.shape[2]] = self.acc
+            self.acc = acc
         self._table_host = host
         self.table = torch.from_numpy(host).to(dev)
         self.valid_buf = valid
@@ -140,12 +159,18 @@ class KVCache:
         assert need_w <= self.width, "map_slots beyond the table width"
         missing = np.argwhere(self._table_host[:, :need_w] < 0)
         if len(missing):
-            self._ensure_pool(self.n_pages + len(missing))
-            ids = np.arange(self.n_pages, self.n_pages + len(missing), dtype=np.int32)
-            self._table_host[missing[:, 0], missing[:, 1]] = ids
-            self.n_pages += len(missing)
+            self._table_host[missing[:, 0], missing[:, 1]] = self._take_pages(len(missing))
             self.table.copy_(torch.from_numpy(self._table_host))
         self.mapped = need_w * PAGE
+
+    def _take_pages(self, n: int) -> np.ndarray:
+        """Ids of n pages of the pool: those handed back first, then new ones."""
+        old = [self._free.pop() for _ in range(min(n, len(self._free)))]
+        new = n - len(old)
+        self._ensure_pool(self.n_pages + new)
+        ids = np.arange(self.n_pages, self.n_pages + new, dtype=np.int32)
+        self.n_pages += new
+        return np.concatenate([np.array(old, dtype=np.int32), ids])
 
     def check_rows(self, B: int):
         """Raise CacheRowsMismatch unless the cache is empty or holds B rows."""
@@ -186,6 +211,89 @@ class KVCache:
         assert cap % PAGE == 0
         B = self._table_host.shape[0]
         self._ensure_width(B, cap // PAGE)
+
+    # -- long contexts ------------------------------------------------------------
+    def _no_graph(self, what: str):
+        if self.static_cap:
+            raise ValueError(f"{what}: a graphed decode holds this cache's tables")
+
+    def track_weights(self) -> "KVCache":
+        """From now on the model adds each slot's attention weight (p in
+        [0, 2^14], over the query heads of a kv head, the layers and the
+        queries at valid slots) to ``acc``."""
+        self._no_graph("track_weights")
+        if not self.tracking:
+            self.tracking = True
+            if self.table is not None:
+                self.acc = torch.zeros(self.table.shape[0], self._dims[1], self.cap,
+                                       dtype=torch.int64, device=self._dims[3])
+        return self
+
+    def evict(self, budget: int, recent: int = 0, sinks: int = 0) -> "KVCache":
+        """At most ``budget`` slots per row stay: the first ``sinks`` and the
+        last ``recent`` valid ones and the heaviest others by ``acc``
+        (kv_select), in their order, at slots 0, 1, ...; the cache is then
+        ``budget`` slots long (rows that keep fewer end in slots that are not
+        valid) and the pages behind them are free. A cache of at most
+        ``budget`` slots stays as it is."""
+        self._no_graph("evict")
+        if not self.tracking:
+            raise ValueError("evict: no weights (call track_weights before the prompt)")
+        if budget < 1 or recent < 0 or sinks < 0 or recent + sinks > budget:
+            raise ValueError(f"evict: recent {recent} and sinks {sinks} of a budget of {budget}")
+        if self.length <= budget:
+            return self
+        from . import torch_ops  # noqa: F401  (registers the operators)
+        ops = torch.ops.detllm_rocm
+        keep, kept = ops.kv_select(self.acc, self.valid_buf, self.length, budget, recent, sinks)
+        # a row's own first pages take its slots; for pages that rows share,
+        # and only for those, new ones do
+        wb = -(-budget // PAGE)
+        host = self._table_host
+        ids, n = np.unique(host[host >= 0], return_counts=True)
+        dst = host[:, :wb].copy()
+        fresh = np.argwhere(np.isin(dst, ids[n > 1]))
+        if len(fresh):
+            dst[fresh[:, 0], fresh[:, 1]] = self._take_pages(len(fresh))
+        dst_dev = torch.from_numpy(dst).to(self._dims[3])
+        ops.kv_compact(self.k_pools, self.v_pools, self.table, dst_dev, keep)
+        self._free += [int(i) for i in np.setdiff1d(ids, dst)][::-1]
+        host[:] = -1
+        host[:, :wb] = dst
+        self.table.copy_(torch.from_numpy(host))
+        self.valid_buf.zero_()
+        self.valid_buf[:, :budget] = keep >= 0
+        self.acc.zero_()
+        self.acc[:, :, :budget] = kept
+        self.length, self.mapped, self.shared = budget, wb * PAGE, 0
+        return self
+
+    def fork(self, rows: int) -> "KVCache":
+        """This one-row cache with ``rows`` rows that begin alike: its full
+        pages are shared (``shared`` slots), the page begun is copied."""
+        self._no_graph("fork")
+        if self.table is None or self.table.shape[0] != 1 or rows < 1:
+            raise ValueError("fork: a cache of one row, into one row or more")
+        full, part = self.length // PAGE, self.length % PAGE
+        row = self._table_host[0]
+        begun = int(row[full]) if part else -1
+        self._free += [int(i) for i in row[full + (1 if part else 0):] if i >= 0]
+        host = np.full((rows, self.width), -1, dtype=np.int32)
+        host[:, :full] = row[:full]
+        if part:
+            host[0, full] = begun
+            host[1:, full] = self._take_pages(rows - 1)
+            to = torch.from_numpy(host[1:, full].copy()).to(self._dims[3]).long()
+            for kp, vp in zip(self.k_pools, self.v_pools):
+                kp[to] = kp[begun].clone()
+                vp[to] = vp[begun].clone()
+        self._table_host = host
+        self.table = torch.from_numpy(host).to(self._dims[3])
+        self.valid_buf = self.valid_buf.repeat(rows, 1)
+        if self.acc is not None:
+            self.acc = self.acc.repeat(rows, 1, 1)
+        self.mapped, self.shared = (full + (1 if part else 0)) * PAGE, full * PAGE
+        return self
 
     def layer_args(self, li: int):
         """(K pool, V pool, table, width) of layer li for the C ABI."""

@@ -38,7 +38,8 @@ import torch
 
 from . import dyadic as dy
 from . import ops
-from ._lib import attn_split_plan, call, gemv_plan, pro_fits, raise_for_error_word
+from ._lib import (attn_acc_work, attn_shared_work, attn_split_plan, call, gemv_plan, pro_fits,
+                   raise_for_error_word)
 from .backends import canonical_backend, gemm_nt, int_gemm, int_gemm_u16i8
 from .guard import NoFloatMode
 from .kvcache import PAGE, KVCache  # noqa: F401  (KVCache is part of this module's API)
@@ -508,6 +509,8 @@ class IntQwen3:
         R, nq, nkv, hd = B * T, self.n_q, self.n_kv, self.hd
         li = L.idx
         valid = ws.valid
+        if cache.acc is not None or (T == 1 and cache.shared and self._joint(B, S, cache.shared)):
+            return self._attend_long(ws, L, B, T, P, ns, st, xm, xk, pos, cache, S_past, S, static)
         plan = self._split_plan(B, S) if T == 1 else None
         if plan is not None:
             # long rows: Q/K/V epilogue, then the split-S attention
@@ -545,6 +548,40 @@ class IntQwen3:
             self._attention_seams(L, B, T, P, ns, st, xm, xk, pos, cache, S_past, S, attn)
         else:
             self._attention(ws, L, B, T, P, ns, st, xm, xk, pos, cache, S_past, S, static, attn)
+        return attn, 1, 0, None
+
+    def _joint(self, B: int, S: int, shared: int) -> bool:
+        """Whether decode attention over S slots reads a forked cache's shared
+        pages once for the batch."""
+        return shared <= S and attn_shared_work(B, S, self.n_q, self.n_kv, shared)[1]
+
+    def _attend_long(self, ws: _Workspace, L: LayerWeights, B, T, P, ns, st, xm, xk, pos,
+                     cache: KVCache, S_past, S, static):
+        """_attend where the cache tracks its weights (the attention adds them
+        to cache.acc) or, else, where its rows share a prefix read once."""
+        nq, nkv, li, valid = self.n_q, self.n_kv, L.idx, ws.valid
+        if T > 1 and self._seams_overridden():
+            raise NotImplementedError("a cache that tracks its weights and overridden attention "
+                                      "seams: the seams' attention does not add to it")
+        q8 = ws.buf("q8", (B * T, nq * self.hd), torch.int8)
+        tpos = ws.buf("tpos", (B, nq, T), I64)
+        attn = ws.buf("attn", (B * T, nq * self.hd), I64)
+        call("detllm_qkv_epilogue", P, ns, st, B, T, nq, nkv, xm, xk, pos,
+             *L.epi, self.rope_cos, self.rope_sin, self.max_pos, q8, tpos, None,
+             *cache.layer_args(li), cache.len_idx if static else None,
+             0 if static else S_past, L.kq_est, self._err)
+        args = (q8, tpos, *cache.layer_args(li), valid, cache.cap, B)
+        s_dev = cache.nslots if static else None
+        if T > 1:
+            call("detllm_attn_prefill_acc", *args, T, S_past, nq, nkv, cache.acc, cache.cap, attn)
+        elif cache.acc is not None:
+            n = attn_acc_work(B, S, nq, nkv)
+            call("detllm_attn_decode_acc", *args, S, nq, nkv, s_dev, cache.acc, cache.cap,
+                 ws.buf("work", (n,), torch.uint8), n, attn, self._err)
+        else:
+            n, _ = attn_shared_work(B, S, nq, nkv, cache.shared)
+            call("detllm_attn_decode_shared", *args, S, nq, nkv, s_dev, cache.shared,
+                 ws.buf("work", (n,), torch.uint8), n, attn, self._err)
         return attn, 1, 0, None
 
     def _partials(self, ws: _Workspace, name: str, R: int, N: int, K: int):
