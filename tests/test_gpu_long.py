@@ -431,3 +431,235 @@ def test_shared_decode_takes_row_0s_pages():
     want = _ops().attn_decode_shared(*args, 286, 256)
     args[4][1:, :2] = -1
     assert torch.equal(_ops().attn_decode_shared(*args, 286, 256), want)
+
+
+# ------------------------------------------------- the operators as they are used
+
+# every attention form once: (operator, arguments behind the cache)
+def _forms(S, T, past, acc):
+    return {"window_decode": lambda a, c: _ops().attn_window_decode(*a, S, 100, 4),
+            "window_decode_split": lambda a, c: _ops().attn_window_decode(*a, S, S, 4),
+            "acc_decode": lambda a, c: _ops().attn_decode_acc(*a, S, acc),
+            "shared_decode": lambda a, c: _ops().attn_decode_shared(*a, S, 256),
+            "window_prefill": lambda a, c: _ops().attn_window_prefill(*c, past, 100, 4),
+            "acc_prefill": lambda a, c: _ops().attn_prefill_acc(*c, past, acc)}
+
+
+def _both(B, n_q, n_kv, S, T, seed):
+    """A decode and a chunk's operands over one cache of S slots."""
+    c = lc.make(B, n_q, n_kv, S, seed, T=T, p_valid=0.9)
+    chunk = _dev(c, seed)
+    one = (chunk[0][:, :, -1].contiguous(), chunk[1][:, :, -1].contiguous()) + chunk[2:]
+    return one, chunk
+
+
+def test_captured_calls_replay():
+    """All forms in one graph, with selection and compaction behind them: each
+    replay, with other queries and eager work in between, gives the eager
+    results."""
+    print("[captured calls]", flush=True)
+    B, n_q, n_kv, S, T = 40, 4, 2, 1200, 70
+    one, chunk = _both(B, n_q, n_kv, S, T, 11)
+    acc = torch.zeros(B, n_kv, S, dtype=I64, device="cuda")
+    wb = 3
+    fresh = torch.arange(one[2].shape[0], one[2].shape[0] + B * wb, dtype=torch.int32,
+                         device="cuda").view(B, wb)
+    one, chunk = (list(a) for a in (one, chunk))
+    for a in (one, chunk):
+        for i in (2, 3):
+            a[i] = torch.cat([a[i], torch.zeros(B * wb, *a[i].shape[1:], dtype=torch.int8,
+                                                device="cuda")])
+    chunk[2], chunk[3] = one[2], one[3]
+    forms = _forms(S, T, S - T, acc)
+
+    def run():
+        out = [f(one, chunk) for f in forms.values()]
+        keep, kept = _ops().kv_select(acc, one[5], S, 300, 30, 4)
+        _ops().kv_compact([one[2]], [one[3]], one[4], fresh, keep)
+        cut = (keep >= 0)
+        left = torch.zeros(B, wb * PAGE, dtype=torch.bool, device="cuda")
+        left[:, :300] = cut
+        out.append(_ops().attn_window_decode(one[0], one[1], one[2], one[3], fresh, left, 300,
+                                             128, 4))
+        return out + [keep, kept]
+
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        run()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = run()
+    for k in range(4):
+        acc.fill_(k)
+        for a in (one, chunk):
+            a[0].copy_(torch.randint(-128, 128, a[0].shape, dtype=torch.int8, device="cuda"))
+        g.replay()
+        torch.cuda.synchronize()
+        got_k, acc_k = [x.clone() for x in got], acc.clone()
+        acc.fill_(k)
+        want = run()
+        for name, x, y in zip(list(forms) + ["cut", "keep", "kept"], got_k, want):
+            assert torch.equal(x, y), (k, name)
+        assert torch.equal(acc_k, acc)
+
+
+def test_other_streams_and_two_at_once():
+    """The operators run on torch's current stream: two streams with their own
+    operands, interleaved, give what each gives alone."""
+    print("[streams]", flush=True)
+    cases = []
+    for seed in (3, 4):
+        one, chunk = _both(36, 4, 2, 900, 40, seed)
+        acc = torch.zeros(36, 2, 900, dtype=I64, device="cuda")
+        cases.append((one, chunk, acc, _forms(900, 40, 860, acc)))
+    alone = [[f(one, chunk) for f in forms.values()] for one, chunk, _, forms in cases]
+    accs = [acc.clone() for _, _, acc, _ in cases]
+    for _, _, acc, _ in cases:
+        acc.zero_()
+    streams = [torch.cuda.Stream() for _ in cases]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = [[], []]
+    for name in cases[0][3]:
+        for i, (one, chunk, _, forms) in enumerate(cases):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(forms[name](one, chunk))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(x, y) for x, y in zip(got[i], alone[i]))
+        assert torch.equal(cases[i][2], accs[i])
+
+
+def test_strided_queries_and_masks():
+    """Queries and constants in another order, and a mask that is a slice at
+    an odd address with rows further apart than the slots."""
+    print("[strides]", flush=True)
+    S, T = 700, 50
+    one, chunk = _both(35, 4, 2, S, T, 21)
+    B, w = one[4].shape
+    acc = torch.zeros(B, 2, S, dtype=I64, device="cuda")
+    forms = _forms(S, T, S - T, acc)
+    wide = torch.ones(B, w * PAGE + 37, dtype=torch.bool, device="cuda")
+    wide[:, 5:5 + S] = one[5][:, :S]
+    mask = wide[:, 5:5 + S]
+
+    def other(a):
+        q = a[0].transpose(1, 0).contiguous().transpose(1, 0)
+        t = a[1].transpose(1, 0).contiguous().transpose(1, 0)
+        assert not q.is_contiguous() and not t.is_contiguous()
+        return (q, t) + tuple(a[2:5]) + (mask,)
+
+    for name, f in forms.items():
+        acc.zero_()
+        want, add = f(one, chunk), acc.clone()
+        acc.zero_()
+        got = f(other(one), other(chunk))
+        assert torch.equal(got, want) and torch.equal(acc, add), name
+    acc.random_(0, 1000)
+    a = _ops().kv_select(acc, one[5][:, :S].contiguous(), S, 200, 20, 4)
+    b = _ops().kv_select(acc, mask, S, 200, 20, 4)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+def test_pages_past_4_gib():
+    """Pages whose bytes lie past 2^32 of their pool."""
+    print("[far pages]", flush=True)
+    one, chunk = _both(33, 16, 8, 640, 20, 31)
+    n = one[2].shape[0]
+    far = (1 << 32) // (8 * PAGE * 128) + 100
+    acc = torch.zeros(33, 8, 640, dtype=I64, device="cuda")
+    forms = _forms(640, 20, 620, acc)
+    want = [f(one, chunk) for f in forms.values()]
+    add = acc.clone()
+    acc.zero_()
+    keep = torch.arange(0, 600, 3, dtype=torch.int32, device="cuda").expand(33, 200).contiguous()
+    kp, vp = (torch.empty(far + n + 66, 8, PAGE, 128, dtype=torch.int8, device="cuda")
+              for _ in range(2))
+    kp[far:far + n], vp[far:far + n] = one[2], one[3]
+    table = one[4] + far
+    move = lambda a: a[:2] + (kp, vp, table, a[5])
+    got = [f(move(one), move(chunk)) for f in forms.values()]
+    assert all(torch.equal(x, y) for x, y in zip(got, want)) and torch.equal(acc, add)
+    dst = torch.arange(far + n, far + n + 66, dtype=torch.int32, device="cuda").view(33, 2)
+    _ops().kv_compact([kp], [vp], table, dst, keep)
+    k, v = unpaged(kp, vp, dst, 200)
+    k0, v0 = unpaged(one[2], one[3], one[4], 600)
+    assert torch.equal(k, k0[:, :, ::3]) and torch.equal(v, v0[:, :, ::3])
+
+
+def test_longest_row():
+    """131071 slots, the most a row may have."""
+    print("[longest row]", flush=True)
+    S = 131071
+    c = lc.make(1, 2, 1, S, seed=41, p_valid=0.9)
+    args = _dev(c, 1)
+    err = torch.zeros(1, dtype=torch.int32, device="cuda")
+    want = _ops().attn_decode(*args, S, err)
+    live = int(c["valid"].sum())
+    assert torch.equal(_ops().attn_window_decode(*args, S, live, 0), want)
+    acc = torch.zeros(1, 1, S, dtype=I64, device="cuda")
+    assert torch.equal(_ops().attn_decode_acc(*args, S, acc), want)
+    out, add = lc.attend(c, S=S)
+    _eq(want, out)
+    _eq(acc, add)
+    want, _ = lc.attend(c, S=S, window=5000, sinks=100)
+    _eq(_ops().attn_window_decode(*args, S, 5000, 100), want)
+    keep, kept = _ops().kv_select(acc, args[5], S, 9000, 300, 50)
+    want_keep, want_kept = lc.select(add, c["valid"], 9000, 300, 50)
+    _eq(keep, want_keep)
+    _eq(kept, want_kept)
+    dst = torch.arange(args[2].shape[0], args[2].shape[0] + 71, dtype=torch.int32,
+                       device="cuda")[None]
+    kp, vp = (torch.cat([x, torch.zeros_like(x[:71])]) for x in args[2:4])
+    _ops().kv_compact([kp], [vp], args[4], dst, keep)
+    k, v = unpaged(kp, vp, dst, 9000)
+    _eq(k[0, 0], c["kc"][0, 0][want_keep[0]])
+    _eq(v[0, 0], c["vc"][0, 0].T[want_keep[0]])
+    two = [x.expand(2, *x.shape[1:]).contiguous() if i in (0, 1, 4, 5) else x
+           for i, x in enumerate(args)]
+    shared = S // PAGE * PAGE
+    both = _ops().attn_decode_shared(*two, S, shared)
+    _eq(both[0], out[0])
+    _eq(both[1], out[0])
+    # a chunk at the end of such a row
+    q = torch.randint(-128, 128, (1, 2, 3, 128), dtype=torch.int8, device="cuda")
+    t = torch.randint(1000, 9000, (1, 2, 3), dtype=I64, device="cuda")
+    want = _ops().attn_prefill(q, t, *args[2:], S - 3)
+    assert torch.equal(_ops().attn_window_prefill(q, t, *args[2:], S - 3, live, 0), want)
+    acc.zero_()
+    assert torch.equal(_ops().attn_prefill_acc(q, t, *args[2:], S - 3, acc), want)
+
+
+@pytest.mark.parametrize("count", [0, 100, 256, 300, 640])
+def test_device_slot_counts(count):
+    """The entry points bound the scanned slots by a device word (a captured
+    step's): the same as that many slots; one above the launch's bound sets
+    bit 4 of the error word and scans the bound."""
+    print(f"[device count {count}]", flush=True)
+    from idempotent_llm_amd._lib import attn_acc_work, attn_shared_work, call
+    B, n_q, n_kv, S, cap = 40, 4, 2, 600, 640
+    one, _ = _both(B, n_q, n_kv, cap, 3, 51)
+    q8, tpos, kp, vp, table, valid = one
+    n = min(count, S)
+    word = torch.tensor([count], dtype=I64, device="cuda")
+    cache = (q8, tpos, kp, vp, table, table.shape[1], valid.view(torch.uint8), valid.shape[1], B)
+    work = torch.empty(1 << 24, dtype=torch.uint8, device="cuda")
+    assert attn_shared_work(B, S, n_q, n_kv, 512)[1]
+    for name, tail, want in (
+            ("detllm_attn_window_decode", (100, 4), lambda: _ops().attn_window_decode(*one, n, 100, 4)),
+            ("detllm_attn_window_decode", (10**6, 0),
+             lambda: _ops().attn_window_decode(*one, n, 10**6, 0)),
+            ("detllm_attn_decode_acc", "acc", lambda: _ops().attn_decode_acc(*one, n, other)),
+            ("detllm_attn_decode_shared", (512,), lambda: _ops().attn_decode_shared(*one, n, 0)),
+            ("detllm_attn_decode_shared", (0,), lambda: _ops().attn_decode_shared(*one, n, 0))):
+        if tail == (512,):
+            table[:, :4] = table[:1, :4].clone()
+        acc, other = (torch.zeros(B, n_kv, cap, dtype=I64, device="cuda") for _ in range(2))
+        args = (acc, cap) if tail == "acc" else tail
+        out = torch.full((B, n_q * 128), 7, dtype=I64, device="cuda")
+        err = torch.zeros(1, dtype=torch.int32, device="cuda")
+        call(name, *cache, S, n_q, n_kv, word, *args, work, work.numel(), out, err)
+        assert torch.equal(out, want()), (name, tail)
+        assert torch.equal(acc, other)
+        assert int(err) == (4 if count > S else 0), (name, tail)
