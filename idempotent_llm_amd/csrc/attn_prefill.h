@@ -97,6 +97,13 @@ __device__ __forceinline__ uint32_t row16_scatter_sum(uint32_t (&v)[16]) {
   return keep + (uint32_t)__builtin_amdgcn_update_dpp(0, (int)send, 0xB1, 0xF, 0xF, false);
 }
 
+// A 64-slot key tile in work: its number, which half of its page it is, its
+// first slot and (windowed form) its validity mask
+struct TileOf {
+  int it, hf, s0;
+  u64 vm;
+};
+
 // The block's work: every query of its tile against the key tiles it sees.
 // WIN: the windowed form (window_pages below), ACC: the accumulating form.
 template <bool WIN, bool ACC>
@@ -295,6 +302,16 @@ __device__ __forceinline__ void prefill_body(const PrefillArgs& a) {
   // fn(st, it, half) per half that holds key slots
   auto halves = [&](const int8_t* stg, int it2, const v4i z, auto&& fn) {
     v4i ka[8], kb[8], sa[4], sb[4];
+    TileOf ta{2 * it2, 0, it2 * 128, 0}, tb{2 * it2 + 1, 1, it2 * 128 + 64, 0};
+    if constexpr (WIN) {  // (read beside the K operands, kept as scalars)
+      const int s0 = __builtin_amdgcn_readfirstlane((int)list[it2] * DI_PAGE);
+      const v4i m = *(const v4i*)(vmask + 2 * it2);
+      auto word = [&](int i) { return (u64)(uint32_t)__builtin_amdgcn_readfirstlane(m[i]); };
+      ta.s0 = s0;
+      tb.s0 = s0 + 64;
+      ta.vm = word(0) | word(1) << 32;
+      tb.vm = word(2) | word(3) << 32;
+    }
     load_k(stg, ka);
     load_k(stg + 64 * 128, kb);
     __builtin_amdgcn_sched_barrier(0);
@@ -307,8 +324,8 @@ __device__ __forceinline__ void prefill_body(const PrefillArgs& a) {
 #pragma unroll
     for (int blk = 0; blk < 4; ++blk) sb[blk] = mfma16(kb[2 * blk + 1], qf1, sb[blk]);
     __builtin_amdgcn_sched_barrier(0);
-    fn(sa, 2 * it2, 0);
-    if (2 * it2 + 1 < ntiles) fn(sb, 2 * it2 + 1, 1);
+    fn(sa, ta);
+    if (2 * it2 + 1 < ntiles) fn(sb, tb);
   };
   // the windowed form: where this lane's window begins, and the extremes of
   // that over the wave
@@ -318,25 +335,22 @@ __device__ __forceinline__ void prefill_body(const PrefillArgs& a) {
     wlo_min = __builtin_amdgcn_readfirstlane(wlo);
     wlo_max = __builtin_amdgcn_readlane(wlo, 15);
   }
-  // tile `it` is visible in full to every query of the wave (wave-uniform)
-  auto full_tile = [&](int it) {
-    if constexpr (WIN) {
-      const int s0 = slot64(it);
-      const u64 vm = vmask[it];
-      const bool all = __builtin_amdgcn_readfirstlane((int)(vm == ~0ull)) != 0;
-      return all && s0 + 63 <= wlim && (s0 >= wlo_max || s0 + 63 < wr.sink_end);
-    }
-    return it < nfull && it * 64 + 63 <= wlim;
+  // the validity mask of a tile
+  auto mask = [&](const TileOf& t) { return WIN ? t.vm : vmask[t.it]; };
+  // the tile is visible in full to every query of the wave (wave-uniform)
+  auto full_tile = [&](const TileOf& t) {
+    if constexpr (WIN)
+      return t.vm == ~0ull && t.s0 + 63 <= wlim && (t.s0 >= wlo_max || t.s0 + 63 < wr.sink_end);
+    return t.it < nfull && t.it * 64 + 63 <= wlim;
   };
-  // no query of the wave sees any slot of tile `it` (wave-uniform; the
-  // windowed form only: a page's other half, the other waves' window ends)
-  auto dead_tile = [&](int it) {
-    const int s0 = slot64(it);
-    return WIN && (s0 > wlim + 15 || (s0 + 63 < wlo_min && s0 >= wr.sink_end));
+  // no query of the wave sees any of its slots (wave-uniform; the windowed form
+  // only: a page's other half, the other waves' window ends)
+  auto dead_tile = [&](const TileOf& t) {
+    return WIN && (t.s0 > wlim + 15 || (t.s0 + 63 < wlo_min && t.s0 >= wr.sink_end));
   };
   // this lane's visibility bits: bit 4 blk + r for slot 16 g + 4 blk + r
-  auto lane_bits = [&](int it, u64 vm) -> uint32_t {
-    const int s0 = slot64(it) + 16 * g;
+  auto lane_bits = [&](const TileOf& t) -> uint32_t {
+    const int s0 = t.s0 + 16 * g;
     const int e = limit - s0;  // last visible offset in the lane's 16
     uint32_t cb = e >= 15 ? 0xFFFFu : (e < 0 ? 0u : (2u << e) - 1u);
     if constexpr (WIN) {
@@ -345,20 +359,20 @@ __device__ __forceinline__ void prefill_body(const PrefillArgs& a) {
       const uint32_t sb = z >= 16 ? 0xFFFFu : (z <= 0 ? 0u : (1u << z) - 1u);
       cb &= wb | sb;
     }
-    return (uint32_t)(vm >> (16 * g)) & cb;
+    return (uint32_t)(mask(t) >> (16 * g)) & cb;
   };
 
   // ---- pass 1: row max over visible slots (scores are int32)
   int mx = INT32_MIN;
-  pass(std::false_type{}, [&](int it2, const int8_t* stg) { halves(stg, it2, v4i{0, 0, 0, 0}, [&](const v4i (&st)[4], int it, int) {
-    if (dead_tile(it)) return;
-    if (full_tile(it)) {
+  pass(std::false_type{}, [&](int it2, const int8_t* stg) { halves(stg, it2, v4i{0, 0, 0, 0}, [&](const v4i (&st)[4], const TileOf& t) {
+    if (dead_tile(t)) return;
+    if (full_tile(t)) {
 #pragma unroll
       for (int blk = 0; blk < 4; ++blk)
 #pragma unroll
         for (int r = 0; r < 4; ++r) mx = max(mx, st[blk][r]);
     } else {
-      const uint32_t bits = lane_bits(it, vmask[it]);
+      const uint32_t bits = lane_bits(t);
 #pragma unroll
       for (int blk = 0; blk < 4; ++blk)
 #pragma unroll
@@ -384,9 +398,9 @@ __device__ __forceinline__ void prefill_body(const PrefillArgs& a) {
   const v4i cinit = v4i{soff, soff, soff, soff};
   const ExpR Et = make_exp(tpos);
   i64 den = 0;
-  pass(std::false_type{}, [&](int it2, const int8_t* stg) { halves(stg, it2, cinit, [&](const v4i (&st)[4], int it, int) {
-    if (dead_tile(it)) return;
-    if (fexp && full_tile(it)) {
+  pass(std::false_type{}, [&](int it2, const int8_t* stg) { halves(stg, it2, cinit, [&](const v4i (&st)[4], const TileOf& t) {
+    if (dead_tile(t)) return;
+    if (fexp && full_tile(t)) {
       uint32_t sum = 0;
 #pragma unroll
       for (int blk = 0; blk < 4; ++blk)
@@ -395,7 +409,7 @@ __device__ __forceinline__ void prefill_body(const PrefillArgs& a) {
       den += sum;
       return;
     }
-    const uint32_t bits = lane_bits(it, vmask[it]);
+    const uint32_t bits = lane_bits(t);
     if (fexp) {
       uint32_t sum = 0;
 #pragma unroll
@@ -443,7 +457,8 @@ __device__ __forceinline__ void prefill_body(const PrefillArgs& a) {
   int voff[2];
 #pragma unroll
   for (int hf = 0; hf < 2; ++hf) voff[hf] = PF_KBYTES + qi * 128 + (((4 * hf + g) ^ pf_vswz(qi)) << 4);
-  pass(std::true_type{}, [&](int it2, const int8_t* stg) { halves(stg, it2, cinit, [&](const v4i (&st)[4], int it, int hf) {
+  pass(std::true_type{}, [&](int it2, const int8_t* stg) { halves(stg, it2, cinit, [&](const v4i (&st)[4], const TileOf& t) {
+    const int hf = t.hf;
     v4i vf[8], vc[2];
 #pragma unroll
     for (int j = 0; j < 8; ++j) vf[j] = *(const v4i*)(stg + voff[hf] + j * 2048);
@@ -451,7 +466,7 @@ __device__ __forceinline__ void prefill_body(const PrefillArgs& a) {
     for (int c = 0; c < 2; ++c) vc[c] = *(const v4i*)(stg + voff[hf] + (2 * wave + c) * 2048);
     __builtin_amdgcn_sched_barrier(0);
     v4i phi, plo;
-    if (dead_tile(it)) {
+    if (dead_tile(t)) {
       // p = 0: bytes -64 and 0 (the tile's column sums count for the block)
       const int m64 = (int)0xC0C0C0C0u;
       phi = v4i{m64, m64, m64, m64};
@@ -461,9 +476,9 @@ __device__ __forceinline__ void prefill_body(const PrefillArgs& a) {
       for (int c = 0; c < 2; ++c) ocs[c] = mfma16(ones, vc[c], ocs[c]);
       return;
     }
-    const bool full = full_tile(it);
+    const bool full = full_tile(t);
     uint32_t bits = 0xFFFFu;
-    if (!full) bits = lane_bits(it, vmask[it]);
+    if (!full) bits = lane_bits(t);
     uint32_t pw[ACC ? 16 : 1];  // (the accumulating form keeps the p)
     auto put = [&](int blk, const uint32_t (&p)[4]) {
       int whi, wlo;
@@ -515,7 +530,7 @@ __device__ __forceinline__ void prefill_body(const PrefillArgs& a) {
       // the 16 queries' sums: lane (qi, g) that of slot 16 g + qi
       const uint32_t sum = row16_scatter_sum(pw);
       if (sum != 0)
-        atomicAdd((unsigned long long*)&accrow[slot64(it) + 16 * g + qi], (unsigned long long)sum);
+        atomicAdd((unsigned long long*)&accrow[t.s0 + 16 * g + qi], (unsigned long long)sum);
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j) {

@@ -214,6 +214,10 @@ __device__ __forceinline__ WinRange window_pages(const uint8_t* vrow, int end1, 
     r.pages = n;
   }
   __syncthreads();
+  r.sink_end = __builtin_amdgcn_readfirstlane(r.sink_end);  // (the same in every lane)
+  r.lo = __builtin_amdgcn_readfirstlane(r.lo);
+  r.pre = __builtin_amdgcn_readfirstlane(r.pre);
+  r.pages = __builtin_amdgcn_readfirstlane(r.pages);
   return r;
 }
 
