@@ -142,16 +142,23 @@ __device__ __forceinline__ void shared_parts(const SharedArgs& a, int kvh, int m
 
 // Maxima or sums of exponentials of NG groups of 16 queries from m0 on, over the
 // tiles [tile0, tend) (64 slots each) of row trow's pages, for part `part`. Each
-// wave takes every fourth tile, a K row read once for its NG groups.
+// wave takes every fourth tile, a K row read once for its NG groups; the
+// queries and their constants are read back from LDS, so that a wave needs about
+// 100 registers and four blocks share a CU.
+constexpr int STAT_QROW = 144;  // bytes between queries in LDS: 16 lanes on 64 banks
 template <int NG>
-struct StatTile {
-  v4i k[8];           // blocks of 16 slots: channels 16 g .. (+ 64)
-  uint32_t f[NG][4];  // the flags of slots 16 g .. + 15 of each group's row
+struct StatLds {
+  __attribute__((aligned(16))) int8_t q[16 * NG * STAT_QROW];
+  double rt[16 * NG], kx[16 * NG];  // of the estimated DI-Exp
+  uint32_t t[16 * NG];
+  i64 tpos[16 * NG];
+  i64 red[4 * 16 * NG];
+  int32_t mx[256];
 };
 template <int NG, bool DEN>
 __device__ __forceinline__ void shared_stat(const SharedArgs& a, int S, int kvh, int m0, int mend,
-                                            int trow, int tile0, int tend, int part, i64* red,
-                                            int32_t (&buf)[256]) {
+                                            int trow, int tile0, int tend, int part, char* lds) {
+  StatLds<NG>& L = *(StatLds<NG>*)lds;
   const int tid = threadIdx.x, lane = tid & 63, qi = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int first = tile0 + wave;
@@ -163,99 +170,107 @@ __device__ __forceinline__ void shared_stat(const SharedArgs& a, int S, int kvh,
     pgv = a.kv.page(trow, (i64)(t < tend ? t : tile0) * 64);
   };
   if (ntiles > 0) load_pages(0);
-  v4i qf[NG][2];
-  i64 tpos[NG];
-  const uint8_t* vrow[NG];
-  bool tok[NG];
+  // the queries to LDS, 8 threads each
 #pragma unroll
-  for (int n = 0; n < NG; ++n) {
-    const int m = m0 + 16 * n + qi;
-    tok[n] = m < mend;
-    const int mc = tok[n] ? m : m0;
-    const i64 gq = a.query(kvh, mc);
-    vrow[n] = a.valid + (i64)(mc >> a.gs) * a.valid_stride;
-    qf[n][0] = *(const v4i*)(a.q8 + gq * 128 + g * 16);
-    qf[n][1] = *(const v4i*)(a.q8 + gq * 128 + 64 + g * 16);
-    tpos[n] = DEN ? a.tpos[gq] : 1;
+  for (int i = tid; i < 16 * NG * 8; i += 256) {
+    const int m = min(m0 + (i >> 3), mend - 1);
+    *(v4i*)(L.q + (i >> 3) * STAT_QROW + (i & 7) * 16) =
+        *(const v4i*)(a.q8 + a.query(kvh, m) * 128 + (i & 7) * 16);
   }
-  auto load = [&](int i, StatTile<NG>& t) {
+  const uint8_t* vrow[NG];
+#pragma unroll
+  for (int n = 0; n < NG; ++n)
+    vrow[n] = a.valid + (i64)(min(m0 + 16 * n + qi, mend - 1) >> a.gs) * a.valid_stride;
+  v4i k[8];
+  uint32_t f[NG][4];
+  bool ok = false;  // the tile's page is mapped
+  auto load = [&](int i) {
     const int s0 = (first + i * 4) * 64, pg = __builtin_amdgcn_readlane(pgv, i & 63);
     const int8_t* kb = a.kv.krow(pg < 0 ? 0 : pg, kvh, (s0 & (DI_PAGE - 1)) + kr) + g * 16;
 #pragma unroll
     for (int blk = 0; blk < 4; ++blk) {
-      t.k[2 * blk] = *(const v4i*)(kb + blk * 512);
-      t.k[2 * blk + 1] = *(const v4i*)(kb + blk * 512 + 64);
+      k[2 * blk] = *(const v4i*)(kb + blk * 512);
+      k[2 * blk + 1] = *(const v4i*)(kb + blk * 512 + 64);
     }
 #pragma unroll
-    for (int n = 0; n < NG; ++n) flags16(vrow[n], s0 + 16 * g, S, t.f[n]);
-    return pg >= 0;
+    for (int n = 0; n < NG; ++n) flags16(vrow[n], s0 + 16 * g, S, f[n]);
+    ok = pg >= 0;
   };
-  StatTile<NG> ta, tb;
-  bool oka = false, okb = false;  // the tile's page is mapped
-  if (ntiles > 0) oka = load(0, ta);
+  if (ntiles > 0) load(0);
+  bool fexp = true;  // block-uniform: every constant below 2^23
+  if (DEN) {
+    i64 none[1];
+    i64 tp = 1;
+    if (tid < 16 * NG) tp = a.tpos[a.query(kvh, min(m0 + tid, mend - 1))];
+    shared_parts<16 * NG, false>(a, kvh, m0, mend, L.mx, none);
+    if (tid < 16 * NG) {
+      const ExpEst E = make_expest(tp);
+      L.rt[tid] = E.rt;
+      L.kx[tid] = dexp_sp_const(E);
+      L.t[tid] = E.t;
+      L.tpos[tid] = tp;
+    }
+    fexp = __syncthreads_and(tp < (i64)PF_SMALL_T) != 0;
+  } else {
+    __syncthreads();
+  }
   int mx[NG];
   i64 den[NG];
-  PfFast F[NG];
-  bool fexp[NG];
 #pragma unroll
   for (int n = 0; n < NG; ++n) {
     mx[n] = INT32_MIN;
     den[n] = 0;
   }
-  if (DEN) {
-    i64 none[1];
-    shared_parts<16 * NG, false>(a, kvh, m0, mend, buf, none);
-#pragma unroll
-    for (int n = 0; n < NG; ++n) {
-      mx[n] = buf[16 * n + qi];
-      F[n] = shared_fast(tpos[n], mx[n], 1);
-      fexp[n] = __ballot(tpos[n] >= (i64)PF_SMALL_T) == 0;
-    }
-  }
-  auto body = [&](int i, const StatTile<NG>& t, bool ok) {
+  for (int i = 0; i < ntiles; ++i) {
     const int sl = (first + i * 4) * 64 + 16 * g;
 #pragma unroll
     for (int n = 0; n < NG; ++n) {
-      const int32_t off = DEN && fexp[n] ? F[n].cx : 0;  // scores arrive as st + off
+      const int q = 16 * n + qi;
+      __builtin_amdgcn_sched_barrier(0);  // (else all groups' queries are read at once)
+      const v4i qf0 = *(const v4i*)(L.q + q * STAT_QROW + g * 16);
+      const v4i qf1 = *(const v4i*)(L.q + q * STAT_QROW + 64 + g * 16);
+      // (where the estimate runs, scores arrive as st + t - mx)
+      ExpEst E{0.0, 0};
+      double kx = 0.0;
+      int off = 0;
+      if (DEN) {
+        E.rt = L.rt[q];
+        E.t = L.t[q];
+        kx = L.kx[q];
+        off = fexp ? (int)(E.t - (uint32_t)L.mx[q]) : 0;
+      }
       const v4i z = v4i{off, off, off, off};
       v4i st[4];
 #pragma unroll
-      for (int blk = 0; blk < 4; ++blk) st[blk] = mfma16(t.k[2 * blk], qf[n][0], z);
+      for (int blk = 0; blk < 4; ++blk) st[blk] = mfma16(k[2 * blk], qf0, z);
 #pragma unroll
-      for (int blk = 0; blk < 4; ++blk) st[blk] = mfma16(t.k[2 * blk + 1], qf[n][1], st[blk]);
-      const uint32_t bits = ok && tok[n] ? flags16_bits(t.f[n], sl, S) : 0u;
+      for (int blk = 0; blk < 4; ++blk) st[blk] = mfma16(k[2 * blk + 1], qf1, st[blk]);
+      const uint32_t bits = ok ? flags16_bits(f[n], sl, S) : 0u;
       if (!DEN) {
 #pragma unroll
         for (int r = 0; r < 16; ++r)
           mx[n] = max(mx[n], (bits >> r) & 1u ? st[r >> 2][r & 3] : INT32_MIN);
-      } else if (fexp[n]) {
+      } else if (DI_LIKELY(fexp)) {
         uint32_t sum = 0;
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           const bool vis = (bits >> r) & 1u;
-          const uint32_t e =
-              dexp_est_sp(vis ? st[r >> 2][r & 3] : (int32_t)F[n].E.t, F[n].E, F[n].kx);
+          const uint32_t e = dexp_est_sp(vis ? st[r >> 2][r & 3] : (int32_t)E.t, E, kx);
           sum += vis ? e : 0u;
         }
         den[n] += sum;
       } else {
-        const ExpR Et = make_exp(tpos[n]);
+        const ExpR Et = make_exp(L.tpos[q]);
+        const int m = L.mx[q];
 #pragma unroll
         for (int r = 0; r < 16; ++r)
           if ((bits >> r) & 1u)
-            den[n] = wadd(den[n], di_exp_neg((u64)(uint32_t)(mx[n] - st[r >> 2][r & 3]), Et));
+            den[n] = wadd(den[n], di_exp_neg((u64)(uint32_t)(m - st[r >> 2][r & 3]), Et));
       }
     }
-  };
-  for (int i = 0; i < ntiles; i += 2) {  // a tile loads while the one before is worked on
-    if (i + 1 < ntiles) okb = load(i + 1, tb);
-    body(i, ta, oka);
     if (i + 1 < ntiles) {
-      if (i + 2 < ntiles) {
-        if (((i + 2) & 63) == 0) load_pages(i + 2);
-        oka = load(i + 2, ta);
-      }
-      body(i + 1, tb, okb);
+      if (((i + 1) & 63) == 0) load_pages(i + 1);
+      load(i + 1);
     }
   }
   // over the lanes of a query, then over the waves
@@ -265,17 +280,17 @@ __device__ __forceinline__ void shared_stat(const SharedArgs& a, int S, int kvh,
     if (DEN) {
       v = group4_sum(den[n]);
     } else {
-      int x = max(mx[n], __shfl_xor(mx[n], 16));
+      const int x = max(mx[n], __shfl_xor(mx[n], 16));
       v = max(x, __shfl_xor(x, 32));
     }
-    if (g == 0) red[(wave * NG + n) * 16 + qi] = v;
+    if (g == 0) L.red[(wave * NG + n) * 16 + qi] = v;
   }
   __syncthreads();
   if (tid < 16 * NG && m0 + tid < mend) {
-    i64 v = red[tid];
+    i64 v = L.red[tid];
 #pragma unroll
     for (int w = 1; w < 4; ++w) {
-      const i64 o = red[w * NG * 16 + tid];
+      const i64 o = L.red[w * NG * 16 + tid];
       v = DEN ? wadd(v, o) : imax(v, o);
     }
     const i64 at = ((i64)kvh * a.parts + part) * a.M + m0 + tid;
@@ -287,10 +302,9 @@ __device__ __forceinline__ void shared_stat(const SharedArgs& a, int S, int kvh,
 // Blocks of the prefix (chunk, query block, kv head), then one per (row, kv
 // head) for the row's own slots.
 template <int NG, bool DEN>
-__global__ __launch_bounds__(256, 2) void k_shared_stat(SharedArgs a) {
+__global__ __launch_bounds__(256, DEN ? 4 : 3) void k_shared_stat(SharedArgs a) {
   keep_hidden_args();
-  __shared__ i64 red[4 * NG * 16];
-  __shared__ int32_t buf[256];
+  __shared__ __attribute__((aligned(16))) char lds[sizeof(StatLds<NG>)];
   const int S = a.scanned(false);
   const int npre = a.nchunks * a.qblocks * a.n_kv;
   const int bid = blockIdx.x;
@@ -298,11 +312,11 @@ __global__ __launch_bounds__(256, 2) void k_shared_stat(SharedArgs a) {
     const int c = bid / (a.qblocks * a.n_kv), r = bid % (a.qblocks * a.n_kv);
     const int end = min(min((c + 1) * a.chunk, a.P), S);
     shared_stat<NG, DEN>(a, S, r % a.n_kv, r / a.n_kv * 16 * NG, a.M, 0, c * (a.chunk / 64),
-                         (end + 63) / 64, c, red, buf);
+                         (end + 63) / 64, c, lds);
   } else {
     const int r = bid - npre, b = r / a.n_kv;
     shared_stat<1, DEN>(a, S, r % a.n_kv, b << a.gs, (b + 1) << a.gs, b, a.P / 64, (S + 63) / 64,
-                        a.nchunks, red, buf);
+                        a.nchunks, lds);
   }
 }
 
