@@ -45,11 +45,22 @@ struct SelectArgs {
   int64_t* kept;
 };
 
+// The wave's OR of v, in lane 63
+__device__ __forceinline__ u64 wave_or(u64 v) {
+  v |= (u64)dpp64<0xB1, 0xF>((i64)v, 0);
+  v |= (u64)dpp64<0x4E, 0xF>((i64)v, 0);
+  v |= (u64)dpp64<0x141, 0xF>((i64)v, 0);
+  v |= (u64)dpp64<0x140, 0xF>((i64)v, 0);
+  v |= (u64)dpp64<0x142, 0xA>((i64)v, 0);
+  v |= (u64)dpp64<0x143, 0xC>((i64)v, 0);
+  return v;
+}
+
 template <int E>
 __global__ __launch_bounds__(SEL_NT) void k_kv_select(SelectArgs a) {
   keep_hidden_args();
   __shared__ int hist[256], red[SEL_NT / 64], pick[3], nlist;
-  __shared__ u64 diff, keys[SEL_RANK];
+  __shared__ u64 least_key, keys[SEL_RANK];
   __shared__ int slots[SEL_RANK];
   const int b = blockIdx.x, tid = threadIdx.x;
   const uint8_t* vrow = a.valid + (i64)b * a.valid_stride;
@@ -59,6 +70,7 @@ __global__ __launch_bounds__(SEL_NT) void k_kv_select(SelectArgs a) {
   auto key_of = [](i64 w) { return (u64)w ^ (1ull << 63); };
   u64 reg[E > 0 ? E : 1];
   if constexpr (E > 0) {
+    // slots tid, tid + 1024, ... load together; LDS turns them into runs
     i64 sum[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) sum[e] = 0;
@@ -69,15 +81,23 @@ __global__ __launch_bounds__(SEL_NT) void k_kv_select(SelectArgs a) {
       for (int q = 0; q < HU; ++q) {
         const int64_t* row = a.acc + ((i64)b * a.n_kv + ::min(h + q, a.n_kv - 1)) * a.acc_stride;
 #pragma unroll
-        for (int e = 0; e < E; ++e) x[q][e] = row[::min(s0 + e, a.S - 1)];
+        for (int e = 0; e < E; ++e) x[q][e] = row[::min(tid + e * SEL_NT, a.S - 1)];
       }
 #pragma unroll
       for (int q = 0; q < HU; ++q)
 #pragma unroll
         for (int e = 0; e < E; ++e) sum[e] = wadd(sum[e], h + q < a.n_kv ? x[q][e] : 0);
     }
+    if constexpr (E == 1) {
+      reg[0] = key_of(sum[0]);
+    } else {
+      extern __shared__ __attribute__((aligned(16))) u64 turn[];  // [1024 E]
 #pragma unroll
-    for (int e = 0; e < E; ++e) reg[e] = key_of(sum[e]);
+      for (int e = 0; e < E; ++e) turn[tid + e * SEL_NT] = key_of(sum[e]);
+      __syncthreads();
+#pragma unroll
+      for (int e = 0; e < E; ++e) reg[e] = turn[s0 + e];
+    }
   }
   // each(f): f(slot, key, valid) of the thread's slots below S, in order
   uint32_t vbits = 0;
@@ -98,10 +118,6 @@ __global__ __launch_bounds__(SEL_NT) void k_kv_select(SelectArgs a) {
   };
   int mine = 0, n;
   each([&](int, u64) { ++mine; });
-  if (tid == 0) {
-    diff = 0;
-    nlist = 0;
-  }
   const int rank0 = block_count_before<SEL_NT>(mine, red, &n);
   // the valid slots of rank [lo, hi) compete for `need` places
   const bool all = n <= a.budget;
@@ -119,21 +135,27 @@ __global__ __launch_bounds__(SEL_NT) void k_kv_select(SelectArgs a) {
   int left = need;   // places for keys whose known digits are `least`
   bool ranked = false;
   if (need > 0) {
-    // the bits in which the competing keys differ from the first of them
-    u64 base = 0, d = 0;
-    bool any = false;
+    // the bits in which the competing keys differ: set in one, clear in another
+    u64 ones = 0, zeros = 0;
     compete([&](int, u64 k) {
-      if (!any) base = k;
-      any = true;
-      d |= k ^ base;
+      ones |= k;
+      zeros |= ~k;
     });
-    if (any && atomicAdd(&nlist, 1) == 0) keys[0] = base;
+    ones = wave_or(ones);
+    zeros = wave_or(zeros);
+    if ((tid & 63) == 63) {
+      keys[tid >> 6] = ones;
+      keys[SEL_NT / 64 + (tid >> 6)] = zeros;
+    }
     __syncthreads();
-    d |= any ? base ^ keys[0] : 0;
-    if (d) atomicOr((unsigned long long*)&diff, d);
-    __syncthreads();
-    const u64 all_diff = diff, first = keys[0];
-    int top = 64 - clz64(all_diff);  // bits [0, top) differ (0: all keys are equal)
+    ones = zeros = 0;
+#pragma unroll
+    for (int w = 0; w < SEL_NT / 64; ++w) {
+      ones |= keys[w];
+      zeros |= keys[SEL_NT / 64 + w];
+    }
+    const u64 first = ones & ~zeros;  // (what all agree on)
+    int top = 64 - clz64(ones & zeros);  // bits [0, top) may differ (0: all keys are equal)
     known = top == 64 ? 0 : ~0ull << top;
     least = first & known;
     int count = hi - lo;  // keys whose known digits are `least`
@@ -190,11 +212,11 @@ __global__ __launch_bounds__(SEL_NT) void k_kv_select(SelectArgs a) {
         ahead += keys[i] > k || (keys[i] == k && slots[i] < s) ? 1 : 0;
       ahead = sum8_i32(ahead);
       if (at < c && (tid & 7) == 0 && ahead == left - 1) {
-        diff = k;
+        least_key = k;
         pick[0] = s;
       }
       __syncthreads();
-      least = diff;
+      least = least_key;
       known = ~0ull;
     }
   }
@@ -433,9 +455,9 @@ int detllm_kv_select(const int64_t* acc, int64_t acc_stride, const uint8_t* vali
   if (S <= SEL_NT) {
     hipLaunchKernelGGL(k_kv_select<1>, grid, block, 0, s, a);
   } else if (S <= 4 * SEL_NT) {
-    hipLaunchKernelGGL(k_kv_select<4>, grid, block, 0, s, a);
+    hipLaunchKernelGGL(k_kv_select<4>, grid, block, 4 * SEL_NT * 8, s, a);
   } else if (S <= SEL_FUSED) {
-    hipLaunchKernelGGL(k_kv_select<16>, grid, block, 0, s, a);
+    hipLaunchKernelGGL(k_kv_select<16>, grid, block, 16 * SEL_NT * 8, s, a);
   } else {
     if (!work || work_bytes < (i64)B * S * 8) return DI_ERANGE;
     hipLaunchKernelGGL(k_kv_weight, dim3((S + 255) / 256, B), dim3(256), 0, s, acc, acc_stride, S,
