@@ -325,8 +325,8 @@ __device__ __forceinline__ void compact_k(const CompactArgs& a, const KVPages& k
 }
 
 // V^T: a kept slot is a byte of each of 128 channel rows, so whole source pages
-// are read, each once, KVC_PAGES at a time: the next ones load to registers
-// while bytes are taken from those in LDS. Thread (tid / 32, tid % 32) makes
+// are read, each once, KVC_PAGES at a time: the two next lots load to registers
+// while bytes are taken from the one in LDS. Thread (tid / 32, tid % 32) makes
 // slots 4 (tid % 32) .. + 3 of channels tid / 32 + 8 u of a page of dst in
 // registers and writes them when every source page of that page has passed. The
 // same order as in compact_k: a page is written when its last source page, and
@@ -357,16 +357,16 @@ __device__ __forceinline__ void compact_v(const CompactArgs& a, const KVPages& k
   }
   if (tid == 0) start[np] = n;
   __syncthreads();
-  v4i pre[KVC_PAGES][4];
-  auto load = [&](int p0) {
+  v4i pa[KVC_PAGES][4], pb[KVC_PAGES][4];
+  auto load = [&](int p0, v4i (&x)[KVC_PAGES][4]) {
 #pragma unroll
     for (int q = 0; q < KVC_PAGES; ++q) {
       const int pg = p0 + q < np ? kv.page(b, (i64)list[p0 + q] * DI_PAGE) : -1;
       const int8_t* from = kv.vchan(pg < 0 ? 0 : pg, h, 0);
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
-        pre[q][u] = v4i{0, 0, 0, 0};
-        if (pg >= 0) pre[q][u] = *(const v4i*)(from + (u * 256 + tid) * 16);
+        x[q][u] = v4i{0, 0, 0, 0};
+        if (pg >= 0) x[q][u] = *(const v4i*)(from + (u * 256 + tid) * 16);
       }
     }
   };
@@ -375,7 +375,13 @@ __device__ __forceinline__ void compact_v(const CompactArgs& a, const KVPages& k
 #pragma unroll
   for (int u = 0; u < 16; ++u) x[u] = 0;
   const int npages = (a.budget + DI_PAGE - 1) / DI_PAGE;
-  int j = 0;  // the page of dst being made
+  int j = 0;  // the page of dst being made, and this thread's source slots of it
+  int s4[4];
+  auto load_slots = [&] {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) s4[r] = krow[::min(j * DI_PAGE + i4 + r, a.budget - 1)];
+  };
+  load_slots();
   auto flush = [&] {
     const int to = j < a.dst_width ? drow[j] : -1;
     if (to >= 0) {
@@ -385,24 +391,24 @@ __device__ __forceinline__ void compact_v(const CompactArgs& a, const KVPages& k
 #pragma unroll
     for (int u = 0; u < 16; ++u) x[u] = 0;
     ++j;
+    load_slots();
   };
-  if (np > 0) load(0);
-  for (int p0 = 0; p0 < np; p0 += KVC_PAGES) {
+  auto step = [&](int p0, v4i (&in)[KVC_PAGES][4]) {
     __syncthreads();  // the last pages have been read
 #pragma unroll
     for (int q = 0; q < KVC_PAGES; ++q)
 #pragma unroll
-      for (int u = 0; u < 4; ++u) *(v4i*)(src[q] + (u * 256 + tid) * 16) = pre[q][u];
+      for (int u = 0; u < 4; ++u) *(v4i*)(src[q] + (u * 256 + tid) * 16) = in[q][u];
     __syncthreads();
-    if (p0 + KVC_PAGES < np) load(p0 + KVC_PAGES);
-    const int end = start[::min(p0 + KVC_PAGES, np)];
+    if (p0 + 2 * KVC_PAGES < np) load(p0 + 2 * KVC_PAGES, in);
+    const int begin = start[p0], end = start[::min(p0 + KVC_PAGES, np)];
     for (;;) {
       // bytes of page j from these source pages
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int i = j * DI_PAGE + i4 + r;
-        if (i >= start[p0] && i < end) {
-          const int s = krow[i], pg = s / DI_PAGE;
+        if (i >= begin && i < end) {
+          const int s = s4[r], pg = s / DI_PAGE;
           int q = 0;
 #pragma unroll
           for (int t = 1; t < KVC_PAGES; ++t) q = p0 + t < np && (int)list[p0 + t] <= pg ? t : q;
@@ -415,6 +421,12 @@ __device__ __forceinline__ void compact_v(const CompactArgs& a, const KVPages& k
       if (end < (j + 1) * DI_PAGE) break;  // block-uniform
       flush();
     }
+  };
+  if (np > 0) load(0, pa);
+  if (np > KVC_PAGES) load(KVC_PAGES, pb);
+  for (int p0 = 0; p0 < np; p0 += 2 * KVC_PAGES) {
+    step(p0, pa);
+    if (p0 + KVC_PAGES < np) step(p0 + KVC_PAGES, pb);
   }
   while (j < npages) flush();
 }
