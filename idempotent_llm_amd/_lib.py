@@ -69,7 +69,7 @@ SIGNATURES = {
     "detllm_attn_decode_acc": [P, P, P, P, P, I, P, L, I, I, I, I, P, P, L, P, L, P, P, S],
     "detllm_kv_select_work": [I, I, P],
     "detllm_kv_select": [P, L, P, L, I, I, I, I, I, I, P, P, P, L, S],
-    "detllm_kv_compact": [P, P, I, P, I, P, I, P, I, I, I, S],
+    "detllm_kv_compact": [P, P, I, I, P, I, P, I, P, I, I, I, S],
     "detllm_attn_decode_shared_work": [I, I, I, I, I, P, P],
     "detllm_attn_decode_shared": [P, P, P, P, P, I, P, L, I, I, I, I, P, I, P, L, P, P, S],
     "detllm_decode_prologue": [P, L, I, L, P, P, P, P, L, S],

@@ -273,7 +273,18 @@ struct CompactArgs {
   const int32_t* table;  // [B][width]
   const int32_t* dst;    // [B][dst_width]
   const int32_t* keep;   // [B][budget] ascending, -1 behind
-  int width, dst_width, budget, n_kv;
+  int width, dst_width, budget, n_kv, n_pages;
+
+  // page of row b's slot s, and the page for j of dst (-1: none, or not of the
+  // pools)
+  __device__ __forceinline__ int from(const KVPages& kv, int b, i64 s) const {
+    const int pg = kv.page(b, s);
+    return pg < n_pages ? pg : -1;
+  }
+  __device__ __forceinline__ int to(int b, int j) const {
+    const int pg = j < dst_width ? dst[(i64)b * dst_width + j] : -1;
+    return pg < n_pages ? pg : -1;
+  }
 };
 
 // K: page after page of dst, 8 lanes a row of 128 bytes. Slot i comes from slot
@@ -284,7 +295,6 @@ struct CompactArgs {
 __device__ __forceinline__ void compact_k(const CompactArgs& a, const KVPages& kv, int h, int b) {
   const int tid = threadIdx.x, npages = (a.budget + DI_PAGE - 1) / DI_PAGE;
   const int32_t* krow = a.keep + (i64)b * a.budget;
-  const int32_t* drow = a.dst + (i64)b * a.dst_width;
   int s[4];  // the next page's source slots of this thread's rows
   auto load_slots = [&](int j) {
 #pragma unroll
@@ -297,7 +307,7 @@ __device__ __forceinline__ void compact_k(const CompactArgs& a, const KVPages& k
   auto load_rows = [&](v4i (&r)[4]) {
     int pg[4];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) pg[u] = kv.page(b, s[u]);
+    for (int u = 0; u < 4; ++u) pg[u] = a.from(kv, b, s[u]);
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       r[u] = v4i{0, 0, 0, 0};
@@ -308,7 +318,7 @@ __device__ __forceinline__ void compact_k(const CompactArgs& a, const KVPages& k
   load_rows(x);
   if (npages > 1) load_slots(1);
   for (int j = 0; j < npages; ++j) {
-    const int to = j < a.dst_width ? drow[j] : -1;
+    const int to = a.to(b, j);
     if (j + 1 < npages) load_rows(y);
     if (j + 2 < npages) load_slots(j + 2);
 #pragma unroll
@@ -338,7 +348,6 @@ __device__ __forceinline__ void compact_v(const CompactArgs& a, const KVPages& k
   __shared__ int red[4];
   const int tid = threadIdx.x;
   const int32_t* krow = a.keep + (i64)b * a.budget;
-  const int32_t* drow = a.dst + (i64)b * a.dst_width;
   int np = 0, n = 0;  // listed pages, kept slots
   for (int i0 = 0; i0 < a.budget; i0 += 256) {
     const int i = i0 + tid;
@@ -361,7 +370,7 @@ __device__ __forceinline__ void compact_v(const CompactArgs& a, const KVPages& k
   auto load = [&](int p0, v4i (&x)[KVC_PAGES][4]) {
 #pragma unroll
     for (int q = 0; q < KVC_PAGES; ++q) {
-      const int pg = p0 + q < np ? kv.page(b, (i64)list[p0 + q] * DI_PAGE) : -1;
+      const int pg = p0 + q < np ? a.from(kv, b, (i64)list[p0 + q] * DI_PAGE) : -1;
       const int8_t* from = kv.vchan(pg < 0 ? 0 : pg, h, 0);
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
@@ -383,7 +392,7 @@ __device__ __forceinline__ void compact_v(const CompactArgs& a, const KVPages& k
   };
   load_slots();
   auto flush = [&] {
-    const int to = j < a.dst_width ? drow[j] : -1;
+    const int to = a.to(b, j);
     if (to >= 0) {
 #pragma unroll
       for (int u = 0; u < 16; ++u) *(uint32_t*)(kv.vchan(to, h, ch + 8 * u) + i4) = x[u];
@@ -480,10 +489,11 @@ int detllm_kv_select(const int64_t* acc, int64_t acc_stride, const uint8_t* vali
   return DI_OK;
 }
 
-int detllm_kv_compact(int8_t* const* kpools, int8_t* const* vpools, int n_layers,
+int detllm_kv_compact(int8_t* const* kpools, int8_t* const* vpools, int n_layers, int n_pages,
                       const int32_t* table, int width, const int32_t* dst, int dst_width,
                       const int32_t* keep, int B, int budget, int n_kv, hipStream_t s) {
-  if (n_layers < 0 || width < 1 || dst_width < 0 || budget < 0 || n_kv < 1) return DI_EINVAL;
+  if (n_layers < 0 || n_pages < 1 || width < 1 || dst_width < 0 || budget < 0 || n_kv < 1)
+    return DI_EINVAL;
   if (B <= 0 || n_layers == 0 || dst_width == 0 || budget == 0) return DI_OK;
   if (!kpools || !vpools || !table || !dst || !keep) return DI_EINVAL;
   if (B > 65535 || n_kv > (1 << 20) || width > KVC_MAXP) return DI_ERANGE;
@@ -498,6 +508,7 @@ int detllm_kv_compact(int8_t* const* kpools, int8_t* const* vpools, int n_layers
     }
     a.table = table; a.dst = dst; a.keep = keep;
     a.width = width; a.dst_width = dst_width; a.budget = budget; a.n_kv = n_kv;
+    a.n_pages = n_pages;
     hipLaunchKernelGGL(k_kv_compact, dim3(2 * n_kv, B, n), dim3(256), 0, s, a);
   }
   DI_LAUNCH_CHECK();

@@ -26,6 +26,7 @@
 #include <torch/library.h>
 
 #include <algorithm>
+#include <set>
 #include <string>
 #include <tuple>
 #include <utility>
@@ -516,6 +517,12 @@ Cache check_cache(const char* op, const Tensor& q8, const Tensor& tpos, const Te
 }
 int as_i32(int64_t v) { return (int)std::min<int64_t>(v, INT32_MAX); }
 
+// The mask as bytes, its rows at least S apart (a broadcast one is copied)
+Tensor mask_rows(const Tensor& valid, int64_t S) {
+  return (valid.size(0) <= 1 || valid.stride(0) >= S ? valid : valid.contiguous()).view(at::kByte);
+}
+int64_t mask_stride(const Tensor& v, int64_t S) { return std::max(v.stride(0), S); }
+
 // acc [B, n_kv, slots]: what a kernel adds to in place
 void check_acc(const char* op, const Tensor& acc, int64_t B, int64_t n_kv, int64_t S,
                const Tensor& like) {
@@ -530,7 +537,7 @@ void check_acc(const char* op, const Tensor& acc, int64_t B, int64_t n_kv, int64
 // The arguments that every attention entry begins with (B and n_q behind them)
 #define DI_CACHE_ARGS                                                                         \
   ptr<int8_t>(qc), i64(tc), ptr<int8_t>(kpool), ptr<int8_t>(vpool), ptr<int32_t>(table),      \
-      c.width, ptr<uint8_t>(v), valid.stride(0)
+      c.width, ptr<uint8_t>(v), mask_stride(v, reach)
 
 Tensor op_attn_window_prefill(const Tensor& q8, const Tensor& tpos, const Tensor& kpool,
                               const Tensor& vpool, const Tensor& table, const Tensor& valid,
@@ -538,12 +545,13 @@ Tensor op_attn_window_prefill(const Tensor& q8, const Tensor& tpos, const Tensor
   constexpr const char* op = "attn_window_prefill";
   rank(q8, 4, op);
   const int64_t T = q8.size(2);
-  DI_CHECK(S_past >= 0 && window >= 1 && sinks >= 0, op, "S_past ", S_past, ", window ", window,
+  DI_CHECK(S_past >= 0 && S_past <= 131071 && window >= 1 && sinks >= 0, op, "S_past ", S_past, ", window ", window,
            ", sinks ", sinks);
-  const Cache c = check_cache(op, q8, tpos, kpool, vpool, table, valid, true, S_past + T);
+  const int64_t reach = S_past + T;
+  const Cache c = check_cache(op, q8, tpos, kpool, vpool, table, valid, true, reach);
   const c10::DeviceGuard guard(q8.device());
   Tensor out = empty({c.B, T, c.n_q * 128}, at::kLong, q8);
-  const Tensor qc = q8.contiguous(), tc = tpos.contiguous(), v = valid.view(at::kByte);
+  const Tensor qc = q8.contiguous(), tc = tpos.contiguous(), v = mask_rows(valid, reach);
   DI_RUN(detllm_attn_window_prefill, DI_CACHE_ARGS, c.B, (int)T, (int)S_past, c.n_q, c.n_kv,
          as_i32(window), as_i32(sinks), ptr<int64_t>(out));
   return out;
@@ -555,12 +563,13 @@ Tensor op_attn_prefill_acc(const Tensor& q8, const Tensor& tpos, const Tensor& k
   constexpr const char* op = "attn_prefill_acc";
   rank(q8, 4, op);
   const int64_t T = q8.size(2);
-  DI_CHECK(S_past >= 0, op, "S_past ", S_past);
-  const Cache c = check_cache(op, q8, tpos, kpool, vpool, table, valid, true, S_past + T);
-  check_acc(op, acc, c.B, c.n_kv, S_past + T, q8);
+  DI_CHECK(S_past >= 0 && S_past <= 131071, op, "S_past ", S_past);
+  const int64_t reach = S_past + T;
+  const Cache c = check_cache(op, q8, tpos, kpool, vpool, table, valid, true, reach);
+  check_acc(op, acc, c.B, c.n_kv, reach, q8);
   const c10::DeviceGuard guard(q8.device());
   Tensor out = empty({c.B, T, c.n_q * 128}, at::kLong, q8);
-  const Tensor qc = q8.contiguous(), tc = tpos.contiguous(), v = valid.view(at::kByte);
+  const Tensor qc = q8.contiguous(), tc = tpos.contiguous(), v = mask_rows(valid, reach);
   DI_RUN(detllm_attn_prefill_acc, DI_CACHE_ARGS, c.B, (int)T, (int)S_past, c.n_q, c.n_kv,
          ptr<int64_t>(acc), acc.size(2), ptr<int64_t>(out));
   mutated(acc);
@@ -575,7 +584,8 @@ Tensor op_attn_window_decode(const Tensor& q8, const Tensor& tpos, const Tensor&
                              int64_t S, int64_t window, int64_t sinks) {
   constexpr const char* op = "attn_window_decode";
   DI_CHECK(window >= 1 && sinks >= 0, op, "window ", window, ", sinks ", sinks);
-  const Cache c = check_cache(op, q8, tpos, kpool, vpool, table, valid, false, S);
+  const int64_t reach = S;
+  const Cache c = check_cache(op, q8, tpos, kpool, vpool, table, valid, false, reach);
   const int win = as_i32(window), sk = as_i32(sinks);
   int64_t bytes = 0;
   check(detllm_attn_window_decode_work(c.B, (int)S, c.n_q, c.n_kv, win, sk, &bytes),
@@ -583,7 +593,7 @@ Tensor op_attn_window_decode(const Tensor& q8, const Tensor& tpos, const Tensor&
   const c10::DeviceGuard guard(q8.device());
   Tensor out = empty({c.B, c.n_q * 128}, at::kLong, q8);
   const Tensor work = scratch(bytes, q8);
-  const Tensor qc = q8.contiguous(), tc = tpos.contiguous(), v = valid.view(at::kByte);
+  const Tensor qc = q8.contiguous(), tc = tpos.contiguous(), v = mask_rows(valid, reach);
   DI_RUN(detllm_attn_window_decode, DI_CACHE_ARGS, c.B, (int)S, c.n_q, c.n_kv, nullptr, win, sk,
          work.data_ptr(), bytes, ptr<int64_t>(out), nullptr);
   return out;
@@ -593,7 +603,8 @@ Tensor op_attn_decode_acc(const Tensor& q8, const Tensor& tpos, const Tensor& kp
                           const Tensor& vpool, const Tensor& table, const Tensor& valid,
                           int64_t S, const Tensor& acc) {
   constexpr const char* op = "attn_decode_acc";
-  const Cache c = check_cache(op, q8, tpos, kpool, vpool, table, valid, false, S);
+  const int64_t reach = S;
+  const Cache c = check_cache(op, q8, tpos, kpool, vpool, table, valid, false, reach);
   check_acc(op, acc, c.B, c.n_kv, S, q8);
   int64_t bytes = 0;
   check(detllm_attn_decode_acc_work(c.B, (int)S, c.n_q, c.n_kv, &bytes),
@@ -601,7 +612,7 @@ Tensor op_attn_decode_acc(const Tensor& q8, const Tensor& tpos, const Tensor& kp
   const c10::DeviceGuard guard(q8.device());
   Tensor out = empty({c.B, c.n_q * 128}, at::kLong, q8);
   const Tensor work = scratch(bytes, q8);
-  const Tensor qc = q8.contiguous(), tc = tpos.contiguous(), v = valid.view(at::kByte);
+  const Tensor qc = q8.contiguous(), tc = tpos.contiguous(), v = mask_rows(valid, reach);
   DI_RUN(detllm_attn_decode_acc, DI_CACHE_ARGS, c.B, (int)S, c.n_q, c.n_kv, nullptr,
          ptr<int64_t>(acc), acc.size(2), work.data_ptr(), bytes, ptr<int64_t>(out), nullptr);
   mutated(acc);
@@ -614,7 +625,8 @@ Tensor op_attn_decode_shared(const Tensor& q8, const Tensor& tpos, const Tensor&
   constexpr const char* op = "attn_decode_shared";
   DI_CHECK(shared >= 0 && shared <= S && shared % 128 == 0, op, shared, " of ", S,
            " slots shared (whole pages of 128)");
-  const Cache c = check_cache(op, q8, tpos, kpool, vpool, table, valid, false, S);
+  const int64_t reach = S;
+  const Cache c = check_cache(op, q8, tpos, kpool, vpool, table, valid, false, reach);
   int64_t bytes = 0;
   check(detllm_attn_decode_shared_work(c.B, (int)S, c.n_q, c.n_kv, (int)shared, &bytes,
                                        nullptr),
@@ -622,7 +634,7 @@ Tensor op_attn_decode_shared(const Tensor& q8, const Tensor& tpos, const Tensor&
   const c10::DeviceGuard guard(q8.device());
   Tensor out = empty({c.B, c.n_q * 128}, at::kLong, q8);
   const Tensor work = scratch(bytes, q8);
-  const Tensor qc = q8.contiguous(), tc = tpos.contiguous(), v = valid.view(at::kByte);
+  const Tensor qc = q8.contiguous(), tc = tpos.contiguous(), v = mask_rows(valid, reach);
   DI_RUN(detllm_attn_decode_shared, DI_CACHE_ARGS, c.B, (int)S, c.n_q, c.n_kv, nullptr,
          (int)shared, work.data_ptr(), bytes, ptr<int64_t>(out), nullptr);
   return out;
@@ -648,8 +660,8 @@ T2 op_kv_select(const Tensor& acc, const Tensor& valid, int64_t S, int64_t budge
   check(detllm_kv_select_work((int)B, (int)S, &bytes), "detllm_kv_select_work");
   const c10::DeviceGuard guard(acc.device());
   Tensor keep = empty({B, budget}, at::kInt, acc), kept = empty({B, n_kv, budget}, at::kLong, acc);
-  const Tensor work = scratch(bytes, acc), v = valid.view(at::kByte);
-  DI_RUN(detllm_kv_select, i64(acc), acc.size(2), ptr<uint8_t>(v), valid.stride(0), (int)B, (int)S,
+  const Tensor work = scratch(bytes, acc), v = mask_rows(valid, S);
+  DI_RUN(detllm_kv_select, i64(acc), acc.size(2), ptr<uint8_t>(v), mask_stride(v, S), (int)B, (int)S,
          (int)n_kv, (int)budget, (int)recent, (int)sinks, ptr<int32_t>(keep), ptr<int64_t>(kept),
          work.data_ptr(), bytes);
   return {keep, kept};
@@ -680,10 +692,16 @@ void op_kv_compact(at::TensorList kpools, at::TensorList vpools, const Tensor& t
                op, "expected contiguous int8 pools [pages, n_kv, 128, 128] on ", table.device());
       (t == &kpools[i] ? k : v).push_back(ptr<int8_t>(*t));
     }
-  DI_CHECK(table.size(1) > 0 && dst.size(1) * 128 >= keep.size(1), op, keep.size(1),
+  for (const auto* pools : {&k, &v})
+    DI_CHECK(std::set<int8_t*>(pools->begin(), pools->end()).size() == pools->size(), op,
+             "a pool is given twice");
+  for (const int8_t* p : v)
+    DI_CHECK(std::find(k.begin(), k.end(), p) == k.end(), op, "a pool is given twice");
+  DI_CHECK(table.size(1) > 0 && table.size(1) <= 1024 && dst.size(1) * 128 >= keep.size(1), op, keep.size(1),
            " slots for ", dst.size(1), " pages");
   const c10::DeviceGuard guard(table.device());
-  DI_RUN(detllm_kv_compact, k.data(), v.data(), (int)k.size(), ptr<int32_t>(table),
+  DI_RUN(detllm_kv_compact, k.data(), v.data(), (int)k.size(), as_i32(kpools[0].size(0)),
+         ptr<int32_t>(table),
          (int)table.size(1), ptr<int32_t>(dst), (int)dst.size(1), ptr<int32_t>(keep), (int)B,
          (int)keep.size(1), (int)kpools[0].size(1));
   for (size_t i = 0; i < kpools.size(); ++i) {

@@ -562,6 +562,62 @@ def test_strided_queries_and_masks():
     assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
 
 
+def test_broadcast_masks():
+    """One mask for all rows (stride 0), and one row whose stride is anything."""
+    print("[broadcast masks]", flush=True)
+    S, T = 300, 40
+    one, chunk = _both(34, 4, 2, S, T, 22)
+    acc = torch.zeros(34, 2, S, dtype=I64, device="cuda")
+    row = one[5][:1, :S].contiguous()
+    for name, f in _forms(S, T, S - T, acc).items():
+        want = f(one[:5] + (row.repeat(34, 1),), chunk[:5] + (row.repeat(34, 1),))
+        got = f(one[:5] + (row.expand(34, S),), chunk[:5] + (row.expand(34, S),))
+        assert torch.equal(got, want), name
+    odd = torch.as_strided(row, (1, S), (1, 1))
+    first = lambda a: tuple(x[:1] if i in (0, 1, 4) else x for i, x in enumerate(a[:5]))
+    a = _ops().attn_window_decode(*first(one), row, S, 100, 4)
+    assert torch.equal(_ops().attn_window_decode(*first(one), odd, S, 100, 4), a)
+    a, b = (_ops().kv_select(acc, m, S, 90, 9, 4) for m in (row.repeat(34, 1), row.expand(34, S)))
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+def test_empty_calls():
+    """No rows, and a chunk of no queries."""
+    print("[empty calls]", flush=True)
+    one, chunk = _both(2, 4, 2, 200, 5, 23)
+    none = lambda a: tuple(x[:0] if i in (0, 1, 4, 5) else x for i, x in enumerate(a))
+    acc = torch.zeros(2, 2, 200, dtype=I64, device="cuda")
+    assert _ops().attn_window_decode(*none(one), 200, 9, 4).shape == (0, 512)
+    assert _ops().attn_decode_acc(*none(one), 200, acc[:0]).shape == (0, 512)
+    assert _ops().attn_decode_shared(*none(one), 200, 128).shape == (0, 512)
+    assert _ops().attn_window_prefill(*none(chunk), 195, 9, 4).shape == (0, 5, 512)
+    assert _ops().attn_prefill_acc(*none(chunk), 195, acc[:0]).shape == (0, 5, 512)
+    short = (chunk[0][:, :, :0], chunk[1][:, :, :0]) + chunk[2:]
+    assert _ops().attn_window_prefill(*short, 195, 9, 4).shape == (2, 0, 512)
+    assert _ops().attn_prefill_acc(*short, 195, acc).shape == (2, 0, 512)
+    keep, kept = _ops().kv_select(acc[:0], one[5][:0], 200, 50, 5, 4)
+    assert keep.shape == (0, 50) and kept.shape == (0, 2, 50)
+    before = one[2].clone()
+    _ops().kv_compact([one[2]], [one[3]], one[4][:0], one[4][:0], keep)
+    assert not acc.any() and torch.equal(one[2], before)
+
+
+def test_compact_ignores_pages_that_are_not_the_pools():
+    """Ids past the pools, in dst or the table, count as not mapped."""
+    print("[compact foreign pages]", flush=True)
+    c = lc.make(1, 1, 1, 256, seed=6)
+    kp, vp, table, w = paged(c["kc"], c["vc"], seed=1)
+    keep = torch.arange(0, 256, 2, dtype=torch.int32, device="cuda")[None]
+    before = kp.clone(), vp.clone()
+    _ops().kv_compact([kp], [vp], table, torch.tensor([[w]], dtype=torch.int32, device="cuda"), keep)
+    assert torch.equal(kp, before[0]) and torch.equal(vp, before[1])
+    kp, vp = (torch.cat([x, torch.full_like(x[:1], 9)]) for x in (kp, vp))
+    table[0, 1] = 1 << 20
+    _ops().kv_compact([kp], [vp], table, torch.tensor([[w]], dtype=torch.int32, device="cuda"), keep)
+    _eq(kp[w, 0, :64], c["kc"][0, 0, 0:128:2])
+    assert not kp[w, 0, 64:].any() and not vp[w, 0, :, 64:].any()
+
+
 def test_pages_past_4_gib():
     """Pages whose bytes lie past 2^32 of their pool."""
     print("[far pages]", flush=True)

@@ -81,6 +81,7 @@ BAD_TAILS = [
     ("attn_window_prefill", 8, (100, 16, -1)), ("attn_window_prefill", 8, (377, 16, 4)),
     ("attn_window_decode", None, (385, 16, 4)), ("attn_window_decode", None, (-1, 16, 4)),
     ("attn_window_decode", None, (200, 0, 4)), ("attn_window_decode", None, (200, 16, -1)),
+    ("attn_window_prefill", 8, (2**63 - 1, 16, 4)), ("attn_prefill_acc", 8, (2**63 - 1, "acc")),
     ("attn_prefill_acc", 8, (-1, "acc")), ("attn_prefill_acc", 8, (377, "acc")),
     ("attn_decode_acc", None, (385, "acc")),
     ("attn_decode_shared", None, (200, 100)), ("attn_decode_shared", None, (200, 256)),
@@ -132,6 +133,7 @@ def test_compact_refuses():
     pool = lambda *s: torch.zeros(*(s or (6, 2, 128, 128)), dtype=I8)
     table, dst = torch.zeros(2, 3, dtype=I32), torch.zeros(2, 2, dtype=I32)
     keep = torch.zeros(2, 200, dtype=I32)
+    same = pool()
     bad = [([], [], table, dst, keep), ([pool()], [pool(), pool()], table, dst, keep),
            ([pool()], [pool(5, 2, 128, 128)], table, dst, keep),
            ([pool(), pool(5, 2, 128, 128)], [pool(), pool()], table, dst, keep),
@@ -142,7 +144,9 @@ def test_compact_refuses():
            ([pool()], [pool()], table, dst[:1], keep), ([pool()], [pool()], table, dst, keep[:1]),
            ([pool()], [pool()], table, dst[:, :1].contiguous(), keep),
            ([pool()], [pool()], table, dst, keep.long()),
-           ([pool()], [pool()], table[:, :0].contiguous(), dst, keep)]
+           ([pool()], [pool()], table[:, :0].contiguous(), dst, keep),
+           ([same, pool()], [pool(), same], table, dst, keep), ([same], [same], table, dst, keep),
+           ([same, same], [pool(), pool()], table, dst, keep)]
     for args in bad:
         with pytest.raises(ValueError, match="kv_compact|dimensions"):
             _call("kv_compact", *args)
@@ -179,11 +183,11 @@ def test_entry_error_codes():
         e["detllm_kv_select"](0, t, 300, t, 300, 2, 300, 2, 100, 97, 4, t, t, t, 1 << 40)
     with pytest.raises(RuntimeError, match="code -34"):
         e["detllm_kv_select"](0, t, 20000, t, 20000, 2, 20000, 2, 100, 9, 4, t, t, None, 0)
-    assert e["detllm_kv_compact"](0, None, None, 0, t, 3, t, 2, t, 2, 100, 2) is None
+    assert e["detllm_kv_compact"](0, None, None, 0, 6, t, 3, t, 2, t, 2, 100, 2) is None
     pools = (ctypes.c_void_p * 1)(0)
     with pytest.raises(RuntimeError, match="code -22"):
-        e["detllm_kv_compact"](0, ctypes.addressof(pools), ctypes.addressof(pools), 1, t, 3, t, 2,
-                               t, 2, 100, 2)
+        e["detllm_kv_compact"](0, ctypes.addressof(pools), ctypes.addressof(pools), 1, 6, t, 3, t,
+                               2, t, 2, 100, 2)
 
 
 def test_scratch_sizes_cover_every_shape():
