@@ -663,6 +663,19 @@ __global__ __launch_bounds__(256) void k_shared_split_pv(SplitArgs sa, int P) {
   split_pv_chunk<G, SharedView>(sa, blockIdx.x, blockIdx.y, blockIdx.z, SharedView{P});
 }
 
+// Whether the four launches pay: they cost 19 us with few rows and 25 with 32
+// and more, whatever the prefix, and a row's own slots cost more there than in
+// the per-row form. us per call, per row / joint, 16 / 8 heads, 40 slots behind
+// the prefix: 4 rows 8192 slots 26.7 / 27.3, 8 rows 4096 23.8 / 24.4, 8192 34.6 /
+// 28.3, 16 rows 2048 21.9 / 22.0, 4096 30.9 / 24.3, 32 rows 2048 23.5 / 25.8, 4096
+// 39.5 / 28.2, 64 rows 1024 22.7 / 27.1, 2048 37.2 / 28.8, 8192 191 / 43; 1000 slots
+// behind 1024: 16 rows 22.8 / 34.9, 64 rows 38.0 / 62.7.
+bool shared_joint(int B, int S, int P) {
+  const i64 saved = (i64)(B - 1) * P;
+  return B > 16 ? saved >= 81920 && S - P <= P / 4
+                : saved >= 24576 && S - P <= imin(P / 16, 512);
+}
+
 struct SharedPlan {
   bool joint;                                          // the prefix read once for the batch
   int ng, qblocks, chunk, nchunks;                     // stat
@@ -674,7 +687,7 @@ SharedPlan shared_plan(int B, int S, int P, int n_q, int n_kv) {
   SharedPlan p{};
   const int G = n_q / n_kv;
   const i64 M = (i64)B * G;
-  p.joint = P > 0 && (i64)(B - 1) * P >= 8192 && S - P <= 4096;
+  p.joint = shared_joint(B, S, P);
   if (!p.joint) {
     i64 at;
     p.split = B > 0 && S > 0 ? decode_chunk(B, S, n_q, n_kv) : 0;

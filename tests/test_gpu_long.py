@@ -375,20 +375,21 @@ SHARED = {
     "group_1": (20, 8, 8, 384, 77, dict(p_valid=0.9)),
     "group_8": (3, 8, 1, 256, 300, dict(p_valid=0.9)),
     "odd_rows": (9, 4, 2, 640, 65, dict(p_valid=0.9)),
-    "two_blocks": (70, 4, 2, 384, 10, {}),
+    "two_blocks": (70, 4, 2, 1280, 10, {}),
     "long": (5, 4, 2, 2048, 130, dict(p_valid=0.95)),
-    "one_group": (8, 2, 1, 1280, 40, dict(p_valid=0.9)),
-    "two_groups": (13, 4, 2, 896, 70, dict(p_valid=0.9)),
-    "one_group_8": (2, 16, 2, 8320, 200, dict(p_valid=0.9)),
-    "four_groups_1": (50, 2, 2, 384, 1, dict(p_valid=0.9)),
-    "no_suffix_joint": (40, 4, 2, 256, 0, dict(p_valid=0.9)),
-    "long_suffix": (10, 4, 2, 1024, 1000, dict(p_valid=0.9)),
-    "many_chunks": (5, 8, 1, 20000 // 128 * 128, 3, dict(p_valid=0.9)),
-    "dead_joint": (40, 4, 2, 256, 20, dict(gaps=((0, 0, 276), (39, 0, 256), (1, 250, 276)))),
-    "wide_tpos_joint": (33, 4, 2, 384, 40, dict(tpos=(0, 62), p_valid=0.8)),
-    "mixed_tpos_joint": (33, 4, 2, 384, 40, dict(tpos=(30, 48), p_valid=0.8)),
-    "flat_joint": (5, 4, 2, 2560, 20, dict(flat_heads=(0, 1), tpos=(38, 39))),
-    "extreme_joint": (33, 2, 2, 384, 70, dict(extreme=(0,), tpos=(28, 40))),
+    # (from here to flat_joint: prefixes read once for the batch)
+    "one_group": (8, 2, 1, 3584, 40, dict(p_valid=0.9)),
+    "two_groups": (13, 4, 2, 2048, 70, dict(p_valid=0.9)),
+    "one_group_8": (2, 16, 2, 24576, 200, dict(p_valid=0.9)),
+    "four_groups_1": (50, 2, 2, 1792, 1, dict(p_valid=0.9)),
+    "no_suffix_joint": (40, 4, 2, 2176, 0, dict(p_valid=0.9)),
+    "long_suffix": (18, 4, 2, 4864, 1000, dict(p_valid=0.9)),
+    "many_chunks": (5, 8, 1, 19968, 3, dict(p_valid=0.9)),
+    "dead_joint": (40, 4, 2, 2176, 20, dict(gaps=((0, 0, 2196), (39, 0, 2176), (1, 2170, 2196)))),
+    "wide_tpos_joint": (33, 4, 2, 2560, 40, dict(tpos=(0, 62), p_valid=0.8)),
+    "mixed_tpos_joint": (33, 4, 2, 2560, 40, dict(tpos=(30, 48), p_valid=0.8)),
+    "extreme_joint": (33, 2, 2, 2560, 70, dict(extreme=(0,), tpos=(28, 40))),
+    "flat_joint": (5, 4, 2, 6144, 20, dict(flat_heads=(0, 1), tpos=(38, 39))),
     "dead_prefix": (3, 4, 2, 256, 50, dict(gaps=((1, 0, 256),))),
     "dead_row": (3, 4, 2, 256, 50, dict(dead_rows=(1,))),
     "wide_tpos": (3, 4, 2, 256, 100, dict(tpos=(0, 62), p_valid=0.8)),
@@ -422,6 +423,10 @@ def test_shared_decode(name):
     if S:
         err = torch.zeros(1, dtype=torch.int32, device="cuda")
         assert torch.equal(out, _ops().attn_decode(*args, S, err))
+    from idempotent_llm_amd._lib import attn_shared_work
+    names = list(SHARED)
+    joint = names.index("one_group") <= names.index(name) <= names.index("flat_joint")
+    assert attn_shared_work(B, S, n_q, n_kv, shared)[1] == (joint or name == "two_blocks")
 
 
 def test_shared_decode_takes_row_0s_pages():
@@ -440,7 +445,8 @@ def _forms(S, T, past, acc):
     return {"window_decode": lambda a, c: _ops().attn_window_decode(*a, S, 100, 4),
             "window_decode_split": lambda a, c: _ops().attn_window_decode(*a, S, S, 4),
             "acc_decode": lambda a, c: _ops().attn_decode_acc(*a, S, acc),
-            "shared_decode": lambda a, c: _ops().attn_decode_shared(*a, S, 256),
+            "shared_decode": lambda a, c: _ops().attn_decode_shared(*a, S, (S - 1) // PAGE * PAGE),
+            "shared_decode_rows": lambda a, c: _ops().attn_decode_shared(*a, S, 128),
             "window_prefill": lambda a, c: _ops().attn_window_prefill(*c, past, 100, 4),
             "acc_prefill": lambda a, c: _ops().attn_prefill_acc(*c, past, acc)}
 
@@ -458,7 +464,7 @@ def test_captured_calls_replay():
     replay, with other queries and eager work in between, gives the eager
     results."""
     print("[captured calls]", flush=True)
-    B, n_q, n_kv, S, T = 40, 4, 2, 1200, 70
+    B, n_q, n_kv, S, T = 40, 4, 2, 2400, 70
     one, chunk = _both(B, n_q, n_kv, S, T, 11)
     acc = torch.zeros(B, n_kv, S, dtype=I64, device="cuda")
     wb = 3
@@ -510,9 +516,9 @@ def test_other_streams_and_two_at_once():
     print("[streams]", flush=True)
     cases = []
     for seed in (3, 4):
-        one, chunk = _both(36, 4, 2, 900, 40, seed)
-        acc = torch.zeros(36, 2, 900, dtype=I64, device="cuda")
-        cases.append((one, chunk, acc, _forms(900, 40, 860, acc)))
+        one, chunk = _both(36, 4, 2, 2500, 40, seed)
+        acc = torch.zeros(36, 2, 2500, dtype=I64, device="cuda")
+        cases.append((one, chunk, acc, _forms(2500, 40, 2460, acc)))
     alone = [[f(one, chunk) for f in forms.values()] for one, chunk, _, forms in cases]
     accs = [acc.clone() for _, _, acc, _ in cases]
     for _, _, acc, _ in cases:
@@ -535,7 +541,7 @@ def test_strided_queries_and_masks():
     """Queries and constants in another order, and a mask that is a slice at
     an odd address with rows further apart than the slots."""
     print("[strides]", flush=True)
-    S, T = 700, 50
+    S, T = 2560, 50
     one, chunk = _both(35, 4, 2, S, T, 21)
     B, w = one[4].shape
     acc = torch.zeros(B, 2, S, dtype=I64, device="cuda")
@@ -621,11 +627,11 @@ def test_compact_ignores_pages_that_are_not_the_pools():
 def test_pages_past_4_gib():
     """Pages whose bytes lie past 2^32 of their pool."""
     print("[far pages]", flush=True)
-    one, chunk = _both(33, 16, 8, 640, 20, 31)
+    one, chunk = _both(33, 16, 8, 2640, 20, 31)
     n = one[2].shape[0]
     far = (1 << 32) // (8 * PAGE * 128) + 100
-    acc = torch.zeros(33, 8, 640, dtype=I64, device="cuda")
-    forms = _forms(640, 20, 620, acc)
+    acc = torch.zeros(33, 8, 2640, dtype=I64, device="cuda")
+    forms = _forms(2640, 20, 2620, acc)
     want = [f(one, chunk) for f in forms.values()]
     add = acc.clone()
     acc.zero_()
@@ -687,30 +693,30 @@ def test_longest_row():
     assert torch.equal(_ops().attn_prefill_acc(q, t, *args[2:], S - 3, acc), want)
 
 
-@pytest.mark.parametrize("count", [0, 100, 256, 300, 640])
+@pytest.mark.parametrize("count", [0, 100, 2176, 2300, 2560])
 def test_device_slot_counts(count):
     """The entry points bound the scanned slots by a device word (a captured
     step's): the same as that many slots; one above the launch's bound sets
     bit 4 of the error word and scans the bound."""
     print(f"[device count {count}]", flush=True)
     from idempotent_llm_amd._lib import attn_acc_work, attn_shared_work, call
-    B, n_q, n_kv, S, cap = 40, 4, 2, 600, 640
+    B, n_q, n_kv, S, cap = 40, 4, 2, 2400, 2560
     one, _ = _both(B, n_q, n_kv, cap, 3, 51)
     q8, tpos, kp, vp, table, valid = one
     n = min(count, S)
     word = torch.tensor([count], dtype=I64, device="cuda")
     cache = (q8, tpos, kp, vp, table, table.shape[1], valid.view(torch.uint8), valid.shape[1], B)
     work = torch.empty(1 << 24, dtype=torch.uint8, device="cuda")
-    assert attn_shared_work(B, S, n_q, n_kv, 512)[1]
+    assert attn_shared_work(B, S, n_q, n_kv, 2176)[1]
     for name, tail, want in (
             ("detllm_attn_window_decode", (100, 4), lambda: _ops().attn_window_decode(*one, n, 100, 4)),
             ("detllm_attn_window_decode", (10**6, 0),
              lambda: _ops().attn_window_decode(*one, n, 10**6, 0)),
             ("detllm_attn_decode_acc", "acc", lambda: _ops().attn_decode_acc(*one, n, other)),
-            ("detllm_attn_decode_shared", (512,), lambda: _ops().attn_decode_shared(*one, n, 0)),
+            ("detllm_attn_decode_shared", (2176,), lambda: _ops().attn_decode_shared(*one, n, 0)),
             ("detllm_attn_decode_shared", (0,), lambda: _ops().attn_decode_shared(*one, n, 0))):
-        if tail == (512,):
-            table[:, :4] = table[:1, :4].clone()
+        if tail == (2176,):
+            table[:, :17] = table[:1, :17].clone()
         acc, other = (torch.zeros(B, n_kv, cap, dtype=I64, device="cuda") for _ in range(2))
         args = (acc, cap) if tail == "acc" else tail
         out = torch.full((B, n_q * 128), 7, dtype=I64, device="cuda")

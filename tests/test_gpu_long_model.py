@@ -144,10 +144,10 @@ def test_evicted_cache_answers_as_a_masked_one(model, lens, budget, recent, sink
         cur, at = a.argmax(-1), at + 1
 
 
-@pytest.mark.parametrize("T,rows", [(200, 3), (256, 2), (1000, 12)])
+@pytest.mark.parametrize("T,rows", [(200, 3), (256, 2), (1950, 14)])
 def test_forked_rows_answer_as_equal_prompts(model, T, rows):
     """Rows forked from one prompt give the logits of as many equal prompts,
-    eager, graphed (the longest case reads its prefix once for the batch) and
+    eager (the longest case reads its prefix once for the batch), graphed and
     as a chunk; evicting them copies what they share."""
     from idempotent_llm_amd.graphed import GraphedDecode
     from idempotent_llm_amd.kvcache import KVCache
@@ -159,7 +159,7 @@ def test_forked_rows_answer_as_equal_prompts(model, T, rows):
     m.forward(ids.expand(rows, T).contiguous(), pos.expand(rows, T).contiguous(), many)
     one.fork(rows)
     one.tracking, acc, one.acc = False, one.acc, None      # (the shared form tracks no weights)
-    assert m._joint(rows, T + 1, one.shared) == (rows == 12)
+    assert m._joint(rows, T + 1, one.shared) == (rows == 14)
     at = torch.full((rows,), T, device="cuda")
     cur = torch.arange(rows, device="cuda") + 5            # the rows part here
     for s in range(3):
