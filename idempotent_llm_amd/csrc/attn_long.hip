@@ -5,11 +5,11 @@
 //
 // Windowed (attn_window.h has the rule): the kernels are attention.hip's over
 // a shorter list of pages, those of the sinks and those from the window's
-// first slot on, so their work follows the window and not the cache. The
-// range is found on the device, per query tile in prefill and per row in
-// decode, because it depends on the row's validity flags: a launch is sized
-// for rows without gaps, and a row whose window spans more slots takes more
-// steps in the same blocks.
+// first slot on that hold a valid slot, so their work follows the window and not
+// the cache. The list is made on the device, per query tile in prefill and per
+// row in decode, because it depends on the row's validity flags: a launch is
+// sized for rows without gaps, and a row whose window spans more pages takes
+// more steps in the same blocks (scores past its LDS go to the scratch).
 //
 // Accumulating: the p of a slot, summed over the query heads of a kv head (and
 // over a tile's queries), is added to acc [B][n_kv][slots]. p is an integer, so
@@ -22,10 +22,22 @@
 
 namespace {
 
+// Bound by issue, as k_attn_prefill: about 28 VALU instructions per pair of a
+// query and a slot it may see (DI-Exp twice, p, packing) beside 42 MFMAs and as
+// many LDS operand reads per 16 x 64 tile, in phases that overlap only in part.
+// 64 queries, a window of 1024 and 4 sinks walk about 1340 slots, 1.3 times what
+// they see (pages and 64-query tiles are whole). 2048 queries behind 6144 slots,
+// 32 heads, window 1024: 129 us, 67 M pairs seen, 267 TOP/s; 3 x 333 queries,
+// window 100: 24 us, most of it the chain of three passes over three pages.
 __global__ __launch_bounds__(256, 2) void k_window_prefill(PrefillArgs a) {
   keep_hidden_args();
   prefill_body<true, false>(a);
 }
+// k_attn_prefill, and per 16 x 64 tile the 16 queries' p of each slot summed over
+// lanes (45 VALU instructions, row16_scatter_sum) and one 64-bit atomic per slot:
+// 2048 queries, 16 heads 74 us against 61.5 without. Sums of a block's four waves
+// joined in LDS first, a fourth of the atomics, measured 1.7 us less and were not
+// kept for it.
 __global__ __launch_bounds__(256, 2) void k_acc_prefill(PrefillArgs a) {
   keep_hidden_args();
   prefill_body<false, true>(a);
@@ -53,6 +65,9 @@ __device__ __forceinline__ WinView win_view(const WinRange& r, const uint16_t* l
   return WinView{list, n, r.sink_end, r.lo};
 }
 
+constexpr int NW = 8;  // waves of the one-block kernels (4: 32 rows, window 2048 behind
+                       // padding 49 us against 40, 32 x 4000 slots 73 against 57)
+
 struct WindowArgs {
   SplitArgs s;
   int window, sinks;
@@ -64,8 +79,11 @@ struct WindowArgs {
 };
 
 // One block per (row, kv head). Scores in LDS; a row whose window spans more
-// slots than that holds keeps them in the scratch.
-template <int G, int NW>
+// slots than that holds keeps them in the scratch. Bound by HBM with many rows
+// (32 x 8000 slots, window 2048: 39 us for 134 MB seen, about 150 MB in whole
+// pages), by the chain flags - list - K - maximum - denominator - p - V with few
+// (one row of 320: 10 us).
+template <int G>
 __global__ __launch_bounds__(64 * NW) void k_window_decode(WindowArgs w) {
   keep_hidden_args();
   extern __shared__ __attribute__((aligned(16))) int32_t sh_scores[];
@@ -139,7 +157,8 @@ __global__ __launch_bounds__(256) void k_window_pv(WindowArgs w) {
   } while (c * w.s.chunk < v.n);
 }
 
-template <int G, bool SCR, int NW>
+// One block per (row, kv head), as k_window_decode: 32 x 4000 slots 57 us, 4.9 TB/s.
+template <int G>
 __global__ __launch_bounds__(64 * NW) void k_acc_decode(DecodeArgs a) {
   keep_hidden_args();
   extern __shared__ __attribute__((aligned(16))) int32_t sh_scores[];
@@ -152,7 +171,7 @@ __global__ __launch_bounds__(64 * NW) void k_acc_decode(DecodeArgs a) {
   for (int i = threadIdx.x; i < npages; i += 64 * NW) pg_lds[i] = a.kv.page(b, (i64)i * DI_PAGE);
   if (npages == 0 && threadIdx.x == 0) pg_lds[0] = -1;
   __syncthreads();
-  decode_body<G, VPRE, SCR, false, NW, false, WholeRow, true>(
+  decode_body<G, VPRE, false, false, NW, false, WholeRow, true>(
       a, S, kvh, b, a.q8 + q0 * 128, a.tpos + q0, sh_scores, pg_lds);
   report_slots(a, over, kvh == 0);
 }
@@ -168,6 +187,11 @@ __global__ __launch_bounds__(256) void k_acc_pv(SplitArgs sa) {
   split_pv_chunk<G, WholeRow, true>(sa, blockIdx.x, blockIdx.y, blockIdx.z);
 }
 
+// Bytes of the one block's scores where a row may need more than its LDS
+i64 one_block_bytes(int B, int S, int n_q, int G) {
+  const i64 spad = ((i64)S + 15) / 16 * 16;
+  return (i64)G * spad * 4 > DECODE_LDS_BYTES ? (i64)B * n_q * spad * 4 : 0;
+}
 // Slots that a launch is sized for: what a query sees, and the rest of the
 // pages at the ends of the two ranges and around two stretches of padding.
 int window_slots(int S, int window, int sinks) {
@@ -283,10 +307,10 @@ int detllm_attn_window_decode(const int8_t* q8, const int64_t* tpos, const int8_
     const dim3 grid(n_kv, B);
     const size_t dyn = (size_t)G * w.lds_slots * 4;
     switch (G) {
-      case 1: hipLaunchKernelGGL((k_window_decode<1, 8>), grid, dim3(512), dyn, s, w); break;
-      case 2: hipLaunchKernelGGL((k_window_decode<2, 8>), grid, dim3(512), dyn, s, w); break;
-      case 4: hipLaunchKernelGGL((k_window_decode<4, 8>), grid, dim3(512), dyn, s, w); break;
-      case 8: hipLaunchKernelGGL((k_window_decode<8, 8>), grid, dim3(512), dyn, s, w); break;
+      case 1: hipLaunchKernelGGL(k_window_decode<1>, grid, dim3(64 * NW), dyn, s, w); break;
+      case 2: hipLaunchKernelGGL(k_window_decode<2>, grid, dim3(64 * NW), dyn, s, w); break;
+      case 4: hipLaunchKernelGGL(k_window_decode<4>, grid, dim3(64 * NW), dyn, s, w); break;
+      case 8: hipLaunchKernelGGL(k_window_decode<8>, grid, dim3(64 * NW), dyn, s, w); break;
     }
   }
   DI_LAUNCH_CHECK();
@@ -301,7 +325,7 @@ int detllm_attn_decode_acc_work(int B, int S, int n_q, int n_kv, int64_t* bytes)
   if (B == 0 || S == 0) return DI_OK;
   const int chunk = decode_chunk(B, S, n_q, n_kv);
   i64 at;
-  *bytes = chunk ? split_bytes(B, S, n_q, chunk, &at) : one_block_bytes(B, S, n_q, n_q / n_kv);
+  if (chunk) *bytes = split_bytes(B, S, n_q, chunk, &at);
   return DI_OK;
 }
 
@@ -321,8 +345,8 @@ int detllm_attn_decode_acc(const int8_t* q8, const int64_t* tpos, const int8_t* 
   const int G = n_q / n_kv;
   const int chunk = S > 0 ? decode_chunk(B, S, n_q, n_kv) : 0;
   DecodeArgs d{q8, tpos, KVPages{(int8_t*)kpool, (int8_t*)vpool, table, width, n_kv}, valid,
-               out, need > 0 ? (int32_t*)work : nullptr, s_dev, S, n_q, n_kv, valid_stride, err,
-               nullptr, nullptr, acc, acc_stride};
+               out, nullptr, s_dev, S, n_q, n_kv, valid_stride, err, nullptr, nullptr, acc,
+               acc_stride};
   if (chunk) {
     const SplitArgs sa = split_args(d, B, chunk, work);
     const dim3 grid(n_kv, B, sa.ns);
@@ -341,18 +365,12 @@ int detllm_attn_decode_acc(const int8_t* q8, const int64_t* tpos, const int8_t* 
     }
   } else {
     const dim3 grid(n_kv, B);
-    const size_t dyn = d.scratch ? 0 : (size_t)G * (((i64)S + 15) / 16 * 16) * 4;
+    const size_t dyn = (size_t)G * (((i64)S + 15) / 16 * 16) * 4;
     switch (G) {
-#define DI_ACC_ONE(G_)                                                                        \
-  case G_:                                                                                    \
-    if (d.scratch) hipLaunchKernelGGL((k_acc_decode<G_, true, 8>), grid, dim3(512), dyn, s, d);  \
-    else hipLaunchKernelGGL((k_acc_decode<G_, false, 8>), grid, dim3(512), dyn, s, d);           \
-    break
-      DI_ACC_ONE(1);
-      DI_ACC_ONE(2);
-      DI_ACC_ONE(4);
-      DI_ACC_ONE(8);
-#undef DI_ACC_ONE
+      case 1: hipLaunchKernelGGL(k_acc_decode<1>, grid, dim3(64 * NW), dyn, s, d); break;
+      case 2: hipLaunchKernelGGL(k_acc_decode<2>, grid, dim3(64 * NW), dyn, s, d); break;
+      case 4: hipLaunchKernelGGL(k_acc_decode<4>, grid, dim3(64 * NW), dyn, s, d); break;
+      case 8: hipLaunchKernelGGL(k_acc_decode<8>, grid, dim3(64 * NW), dyn, s, d); break;
     }
   }
   DI_LAUNCH_CHECK();

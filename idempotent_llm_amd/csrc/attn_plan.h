@@ -11,12 +11,12 @@ namespace {
 //
 // Few pairs of (row, kv head) leave CUs idle, so long rows are cut; two launches
 // and a denominator that every chunk block sums over the whole row cost more the
-// more heads a kv head has. From 12288 / G slots on the one block's scores are
-// past its 48 KiB of LDS and the cut form is the better one at any number of
-// pairs, but at one head (32 x 8000 slots 113 / 123 us). us per call, one block /
+// more heads a kv head has. Past 12288 / G slots the one block's scores leave its
+// 48 KiB of LDS and every row is cut. us per call, one block /
 // cut (accumulating form, 8 kv heads):
 //   G = 1: 8 pairs 768 slots 11.0 / 10.2, 64 pairs 768 11.1 / 12.1, 1024 14.1 / 11.5,
-//     128 pairs 1536 19.0 / 19.3, 2048 23.5 / 22.5, 4096 44 / 33
+//     128 pairs 1536 19.0 / 19.3, 2048 23.5 / 22.5, 4096 44 / 33, 256 pairs 8000
+//     113 / 123
 //   G = 2: 8 pairs 768 12.0 / 12.9, 1024 13.7 / 13.0, 64 pairs 768 12.2 / 13.2,
 //     1024 15.1 / 14.1, 128 pairs 2048 24.9 / 26.1, 3000 33.3 / 32.6, 256 pairs
 //     8000 175 / 131
@@ -28,7 +28,7 @@ namespace {
 inline int decode_chunk(int B, int n, int n_q, int n_kv) {
   const int G = n_q / n_kv;
   const i64 pairs = (i64)B * n_kv;
-  int from = G == 1 && pairs > 128 ? INT32_MAX : 12288 / G + 1;
+  int from = 12288 / G + 1;
   if (G == 1) from = pairs <= 32 ? 768 : pairs <= 64 ? 960 : pairs <= 128 ? 1920 : from;
   if (G == 2) from = pairs <= 64 ? 960 : pairs <= 128 ? 2816 : from;
   if (G == 4) from = pairs <= 32 ? 1280 : pairs <= 64 ? 1664 : from;
@@ -44,10 +44,6 @@ inline i64 split_bytes(int B, int S, int n_q, int chunk, i64* cmax_at) {
   const i64 ns = ((i64)S + chunk - 1) / chunk, rows = (i64)B * n_q;
   *cmax_at = rows * ns * chunk * 4;
   return *cmax_at + (rows * ns * 4 + 15) / 16 * 16;
-}
-inline i64 one_block_bytes(int B, int S, int n_q, int G) {
-  const i64 spad = ((i64)S + 15) / 16 * 16;
-  return (i64)G * spad * 4 > DECODE_LDS_BYTES ? (i64)B * n_q * spad * 4 : 0;
 }
 inline int heads_ok(int n_q, int n_kv) {
   if (n_q <= 0 || n_kv <= 0 || n_q % n_kv) return DI_EINVAL;

@@ -21,6 +21,13 @@
 // in attn_prefill.h: S^T = K . Q^T, a lane holds one query (column qi = lane % 16)
 // and 16 slots (16 g + 4 blk + r, g = lane / 16) of a 64-slot tile.
 //
+// 64 rows behind 8192 slots, 200 of their own, 16 / 8 heads: 50 us (maxima 11,
+// sums 12, P.V of the prefix 16, the rest 12), 191 in the per-row form; the 46 MB
+// take 10 us and the products 2. What is left is the launches' own chains (the
+// first load, the parts' join and the block's end: 4 to 7 us each with one slot
+// per row), so fewer and larger parts or another number of blocks change
+// nothing: 256, 512 and 1024 blocks of maxima 11.0, 11.2, 11.3 us.
+//
 // Few rows or short prefixes do not pay for four launches and take
 // attention.hip's kernels, the prefix's pages looked up in row 0.
 
@@ -635,7 +642,7 @@ struct SharedView {
   }
   __device__ __forceinline__ bool sees(int) const { return true; }
 };
-template <int G, bool SCR>
+template <int G>
 __global__ __launch_bounds__(512) void k_shared_one(DecodeArgs a, int P) {
   keep_hidden_args();
   extern __shared__ __attribute__((aligned(16))) int32_t sh_scores[];
@@ -649,7 +656,7 @@ __global__ __launch_bounds__(512) void k_shared_one(DecodeArgs a, int P) {
   for (int i = threadIdx.x; i < npages; i += 512) pg_lds[i] = v.page(a.kv, b, i * DI_PAGE);
   if (npages == 0 && threadIdx.x == 0) pg_lds[0] = -1;  // S = 0: loads read page 0
   __syncthreads();
-  decode_body<G, VPRE, SCR, false, 8>(a, S, kvh, b, a.q8 + q0 * 128, a.tpos + q0, sh_scores, pg_lds);
+  decode_body<G, VPRE, false, false, 8>(a, S, kvh, b, a.q8 + q0 * 128, a.tpos + q0, sh_scores, pg_lds);
   report_slots(a, over, kvh == 0);
 }
 template <int G>
@@ -691,7 +698,7 @@ SharedPlan shared_plan(int B, int S, int P, int n_q, int n_kv) {
   if (!p.joint) {
     i64 at;
     p.split = B > 0 && S > 0 ? decode_chunk(B, S, n_q, n_kv) : 0;
-    p.bytes = p.split ? split_bytes(B, S, n_q, p.split, &at) : one_block_bytes(B, S, n_q, G);
+    p.bytes = p.split ? split_bytes(B, S, n_q, p.split, &at) : 0;
     return p;
   }
   p.ng = p.qw = M <= 16 ? 1 : M <= 32 ? 2 : 4;
@@ -747,8 +754,7 @@ int detllm_attn_decode_shared(const int8_t* q8, const int64_t* tpos, const int8_
   const int G = n_q / n_kv;
   const KVPages kv{(int8_t*)kpool, (int8_t*)vpool, table, width, n_kv};
   if (!p.joint) {
-    const DecodeArgs d{q8, tpos, kv, valid, out, p.bytes > 0 ? (int32_t*)work : nullptr, s_dev, S,
-                       n_q, n_kv, valid_stride, err};
+    const DecodeArgs d{q8, tpos, kv, valid, out, nullptr, s_dev, S, n_q, n_kv, valid_stride, err};
     if (p.split) {
       const SplitArgs sa = split_args(d, B, p.split, work);
       const dim3 grid(n_kv, B, sa.ns);
@@ -767,18 +773,12 @@ int detllm_attn_decode_shared(const int8_t* q8, const int64_t* tpos, const int8_
       }
     } else {
       const dim3 grid(n_kv, B);
-      const size_t dyn = d.scratch ? 0 : (size_t)G * (((i64)S + 15) / 16 * 16) * 4;
+      const size_t dyn = (size_t)G * (((i64)S + 15) / 16 * 16) * 4;
       switch (G) {
-#define DI_SHARED_ONE(G_)                                                                         \
-  case G_:                                                                                        \
-    if (d.scratch) hipLaunchKernelGGL((k_shared_one<G_, true>), grid, dim3(512), dyn, s, d, shared); \
-    else hipLaunchKernelGGL((k_shared_one<G_, false>), grid, dim3(512), dyn, s, d, shared);       \
-    break
-        DI_SHARED_ONE(1);
-        DI_SHARED_ONE(2);
-        DI_SHARED_ONE(4);
-        DI_SHARED_ONE(8);
-#undef DI_SHARED_ONE
+        case 1: hipLaunchKernelGGL(k_shared_one<1>, grid, dim3(512), dyn, s, d, shared); break;
+        case 2: hipLaunchKernelGGL(k_shared_one<2>, grid, dim3(512), dyn, s, d, shared); break;
+        case 4: hipLaunchKernelGGL(k_shared_one<4>, grid, dim3(512), dyn, s, d, shared); break;
+        case 8: hipLaunchKernelGGL(k_shared_one<8>, grid, dim3(512), dyn, s, d, shared); break;
       }
     }
     DI_LAUNCH_CHECK();

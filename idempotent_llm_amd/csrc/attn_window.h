@@ -12,7 +12,7 @@
 // pages it scans are then those of the two ranges that hold a valid slot: a row
 // whose window reaches back over padding does not scan the padding's pages (32
 // rows of 8000 slots, a window of 2048 behind prompts padded by up to 3000
-// slots: 110 -> @@ us).
+// slots: 110 us with them, 49 without, on four waves a block).
 #pragma once
 
 #include "common.h"

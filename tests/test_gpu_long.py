@@ -59,7 +59,10 @@ WINDOW_DECODE = {
     "long": (1, 4, 2, 5000, 2500, 4, dict(p_valid=0.98)),
     "long_gap": (2, 4, 2, 6000, 900, 4, dict(gaps=((0, 1000, 5600), (1, 3, 5990)))),
     "long_gap_split": (2, 4, 2, 9000, 2000, 4, dict(gaps=((0, 500, 8600), (1, 2500, 8000)))),
-    "scratch": (1, 8, 1, 8000, 300, 4, dict(gaps=((0, 200, 7900),))),
+    "long_gap_8": (1, 8, 1, 8000, 300, 4, dict(gaps=((0, 200, 7900),))),
+    "sparse_scratch": (2, 8, 1, 8000, 600, 4, dict(p_valid=0.08)),
+    "sparse_scratch_2": (3, 4, 2, 9000, 100, 4, dict(p_valid=0.01)),
+    "sparse_split": (1, 4, 2, 9000, 1500, 70, dict(p_valid=0.2)),
     "wide_tpos": (2, 4, 2, 400, 120, 4, dict(tpos=(0, 62), p_valid=0.8)),
     "wide_tpos_long": (1, 4, 2, 3000, 1500, 4, dict(tpos=(0, 62), p_valid=0.8)),
     "flat": (1, 2, 1, 4000, 3000, 4, dict(flat_heads=(0, 1), tpos=(38, 39))),
@@ -165,7 +168,8 @@ ACC_DECODE = {
     "group_8_long": (1, 8, 1, 2500, dict(p_valid=0.9)),
     "long": (1, 4, 2, 3333, dict(p_valid=0.9)),
     "many_rows_long": (33, 8, 4, 1300, dict(p_valid=0.9)),
-    "scratch": (17, 64, 8, 1700, dict(p_valid=0.9)),
+    "group_8_rows": (17, 64, 8, 1700, dict(p_valid=0.9)),
+    "group_1_rows": (130, 1, 1, 12300, dict(p_valid=0.9)),
     "dead_rows": (3, 2, 2, 300, dict(dead_rows=(0, 2))),
     "last_slot_dead": (2, 2, 1, 300, dict(gaps=((1, 290, 300),))),
     "wide_tpos": (2, 4, 2, 400, dict(tpos=(0, 40), p_valid=0.8)),
