@@ -280,6 +280,7 @@ struct CompactArgs {
   const int32_t* dst;    // [B][dst_width]
   const int32_t* keep;   // [B][budget] ascending, -1 behind
   int width, dst_width, budget, n_kv, n_pages;
+  int nseg, per;         // parts of dst's pages (one block each), pages of a part
 
   // page of row b's slot s, and the page for j of dst (-1: none, or not of the
   // pools)
@@ -298,8 +299,9 @@ struct CompactArgs {
 // earlier one: everything it held for later pages has been read, because the
 // reads of a page end before its writes begin (the barrier) and those of the
 // page after it come from places behind it.
-__device__ __forceinline__ void compact_k(const CompactArgs& a, const KVPages& kv, int h, int b) {
-  const int tid = threadIdx.x, npages = (a.budget + DI_PAGE - 1) / DI_PAGE;
+__device__ __forceinline__ void compact_k(const CompactArgs& a, const KVPages& kv, int h, int b,
+                                          int j0, int j1) {
+  const int tid = threadIdx.x;
   const int32_t* krow = a.keep + (i64)b * a.budget;
   int s[4];  // the next page's source slots of this thread's rows
   auto load_slots = [&](int j) {
@@ -320,13 +322,13 @@ __device__ __forceinline__ void compact_k(const CompactArgs& a, const KVPages& k
       if (pg[u] >= 0) r[u] = *(const v4i*)(kv.krow(pg[u], h, s[u] & (DI_PAGE - 1)) + (tid & 7) * 16);
     }
   };
-  load_slots(0);
+  load_slots(j0);
   load_rows(x);
-  if (npages > 1) load_slots(1);
-  for (int j = 0; j < npages; ++j) {
+  if (j0 + 1 < j1) load_slots(j0 + 1);
+  for (int j = j0; j < j1; ++j) {
     const int to = a.to(b, j);
-    if (j + 1 < npages) load_rows(y);
-    if (j + 2 < npages) load_slots(j + 2);
+    if (j + 1 < j1) load_rows(y);
+    if (j + 2 < j1) load_slots(j + 2);
 #pragma unroll
     for (int u = 0; u < 4; ++u) asm volatile("" ::"v"(x[u]));  // (this page's reads have ended)
     __syncthreads();
@@ -347,7 +349,8 @@ __device__ __forceinline__ void compact_k(const CompactArgs& a, const KVPages& k
 // registers and writes them when every source page of that page has passed. The
 // same order as in compact_k: a page is written when its last source page, and
 // all before it, are in LDS or behind.
-__device__ __forceinline__ void compact_v(const CompactArgs& a, const KVPages& kv, int h, int b) {
+__device__ __forceinline__ void compact_v(const CompactArgs& a, const KVPages& kv, int h, int b,
+                                          int j0, int j1) {
   __shared__ __attribute__((aligned(16))) int8_t src[KVC_PAGES][128 * DI_PAGE];
   __shared__ uint16_t list[KVC_MAXP];    // source pages with kept slots, ascending
   __shared__ int32_t start[KVC_MAXP + 1];  // the first kept slot from each
@@ -355,11 +358,12 @@ __device__ __forceinline__ void compact_v(const CompactArgs& a, const KVPages& k
   const int tid = threadIdx.x;
   const int32_t* krow = a.keep + (i64)b * a.budget;
   int np = 0, n = 0;  // listed pages, kept slots
-  for (int i0 = 0; i0 < a.budget; i0 += 256) {
+  const int ifirst = j0 * DI_PAGE, iend = ::min(j1 * DI_PAGE, a.budget);
+  for (int i0 = ifirst; i0 < iend; i0 += 256) {
     const int i = i0 + tid;
-    const int s = i < a.budget ? krow[i] : -1;
-    const int before_s = i > 0 && i < a.budget ? krow[i - 1] : -1;
-    const bool lead = s >= 0 && (i == 0 || s / DI_PAGE != before_s / DI_PAGE);
+    const int s = i < iend ? krow[i] : -1;
+    const int before_s = i > ifirst && i < iend ? krow[i - 1] : -1;
+    const bool lead = s >= 0 && (i == ifirst || s / DI_PAGE != before_s / DI_PAGE);
     int total;
     const int before = block_count_before<256>((lead ? 1 : 0) | (s >= 0 ? 0x10000 : 0), red, &total);
     const int at = np + (before & 0xFFFF);
@@ -370,7 +374,7 @@ __device__ __forceinline__ void compact_v(const CompactArgs& a, const KVPages& k
     np = ::min(np + (total & 0xFFFF), KVC_MAXP);
     n += total >> 16;
   }
-  if (tid == 0) start[np] = n;
+  if (tid == 0) start[np] = ifirst + n;
   __syncthreads();
   v4i pa[KVC_PAGES][4], pb[KVC_PAGES][4];
   auto load = [&](int p0, v4i (&x)[KVC_PAGES][4]) {
@@ -389,8 +393,7 @@ __device__ __forceinline__ void compact_v(const CompactArgs& a, const KVPages& k
   uint32_t x[16];
 #pragma unroll
   for (int u = 0; u < 16; ++u) x[u] = 0;
-  const int npages = (a.budget + DI_PAGE - 1) / DI_PAGE;
-  int j = 0;  // the page of dst being made, and this thread's source slots of it
+  int j = j0;  // the page of dst being made, and this thread's source slots of it
   int s4[4];
   auto load_slots = [&] {
 #pragma unroll
@@ -443,15 +446,35 @@ __device__ __forceinline__ void compact_v(const CompactArgs& a, const KVPages& k
     step(p0, pa);
     if (p0 + KVC_PAGES < np) step(p0 + KVC_PAGES, pb);
   }
-  while (j < npages) flush();
+  while (j < j1) flush();
 }
 
+// Where the (kv head, K or V, row, layer) blocks alone leave the card idle, dst's
+// pages are cut into parts, about four blocks per CU. That holds for rows whose
+// dst pages are none of their table's; where one is, the order above has to be
+// kept and the row's first block takes all parts. Kept of a row's slots, new pages
+// against its own: 150 of 400 (8 layers, 8 heads) 7.5 and 8.7 us, 2000 of 4000 (2
+// layers, 2 heads) 8.6 and 54, 20000 of 131000 (1 layer, 8 heads) 179 and 1332.
 __global__ __launch_bounds__(256) void k_kv_compact(CompactArgs a) {
   keep_hidden_args();
-  const int h = blockIdx.x >> 1, b = blockIdx.y;
+  const int seg = blockIdx.x / (2 * a.n_kv), hk = blockIdx.x % (2 * a.n_kv);
+  const int h = hk >> 1, b = blockIdx.y, npages = (a.budget + DI_PAGE - 1) / DI_PAGE;
   const KVPages kv{a.k[blockIdx.z], a.v[blockIdx.z], a.table, a.width, a.n_kv};
-  if (blockIdx.x & 1) compact_v(a, kv, h, b);
-  else compact_k(a, kv, h, b);
+  int j0 = seg * a.per, j1 = ::min(j0 + a.per, npages);
+  if (a.nseg > 1) {  // block-uniform
+    bool hit = false;
+    const int nd = ::min(a.dst_width, npages);
+    for (int t = threadIdx.x; t < a.width; t += 256) {
+      const int x = a.table[(i64)b * a.width + t];
+      for (int j = 0; j < nd; ++j) hit |= x >= 0 && a.dst[(i64)b * a.dst_width + j] == x;
+    }
+    if (__syncthreads_or(hit)) {
+      if (seg > 0) return;
+      j1 = npages;
+    }
+  }
+  if (hk & 1) compact_v(a, kv, h, b, j0, j1);
+  else compact_k(a, kv, h, b, j0, j1);
 }
 
 constexpr int SEL_FUSED = 16 * SEL_NT;  // slots per row whose keys fit registers
@@ -502,7 +525,8 @@ int detllm_kv_compact(int8_t* const* kpools, int8_t* const* vpools, int n_layers
     return DI_EINVAL;
   if (B <= 0 || n_layers == 0 || dst_width == 0 || budget == 0) return DI_OK;
   if (!kpools || !vpools || !table || !dst || !keep) return DI_EINVAL;
-  if (B > 65535 || n_kv > (1 << 20) || width > KVC_MAXP) return DI_ERANGE;
+  if (B > 65535 || n_kv > (1 << 20) || width > KVC_MAXP || budget > KVC_MAXP * DI_PAGE)
+    return DI_ERANGE;
   for (int l = 0; l < n_layers; ++l)
     if (!kpools[l] || !vpools[l]) return DI_EINVAL;
   for (int l0 = 0; l0 < n_layers; l0 += KVC_LAYERS) {
@@ -515,7 +539,10 @@ int detllm_kv_compact(int8_t* const* kpools, int8_t* const* vpools, int n_layers
     a.table = table; a.dst = dst; a.keep = keep;
     a.width = width; a.dst_width = dst_width; a.budget = budget; a.n_kv = n_kv;
     a.n_pages = n_pages;
-    hipLaunchKernelGGL(k_kv_compact, dim3(2 * n_kv, B, n), dim3(256), 0, s, a);
+    const i64 blocks = 2 * (i64)n_kv * B * n, npages = ((i64)budget + DI_PAGE - 1) / DI_PAGE;
+    a.per = (int)imax(npages * blocks / 1024, 1);
+    a.nseg = (int)((npages + a.per - 1) / a.per);
+    hipLaunchKernelGGL(k_kv_compact, dim3((unsigned)(2 * n_kv * a.nseg), B, n), dim3(256), 0, s, a);
   }
   DI_LAUNCH_CHECK();
   return DI_OK;

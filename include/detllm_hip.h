@@ -438,8 +438,7 @@ int detllm_kv_select(const int64_t* acc, int64_t acc_stride, const uint8_t* vali
  * past row b's last kept one, and those of kept slots whose page is not mapped,
  * become 0. kpools / vpools: HOST arrays of n_layers device pointers, all
  * different, of n_pages pages each (a page id past them counts as -1); width at
- * most 1024. keep as
- * detllm_kv_select writes it. The page dst[b][j] may be one of row b's pages
+ * most 1024, budget at most 131072. keep as detllm_kv_select writes it. The page dst[b][j] may be one of row b's pages
  * table[b][0..j]; otherwise no page of dst is in table, and none is in dst
  * twice. */
 int detllm_kv_compact(int8_t* const* kpools, int8_t* const* vpools, int n_layers, int n_pages,

@@ -346,6 +346,35 @@ def test_compact(name, in_place):
         assert torch.equal(kp[others], k0[others]) and torch.equal(vp[others], v0[others])
 
 
+@pytest.mark.parametrize("n_kv, layers, S, budget", [(2, 1, 2000, 900), (8, 2, 4300, 3000)])
+def test_compact_mixed_rows(n_kv, layers, S, budget):
+    """Rows of one call whose pages are their own, their own behind a new one,
+    new, and their own but for the first."""
+    print(f"[compact mixed {n_kv} {layers} {S} {budget}]", flush=True)
+    B, rng, wb = 4, np.random.default_rng(budget), -(-budget // PAGE)
+    keep = np.stack([np.sort(rng.choice(S, budget, replace=False)) for _ in range(B)])
+    keep[3, budget // 2:] = -1
+    keep = keep.astype(np.int32)
+    kps, vps, want = [], [], []
+    for i in range(layers):
+        kc = rng.integers(-128, 128, (B, n_kv, S, 128), dtype=np.int8)
+        vc = rng.integers(-128, 128, (B, n_kv, 128, S), dtype=np.int8)
+        kp, vp, table, w = paged(kc, vc, seed=3)
+        extra = torch.full((B * wb,) + kp.shape[1:], 77, dtype=torch.int8, device="cuda")
+        kps.append(torch.cat([kp, extra]))
+        vps.append(torch.cat([vp, extra]))
+        want.append(_compacted(kc, vc, keep))
+    dst = torch.arange(B * w, B * (w + wb), dtype=torch.int32, device="cuda").view(B, wb)
+    dst[0] = table[0, :wb]
+    dst[1, 1:] = table[1, :wb - 1]
+    dst[3, 1:] = table[3, 1:wb]
+    _ops().kv_compact(kps, vps, table, dst, torch.from_numpy(keep).cuda())
+    for (k, v), kp, vp in zip(want, kps, vps):
+        got_k, got_v = unpaged(kp, vp, dst, wb * PAGE)
+        _eq(got_k, k)
+        _eq(got_v, v)
+
+
 def test_compact_skips_unmapped_pages():
     """dst -1: nothing is written; a kept slot whose page is not mapped
     becomes 0."""

@@ -124,9 +124,9 @@ def test_evicted_cache_answers_as_a_masked_one(model, lens, budget, recent, sink
         mask = torch.zeros_like(full.valid_buf)
         for b in range(B):
             mask[b, full_slots[b][full_slots[b] >= 0]] = True
-        pages = cut.n_pages
+        pool = cut.k_pools[0].data_ptr()
         cut.evict(budget, recent, sinks)
-        assert cut.length == budget and cut.n_pages == pages
+        assert cut.length == budget and cut.k_pools[0].data_ptr() == pool
         assert torch.equal(cut.valid, keep >= 0) and torch.equal(cut.acc[:, :, :budget], kept)
         used = cut._table_host[cut._table_host >= 0]
         assert len(set(used.tolist())) == used.size and not set(used.tolist()) & set(cut._free)
