@@ -464,9 +464,9 @@ __global__ __launch_bounds__(256, 2) void k_shared_pv(SharedArgs a) {
   const v4i ones = v4i{0x01010101, 0x01010101, 0x01010101, 0x01010101};
   for (int i = 0; i < np; ++i) {
     const bool mapped = __builtin_amdgcn_readlane(pgv, i) >= 0;
-    // this wave's loads of the page are done; after the barrier every wave's are,
-    // and the other stage is free
-    wait_vmcnt<0>();
+    // this wave's loads of the page are done and its LDS reads of the last one;
+    // after the barrier every wave's are, and the other stage is free
+    __builtin_amdgcn_s_waitcnt(0);
     __builtin_amdgcn_s_barrier();
     if (i + 1 < np) issue(i + 1);
     const int8_t* stg = ring + (i & 1) * STAGE;
