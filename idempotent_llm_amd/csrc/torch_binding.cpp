@@ -692,13 +692,14 @@ void op_kv_compact(at::TensorList kpools, at::TensorList vpools, const Tensor& t
                op, "expected contiguous int8 pools [pages, n_kv, 128, 128] on ", table.device());
       (t == &kpools[i] ? k : v).push_back(ptr<int8_t>(*t));
     }
-  for (const auto* pools : {&k, &v})
-    DI_CHECK(std::set<int8_t*>(pools->begin(), pools->end()).size() == pools->size(), op,
-             "a pool is given twice");
-  for (const int8_t* p : v)
-    DI_CHECK(std::find(k.begin(), k.end(), p) == k.end(), op, "a pool is given twice");
-  DI_CHECK(table.size(1) > 0 && table.size(1) <= 1024 && dst.size(1) * 128 >= keep.size(1), op, keep.size(1),
-           " slots for ", dst.size(1), " pages");
+  std::vector<int8_t*> all(k);
+  all.insert(all.end(), v.begin(), v.end());
+  std::sort(all.begin(), all.end());
+  for (size_t i = 1; i < all.size(); ++i)
+    DI_CHECK(all[i] - all[i - 1] >= kpools[0].numel(), op, "a pool is given twice, or two overlap");
+  DI_CHECK(table.size(1) > 0 && table.size(1) <= 1024 && keep.size(1) <= 1024 * 128 &&
+               dst.size(1) * 128 >= keep.size(1),
+           op, keep.size(1), " slots for ", dst.size(1), " pages, a table of ", table.size(1));
   const c10::DeviceGuard guard(table.device());
   DI_RUN(detllm_kv_compact, k.data(), v.data(), (int)k.size(), as_i32(kpools[0].size(0)),
          ptr<int32_t>(table),

@@ -133,7 +133,7 @@ def test_compact_refuses():
     pool = lambda *s: torch.zeros(*(s or (6, 2, 128, 128)), dtype=I8)
     table, dst = torch.zeros(2, 3, dtype=I32), torch.zeros(2, 2, dtype=I32)
     keep = torch.zeros(2, 200, dtype=I32)
-    same = pool()
+    same, wide = pool(), pool(9, 2, 128, 128)
     bad = [([], [], table, dst, keep), ([pool()], [pool(), pool()], table, dst, keep),
            ([pool()], [pool(5, 2, 128, 128)], table, dst, keep),
            ([pool(), pool(5, 2, 128, 128)], [pool(), pool()], table, dst, keep),
@@ -146,7 +146,11 @@ def test_compact_refuses():
            ([pool()], [pool()], table, dst, keep.long()),
            ([pool()], [pool()], table[:, :0].contiguous(), dst, keep),
            ([same, pool()], [pool(), same], table, dst, keep), ([same], [same], table, dst, keep),
-           ([same, same], [pool(), pool()], table, dst, keep)]
+           ([same, same], [pool(), pool()], table, dst, keep),
+           ([wide[:6]], [wide[3:]], table, dst, keep),
+           ([pool()], [pool()], torch.zeros(2, 1025, dtype=I32), dst, keep),
+           ([pool()], [pool()], table, torch.zeros(2, 1025, dtype=I32),
+            torch.zeros(2, 131073, dtype=I32))]
     for args in bad:
         with pytest.raises(ValueError, match="kv_compact|dimensions"):
             _call("kv_compact", *args)
@@ -188,6 +192,10 @@ def test_entry_error_codes():
     with pytest.raises(RuntimeError, match="code -22"):
         e["detllm_kv_compact"](0, ctypes.addressof(pools), ctypes.addressof(pools), 1, 6, t, 3, t,
                                2, t, 2, 100, 2)
+    for width, budget in ((1025, 100), (3, 131073)):
+        with pytest.raises(RuntimeError, match="code -34"):
+            e["detllm_kv_compact"](0, ctypes.addressof(pools), ctypes.addressof(pools), 1, 6, t,
+                                   width, t, 2, t, 2, budget, 2)
 
 
 def test_scratch_sizes_cover_every_shape():
