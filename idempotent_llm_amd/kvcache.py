@@ -29,7 +29,8 @@ For long contexts (no counterpart in the reference):
   layer and returns the other pages. Positions are the caller's, so decoding
   goes on where it was;
 * ``fork(rows)`` makes a one-row cache one of ``rows`` rows that share its full
-  pages (``shared`` slots); decode attention reads these once for the batch.
+  pages (``shared`` slots); decode attention reads these once for the batch
+  where that pays and the cache does not track its weights.
 """
 
 from __future__ import annotations
