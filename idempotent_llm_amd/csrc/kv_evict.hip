@@ -272,13 +272,14 @@ __global__ __launch_bounds__(SEL_NT) void k_kv_select(SelectArgs a) {
 constexpr int KVC_LAYERS = 32;  // layers per launch (pool pointers by value)
 constexpr int KVC_PAGES = 2;    // source pages of V in LDS at once
 constexpr int KVC_MAXP = 1024;  // pages of V listed at once
+constexpr int KVC_MAXDST = 1 << 23;  // pages of dst (their slots are numbered in 32 bits)
 
 struct CompactArgs {
   int8_t* k[KVC_LAYERS];
   int8_t* v[KVC_LAYERS];
   const int32_t* table;  // [B][width]
   const int32_t* dst;    // [B][dst_width]
-  const int32_t* keep;   // [B][budget] ascending, -1 behind
+  const int32_t* keep;   // [B][budget] ascending, -1 behind (budget 0: any address)
   int width, dst_width, budget, n_kv, n_pages;
   int nseg, per;         // parts of dst's pages (one block each), pages of a part
 
@@ -397,7 +398,7 @@ __device__ __forceinline__ void compact_v(const CompactArgs& a, const KVPages& k
   int s4[4];
   auto load_slots = [&] {
 #pragma unroll
-    for (int r = 0; r < 4; ++r) s4[r] = krow[::min(j * DI_PAGE + i4 + r, a.budget - 1)];
+    for (int r = 0; r < 4; ++r) s4[r] = krow[::max(::min(j * DI_PAGE + i4 + r, a.budget - 1), 0)];
   };
   load_slots();
   auto flush = [&] {
@@ -458,15 +459,14 @@ __device__ __forceinline__ void compact_v(const CompactArgs& a, const KVPages& k
 __global__ __launch_bounds__(256) void k_kv_compact(CompactArgs a) {
   keep_hidden_args();
   const int seg = blockIdx.x / (2 * a.n_kv), hk = blockIdx.x % (2 * a.n_kv);
-  const int h = hk >> 1, b = blockIdx.y, npages = (a.budget + DI_PAGE - 1) / DI_PAGE;
+  const int h = hk >> 1, b = blockIdx.y, npages = a.dst_width;  // (zeros past the budget)
   const KVPages kv{a.k[blockIdx.z], a.v[blockIdx.z], a.table, a.width, a.n_kv};
   int j0 = seg * a.per, j1 = ::min(j0 + a.per, npages);
   if (a.nseg > 1) {  // block-uniform
     bool hit = false;
-    const int nd = ::min(a.dst_width, npages);
     for (int t = threadIdx.x; t < a.width; t += 256) {
       const int x = a.table[(i64)b * a.width + t];
-      for (int j = 0; j < nd; ++j) hit |= x >= 0 && a.dst[(i64)b * a.dst_width + j] == x;
+      for (int j = 0; j < npages; ++j) hit |= x >= 0 && a.dst[(i64)b * a.dst_width + j] == x;
     }
     if (__syncthreads_or(hit)) {
       if (seg > 0) return;
@@ -523,9 +523,10 @@ int detllm_kv_compact(int8_t* const* kpools, int8_t* const* vpools, int n_layers
                       const int32_t* keep, int B, int budget, int n_kv, hipStream_t s) {
   if (n_layers < 0 || n_pages < 1 || width < 1 || dst_width < 0 || budget < 0 || n_kv < 1)
     return DI_EINVAL;
-  if (B <= 0 || n_layers == 0 || dst_width == 0 || budget == 0) return DI_OK;
-  if (!kpools || !vpools || !table || !dst || !keep) return DI_EINVAL;
-  if (B > 65535 || n_kv > (1 << 20) || width > KVC_MAXP || budget > KVC_MAXP * DI_PAGE)
+  if (B <= 0 || n_layers == 0 || dst_width == 0) return DI_OK;
+  if (!kpools || !vpools || !table || !dst || (!keep && budget > 0)) return DI_EINVAL;
+  if (B > 65535 || n_kv > (1 << 20) || width > KVC_MAXP || budget > KVC_MAXP * DI_PAGE ||
+      dst_width > KVC_MAXDST)
     return DI_ERANGE;
   for (int l = 0; l < n_layers; ++l)
     if (!kpools[l] || !vpools[l]) return DI_EINVAL;
@@ -536,11 +537,11 @@ int detllm_kv_compact(int8_t* const* kpools, int8_t* const* vpools, int n_layers
       a.k[l] = kpools[l0 + l];
       a.v[l] = vpools[l0 + l];
     }
-    a.table = table; a.dst = dst; a.keep = keep;
+    a.table = table; a.dst = dst; a.keep = budget > 0 ? keep : dst;
     a.width = width; a.dst_width = dst_width; a.budget = budget; a.n_kv = n_kv;
     a.n_pages = n_pages;
-    const i64 blocks = 2 * (i64)n_kv * B * n, npages = ((i64)budget + DI_PAGE - 1) / DI_PAGE;
-    a.per = (int)imax(npages * blocks / 1024, 1);
+    const i64 blocks = 2 * (i64)n_kv * B * n, npages = dst_width;
+    a.per = (int)imin(imax(npages * blocks / 1024, 1), npages);
     a.nseg = (int)((npages + a.per - 1) / a.per);
     hipLaunchKernelGGL(k_kv_compact, dim3((unsigned)(2 * n_kv * a.nseg), B, n), dim3(256), 0, s, a);
   }

@@ -698,7 +698,7 @@ void op_kv_compact(at::TensorList kpools, at::TensorList vpools, const Tensor& t
   for (size_t i = 1; i < all.size(); ++i)
     DI_CHECK(all[i] - all[i - 1] >= kpools[0].numel(), op, "a pool is given twice, or two overlap");
   DI_CHECK(table.size(1) > 0 && table.size(1) <= 1024 && keep.size(1) <= 1024 * 128 &&
-               dst.size(1) * 128 >= keep.size(1),
+               dst.size(1) * 128 >= keep.size(1) && dst.size(1) <= (1 << 23),
            op, keep.size(1), " slots for ", dst.size(1), " pages, a table of ", table.size(1));
   const c10::DeviceGuard guard(table.device());
   DI_RUN(detllm_kv_compact, k.data(), v.data(), (int)k.size(), as_i32(kpools[0].size(0)),

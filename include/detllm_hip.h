@@ -435,12 +435,13 @@ int detllm_kv_select(const int64_t* acc, int64_t acc_stride, const uint8_t* vali
 
 /* detllm_kv_compact: slot keep[b][i] of every layer's K and V copied to slot i
  * of the pages dst [B][dst_width] (-1: not written); the slots of these pages
- * past row b's last kept one, and those of kept slots whose page is not mapped,
- * become 0. kpools / vpools: HOST arrays of n_layers device pointers, all
- * different, of n_pages pages each (a page id past them counts as -1); width at
- * most 1024, budget at most 131072. keep as detllm_kv_select writes it. The page dst[b][j] may be one of row b's pages
- * table[b][0..j]; otherwise no page of dst is in table, and none is in dst
- * twice. */
+ * past row b's last kept one (whole pages past the budget among them), and those
+ * of kept slots whose page is not mapped, become 0. kpools / vpools: HOST arrays
+ * of n_layers device pointers, all different, of n_pages pages each (a page id
+ * past them counts as -1); width at most 1024, budget at most 131072, dst_width
+ * at most 2^23. keep as detllm_kv_select writes it. The page dst[b][j] may be one
+ * of row b's pages table[b][0..j]; otherwise no page of dst is in table, and none
+ * is in dst twice. */
 int detllm_kv_compact(int8_t* const* kpools, int8_t* const* vpools, int n_layers, int n_pages,
                       const int32_t* table, int width, const int32_t* dst, int dst_width,
                       const int32_t* keep, int B, int budget, int n_kv, hipStream_t s);

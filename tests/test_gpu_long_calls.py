@@ -1,0 +1,64 @@
+"""GPU checks of calls that the long-cache operators' contracts allow beside
+the ordinary ones of test_gpu_long.py. Integer arithmetic: exact equality."""
+
+import numpy as np
+import pytest
+import torch
+
+from pagedcache import PAGE, paged, unpaged
+
+pytestmark = pytest.mark.gpu
+I64 = torch.int64
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _need_gpu():
+    if not torch.cuda.is_available():
+        pytest.skip("needs a GPU")
+    from idempotent_llm_amd import _lib, torch_ops  # noqa: F401
+    _lib.load()
+
+
+def _ops():
+    return torch.ops.detllm_rocm
+
+
+# B, n_kv, slots, kept (the budget), pages of dst
+WIDER = {
+    "one_more": (2, 2, 300, 100, 2),
+    "whole_page": (1, 1, 300, 128, 2),
+    "many": (3, 2, 900, 200, 7),
+    "all_zero": (2, 1, 300, 0, 2),
+    "parts": (1, 1, 5000, 3000, 40),
+}
+
+
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("name", list(WIDER))
+def test_compact_to_more_pages_than_the_budget(name, in_place):
+    """Pages of dst behind the budget's become 0 like the slots behind the
+    last kept one."""
+    B, n_kv, S, budget, wide = WIDER[name]
+    print(f"[compact wider {name} in_place={in_place}]", flush=True)
+    rng = np.random.default_rng(wide)
+    kc = rng.integers(-128, 128, (B, n_kv, S, 128), dtype=np.int8)
+    vc = rng.integers(-128, 128, (B, n_kv, 128, S), dtype=np.int8)
+    kp, vp, table, w = paged(kc, vc, seed=5)
+    keep = np.stack([np.sort(rng.choice(S, budget, replace=False)) for _ in range(B)])
+    keep = keep.astype(np.int32)
+    fresh = torch.arange(B * w, B * (w + wide), dtype=torch.int32, device="cuda").view(B, wide)
+    dst = fresh.clone()
+    if in_place:
+        dst[:, :min(w, wide)] = table[:, :min(w, wide)]
+    kp, vp = (torch.cat([x, torch.full((B * wide,) + x.shape[1:], 77, dtype=torch.int8,
+                                       device="cuda")]) for x in (kp, vp))
+    before = kp.clone(), vp.clone()
+    _ops().kv_compact([kp], [vp], table, dst, torch.from_numpy(keep).cuda())
+    k, v = (x.cpu().numpy() for x in unpaged(kp, vp, dst, wide * PAGE))
+    for b in range(B):
+        assert np.array_equal(k[b, :, :budget], kc[b][:, keep[b]])
+        assert np.array_equal(v[b, :, :budget], vc[b].transpose(0, 2, 1)[:, keep[b]])
+    assert not k[:, :, budget:].any() and not v[:, :, budget:].any()
+    others = torch.ones(kp.shape[0], dtype=torch.bool, device="cuda")
+    others[dst.reshape(-1).long()] = False
+    assert torch.equal(kp[others], before[0][others]) and torch.equal(vp[others], before[1][others])
