@@ -253,15 +253,16 @@ __global__ __launch_bounds__(SEL_NT) void k_kv_select(SelectArgs a) {
   kept_each([&](int) { ++c; });
   int place = block_count_before<SEL_NT>(c, red, &total);
   kept_each([&](int s) { krow[place++] = s; });
-  for (int i = total + tid; i < a.budget; i += SEL_NT) krow[i] = -1;
+  // (unsigned: a budget near 2^31 plus a step of SEL_NT passes an int)
+  for (uint32_t i = total + tid; i < (uint32_t)a.budget; i += SEL_NT) krow[i] = -1;
   __syncthreads();
-  for (int p = tid; p < a.budget; p += SEL_NT) {
-    const int s = p < total ? krow[p] : 0;
+  for (uint32_t p = tid; p < (uint32_t)a.budget; p += SEL_NT) {
+    const int s = p < (uint32_t)total ? krow[p] : 0;
     const int64_t* from = a.acc + (i64)b * a.n_kv * a.acc_stride + s;
     int64_t* to = a.kept + (i64)b * a.n_kv * a.budget + p;
 #pragma unroll 8
     for (int h = 0; h < a.n_kv; ++h)
-      to[(i64)h * a.budget] = p < total ? from[(i64)h * a.acc_stride] : 0;
+      to[(i64)h * a.budget] = p < (uint32_t)total ? from[(i64)h * a.acc_stride] : 0;
   }
 }
 

@@ -62,3 +62,19 @@ def test_compact_to_more_pages_than_the_budget(name, in_place):
     others = torch.ones(kp.shape[0], dtype=torch.bool, device="cuda")
     others[dst.reshape(-1).long()] = False
     assert torch.equal(kp[others], before[0][others]) and torch.equal(vp[others], before[1][others])
+
+
+def test_select_with_the_largest_budget():
+    """2^31 - 2 places for 300 slots: everything stays, -1 and 0 behind it."""
+    print("[select largest budget]", flush=True)
+    S, budget = 300, 2**31 - 2
+    acc = torch.arange(1, S + 1, dtype=I64, device="cuda").view(1, 1, S)
+    valid = torch.arange(S, device="cuda")[None] % 3 != 1
+    live = valid[0].nonzero()[:, 0]
+    n = len(live)
+    keep, kept = _ops().kv_select(acc, valid, S, budget, 0, 0)
+    torch.cuda.synchronize()
+    assert keep.shape == (1, budget) and kept.shape == (1, 1, budget)
+    assert torch.equal(keep[0, :n].long(), live) and torch.equal(kept[0, 0, :n], acc[0, 0, live])
+    assert int(keep[0, n:].max()) == -1 and int(keep[0, n:].min()) == -1
+    assert int(kept[0, 0, n:].max()) == 0 and int(kept[0, 0, n:].min()) == 0
