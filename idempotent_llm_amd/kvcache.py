@@ -260,7 +260,10 @@ class KVCache:
         if len(fresh):
             dst[fresh[:, 0], fresh[:, 1]] = self._take_pages(len(fresh))
         dst_dev = torch.from_numpy(dst).to(self._dims[3])
-        ops.kv_compact(self.k_pools, self.v_pools, self.table, dst_dev, keep)
+        # (the columns that hold the slots: a table grown by doubling may have more
+        # than kv_compact's 1024)
+        table = self.table[:, :-(-self.length // PAGE)].contiguous()
+        ops.kv_compact(self.k_pools, self.v_pools, table, dst_dev, keep)
         self._free += [int(i) for i in np.setdiff1d(ids, dst)][::-1]
         host[:] = -1
         host[:, :wb] = dst

@@ -1,6 +1,8 @@
 """GPU checks of calls that the long-cache operators' contracts allow beside
 the ordinary ones of test_gpu_long.py. Integer arithmetic: exact equality."""
 
+from types import SimpleNamespace
+
 import numpy as np
 import pytest
 import torch
@@ -78,3 +80,29 @@ def test_select_with_the_largest_budget():
     assert torch.equal(keep[0, :n].long(), live) and torch.equal(kept[0, 0, :n], acc[0, 0, live])
     assert int(keep[0, n:].max()) == -1 and int(keep[0, n:].min()) == -1
     assert int(kept[0, 0, n:].max()) == 0 and int(kept[0, 0, n:].min()) == 0
+
+
+@pytest.mark.parametrize("slots,pages", [((70000, 70100), 1094), ((131071,), 1024),
+                                         ((66000, 66049), 1032)])
+def test_evict_of_long_caches(slots, pages):
+    """Caches whose table doubled past 1024 pages, and the longest one."""
+    from idempotent_llm_amd.kvcache import KVCache
+    print(f"[evict long {slots}]", flush=True)
+    model = SimpleNamespace(n_layers=2, n_kv=1, hd=128, device=torch.device("cuda"))
+    c = KVCache().track_weights()
+    for n in slots:
+        c.reserve(model, 2, n)
+    S = c.length = slots[-1]
+    assert c.width == pages
+    g = torch.Generator(device="cuda").manual_seed(S)
+    for pool in c.k_pools + c.v_pools:
+        pool.copy_(torch.randint(-128, 128, pool.shape, dtype=torch.int8, device="cuda",
+                                 generator=g))
+    c.valid_buf[:, :S] = torch.rand(2, S, device="cuda", generator=g) < 0.9
+    c.acc[:, :, :S] = torch.randint(0, 1 << 40, (2, 1, S), device="cuda", generator=g)
+    keep, kept = _ops().kv_select(c.acc, c.valid_buf, S, 900, 50, 4)
+    at = keep.long()[:, None, :, None].expand(2, 1, 900, 128)
+    want = [x.gather(2, at) for x in c.k8 + c.v8]
+    c.evict(900, 50, 4)
+    assert c.length == 900 and bool(c.valid.all()) and torch.equal(c.acc[:, :, :900], kept)
+    assert all(torch.equal(x, y) for x, y in zip(c.k8 + c.v8, want))
