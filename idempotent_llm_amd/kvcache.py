@@ -35,6 +35,8 @@ For long contexts (no counterpart in the reference):
 
 from __future__ import annotations
 
+from contextlib import contextmanager
+
 import numpy as np
 import torch
 
@@ -166,12 +168,21 @@ class KVCache:
 
     def _take_pages(self, n: int) -> np.ndarray:
         """Ids of n pages of the pool: those handed back first, then new ones."""
-        old = [self._free.pop() for _ in range(min(n, len(self._free)))]
-        new = n - len(old)
-        self._ensure_pool(self.n_pages + new)
+        new = max(0, n - len(self._free))
+        self._ensure_pool(self.n_pages + new)      # (may raise: before any page is taken)
+        old = [self._free.pop() for _ in range(n - new)]
         ids = np.arange(self.n_pages, self.n_pages + new, dtype=np.int32)
         self.n_pages += new
         return np.concatenate([np.array(old, dtype=np.int32), ids])
+
+    @contextmanager
+    def _pages_as_before_if_it_raises(self):
+        free, n_pages = list(self._free), self.n_pages
+        try:
+            yield
+        except BaseException:
+            self._free, self.n_pages = free, n_pages
+            raise
 
     def check_rows(self, B: int):
         """Raise CacheRowsMismatch unless the cache is empty or holds B rows."""
@@ -257,19 +268,21 @@ class KVCache:
         dst = host[:, :wb].copy()
         spare = len(self._free) + self.k_pools[0].shape[0] - self.n_pages
         fresh = np.argwhere(np.isin(dst, ids[n > 1]) | (spare >= dst.size))
-        if len(fresh):
-            dst[fresh[:, 0], fresh[:, 1]] = self._take_pages(len(fresh))
-        dst_dev = torch.from_numpy(dst).to(self._dims[3])
-        # (the columns that hold the slots: a table grown by doubling may have more
-        # than kv_compact's 1024)
-        table = self.table[:, :-(-self.length // PAGE)].contiguous()
-        ops.kv_compact(self.k_pools, self.v_pools, table, dst_dev, keep)
+        with self._pages_as_before_if_it_raises():
+            if len(fresh):
+                dst[fresh[:, 0], fresh[:, 1]] = self._take_pages(len(fresh))
+            dst_dev = torch.from_numpy(dst).to(self._dims[3])
+            there = keep >= 0
+            # (the columns that hold the slots: a table grown by doubling may have
+            # more than kv_compact's 1024)
+            table = self.table[:, :-(-self.length // PAGE)].contiguous()
+            ops.kv_compact(self.k_pools, self.v_pools, table, dst_dev, keep)
         self._free += [int(i) for i in np.setdiff1d(ids, dst)][::-1]
         host[:] = -1
         host[:, :wb] = dst
         self.table.copy_(torch.from_numpy(host))
         self.valid_buf.zero_()
-        self.valid_buf[:, :budget] = keep >= 0
+        self.valid_buf[:, :budget] = there
         self.acc.zero_()
         self.acc[:, :, :budget] = kept
         self.length, self.mapped, self.shared = budget, wb * PAGE, 0
@@ -284,21 +297,21 @@ class KVCache:
         full, part = self.length // PAGE, self.length % PAGE
         row = self._table_host[0]
         begun = int(row[full]) if part else -1
-        self._free += [int(i) for i in row[full + (1 if part else 0):] if i >= 0]
         host = np.full((rows, self.width), -1, dtype=np.int32)
         host[:, :full] = row[:full]
-        if part:
-            host[0, full] = begun
-            host[1:, full] = self._take_pages(rows - 1)
-            to = torch.from_numpy(host[1:, full].copy()).to(self._dims[3]).long()
-            for kp, vp in zip(self.k_pools, self.v_pools):
-                kp[to] = kp[begun].clone()
-                vp[to] = vp[begun].clone()
-        self._table_host = host
-        self.table = torch.from_numpy(host).to(self._dims[3])
-        self.valid_buf = self.valid_buf.repeat(rows, 1)
-        if self.acc is not None:
-            self.acc = self.acc.repeat(rows, 1, 1)
+        with self._pages_as_before_if_it_raises():
+            self._free += [int(i) for i in row[full + (1 if part else 0):] if i >= 0]
+            if part:
+                host[0, full] = begun
+                host[1:, full] = self._take_pages(rows - 1)
+                to = torch.from_numpy(host[1:, full].copy()).to(self._dims[3]).long()
+                for kp, vp in zip(self.k_pools, self.v_pools):
+                    kp[to] = kp[begun].clone()
+                    vp[to] = vp[begun].clone()
+            table = torch.from_numpy(host).to(self._dims[3])
+            valid = self.valid_buf.repeat(rows, 1)
+            acc = None if self.acc is None else self.acc.repeat(rows, 1, 1)
+        self._table_host, self.table, self.valid_buf, self.acc = host, table, valid, acc
         self.mapped, self.shared = (full + (1 if part else 0)) * PAGE, full * PAGE
         return self
 

@@ -70,3 +70,74 @@ def test_evict_of_a_table_past_1024_pages(eviction):
     c.evict(500, 10, 4)
     assert torch.equal(eviction[0], table[:, :548]) and c.length == 500
     assert (c._table_host[:, :4] >= 0).all() and (c._table_host[:, 4:] == -1).all()
+
+
+def _books(c):
+    return sorted(c._free), c.n_pages, c._table_host.tolist(), c.table.tolist(), c.length, c.shared
+
+
+def test_a_failed_eviction_keeps_its_pages(eviction, monkeypatch):
+    """Pages taken for a move that is refused are not lost, whether they were
+    free ones or new, and the cache evicts once the cause is gone."""
+    for free in ((), (0, 3)):
+        c = _tracked(1000, 1100)
+        c._free += [c.n_pages + i for i in range(len(free))]
+        c.n_pages += len(free)
+        c._ensure_pool(c.n_pages + 40)
+        before = _books(c)
+        good = torch.ops.detllm_rocm.kv_compact
+
+        def refuse(*args):
+            raise ValueError("kv_compact")
+
+        monkeypatch.setattr(torch.ops.detllm_rocm, "kv_compact", refuse)
+        for _ in range(3):
+            with pytest.raises(ValueError):
+                c.evict(300, 10, 4)
+            assert _books(c) == before
+        monkeypatch.setattr(torch.ops.detllm_rocm, "kv_compact", good)
+        c.evict(300, 10, 4)
+        assert c.length == 300
+        used = c._table_host[c._table_host >= 0].tolist()
+        assert sorted(used + c._free) == list(range(c.n_pages))
+
+
+def test_a_failed_fork_keeps_its_pages(monkeypatch):
+    """No memory for the pages begun: the cache stays the one row it was."""
+    c = KVCache()
+    c.reserve(_model(), 1, 700)
+    c.length = 200                          # pages behind the one begun are handed back
+    before = _books(c)
+
+    def no_memory(need):
+        raise MemoryError
+
+    monkeypatch.setattr(c, "_ensure_pool", no_memory)
+    with pytest.raises(MemoryError):
+        c.fork(9)
+    assert _books(c) == before
+    monkeypatch.undo()
+    v_pools, c.v_pools = c.v_pools, [None]              # ... or fails behind the pages taken
+    with pytest.raises(TypeError):
+        c.fork(3)
+    assert _books(c) == before
+    c.v_pools = v_pools
+    c.fork(9)
+    used = set(c._table_host[c._table_host >= 0].tolist())
+    assert not used & set(c._free) and used | set(c._free) == set(range(c.n_pages))
+
+
+def test_free_pages_stay_free_when_the_pool_cannot_grow(monkeypatch):
+    c = _tracked(300)
+    c._ensure_width(2, 9)
+    c._free += [c.n_pages]
+    c.n_pages += 1
+
+    def no_memory(need):
+        raise MemoryError
+
+    monkeypatch.setattr(c, "_ensure_pool", no_memory)
+    before = _books(c)
+    with pytest.raises(MemoryError):
+        c.map_slots(c.cap)
+    assert _books(c) == before
