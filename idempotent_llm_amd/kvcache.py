@@ -142,14 +142,14 @@ class KVCache:
         if self.table is not None:
             host[:, :self.width] = self._table_host
             valid[:, :self.valid_buf.shape[1]] = self.valid_buf
+        acc = self.acc
         if self.tracking:
             acc = torch.zeros(B, self._dims[1], width * PAGE, dtype=torch.int64, device=dev)
             if self.acc is not None:
                 acc[:, :, :self.acc.shape[2]] = self.acc
-            self.acc = acc
-        self._table_host = host
-        self.table = torch.from_numpy(host).to(dev)
-        self.valid_buf = valid
+        table = torch.from_numpy(host).to(dev)
+        # (together: the attention takes acc's row stride from the table's width)
+        self._table_host, self.table, self.valid_buf, self.acc = host, table, valid, acc
 
     def map_slots(self, upto: int):
         """Map pages so every row's slots [0, upto) have one. Only new pages

@@ -141,3 +141,19 @@ def test_free_pages_stay_free_when_the_pool_cannot_grow(monkeypatch):
     with pytest.raises(MemoryError):
         c.map_slots(c.cap)
     assert _books(c) == before
+
+
+def test_a_table_that_cannot_grow_keeps_its_accumulators(monkeypatch):
+    """acc is as wide as the table, also where the wider table fails."""
+    c = _tracked(300)
+
+    def no_memory(x):
+        raise MemoryError
+
+    with monkeypatch.context() as m:
+        m.setattr(torch, "from_numpy", no_memory)
+        with pytest.raises(MemoryError):
+            c._ensure_width(2, 9)
+    assert c.acc.shape[2] == c.valid_buf.shape[1] == c.cap == c._table_host.shape[1] * PAGE
+    c._ensure_width(2, 9)
+    assert c.acc.shape[2] == c.valid_buf.shape[1] == c.cap == 9 * PAGE
