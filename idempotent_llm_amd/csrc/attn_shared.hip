@@ -670,17 +670,27 @@ __global__ __launch_bounds__(256) void k_shared_split_pv(SplitArgs sa, int P) {
   split_pv_chunk<G, SharedView>(sa, blockIdx.x, blockIdx.y, blockIdx.z, SharedView{P});
 }
 
-// Whether the four launches pay: they cost 19 us with few rows and 25 with 32
-// and more, whatever the prefix, and a row's own slots cost more there than in
-// the per-row form. us per call, per row / joint, 16 / 8 heads, 40 slots behind
-// the prefix: 4 rows 8192 slots 26.7 / 27.3, 8 rows 4096 23.8 / 24.4, 8192 34.6 /
-// 28.3, 16 rows 2048 21.9 / 22.0, 4096 30.9 / 24.3, 32 rows 2048 23.5 / 25.8, 4096
-// 39.5 / 28.2, 64 rows 1024 22.7 / 27.1, 2048 37.2 / 28.8, 8192 191 / 43; 1000 slots
-// behind 1024: 16 rows 22.8 / 34.9, 64 rows 38.0 / 62.7.
-bool shared_joint(int B, int S, int P) {
+// Whether the four launches pay: they cost 19 us with few rows and 25 with 17
+// and more (the queries then fill blocks of four groups), whatever the prefix, and
+// a row's own slots cost more there than in the per-row form. The rule bounds
+// these by the prefix and grows no stricter with fewer of them. us per call, per
+// row / joint, 40 slots behind the prefix:
+//   16 / 8 heads: 4 rows 8192 slots 26.7 / 27.3, 8 rows 4096 23.8 / 24.4, 8192 34.6 /
+//     28.3, 16 rows 2048 23.0 / 21.5, 4096 32.0 / 25.1; 17 rows 2048 22.9 / 25.0, 2560
+//     27.3 / 25.6, 4096 40.0 / 27.8, 8192 56.7 / 31.6; 32 rows 2048 24.0 / 26.7, 2560
+//     28.4 / 27.5, 4096 40.5 / 28.7; 33 rows 2048 36.4 / 27.9; 64 rows 1024 23.4 / 28.1,
+//     1280 27.9 / 28.5, 1536 30.9 / 28.9, 2048 37.8 / 29.8, 8192 191 / 43; 100 rows 1024
+//     41.7 / 34.6
+//   17 rows 2048, 2560 and 4096: 8 / 8 heads 21.6 / 21.7, 25.8 / 22.5, 38.2 / 25.2; 32 / 8
+//     26.2 / 26.3, 30.8 / 29.0, 48.3 / 30.1; 8 / 1 35.6 / 28.7, 37.7 / 30.9, 48.6 / 33.1; 4 /
+//     2 16.4 / 25.5, 16.6 / 25.9, 22.1 / 26.6 (so few heads: by the slots saved alone)
+//   more slots behind the prefix, 16 / 8 heads: 17 rows 1000 behind 4096 48.4 / 42.1,
+//     2000 56.8 / 61.9; 16 rows 1000 behind 1024 22.8 / 34.9, 64 rows 38.0 / 62.7
+bool shared_joint(int B, int S, int P, int n_q) {
   const i64 saved = (i64)(B - 1) * P;
-  return B > 16 ? saved >= 81920 && S - P <= P / 4
-                : saved >= 24576 && S - P <= imin(P / 16, 512);
+  if (B <= 16) return saved >= 24576 && S - P <= imin(P / 16, 512);
+  const bool pays = saved >= 81920 || (n_q >= 8 && (P >= 2560 || (P >= 1536 && saved >= 65536)));
+  return pays && S - P <= P / 4;
 }
 
 struct SharedPlan {
@@ -694,7 +704,7 @@ SharedPlan shared_plan(int B, int S, int P, int n_q, int n_kv) {
   SharedPlan p{};
   const int G = n_q / n_kv;
   const i64 M = (i64)B * G;
-  p.joint = shared_joint(B, S, P);
+  p.joint = shared_joint(B, S, P, n_q);
   if (!p.joint) {
     i64 at;
     p.split = B > 0 && S > 0 ? decode_chunk(B, S, n_q, n_kv) : 0;

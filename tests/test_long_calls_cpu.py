@@ -157,3 +157,18 @@ def test_a_table_that_cannot_grow_keeps_its_accumulators(monkeypatch):
     assert c.acc.shape[2] == c.valid_buf.shape[1] == c.cap == c._table_host.shape[1] * PAGE
     c._ensure_width(2, 9)
     assert c.acc.shape[2] == c.valid_buf.shape[1] == c.cap == 9 * PAGE
+
+
+def test_a_prefix_that_16_rows_read_once_17_do_too():
+    """The shared form's rule at prefixes where it pays on both sides of 16
+    rows, and few slots behind them hold it where more do."""
+    from idempotent_llm_amd._lib import attn_shared_work
+    joint = lambda B, S, P, n_q=16, n_kv=8: attn_shared_work(B, S, n_q, n_kv, P)[1]
+    for n_q, n_kv in ((16, 8), (8, 8), (32, 8), (64, 8), (8, 1)):
+        for P in (2560, 4096, 8192, 130944):
+            rows = [joint(B, P + 40, P, n_q, n_kv) for B in range(1, 80)]
+            assert rows == sorted(rows) and rows[16], (n_q, n_kv, P)
+    for B in (2, 8, 16, 17, 24, 64, 300):
+        for P in (128, 1024, 1536, 2048, 4096, 24576):
+            own = [joint(B, P + n, P) for n in range(0, P + 1, 8)]
+            assert own == sorted(own, reverse=True), (B, P)
