@@ -80,9 +80,26 @@ class GraphedDecode:
             raise IndexError(f"decode past {DEC_MAX_SLOTS} cache slots is not supported "
                              "(int32 accumulators of the decode attention)")
         self.cache.resize(cap)
-        self.cache.static_cap = self.cache.cap   # a planned cache may already be wider
+        c = self.cache
+        c.static_cap = c.cap   # a planned cache may already be wider
         self.graph = None   # a captured graph references the old tables
         self.graph_pick = None
+        # a forked cache: the slots up to which the prefix is read once
+        most = min(c.static_cap, DEC_MAX_SLOTS)
+        self._joint = 0 if c.acc is not None else self.model._joint_slots(self.B, c.shared, most)
+        c.static_scan = 0
+
+    def _size_scan(self):
+        """What this step's attention is sized for: the tables' slots, or those
+        over which a shared prefix is read once, as long as they are enough (the
+        capacity would count as the rows' own slots there). A captured graph is of
+        one size."""
+        c = self.cache
+        scan = self._joint if self.length + 1 <= self._joint else c.static_cap
+        if scan != c.static_scan:
+            c.static_scan = scan
+            self.graph = None
+            self.graph_pick = None
 
     def _map_next(self):
         """Pages for this step's slot (a no-op within a mapped page); a pool
@@ -148,6 +165,7 @@ class GraphedDecode:
         c = self.cache
         if self.length + 1 > c.static_cap:
             self._grow_to(_next_bucket(self.length + 1))
+        self._size_scan()
         self._map_next()
         self._prologue()
         self.ids_buf.copy_(cur_ids.view(self.B, 1))
@@ -171,6 +189,7 @@ class GraphedDecode:
         c = self.cache
         if self.length + 1 > c.static_cap:
             self._grow_to(_next_bucket(self.length + 1))
+        self._size_scan()
         self._map_next()
         self._prologue()
         if cur_ids is not None:

@@ -60,7 +60,8 @@ class KVCache:
         self.mapped = 0             # slots [0, mapped) are mapped on every row
         self.valid_buf = None       # [B, width * PAGE] bool
         self.length = 0
-        self.static_cap = 0
+        self.static_cap = 0         # slots of a graphed decode's tables (0: eager)
+        self.static_scan = 0        # slots its steps' attention is sized for
         self.len_idx = None         # [1] int64 device: slot written by a graphed step
         self.nslots = None          # [1] int64 device: slots visible to a graphed step
         self.pool_generation = 0

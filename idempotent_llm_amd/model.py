@@ -368,7 +368,7 @@ class IntQwen3:
         if static:
             # the step's slot flag is set before the replay (graphed.py)
             assert T == 1, "graphed (static-capacity) mode decodes one token per row"
-            S = min(cache.static_cap, DEC_MAX_SLOTS)
+            S = min(cache.static_scan or cache.static_cap, DEC_MAX_SLOTS)
         else:
             S = S_past + T
             cache.reserve(self, B, S)
@@ -554,6 +554,17 @@ class IntQwen3:
         """Whether decode attention over S slots reads a forked cache's shared
         pages once for the batch."""
         return shared <= S and attn_shared_work(B, S, self.n_q, self.n_kv, shared)[1]
+
+    def _joint_slots(self, B: int, shared: int, cap: int) -> int:
+        """The most slots up to cap over which _joint holds (0: none). The rule
+        bounds the slots behind the prefix, so it holds for fewer as well."""
+        if not shared or shared > cap or not self._joint(B, shared, shared):
+            return 0
+        lo, hi = shared, cap + 1      # holds for lo, not for hi (past the capacity)
+        while hi - lo > 1:
+            mid = (lo + hi) // 2
+            lo, hi = (mid, hi) if self._joint(B, mid, shared) else (lo, mid)
+        return lo
 
     def _attend_long(self, ws: _Workspace, L: LayerWeights, B, T, P, ns, st, xm, xk, pos,
                      cache: KVCache, S_past, S, static):
