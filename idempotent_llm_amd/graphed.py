@@ -66,6 +66,7 @@ class GraphedDecode:
         self.pos_buf = self.pos0.view(self.B, 1).clone()
         cache.len_idx = torch.zeros(1, dtype=I64, device=dev)
         cache.nslots = torch.zeros(1, dtype=I64, device=dev)
+        self._len_idx = cache.len_idx    # (this decode holds the cache while it is the cache's)
         nch = -(-model.vocab // GREEDY_CHUNK)
         self._pick_scratch = (torch.empty(self.B, nch, dtype=I64, device=dev),
                               torch.empty(self.B, nch, dtype=I64, device=dev))
@@ -88,6 +89,23 @@ class GraphedDecode:
         most = min(c.static_cap, DEC_MAX_SLOTS)
         self._joint = 0 if c.acc is not None else self.model._joint_slots(self.B, c.shared, most)
         c.static_scan = 0
+
+    def release(self) -> KVCache:
+        """The cache, back in eager use (chunks, evict, fork, track_weights)
+        with what the steps added; another GraphedDecode may take it up. This one
+        takes no further step."""
+        c = self._held()
+        torch.cuda.synchronize()         # (replays in flight read its tables)
+        self.graph = self.graph_pick = self.cache = None
+        if c.len_idx is self._len_idx:   # (else another decode has it by now)
+            c.static_cap = c.static_scan = 0
+            c.len_idx = c.nslots = None
+        return c
+
+    def _held(self) -> KVCache:
+        if self.cache is None:
+            raise ValueError("GraphedDecode: its cache was released")
+        return self.cache
 
     def _size_scan(self):
         """What this step's attention is sized for: the tables' slots, or those
@@ -162,7 +180,7 @@ class GraphedDecode:
     def step(self, cur_ids: torch.Tensor) -> torch.Tensor:
         """cur_ids int64 [B] (device). Returns int32 logits [B, vocab]; the
         buffer is reused by the next step — clone to keep."""
-        c = self.cache
+        c = self._held()
         if self.length + 1 > c.static_cap:
             self._grow_to(_next_bucket(self.length + 1))
         self._size_scan()
@@ -186,7 +204,7 @@ class GraphedDecode:
         Returns the picked ids, int64 [B] (the next step's input buffer —
         clone to keep); the step's logits are in ``self.out_pick[:, 0]``.
         Same tokens and logits as ``greedy_pick(step(cur_ids))``."""
-        c = self.cache
+        c = self._held()
         if self.length + 1 > c.static_cap:
             self._grow_to(_next_bucket(self.length + 1))
         self._size_scan()

@@ -228,7 +228,8 @@ class KVCache:
     # -- long contexts ------------------------------------------------------------
     def _no_graph(self, what: str):
         if self.static_cap:
-            raise ValueError(f"{what}: a graphed decode holds this cache's tables")
+            raise ValueError(f"{what}: a graphed decode holds this cache's tables "
+                             "(GraphedDecode.release gives them back)")
 
     def track_weights(self) -> "KVCache":
         """From now on the model adds each slot's attention weight (p in

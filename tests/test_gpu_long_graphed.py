@@ -70,3 +70,71 @@ def test_graphed_forks_read_the_prefix_once(model, monkeypatch, T, rows, joint_s
             assert torch.equal(got, want)
         cur = m.greedy_pick(want)
     m.raise_if_device_error()
+
+
+@pytest.mark.parametrize("greedy", [False, True])
+def test_weights_of_graphed_steps_drive_an_eviction(model, greedy):
+    """decode, evict, decode with the steps graphed: the cache is released for
+    the eviction, and tokens, weights and pages are those of eager steps."""
+    from idempotent_llm_amd.graphed import GraphedDecode
+    from idempotent_llm_amd.kvcache import KVCache
+    print(f"[graphed evict {greedy}]", flush=True)
+    m, B, T = model, 3, 200
+    g = torch.Generator().manual_seed(9)
+    ids = torch.randint(0, m.vocab, (B, T), generator=g).cuda()
+    pos = torch.arange(T, device="cuda").expand(B, T).contiguous()
+    lens = torch.tensor((200, 150, 180), device="cuda")
+    valid = torch.arange(T, device="cuda")[None] < lens[:, None]
+    eager, graphed = KVCache().track_weights(), KVCache().track_weights()
+    for c in (eager, graphed):
+        m.forward(ids, pos, c, valid)
+    cur, at = ids[:, 0].clone(), lens
+    for turn in range(3):
+        gd = GraphedDecode(m, graphed, at)
+        with pytest.raises(ValueError, match="graphed"):
+            graphed.evict(128, 30, 4)
+        for s in range(4):
+            want = _step(m, eager, cur, at)
+            if greedy:
+                got = gd.step_greedy(cur).clone()
+                assert torch.equal(gd.out_pick[:, 0], want)
+                assert torch.equal(got, m.greedy_pick(want))
+            else:
+                assert torch.equal(gd.step(cur), want)
+            cur, at = m.greedy_pick(want), at + 1
+        assert gd.release() is graphed and graphed.length == eager.length
+        for f in (lambda: gd.step(cur), lambda: gd.step_greedy(cur), gd.release):
+            with pytest.raises(ValueError, match="released"):
+                f()
+        n = eager.length
+        assert torch.equal(graphed.acc[:, :, :n], eager.acc[:, :, :n])
+        assert torch.equal(graphed.valid, eager.valid)
+        for c in (eager, graphed):
+            c.evict(128, 30, 4)
+        assert torch.equal(graphed.acc[:, :, :128], eager.acc[:, :, :128])
+        assert all(torch.equal(x, y) for x, y in zip(graphed.k8 + graphed.v8, eager.k8 + eager.v8))
+    # eager chunks work on it as well
+    chunk = ids[:, :7].contiguous()
+    where = at[:, None] + torch.arange(7, device="cuda")
+    assert torch.equal(m.forward(chunk, where, eager)[0], m.forward(chunk, where, graphed)[0])
+
+
+def test_release_leaves_a_cache_that_another_decode_took(model):
+    from idempotent_llm_amd.graphed import GraphedDecode
+    from idempotent_llm_amd.kvcache import KVCache
+    print("[release of a cache taken over]", flush=True)
+    m = model
+    ids, pos = _prompt(m, 50, 3)
+    one, ref = KVCache(), KVCache()
+    for c in (one, ref):
+        m.forward(ids, pos, c)
+    at, cur = torch.tensor([50], device="cuda"), ids[:, 0].clone()
+    first = GraphedDecode(m, one, at)
+    assert torch.equal(first.step(cur), _step(m, ref, cur, at))
+    second = GraphedDecode(m, one, at + 1)
+    first.release()
+    assert one.static_cap
+    for s in (1, 2):
+        assert torch.equal(second.step(cur), _step(m, ref, cur, at + s))
+    second.release()
+    assert not one.static_cap and one.length == ref.length
