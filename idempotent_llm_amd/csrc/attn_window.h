@@ -131,20 +131,6 @@ struct ValidScan {
   }
 };
 
-// One past the n-th valid slot of [0, end) (`end` if there are fewer; 0 for
-// n <= 0), and the n-th valid slot from end - 1 backward (0 if there are fewer;
-// n >= 1). Every thread of the block calls them and gets the result.
-template <int NT>
-__device__ __forceinline__ int nth_valid_end(const uint8_t* vrow, int end, int n) {
-  __shared__ int red[NT / 64], found[2];
-  return n <= 0 ? 0 : ValidScan<NT>{red, found}.forward(vrow, end, n, 0, 0);
-}
-template <int NT>
-__device__ __forceinline__ int nth_valid_back(const uint8_t* vrow, int end, int n) {
-  __shared__ int red[NT / 64], found[2];
-  return ValidScan<NT>{red, found}.backward(vrow, end, n, (end + 15) & ~15, 0);
-}
-
 // What queries see from the one at slot end1 - 1 on (its window begins lowest),
 // below slot `end`.
 struct WinRange {
