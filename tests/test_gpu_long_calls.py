@@ -106,3 +106,57 @@ def test_evict_of_long_caches(slots, pages):
     c.evict(900, 50, 4)
     assert c.length == 900 and bool(c.valid.all()) and torch.equal(c.acc[:, :, :900], kept)
     assert all(torch.equal(x, y) for x, y in zip(c.k8 + c.v8, want))
+
+
+# B, n_q, n_kv, S, window and sinks or None: the forms that need scratch
+SCRATCH = {
+    "window_cut": (1, 16, 8, 5000, (4000, 4)),
+    "window_cut_rows": (40, 4, 2, 9000, (8000, 4)),
+    "window_scores": (2, 8, 1, 8000, (300, 4)),
+    "acc_cut": (3, 16, 8, 5000, None),
+    "acc_cut_8": (1, 8, 1, 2500, None),
+    "shared_cut": (2, 16, 8, 4500, 4352),
+    "shared_once": (33, 16, 8, 2640, 2560),
+    "shared_once_few": (8, 4, 1, 4200, 4096),
+    "shared_once_many": (20, 64, 8, 4240, 4096),
+}
+
+
+@pytest.mark.parametrize("name", list(SCRATCH))
+def test_scratch_is_enough(name):
+    """Every form writes the bytes that its planner names and none behind."""
+    import ctypes
+    from idempotent_llm_amd._lib import attn_acc_work, attn_shared_work, call, load
+    B, n_q, n_kv, S, extra = SCRATCH[name]
+    print(f"[scratch {name}]", flush=True)
+    g = torch.Generator(device="cuda").manual_seed(S)
+    w = -(-S // PAGE)
+    rnd = lambda *s: torch.randint(-128, 128, s, dtype=torch.int8, device="cuda", generator=g)
+    kp, vp, q8 = rnd(B * w, n_kv, 128, 128), rnd(B * w, n_kv, 128, 128), rnd(B, n_q, 128)
+    tpos = torch.randint(1500, 24000, (B, n_q), dtype=I64, device="cuda", generator=g)
+    table = torch.randperm(B * w, device="cuda", generator=g).view(B, w).to(torch.int32)
+    valid = torch.rand(B, w * PAGE, device="cuda", generator=g) < 0.9
+    if name.startswith("shared"):
+        table[:, :extra // PAGE] = table[:1, :extra // PAGE].clone()
+        n, joint = attn_shared_work(B, S, n_q, n_kv, extra)
+        assert joint == ("once" in name)
+        entry, tail = "detllm_attn_decode_shared", (extra,)
+    elif name.startswith("acc"):
+        acc = torch.zeros(B, n_kv, S, dtype=I64, device="cuda")
+        n, entry, tail = attn_acc_work(B, S, n_q, n_kv), "detllm_attn_decode_acc", (acc, S)
+    else:
+        bytes_ = ctypes.c_int64(0)
+        assert load().detllm_attn_window_decode_work(B, S, n_q, n_kv, *extra,
+                                                     ctypes.byref(bytes_)) == 0
+        n, entry, tail = bytes_.value, "detllm_attn_window_decode", extra
+    assert n > 0
+    err = torch.zeros(1, dtype=torch.int32, device="cuda")
+    want = _ops().attn_decode(q8, tpos, kp, vp, table, valid, S, err)
+    if name.startswith("window"):
+        want = _ops().attn_window_decode(q8, tpos, kp, vp, table, valid, S, *extra)
+    out = torch.zeros(B, n_q * 128, dtype=I64, device="cuda")
+    work = torch.full((2 * n + (1 << 20),), 0xA5, dtype=torch.uint8, device="cuda")
+    call(entry, q8, tpos, kp, vp, table, w, valid.view(torch.uint8), w * PAGE, B, S, n_q, n_kv,
+         None, *tail, work, n, out, err)
+    assert torch.equal(out, want) and int(err) == 0
+    assert bool((work[n:] == 0xA5).all())

@@ -172,3 +172,70 @@ def test_a_prefix_that_16_rows_read_once_17_do_too():
         for P in (128, 1024, 1536, 2048, 4096, 24576):
             own = [joint(B, P + n, P) for n in range(0, P + 1, 8)]
             assert own == sorted(own, reverse=True), (B, P)
+
+
+# ------------------------------------------------------------------ scratch
+
+def _cdiv(a, b):
+    return -(-a // b)
+
+
+def _split_bytes(B, S, n_q, chunk):
+    """Scores [B][n_q][ns * chunk] and chunk maxima [B][n_q][ns], int32."""
+    ns = _cdiv(S, chunk)
+    return B * n_q * ns * chunk * 4 + _cdiv(B * n_q * ns * 4, 16) * 16
+
+
+HEADS = ((8, 8), (16, 8), (32, 8), (64, 8), (8, 1), (4, 2))
+LDS = 48 * 1024     # of scores in the one-block kernels
+
+
+@pytest.mark.parametrize("n_q,n_kv", HEADS)
+def test_scratch_holds_what_the_forms_write(n_q, n_kv):
+    """Each planner's bytes are those of one of the forms that the size may
+    take: none where the scores fit a block's LDS, else the scores (and what
+    the cut form adds)."""
+    import ctypes
+    from idempotent_llm_amd._lib import attn_acc_work, attn_split_plan, load
+    G = n_q // n_kv
+    out = ctypes.c_int64(0)
+    for B in (1, 3, 16, 64, 300):
+        for S in (1, 127, 700, 960, 1700, 5000, 12289, 40000, 131071):
+            spad = _cdiv(S, 16) * 16
+            chunk, ns = attn_split_plan(B, S, n_q, n_kv)
+            forms = [_split_bytes(B, S, n_q, chunk)] if ns > 1 else []
+            if G * spad * 4 <= LDS:
+                forms.append(0)
+            assert attn_acc_work(B, S, n_q, n_kv) in forms, (B, S)
+            for window, sinks in ((1, 0), (200, 4), (3000, 64), (2**31 - 1, 2**31 - 1)):
+                assert load().detllm_attn_window_decode_work(B, S, n_q, n_kv, window, sinks,
+                                                             ctypes.byref(out)) == 0
+                chunk, ns = attn_split_plan(B, min(S, window + sinks + 6 * PAGE), n_q, n_kv)
+                forms = [0 if G * spad * 4 <= LDS else B * n_q * spad * 4]
+                if ns > 1:      # + the rows' ranges (16 bytes) and page lists
+                    forms.append(_split_bytes(B, S, n_q, chunk) + B * (16 + 2 * _cdiv(S, PAGE)))
+                assert out.value in forms, (B, S, window)
+
+
+@pytest.mark.parametrize("n_q,n_kv", HEADS)
+def test_scratch_of_a_prefix_read_once(n_q, n_kv):
+    """For each query maxima (4 bytes) and denominators (8) of every part, and
+    the prefix's partial contexts (512): the parts of the launches' plan."""
+    from idempotent_llm_amd._lib import attn_shared_work
+    G, seen = n_q // n_kv, 0
+    for B in (2, 5, 9, 17, 40, 64, 200):
+        for P in (1536, 2048, 4096, 8192, 24576, 130944):
+            n, joint = attn_shared_work(B, P + 40, n_q, n_kv, P)
+            if not joint:
+                continue
+            seen += 1
+            M = B * G
+            ng = 1 if M <= 16 else 2 if M <= 32 else 4
+            blocks = _cdiv(M, 16 * ng) * n_kv
+            chunk = _cdiv(_cdiv(P // 64, max(512 // blocks, 1)), 4) * 4 * 64
+            parts = _cdiv(P, chunk) + 1
+            pages = min(max(_cdiv(P // PAGE, max(256 // blocks, 1)), 1), 8)
+            parts2 = _cdiv(P // PAGE, pages) * (4 // ng)
+            rows = n_kv * M
+            assert n >= _cdiv(rows * parts * 12, 64) * 64 + rows * parts2 * 512, (B, P)
+    assert seen > 10
