@@ -36,8 +36,9 @@ __global__ __launch_bounds__(256, 2) void k_window_prefill(PrefillArgs a) {
 // k_attn_prefill, and per 16 x 64 tile the 16 queries' p of each slot summed over
 // lanes (45 VALU instructions, row16_scatter_sum) and one 64-bit atomic per slot:
 // 2048 queries, 16 heads 74 us against 61.5 without. Sums of a block's four waves
-// joined in LDS first, a fourth of the atomics, measured 1.7 us less and were not
-// kept for it.
+// joined in LDS first, a fourth of the atomics, measured 1.7 us less (2 %) and were
+// not kept: they need a barrier per 64-slot half, where the waves now meet once a
+// page, and not at all where the pages are resident.
 __global__ __launch_bounds__(256, 2) void k_acc_prefill(PrefillArgs a) {
   keep_hidden_args();
   prefill_body<false, true>(a);

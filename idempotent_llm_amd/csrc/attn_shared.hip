@@ -390,7 +390,9 @@ __device__ __forceinline__ void shared_p(const SharedRow& R, const v4i (&st)[4],
 // its 4 waves are the QW groups times SW = 4 / QW shares of the 64-slot tiles.
 // K and V pages go through LDS as in attn_prefill.h, two pages deep; the
 // validity bits of the block's rows and pages are made first.
-constexpr int SH_MAXP = 8;  // pages per block at most (the bits' LDS)
+constexpr int SH_MAXP = 8;  // pages per block at most (the bits' LDS), so the partial
+                            // contexts grow with rows x prefix: 268 MB of scratch for
+                            // 64 rows of 64 / 8 heads behind 130944 slots
 template <int QW>
 __global__ __launch_bounds__(256, 2) void k_shared_pv(SharedArgs a) {
   keep_hidden_args();

@@ -27,7 +27,8 @@ For long contexts (no counterpart in the reference):
   all layers, to ``acc`` [B, n_kv, slots], and ``evict(budget, recent, sinks)``
   keeps the slots that kv_select picks by it, moves them together in every
   layer and returns the other pages. Positions are the caller's, so decoding
-  goes on where it was;
+  goes on where it was. A graphed decode hands its cache back for it
+  (GraphedDecode.release);
 * ``fork(rows)`` makes a one-row cache one of ``rows`` rows that share its full
   pages (``shared`` slots); decode attention reads these once for the batch
   where that pays and the cache does not track its weights.

@@ -449,7 +449,10 @@ int detllm_kv_compact(int8_t* const* kpools, int8_t* const* vpools, int n_layers
 /* detllm_attn_decode of a batch whose rows share their first `shared` slots (a
  * multiple of 128, at most S): row 0's pages stand for those of every row
  * there, and are read once for the batch where that pays (then *joint, which
- * may be null, is 1). valid is each row's own. */
+ * may be null, is 1; what is 1 for S is so for fewer slots behind the prefix).
+ * S bounds the scan, s_dev counts within it: a captured step whose rows have few
+ * slots behind the prefix gives S their bound and not the table's capacity.
+ * valid is each row's own. */
 int detllm_attn_decode_shared_work(int B, int S, int n_q, int n_kv, int shared, int64_t* bytes,
                                    int* joint);
 int detllm_attn_decode_shared(const int8_t* q8, const int64_t* tpos, const int8_t* kpool,
