@@ -24,10 +24,14 @@ struct DecodeArgs {
   // outputs v = out * om (int64, wrapping) and 0
   const int64_t* om;
   int64_t* ext;
-  // accumulating form (ACC): acc [B][n_kv][acc_stride], each slot's p summed
-  // over the kv head's query heads is added
+};
+// Of the accumulating form (ACC): each slot's p, summed over the kv head's query
+// heads, is added to acc [B][n_kv][stride]. An argument of its own, so that the
+// other kernels' arguments stay where they were: 16 bytes more in DecodeArgs moved
+// those of the fused kernel behind it and cost its launch 0.3 of 10.5 us.
+struct AccInto {
   int64_t* acc;
-  i64 acc_stride;
+  i64 stride;
 };
 
 constexpr int DEC_MAX_PAGES = 1024;  // ceil(131071 / DI_PAGE)
@@ -215,7 +219,7 @@ struct OmPre {
 };
 
 // OMP: omp holds the merge factors (else decode_body loads them when a.ext
-// is set). View: the slots (WholeRow above); ACC: their p are added to a.acc.
+// is set). View: the slots (WholeRow above); ACC: their p are added to `into`.
 template <int G, int VP, bool SCR, bool PRE = false, int NW = 4, bool OMP = false,
           class View = WholeRow, bool ACC = false>
 __device__ __forceinline__ void decode_body(const DecodeArgs& a, int S, int kvh, int b,
@@ -223,7 +227,8 @@ __device__ __forceinline__ void decode_body(const DecodeArgs& a, int S, int kvh,
                                             int32_t* sh_scores, const int32_t* pg_lds,
                                             const KPre<8 / NW>& pre = KPre<8 / NW>{},
                                             const OmPre<G, 8 / NW>& omp = OmPre<G, 8 / NW>{},
-                                            const View& view = View{}) {
+                                            const View& view = View{},
+                                            const AccInto& into = AccInto{}) {
   static_assert(G <= 8, "query heads per kv head");
   static_assert(NW == 4 || NW == 8, "waves per block");
   constexpr int NT = NW * 64;  // threads
@@ -509,7 +514,7 @@ __device__ __forceinline__ void decode_body(const DecodeArgs& a, int S, int kvh,
   if constexpr (ACC) {
     // (a query at a slot that is not valid adds nothing)
     if (S > 0 && vrow[S - 1] != 0)
-      acc_add<G, NT>(sc, Spad, S, a.acc + ((i64)b * a.n_kv + kvh) * a.acc_stride);
+      acc_add<G, NT>(sc, Spad, S, into.acc + ((i64)b * a.n_kv + kvh) * into.stride);
   }
   // ---- P.V on MFMA
   v4i chi[NB], clo[NB];
@@ -681,10 +686,11 @@ __device__ __forceinline__ void split_scores_chunk(const SplitArgs& sa, int kvh,
   }
 }
 
-// ACC: the chunk's p are added to a.acc.
+// ACC: the chunk's p are added to `into`.
 template <int G, class View = WholeRow, bool ACC = false>
 __device__ __forceinline__ void split_pv_chunk(const SplitArgs& sa, int kvh, int b, int c,
-                                               const View& view = View{}) {
+                                               const View& view = View{},
+                                               const AccInto& into = AccInto{}) {
   const DecodeArgs& a = sa.d;
   extern __shared__ __attribute__((aligned(16))) int32_t p_lds[];  // [G][chunk] packed p
   __shared__ i64 red_buf[32];
@@ -814,7 +820,7 @@ __device__ __forceinline__ void split_pv_chunk(const SplitArgs& sa, int kvh, int
   if constexpr (ACC) {
     if (a.valid[(i64)b * a.valid_stride + S - 1] != 0)
       acc_add<G, 256>(p_lds, sa.chunk, hi - lo,
-                      a.acc + ((i64)b * a.n_kv + kvh) * a.acc_stride + lo);
+                      into.acc + ((i64)b * a.n_kv + kvh) * into.stride + lo);
   }
   // P.V of the chunk
   v4i chi[2] = {v4i{0, 0, 0, 0}, v4i{0, 0, 0, 0}}, clo[2] = {v4i{0, 0, 0, 0}, v4i{0, 0, 0, 0}};

@@ -160,7 +160,7 @@ __global__ __launch_bounds__(256) void k_window_pv(WindowArgs w) {
 
 // One block per (row, kv head), as k_window_decode: 32 x 4000 slots 57 us, 4.9 TB/s.
 template <int G>
-__global__ __launch_bounds__(64 * NW) void k_acc_decode(DecodeArgs a) {
+__global__ __launch_bounds__(64 * NW) void k_acc_decode(DecodeArgs a, AccInto into) {
   keep_hidden_args();
   extern __shared__ __attribute__((aligned(16))) int32_t sh_scores[];
   __shared__ int32_t pg_lds[DEC_MAX_PAGES];
@@ -173,7 +173,8 @@ __global__ __launch_bounds__(64 * NW) void k_acc_decode(DecodeArgs a) {
   if (npages == 0 && threadIdx.x == 0) pg_lds[0] = -1;
   __syncthreads();
   decode_body<G, VPRE, false, false, NW, false, WholeRow, true>(
-      a, S, kvh, b, a.q8 + q0 * 128, a.tpos + q0, sh_scores, pg_lds);
+      a, S, kvh, b, a.q8 + q0 * 128, a.tpos + q0, sh_scores, pg_lds, KPre<8 / NW>{},
+      OmPre<G, 8 / NW>{}, WholeRow{}, into);
   report_slots(a, over, kvh == 0);
 }
 
@@ -183,9 +184,9 @@ __global__ __launch_bounds__(256) void k_acc_scores(SplitArgs sa) {
   split_scores_chunk<G>(sa, blockIdx.x, blockIdx.y, blockIdx.z);
 }
 template <int G>
-__global__ __launch_bounds__(256) void k_acc_pv(SplitArgs sa) {
+__global__ __launch_bounds__(256) void k_acc_pv(SplitArgs sa, AccInto into) {
   keep_hidden_args();
-  split_pv_chunk<G, WholeRow, true>(sa, blockIdx.x, blockIdx.y, blockIdx.z);
+  split_pv_chunk<G, WholeRow, true>(sa, blockIdx.x, blockIdx.y, blockIdx.z, WholeRow{}, into);
 }
 
 // Bytes of the one block's scores where a row may need more than its LDS
@@ -345,9 +346,9 @@ int detllm_attn_decode_acc(const int8_t* q8, const int64_t* tpos, const int8_t* 
   if (need > 0 && (!work || work_bytes < need)) return DI_ERANGE;
   const int G = n_q / n_kv;
   const int chunk = S > 0 ? decode_chunk(B, S, n_q, n_kv) : 0;
-  DecodeArgs d{q8, tpos, KVPages{(int8_t*)kpool, (int8_t*)vpool, table, width, n_kv}, valid,
-               out, nullptr, s_dev, S, n_q, n_kv, valid_stride, err, nullptr, nullptr, acc,
-               acc_stride};
+  const DecodeArgs d{q8, tpos, KVPages{(int8_t*)kpool, (int8_t*)vpool, table, width, n_kv}, valid,
+                     out, nullptr, s_dev, S, n_q, n_kv, valid_stride, err};
+  const AccInto into{acc, acc_stride};
   if (chunk) {
     const SplitArgs sa = split_args(d, B, chunk, work);
     const dim3 grid(n_kv, B, sa.ns);
@@ -356,7 +357,7 @@ int detllm_attn_decode_acc(const int8_t* q8, const int64_t* tpos, const int8_t* 
 #define DI_ACC_SPLIT(G_)                                                  \
   case G_:                                                                \
     hipLaunchKernelGGL(k_acc_scores<G_>, grid, dim3(256), 0, s, sa);      \
-    hipLaunchKernelGGL(k_acc_pv<G_>, grid, dim3(256), dyn, s, sa);        \
+    hipLaunchKernelGGL(k_acc_pv<G_>, grid, dim3(256), dyn, s, sa, into);  \
     break
       DI_ACC_SPLIT(1);
       DI_ACC_SPLIT(2);
@@ -368,10 +369,10 @@ int detllm_attn_decode_acc(const int8_t* q8, const int64_t* tpos, const int8_t* 
     const dim3 grid(n_kv, B);
     const size_t dyn = (size_t)G * (((i64)S + 15) / 16 * 16) * 4;
     switch (G) {
-      case 1: hipLaunchKernelGGL(k_acc_decode<1>, grid, dim3(64 * NW), dyn, s, d); break;
-      case 2: hipLaunchKernelGGL(k_acc_decode<2>, grid, dim3(64 * NW), dyn, s, d); break;
-      case 4: hipLaunchKernelGGL(k_acc_decode<4>, grid, dim3(64 * NW), dyn, s, d); break;
-      case 8: hipLaunchKernelGGL(k_acc_decode<8>, grid, dim3(64 * NW), dyn, s, d); break;
+      case 1: hipLaunchKernelGGL(k_acc_decode<1>, grid, dim3(64 * NW), dyn, s, d, into); break;
+      case 2: hipLaunchKernelGGL(k_acc_decode<2>, grid, dim3(64 * NW), dyn, s, d, into); break;
+      case 4: hipLaunchKernelGGL(k_acc_decode<4>, grid, dim3(64 * NW), dyn, s, d, into); break;
+      case 8: hipLaunchKernelGGL(k_acc_decode<8>, grid, dim3(64 * NW), dyn, s, d, into); break;
     }
   }
   DI_LAUNCH_CHECK();
