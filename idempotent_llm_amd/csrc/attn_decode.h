@@ -642,8 +642,7 @@ __device__ __forceinline__ void split_scores_chunk(const SplitArgs& sa, int kvh,
   const int blo = lo / 16, bhi = (hi + 15) / 16;
   for (int blk0 = blo + wave; blk0 < bhi; blk0 += 16) {
     v4i kb[4][2];
-    int vraw[4], vf[4];
-    bool ok[4];
+    int vraw[4], vf[4], ok[4];
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       const int s = (blk0 + u * 4) * 16 + l16;
@@ -653,10 +652,11 @@ __device__ __forceinline__ void split_scores_chunk(const SplitArgs& sa, int kvh,
       kb[u][0] = *(const v4i*)(kr + grp * 16);
       kb[u][1] = *(const v4i*)(kr + 64 + grp * 16);
       vraw[u] = vrow[view.slot(sc_)];  // masked at use (no wait per block)
-      ok[u] = pg >= 0 && view.sees(view.slot(sc_));
+      ok[u] = pg >= 0 && view.sees(view.slot(sc_)) ? 0xFF : 0;
+      asm("" : "+v"(ok[u]));  // (opaque, or the flag's load moves behind a branch on it)
     }
 #pragma unroll
-    for (int u = 0; u < 4; ++u) vf[u] = ok[u] ? vraw[u] : 0;
+    for (int u = 0; u < 4; ++u) vf[u] = vraw[u] & ok[u];
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       const int blk = blk0 + u * 4;
