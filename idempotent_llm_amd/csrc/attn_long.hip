@@ -29,9 +29,9 @@ namespace {
 // they see (pages and 64-query tiles are whole). 2048 queries behind 6144 slots,
 // 32 heads, window 1024: 129 us, 67 M pairs seen, 267 TOP/s; 3 x 333 queries,
 // window 100: 24 us, most of it the chain of three passes over three pages.
-__global__ __launch_bounds__(256, 2) void k_window_prefill(PrefillArgs a) {
+__global__ __launch_bounds__(256, 2) void k_window_prefill(PrefillArgs a, PrefillForm form) {
   keep_hidden_args();
-  prefill_body<true, false>(a);
+  prefill_body<true, false>(a, form);
 }
 // k_attn_prefill, and per 16 x 64 tile the 16 queries' p of each slot summed over
 // lanes (45 VALU instructions, row16_scatter_sum) and one 64-bit atomic per slot:
@@ -39,9 +39,9 @@ __global__ __launch_bounds__(256, 2) void k_window_prefill(PrefillArgs a) {
 // joined in LDS first, a fourth of the atomics, measured 1.7 us less (2 %) and were
 // not kept: they need a barrier per 64-slot half, where the waves now meet once a
 // page, and not at all where the pages are resident.
-__global__ __launch_bounds__(256, 2) void k_acc_prefill(PrefillArgs a) {
+__global__ __launch_bounds__(256, 2) void k_acc_prefill(PrefillArgs a, PrefillForm form) {
   keep_hidden_args();
-  prefill_body<false, true>(a);
+  prefill_body<false, true>(a, form);
 }
 
 __host__ __device__ constexpr int pages_of(int S) { return (S + DI_PAGE - 1) / DI_PAGE; }
@@ -216,11 +216,11 @@ int detllm_attn_window_prefill(const int8_t* q8, const int64_t* tpos, const int8
     return DI_EINVAL;
   if (S > DEC_MAX_S) return DI_ERANGE;  // int32 MFMA accumulators of P.V
   PrefillArgs a{q8, tpos, KVPages{(int8_t*)kpool, (int8_t*)vpool, table, width, n_kv}, valid, out,
-                T, (int)S, S_past, n_q, n_kv, B, valid_stride, window, sinks};
+                T, (int)S, S_past, n_q, n_kv, B, valid_stride};
   const i64 pairs = (i64)(((T + 63) / 64 + 1) / 2) * n_q * B;
   if (2 * pairs > 0x7fffffff) return DI_ERANGE;
   hipLaunchKernelGGL(k_window_prefill, dim3((unsigned)(2 * pairs)), dim3(256),
-                     prefill_lds(S, true), s, a);
+                     prefill_lds(S, true), s, a, PrefillForm{window, sinks, nullptr, 0});
   DI_LAUNCH_CHECK();
   return DI_OK;
 }
@@ -238,10 +238,11 @@ int detllm_attn_prefill_acc(const int8_t* q8, const int64_t* tpos, const int8_t*
     return DI_EINVAL;
   if (S > DEC_MAX_S) return DI_ERANGE;
   PrefillArgs a{q8, tpos, KVPages{(int8_t*)kpool, (int8_t*)vpool, table, width, n_kv}, valid, out,
-                T, (int)S, S_past, n_q, n_kv, B, valid_stride, 0, 0, acc, acc_stride};
+                T, (int)S, S_past, n_q, n_kv, B, valid_stride};
   const i64 pairs = (i64)(((T + 63) / 64 + 1) / 2) * n_q * B;
   if (2 * pairs > 0x7fffffff) return DI_ERANGE;
-  hipLaunchKernelGGL(k_acc_prefill, dim3((unsigned)(2 * pairs)), dim3(256), prefill_lds(S), s, a);
+  hipLaunchKernelGGL(k_acc_prefill, dim3((unsigned)(2 * pairs)), dim3(256), prefill_lds(S), s, a,
+                     PrefillForm{0, 0, acc, acc_stride});
   DI_LAUNCH_CHECK();
   return DI_OK;
 }
