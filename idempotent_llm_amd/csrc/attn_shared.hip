@@ -22,7 +22,7 @@
 // and 16 slots (16 g + 4 blk + r, g = lane / 16) of a 64-slot tile.
 //
 // 64 rows behind 8192 slots, 200 of their own, 16 / 8 heads: 50 us (maxima 11,
-// sums 12, P.V of the prefix 16, the rest 12), 191 in the per-row form; the 46 MB
+// sums 12, P.V of the prefix 16, the rest 12), 145 in the per-row form; the 46 MB
 // take 10 us and the products 2. What is left is the launches' own chains (the
 // first load, the parts' join and the block's end: 4 to 7 us each with one slot
 // per row), so fewer and larger parts or another number of blocks change
@@ -681,7 +681,7 @@ __global__ __launch_bounds__(256) void k_shared_split_pv(SplitArgs sa, int P) {
 //     28.3, 16 rows 2048 23.0 / 21.5, 4096 32.0 / 25.1; 17 rows 2048 22.9 / 25.0, 2560
 //     27.3 / 25.6, 4096 40.0 / 27.8, 8192 56.7 / 31.6; 32 rows 2048 24.0 / 26.7, 2560
 //     28.4 / 27.5, 4096 40.5 / 28.7; 33 rows 2048 36.4 / 27.9; 64 rows 1024 23.4 / 28.1,
-//     1280 27.9 / 28.5, 1536 30.9 / 28.9, 2048 37.8 / 29.8, 8192 191 / 43; 100 rows 1024
+//     1280 27.9 / 28.5, 1536 30.9 / 28.9, 2048 37.8 / 29.8, 8192 144 / 44; 100 rows 1024
 //     41.7 / 34.6
 //   17 rows 2048, 2560 and 4096: 8 / 8 heads 21.6 / 21.7, 25.8 / 22.5, 38.2 / 25.2; 32 / 8
 //     26.2 / 26.3, 30.8 / 29.0, 48.3 / 30.1; 8 / 1 35.6 / 28.7, 37.7 / 30.9, 48.6 / 33.1; 4 /
