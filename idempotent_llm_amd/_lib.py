@@ -72,6 +72,13 @@ SIGNATURES = {
     "detllm_kv_compact": [P, P, I, I, P, I, P, I, P, I, I, I, S],
     "detllm_attn_decode_shared_work": [I, I, I, I, I, P, P],
     "detllm_attn_decode_shared": [P, P, P, P, P, I, P, L, I, I, I, I, P, I, P, L, P, P, S],
+    "detllm_packed_plan_work": [I, I, P],
+    "detllm_packed_plan": [P, I, P, I, P, P, P, I, I, P, P, P, P, P, L, P, S],
+    "detllm_qkv_epilogue_packed": [P, I, L, I, I, I, P, P, P, P, P, L, P, L, P, L, P, L, P, L, P,
+                                   L, P, P, P, P, P, P, P, P, L, P, P, P, P, I, P, P, S],
+    "detllm_attn_packed_work": [I, I, I, I, I, I, P],
+    "detllm_attn_packed": [P, P, P, P, I, P, I, P, P, I, I, I, I, I, I, P, L, P, P, S],
+    "detllm_lora_add": [P, P, P, P, P, P, P, I, I, I, I, I, S],
     "detllm_decode_prologue": [P, L, I, L, P, P, P, P, L, S],
     "detllm_op_quant_i8_pertoken": [P, P, P, I, I, P, P, P, S],
     "detllm_op_requant_i32_common": [P, P, P, I, L, I, I, I, P, P, S],
@@ -89,7 +96,8 @@ SIGNATURES = {
 # host-only entry points (no device work, so no stream argument)
 HOST_ONLY = frozenset({"detllm_igemv_plan", "detllm_attn_split_plan",
                        "detllm_attn_window_decode_work", "detllm_attn_decode_acc_work",
-                       "detllm_kv_select_work", "detllm_attn_decode_shared_work"})
+                       "detllm_kv_select_work", "detllm_attn_decode_shared_work",
+                       "detllm_packed_plan_work", "detllm_attn_packed_work"})
 
 _CT = {P: ctypes.c_void_p, I: ctypes.c_int, L: ctypes.c_int64, S: ctypes.c_void_p}
 
@@ -179,6 +187,16 @@ def attn_shared_work(B: int, S: int, n_q: int, n_kv: int, shared: int):
     return out.value, bool(joint.value)
 
 
+def packed_work(N: int, B: int, S: int, max_new: int, n_q: int, n_kv: int) -> int:
+    """Bytes of scratch of detllm_attn_packed at this shape."""
+    out = ctypes.c_int64(0)
+    rc = load().detllm_attn_packed_work(int(N), int(B), int(S), int(max_new), int(n_q), int(n_kv),
+                                        ctypes.byref(out))
+    if rc != 0:
+        raise RuntimeError(f"detllm_attn_packed_work failed (code {rc})")
+    return out.value
+
+
 def pro_fits(K: int, ksplit: int) -> bool:
     """True when the fused decode GEMVs (detllm_igemv_resnormq /
     detllm_igemv_merge / detllm_igemv_swiglu) cover a K split of ``ksplit``: each split a whole
@@ -194,7 +212,7 @@ def pro_fits(K: int, ksplit: int) -> bool:
 
 
 # bits of the device error word (include/detllm_hip.h)
-ERR_TOKEN, ERR_POSITION, ERR_SLOTS = 1, 2, 4
+ERR_TOKEN, ERR_POSITION, ERR_SLOTS, ERR_PAGES = 1, 2, 4, 8
 
 
 def raise_for_error_word(word: int, vocab=None, max_pos=None) -> None:
@@ -211,6 +229,8 @@ def raise_for_error_word(word: int, vocab=None, max_pos=None) -> None:
         msgs.append(f"position out of range for the RoPE tables (size {max_pos})")
     if word & ERR_SLOTS:
         msgs.append("device slot count exceeded the slots the attention launch was sized for")
+    if word & ERR_PAGES:
+        msgs.append("too few free pages for the step")
     raise IndexError("; ".join(msgs))
 
 

@@ -28,7 +28,7 @@ LIB = os.path.join(PKG, "libdetllm_hip.so")
 NATIVE = os.path.join(PKG, "_native.so")
 HOST_LIB = os.path.join(PKG, "libdetllm_intops_host.so")
 HIP_SOURCES = ("gemm.hip", "rowops.hip", "attention.hip", "attn_long.hip", "attn_shared.hip",
-               "kv_evict.hip")
+               "kv_evict.hip", "attn_packed.hip", "packed_plan.hip", "lora.hip")
 ARCH = "gfx950"
 HIPCC_FLAGS = ["-O3", "-std=c++17", f"--offload-arch={ARCH}", "-fPIC",
                "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",

@@ -1,0 +1,921 @@
+// The blocks of the packed attention (attn_packed.hip, gfx950).
+#pragma once
+
+#include "attn_tiles.h"
+
+namespace {
+
+constexpr int PACKED_MAX_S = 131071;    // int32 accumulators: 128 * 128 * S < 2^31
+constexpr int PACKED_MAX_ROWS = 65536;  // rows of a batch
+constexpr int FEW_SLOTS = 2048;         // slots of a few-row unit in a block of eight waves
+constexpr int FEW_ONE_SLOTS = 1024;     // and of four
+
+// Passes
+constexpr int PH_MAX = 1, PH_DEN = 2, PH_PV = 4, PH_ALL = 7;
+
+struct PackedArgs {
+  const int8_t* q8;     // [N][n_q][128]
+  const int64_t* tpos;  // [N][n_q]
+  KVPages kv;
+  int n_pages;
+  const int32_t* cu;    // [B + 1]
+  const int32_t* past;  // [B]
+  int N, B, S, max_new, n_q, n_kv;
+  int lg;        // log2 of the query heads per kv head
+  int few_rows;  // query rows of a few-row unit at most (its rows of scores)
+  int units, chunk, nch;
+  int32_t* scores;  // few-row units: [B][n_kv][few_rows][nch * chunk]
+  int32_t* smax;    // [units][n_kv][nch][64]: maxima of the visible scores
+  int64_t* sden;    // the same of partial denominators
+  int32_t* part;    // [nch][N][n_q * 128] contexts (null: one chunk, straight to out)
+  int64_t* out;     // [N][n_q * 128]
+  int32_t* err;
+};
+
+// Never a score: |q . k| <= 2^21
+constexpr int32_t NO_SCORE = INT32_MIN;
+
+// What a block works on
+struct Work {
+  bool live;  // else: no such unit (spare: its number among those, of `spares`)
+  bool few;   // the row has at most 16 query rows
+  bool bad;   // the row's slots or tokens are past the launch's bounds
+  int b, tile, unit, kvh, c;
+  int tok0, T, past;  // the row's first token row, its tokens and filled slots
+  int len;            // slots that its tokens see (past + T, bounded)
+  int ntok;           // token rows of all rows
+  int spare, spares;
+};
+
+// Last slot that token t of a row at `past` sees
+__device__ __forceinline__ int row_limit(const PackedArgs& a, int past, int t) {
+  const i64 l = (i64)::max(past, 0) + t;
+  return (int)imin(l, (i64)a.S - 1);
+}
+
+// Inclusive sum over the lanes: within rows of 16 (row shifts by 1, 2, 4, 8),
+// then the rows' totals (broadcasts of lanes 15 and 31)
+__device__ __forceinline__ int wave_scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);
+  return v + __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);
+}
+
+// Every LDS read of the wave done (before a barrier that frees what it read)
+__device__ __forceinline__ void wait_lds() { __builtin_amdgcn_s_waitcnt(0xC07F); }
+
+// The unit of this block, found by every wave for itself. Blocks: kv heads
+// fastest (with 8 of them a head's blocks share an XCD, so its L2 holds their K
+// and V), then chunks, then units from the last row's last tile on (the tiles of
+// a prompt that see most go first).
+__device__ __forceinline__ Work find_work(const PackedArgs& a) {
+  Work w{};
+  const int lane = threadIdx.x & 63;
+  const int bid = blockIdx.x;
+  w.kvh = bid % a.n_kv;
+  const int rest = bid / a.n_kv;
+  w.c = rest % a.nch;
+  const int want = a.units - 1 - rest / a.nch;
+  w.unit = want;
+  w.ntok = ::min(::max(a.cu[a.B], 0), a.N);
+  int base = 0;
+  for (int b0 = 0; b0 < a.B; b0 += 64) {
+    const int b = b0 + lane, bc = ::min(b, a.B - 1);
+    const int past = a.past[bc];
+    const int c0 = ::min(::max(a.cu[bc], 0), a.N), c1 = ::min(::max(a.cu[bc + 1], c0), a.N);
+    const int T = b < a.B ? ::min(c1 - c0, a.max_new) : 0;
+    const i64 R = (i64)T << a.lg;
+    const int n = R <= 16 ? (T > 0 ? 1 : 0) : (int)((R + 63) >> 6);
+    const int over = c1 - c0 > a.max_new;
+    const int incl = wave_scan(n);
+    const int tot = __builtin_amdgcn_readlane(incl, 63);
+    if (!w.live && want < base + tot) {
+      const int l = __ffsll((unsigned long long)__ballot(base + incl > want)) - 1;
+      w.live = true;
+      w.b = b0 + l;
+      w.tile = want - base - (__builtin_amdgcn_readlane(incl, l) - __builtin_amdgcn_readlane(n, l));
+      w.tok0 = __builtin_amdgcn_readlane(c0, l);
+      w.T = __builtin_amdgcn_readlane(T, l);
+      w.bad = __builtin_amdgcn_readlane(over, l) != 0;
+      w.past = __builtin_amdgcn_readlane(past, l);
+    }
+    base += tot;
+  }
+  if (!w.live) {
+    w.spare = want - base;
+    w.spares = a.units - base;
+    return w;
+  }
+  const i64 end = (i64)w.past + w.T;
+  w.bad = w.bad || w.past < 0 || end > (i64)a.S;
+  w.past = ::max(w.past, 0);
+  w.len = row_limit(a, w.past, w.T - 1) + 1;
+  w.few = (w.T << a.lg) <= 16;
+  return w;
+}
+
+// Slots outside the launch's bound: DI_ERR_SLOTS, once a row
+__device__ __forceinline__ void report_row(const PackedArgs& a, const Work& w) {
+  if (w.bad && w.tile == 0 && w.kvh == 0 && w.c == 0 && threadIdx.x == 0 && a.err)
+    atomicOr(a.err, DI_ERR_SLOTS);
+}
+
+// Token rows behind the last row's: zeros, shared among the blocks without a unit
+__device__ __forceinline__ void zero_tail(const PackedArgs& a, const Work& w) {
+  if (w.c != 0) return;
+  const int cols = 128 << a.lg;
+  for (int tok = w.ntok + w.spare; tok < a.N; tok += w.spares) {
+    int64_t* o = a.out + ((i64)tok * a.n_kv + w.kvh) * cols;
+    for (int i = threadIdx.x; i < cols; i += blockDim.x) o[i] = 0;
+  }
+}
+
+// The page of row b's slots [128 j, 128 j + 128): -1 when not mapped
+__device__ __forceinline__ int packed_page(const PackedArgs& a, int b, int j) {
+  const int pg = j < a.kv.width ? a.kv.table[(i64)b * a.kv.width + j] : -1;
+  return pg < a.n_pages ? pg : -1;
+}
+
+// ---- DI-Exp and probabilities of a query row
+//
+// For tpos < 2^17 (a wave's rows decide together; else the integer forms):
+// with n = m - s >= 0, t = tpos, sp = t - n, the exponential is
+// e = ((q + 1) t - n) >> (q + 1), q = n div t (intops.h, dexp_est). The scores'
+// accumulators start from 0x4B400000 + t - m, so that they arrive as the bits of
+// the float 1.5 2^23 + sp (|sp| < 2^22: |n| <= 2^22). Then
+//   x = clamp01(b - sp a), a = fl(1 / 31 t), b = fl((1.5 + 0.5 / t) / 31):
+//     31 x is (n + 0.5) / t + 0.5 within 2^-18.3 where that is below 31 (a, b and
+//     the fma are off by at most half a step, on values up to 32 / 31), and a
+//     quotient (n + 0.5) / t + 0.5 is at least 0.5 / t >= 2^-18 from the next half-integer,
+//   so fma(x, 31, 2^23) rounds to 2^23 + q + 1, q + 1 in its low bits.
+// From 31 on the shift is 31 and (31 t + sp) in 22 bits, whatever its sign,
+// shifts to the 0 that e is there. Of these operations the fmas, the
+// subtraction, the AND and the shift issue in two cycles a wave, the multiply-add
+// in four: 17 cycles against 26 through doubles (conversions, and the minimum of
+// the shift).
+//
+// p = floor((e 2^14 + floor(den / 2)) / den) is e 2^14 / den rounded to nearest,
+// halves up (for odd den there are none). In double, r = fl(2^14 / den) (1 + 2^-50)
+// and fma(e, r, 2^52 + 128) rounds e r once, to an integer: a half goes up, since
+// r exceeds 2^14 / den by 2^-51 of it at least, and another value is 1 / (2 den) from the
+// next half, more than the 2^14 2^-49 that r adds, for den < 2^34. The low word
+// is p + 128: its second byte H and its first L give p = 256 H + (L - 128), and
+// L - 128 as a byte is L ^ 0x80, so the bytes are two int8 operands.
+struct RowExp {
+  float a, b;
+  uint32_t t;
+  int32_t c0;  // the accumulators' start
+};
+constexpr i64 FAST_T = (i64)1 << 17;
+constexpr i64 FAST_DEN = (i64)1 << 34;
+
+__device__ __forceinline__ RowExp make_rowexp(i64 t, int32_t mx) {
+  RowExp E;
+  const double d = (double)t;
+  E.a = (float)(1.0 / (31.0 * d));
+  E.b = (float)((1.5 + 0.5 / d) / 31.0);
+  E.t = (uint32_t)t;
+  E.c0 = (int32_t)(0x4B400000u + (uint32_t)t - (uint32_t)mx);
+  return E;
+}
+__device__ __forceinline__ uint32_t row_exp(int32_t F, const RowExp& E) {
+  const float sp = __builtin_bit_cast(float, F) - 12582912.0f;
+  const float x = __builtin_amdgcn_fmed3f(__builtin_fmaf(sp, -E.a, E.b), 0.0f, 1.0f);
+  const uint32_t y = __builtin_bit_cast(uint32_t, __builtin_fmaf(x, 31.0f, 8388608.0f));
+  const uint32_t m = mad_u24(y, E.t, (uint32_t)F) & 0x3FFFFFu;
+  return m >> (y & 31u);
+}
+
+__device__ __forceinline__ double make_rowp(i64 den) {
+  const double r = 16384.0 / (double)den;
+  return fma(r, 0x1p-50, r);
+}
+__device__ __forceinline__ uint32_t row_p128(uint32_t e, double r) {  // p + 128
+  const double y = fma((double)e, r, 0x1p52 + 128.0);
+  return (uint32_t)__builtin_bit_cast(u64, y);
+}
+// Four words p + 128 as the operands' bytes
+__device__ __forceinline__ void pack4(const uint32_t (&w)[4], int& hi, int& lo) {
+  const uint32_t a = __builtin_amdgcn_perm(w[1], w[0], 0x05010400u);  // L0 L1 H0 H1
+  const uint32_t b = __builtin_amdgcn_perm(w[3], w[2], 0x05010400u);
+  lo = (int)(__builtin_amdgcn_perm(b, a, 0x05040100u) ^ 0x80808080u);
+  hi = (int)__builtin_amdgcn_perm(b, a, 0x07060302u);
+}
+
+// The integer forms
+struct RowSlow {
+  ExpR E;
+  Recip R;
+};
+__device__ __forceinline__ i64 slow_exp(int32_t st, int32_t mx, const ExpR& E) {
+  return di_exp_neg((u64)(uint32_t)(mx - st), E);
+}
+__device__ __forceinline__ uint32_t slow_p128(i64 e, const Recip& R) {
+  return (uint32_t)to_i32(rhad_r(shl(e, 14), R)) + 128u;
+}
+
+__device__ __forceinline__ int max16(int v) {  // over the lanes of one query row
+  v = ::max(v, __shfl_xor(v, 16));
+  return ::max(v, __shfl_xor(v, 32));
+}
+
+// ------------------------------------------------------------- few-row units
+//
+// One row, at most 16 query rows (token t and head g: row t G + g). S^T = K . Q^T
+// on v_mfma_i32_16x16x64_i8 with K's rows straight from the cache: MFMA row i of
+// block blk is slot 16 (i / 4) + 4 blk + i % 4 of a 64-slot tile, so that lane (qi, g4)
+// of a wave receives query row qi's scores of the 16 slots 16 g4 .. + 15, which are
+// its bytes of the P operand. Each byte of K and V is read once; what bounds it
+// is HBM, or, for short rows, one chain of loads and three block reductions. The
+// arithmetic of the query rows that are not there (14 of 16 at one token and two
+// heads) is 5 cycles a slot and CU against the 31 that its 256 bytes take.
+
+template <int NW>
+struct FewLds {
+  int32_t mx[NW][16];
+  int64_t den[NW][16];
+  int32_t ctx[16][128];
+};
+
+struct FewRow {
+  bool on;     // the lane's query row is there
+  int limit;   // the last slot it sees (-1: none)
+  i64 tpos;
+  v4i q0, q1;
+};
+
+__device__ __forceinline__ FewRow few_row(const PackedArgs& a, const Work& w) {
+  const int lane = threadIdx.x & 63, qi = lane & 15, g4 = lane >> 4;
+  FewRow r;
+  const int t = qi >> a.lg, g = qi & ((1 << a.lg) - 1);
+  r.on = qi < (w.T << a.lg);
+  const i64 row = (i64)(w.tok0 + (r.on ? t : 0)) * a.n_q + (w.kvh << a.lg) + g;
+  r.limit = r.on ? row_limit(a, w.past, t) : -1;
+  const i64 tp = a.tpos[row];
+  const v4i q0 = *(const v4i*)(a.q8 + row * 128 + g4 * 16);
+  const v4i q1 = *(const v4i*)(a.q8 + row * 128 + 64 + g4 * 16);
+  r.tpos = r.on ? tp : 1;
+  const v4i z = v4i{0, 0, 0, 0};
+  r.q0 = r.on ? q0 : z;
+  r.q1 = r.on ? q1 : z;
+  return r;
+}
+
+// K operands of the 64-slot half hf of a page (a page that is not there reads page 0)
+__device__ __forceinline__ void few_k(const PackedArgs& a, int pg, int kvh, int hf, v4i (&k)[8]) {
+  const int lane = threadIdx.x & 63, qi = lane & 15, g4 = lane >> 4;
+  const int8_t* p = a.kv.krow(::max(pg, 0), kvh, hf * 64 + 16 * (qi >> 2) + (qi & 3)) + g4 * 16;
+#pragma unroll
+  for (int blk = 0; blk < 4; ++blk) {
+    k[2 * blk] = *(const v4i*)(p + blk * 512);
+    k[2 * blk + 1] = *(const v4i*)(p + blk * 512 + 64);
+  }
+}
+// V operands: channel 16 j + qi, slots 16 g4 .. + 15 of the half
+__device__ __forceinline__ void few_v(const PackedArgs& a, int pg, int kvh, int hf, v4i (&v)[8]) {
+  const int lane = threadIdx.x & 63, qi = lane & 15, g4 = lane >> 4;
+  const int8_t* p = a.kv.vchan(::max(pg, 0), kvh, qi) + hf * 64 + g4 * 16;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = *(const v4i*)(p + j * 16 * DI_PAGE);
+}
+__device__ __forceinline__ void few_scores(const v4i (&k)[8], const FewRow& r, v4i (&st)[4]) {
+  const v4i z = v4i{0, 0, 0, 0};
+#pragma unroll
+  for (int blk = 0; blk < 4; ++blk) st[blk] = mfma16(k[2 * blk], r.q0, z);
+#pragma unroll
+  for (int blk = 0; blk < 4; ++blk) st[blk] = mfma16(k[2 * blk + 1], r.q1, st[blk]);
+}
+// bit i: the lane's query row sees slot s0 + i, i < 16
+__device__ __forceinline__ uint32_t seen16(int limit, int s0) {
+  const int e = limit - s0;
+  return e >= 15 ? 0xFFFFu : (e < 0 ? 0u : (2u << e) - 1u);
+}
+
+// sum p v of a tile into the accumulators
+__device__ __forceinline__ void pv16(const v4i& phi, const v4i& plo, const v4i (&v)[8], v4i (&hi)[8],
+                                     v4i (&lo)[8]) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    hi[j] = mfma16(phi, v[j], hi[j]);
+    lo[j] = mfma16(plo, v[j], lo[j]);
+  }
+}
+
+// The tile's operands from its 16 scores a lane; `bits` of them are seen
+__device__ __forceinline__ void few_probs(const v4i (&st)[4], uint32_t bits, bool fast,
+                                          const RowExp& E, double rp, int32_t mx, const RowSlow& sl,
+                                          v4i& phi, v4i& plo) {
+#pragma unroll
+  for (int blk = 0; blk < 4; ++blk) {
+    uint32_t w4[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const bool vis = (bits >> (4 * blk + r)) & 1u;
+      if (fast) {
+        const uint32_t e = row_exp(st[blk][r] + E.c0, E);
+        w4[r] = row_p128(vis ? e : 0u, rp);
+      } else {
+        w4[r] = vis ? slow_p128(slow_exp(st[blk][r], mx, sl.E), sl.R) : 128u;
+      }
+    }
+    int h, l;
+    pack4(w4, h, l);
+    phi[blk] = h;
+    plo[blk] = l;
+  }
+}
+__device__ __forceinline__ i64 few_den(const v4i (&st)[4], uint32_t bits, bool fast, const RowExp& E,
+                                       int32_t mx, const ExpR& Es) {
+  i64 den = 0;
+  if (fast) {
+    uint32_t sum = 0;
+#pragma unroll
+    for (int blk = 0; blk < 4; ++blk)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const uint32_t e = row_exp(st[blk][r] + E.c0, E);
+        sum += (bits >> (4 * blk + r)) & 1u ? e : 0u;
+      }
+    return sum;
+  }
+#pragma unroll
+  for (int blk = 0; blk < 4; ++blk)
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if ((bits >> (4 * blk + r)) & 1u) den = wadd(den, slow_exp(st[blk][r], mx, Es));
+  return den;
+}
+
+// The waves' contexts (accumulators of query row 4 g4 + r, channel 16 j + qi) added
+// up in LDS, then written: to out, or to a chunk's part
+template <int NW>
+__device__ __forceinline__ void few_store(const PackedArgs& a, const Work& w, FewLds<NW>& lds,
+                                          const v4i (&hi)[8], const v4i (&lo)[8], bool any) {
+  const int lane = threadIdx.x & 63, qi = lane & 15, g4 = lane >> 4;
+  const int R = w.T << a.lg;
+  if (any) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (4 * g4 + r < R) atomicAdd(&lds.ctx[4 * g4 + r][16 * j + qi], hi[j][r] * 256 + lo[j][r]);
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < R * 128; i += NW * 64) {
+    const int row = i >> 7, t = row >> a.lg, g = row & ((1 << a.lg) - 1);
+    const i64 at = ((i64)(w.tok0 + t) * a.n_q + (w.kvh << a.lg) + g) * 128 + (i & 127);
+    const int x = lds.ctx[row][i & 127];
+    if (a.part) a.part[(i64)w.c * a.N * a.n_q * 128 + at] = x;
+    else a.out[at] = x;
+  }
+}
+
+// A whole row of at most 64 NW NT slots: tile i of wave v is tile i NW + v
+template <int NW, int NT>
+__device__ __forceinline__ void few_one(const PackedArgs& a, const Work& w, FewLds<NW>& lds) {
+  const int lane = threadIdx.x & 63, qi = lane & 15, g4 = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const int ntiles = (w.len + 63) / 64;
+  int pg[NT];
+#pragma unroll
+  for (int i = 0; i < NT; ++i) {
+    const int it = i * NW + wave;
+    pg[i] = it < ntiles ? packed_page(a, w.b, it >> 1) : -1;
+  }
+  const FewRow row = few_row(a, w);
+  for (int i = threadIdx.x; i < 16 * 128; i += NW * 64) ((int32_t*)lds.ctx)[i] = 0;
+  v4i st[NT][4];
+  {
+    v4i k[NT][8];
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+      pg[i] = __builtin_amdgcn_readfirstlane(pg[i]);
+      if (i * NW + wave < ntiles) few_k(a, pg[i], w.kvh, (i * NW + wave) & 1, k[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+      if (i * NW + wave < ntiles) few_scores(k[i], row, st[i]);
+  }
+  // the first V operands load under the reductions
+  v4i v0[8];
+  if (wave < ntiles) few_v(a, pg[0], w.kvh, wave & 1, v0);
+  auto bits = [&](int i) {
+    const int it = i * NW + wave;
+    return it < ntiles && pg[i] >= 0 ? seen16(row.limit, it * 64 + 16 * g4) : 0u;
+  };
+  int mx = NO_SCORE;
+#pragma unroll
+  for (int i = 0; i < NT; ++i)
+    if (i * NW + wave < ntiles) {
+      const uint32_t bb = bits(i);
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        if ((bb >> e) & 1u) mx = ::max(mx, st[i][e >> 2][e & 3]);
+    }
+  mx = max16(mx);
+  if (g4 == 0) lds.mx[wave][qi] = mx;
+  __syncthreads();
+#pragma unroll
+  for (int v = 0; v < NW; ++v) mx = ::max(mx, lds.mx[v][qi]);
+  if (mx == NO_SCORE) mx = 0;  // nothing seen: max := 0, every p = 0
+  const bool fast_e = __ballot(row.tpos >= FAST_T) == 0;
+  const RowExp E = make_rowexp(row.tpos, mx);
+  RowSlow sl;
+  if (!fast_e) sl.E = make_exp(row.tpos);
+  i64 den = 0;
+#pragma unroll
+  for (int i = 0; i < NT; ++i)
+    if (i * NW + wave < ntiles) den = wadd(den, few_den(st[i], bits(i), fast_e, E, mx, sl.E));
+  den = group4_sum(den);
+  if (g4 == 0) lds.den[wave][qi] = den;
+  __syncthreads();
+  den = 0;
+#pragma unroll
+  for (int v = 0; v < NW; ++v) den = wadd(den, lds.den[v][qi]);
+  den = imax(den, 1);
+  const bool fast = fast_e && __ballot(den >= FAST_DEN) == 0;
+  const double rp = make_rowp(den);
+  if (!fast) {
+    sl.E = make_exp(row.tpos);
+    sl.R = make_recip(den);
+  }
+  v4i hi[8], lo[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) hi[j] = lo[j] = v4i{0, 0, 0, 0};
+#pragma unroll
+  for (int i = 0; i < NT; ++i) {
+    const int it = i * NW + wave;
+    if (it < ntiles) {
+      v4i v[8], phi, plo;
+      if (i > 0) few_v(a, pg[i], w.kvh, it & 1, v);
+      few_probs(st[i], bits(i), fast, E, rp, mx, sl, phi, plo);
+      pv16(phi, plo, i > 0 ? v : v0, hi, lo);
+    }
+  }
+  few_store<NW>(a, w, lds, hi, lo, wave < ntiles);
+}
+
+// The place of a unit's chunk in smax and sden
+__device__ __forceinline__ i64 cell(const PackedArgs& a, const Work& w, int c) {
+  return (((i64)w.unit * a.n_kv + w.kvh) * a.nch + c) * 64;
+}
+// Over a row's chunks [0, nc): the maximum and, with DEN, the denominator of query
+// row i of the unit (lanes that share i take chunks in turn)
+template <bool DEN>
+__device__ __forceinline__ void over_chunks(const PackedArgs& a, const Work& w, int nc, int i,
+                                            int32_t* mx, i64* den) {
+  const int g4 = (threadIdx.x & 63) >> 4;
+  int m = NO_SCORE;
+  i64 d = 0;
+  for (int c0 = 0; c0 < nc; c0 += 16) {
+    int x[4];
+    i64 y[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int c = ::min(c0 + 4 * u + g4, nc - 1);
+      const i64 at = cell(a, w, c) + i;
+      x[u] = a.smax[at];
+      if (DEN) y[u] = a.sden[at];
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      m = ::max(m, x[u]);
+      if (DEN && c0 + 4 * u + g4 < nc) d = wadd(d, y[u]);
+    }
+  }
+  m = max16(m);
+  *mx = m == NO_SCORE ? 0 : m;
+  if (DEN) *den = imax(group4_sum(d), 1);
+}
+
+// One pass over chunk w.c of a few-row unit, four waves
+template <int PH>
+__device__ __forceinline__ void few_phase(const PackedArgs& a, const Work& w, FewLds<4>& lds) {
+  const int lane = threadIdx.x & 63, qi = lane & 15, g4 = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const int lo_s = w.c * a.chunk, hi_s = ::min(w.len, lo_s + a.chunk);
+  if (lo_s >= hi_s) return;
+  const int R = w.T << a.lg, nc = (w.len + a.chunk - 1) / a.chunk;
+  const i64 pitch = (i64)a.nch * a.chunk;
+  int32_t* const sc = a.scores + (((i64)w.b * a.n_kv + w.kvh) * a.few_rows) * pitch;
+  const int t0 = lo_s / 64, t1 = (hi_s + 63) / 64;
+  if constexpr (PH == PH_MAX) {
+    const FewRow row = few_row(a, w);
+    int mx = NO_SCORE;
+    // two tiles of K in flight a wave
+    for (int it = t0 + wave; it < t1; it += 8) {
+      v4i k[2][8];
+      int pg[2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+        pg[u] = __builtin_amdgcn_readfirstlane(it + 4 * u < t1 ? packed_page(a, w.b, (it + 4 * u) >> 1) : -1);
+#pragma unroll
+      for (int u = 0; u < 2; ++u) few_k(a, pg[u], w.kvh, (it + 4 * u) & 1, k[u]);
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int x = it + 4 * u;
+        if (x < t1) {
+          v4i st[4];
+          few_scores(k[u], row, st);
+          const uint32_t bb = pg[u] >= 0 ? seen16(row.limit, x * 64 + 16 * g4) : 0u;
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            int& s = ((int*)&st[e >> 2])[e & 3];
+            s = (bb >> e) & 1u ? s : NO_SCORE;
+            mx = ::max(mx, s);
+          }
+          if (row.on) {
+            v4i* o = (v4i*)(sc + qi * pitch + x * 64 + 16 * g4);
+#pragma unroll
+            for (int blk = 0; blk < 4; ++blk) o[blk] = st[blk];
+          }
+        }
+      }
+    }
+    mx = max16(mx);
+    if (g4 == 0) lds.mx[wave][qi] = mx;
+    __syncthreads();
+    if (threadIdx.x < 16) {
+#pragma unroll
+      for (int v = 0; v < 4; ++v) mx = ::max(mx, lds.mx[v][qi]);
+      a.smax[cell(a, w, w.c) + qi] = mx;
+    }
+  } else if constexpr (PH == PH_DEN) {
+    // a query row a wave, four slots a lane and load (chunks end on whole tiles)
+    for (int r = wave; r < R; r += 4) {
+      int m = NO_SCORE;
+      for (int c = lane; c < nc; c += 64) m = ::max(m, a.smax[cell(a, w, c) + r]);
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) m = ::max(m, __shfl_xor(m, d));
+      const int mx = m == NO_SCORE ? 0 : m;
+      const int t = r >> a.lg, g = r & ((1 << a.lg) - 1);
+      const i64 tpos = a.tpos[(i64)(w.tok0 + t) * a.n_q + (w.kvh << a.lg) + g];
+      const bool fast = tpos < FAST_T;  // (one row: uniform)
+      const RowExp E = make_rowexp(fast ? tpos : 1, mx);
+      ExpR Es{};
+      if (!fast) Es = make_exp(tpos);
+      const int32_t* src = sc + r * pitch;
+      i64 den = 0;
+      for (int s0 = lo_s + 4 * lane; s0 < t1 * 64; s0 += 1024) {
+        v4i x[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) x[u] = *(const v4i*)(src + (s0 + 256 * u < t1 * 64 ? s0 + 256 * u : s0));
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          if (s0 + 256 * u < t1 * 64) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int v = x[u][i];
+              if (fast) {
+                const uint32_t e = row_exp(v + E.c0, E);
+                den += v == NO_SCORE ? 0u : e;
+              } else if (v != NO_SCORE) {
+                den = wadd(den, slow_exp(v, mx, Es));
+              }
+            }
+          }
+      }
+      den = wave_sum(den);
+      if (lane == 0) a.sden[cell(a, w, w.c) + r] = den;
+    }
+  } else {
+    const FewRow row = few_row(a, w);
+    for (int i = threadIdx.x; i < 16 * 128; i += 256) ((int32_t*)lds.ctx)[i] = 0;
+    int32_t mx;
+    i64 den;
+    over_chunks<true>(a, w, nc, qi, &mx, &den);
+    if (!row.on) {
+      mx = 0;
+      den = 1;
+    }
+    const bool fast = __ballot(row.tpos >= FAST_T || den >= FAST_DEN) == 0;
+    const RowExp E = make_rowexp(row.tpos, mx);
+    const double rp = make_rowp(den);
+    RowSlow sl;
+    if (!fast) {
+      sl.E = make_exp(row.tpos);
+      sl.R = make_recip(den);
+    }
+    v4i hi[8], lo[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) hi[j] = lo[j] = v4i{0, 0, 0, 0};
+    __syncthreads();  // ctx is zero
+    const int32_t* src = sc + (row.on ? qi : 0) * pitch + 16 * g4;
+    for (int it = t0 + wave; it < t1; it += 8) {
+      v4i v[2][8], st[2][4];
+      int pg[2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+        pg[u] = __builtin_amdgcn_readfirstlane(it + 4 * u < t1 ? packed_page(a, w.b, (it + 4 * u) >> 1) : -1);
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int x = it + 4 * u < t1 ? it + 4 * u : it;
+#pragma unroll
+        for (int blk = 0; blk < 4; ++blk) st[u][blk] = *(const v4i*)(src + x * 64 + 4 * blk);
+        few_v(a, pg[u], w.kvh, (it + 4 * u) & 1, v[u]);
+      }
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+        if (it + 4 * u < t1) {
+          uint32_t bb = 0;
+#pragma unroll
+          for (int e = 0; e < 16; ++e) bb |= (st[u][e >> 2][e & 3] != NO_SCORE ? 1u : 0u) << e;
+          v4i phi, plo;
+          few_probs(st[u], row.on ? bb : 0u, fast, E, rp, mx, sl, phi, plo);
+          pv16(phi, plo, v[u], hi, lo);
+        }
+    }
+    few_store<4>(a, w, lds, hi, lo, true);
+  }
+}
+
+// ------------------------------------------------------------- 64 query rows
+//
+// Four waves of 16 query rows (row i: token i / G, head i % G of the kv head, so K
+// and V are read once for the kv head's query heads); key pages reach LDS by
+// direct-to-LDS loads, a 64 KB ring of them ahead of the pass, one barrier per
+// page, their 16-byte chunks swizzled against bank conflicts.
+
+constexpr int TL_K = 128 * 128;       // K page: 128 slot rows of 128 B
+constexpr int TL_V = 128 * 128;       // V page: 128 channel rows of 128 B
+constexpr int TL_RING = 64 * 1024;
+constexpr int TL_RESIDENT = TL_RING / (TL_K + TL_V);  // pages that stay for all three passes
+constexpr int TL_PAGES = 1024;        // pages of the longest row
+
+struct TileLds {
+  union {
+    __attribute__((aligned(1024))) int8_t ring[TL_RING];
+    FewLds<4> few;
+  };
+  int32_t pages[TL_PAGES];
+};
+
+// Physical chunk = logical ^ swizzle, so that the operand reads below take LDS's
+// full rate: bits 0, 1 and 4 of a K row, the low 3 bits of a V row
+__device__ __forceinline__ int tl_kswz(int row) { return (row & 3) | ((row >> 2) & 4); }
+__device__ __forceinline__ int tl_vswz(int d) { return d & 7; }
+
+template <int PH>
+__device__ __forceinline__ void tile_body(const PackedArgs& a, const Work& w, TileLds& lds) {
+  const int tid = threadIdx.x, lane = tid & 63, qi = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int R = w.T << a.lg;             // the row's query rows
+  const int r0 = w.tile * 64;            // the tile's first
+  const int rl = ::min(r0 + 63, R - 1);  // and last
+  // the tile's slots, and the chunk's of those
+  const int end = row_limit(a, w.past, rl >> a.lg) + 1;
+  const int lo_s = PH == PH_ALL ? 0 : w.c * a.chunk;
+  const int hi_s = PH == PH_ALL ? end : ::min(end, lo_s + a.chunk);
+  if (lo_s >= hi_s) return;
+  const int p0 = lo_s / DI_PAGE, np = (hi_s + DI_PAGE - 1) / DI_PAGE - p0;
+  const int wr0 = r0 + wave * 16;          // the wave's first query row
+  const bool work = wr0 < R;               // (waves without one only load)
+  const int qr = ::min(wr0 + qi, R - 1);   // the lane's (rows past the last: the last, not stored)
+  const int t = qr >> a.lg;
+  const int limit = row_limit(a, w.past, t);
+  const int wlim = row_limit(a, w.past, ::min(wr0, R - 1) >> a.lg);        // the wave's smallest
+  const int wmax = row_limit(a, w.past, ::min(wr0 + 15, R - 1) >> a.lg);   // and largest limit
+  const i64 qrow = (i64)(w.tok0 + t) * a.n_q + (w.kvh << a.lg) + (qr & ((1 << a.lg) - 1));
+  const v4i qf0 = *(const v4i*)(a.q8 + qrow * 128 + g * 16);
+  const v4i qf1 = *(const v4i*)(a.q8 + qrow * 128 + 64 + g * 16);
+  const i64 tpos = a.tpos[qrow];
+
+  int koffl[4], voffl[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int row = (wave * 4 + j) * 8 + (lane >> 3);
+    koffl[j] = row * 128 + ((lane & 7) ^ tl_kswz(row)) * 16;
+    voffl[j] = row * DI_PAGE + ((lane & 7) ^ tl_vswz(row)) * 16;
+  }
+  // a page that is not there: a view of no bytes, whose loads read 0
+  auto issue = [&](int page, int8_t* st, bool with_v) {
+    const int pg = __builtin_amdgcn_readfirstlane(page);
+    const int pgc = pg < 0 ? 0 : pg, n = pg < 0 ? 0 : DI_PAGE * 128;
+    const __amdgpu_buffer_rsrc_t krs = __builtin_amdgcn_make_buffer_rsrc(
+        (void*)a.kv.krow(pgc, w.kvh, 0), (short)0, n, 0x00020000);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(krs, (lds_ptr_t)(st + (wave * 4 + j) * 1024), 16,
+                                               koffl[j], 0, 0, 0);
+    if (with_v) {
+      const __amdgpu_buffer_rsrc_t vrs = __builtin_amdgcn_make_buffer_rsrc(
+          (void*)a.kv.vchan(pgc, w.kvh, 0), (short)0, n, 0x00020000);
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(
+            vrs, (lds_ptr_t)(st + TL_K + (wave * 4 + j) * 1024), 16, voffl[j], 0, 0, 0);
+    }
+  };
+  const bool resident = PH == PH_ALL && np <= TL_RESIDENT;
+  for (int i = tid; i < np; i += 256) lds.pages[i] = packed_page(a, w.b, p0 + i);
+  if (resident)
+    for (int i = 0; i < np; ++i)
+      issue(packed_page(a, w.b, p0 + i), lds.ring + i * (TL_K + TL_V), true);
+  wait_vmcnt<0>();  // queries, page ids; a resident tile's pages
+  __syncthreads();
+
+  // One pass over the pages; body(i, stage) runs with page i in LDS. Each wave
+  // waits for its own loads of the page (they complete in order), then one
+  // barrier publishes every wave's part and frees the stage that the next issue
+  // overwrites.
+  auto pass = [&](auto kv, auto&& body) {
+    constexpr bool KV = decltype(kv)::value;
+    constexpr int STAGE = KV ? TL_K + TL_V : TL_K;
+    constexpr int ST = TL_RING / STAGE;
+    constexpr int LPT = KV ? 8 : 4;  // loads per page and wave
+    if (resident) {
+      for (int i = 0; i < np; ++i) body(i, lds.ring + i * (TL_K + TL_V));
+      return;
+    }
+    wait_lds();
+    __builtin_amdgcn_s_barrier();  // the pass before is done with the ring
+#pragma unroll
+    for (int s = 0; s < ST - 1; ++s)
+      if (s < np) issue(lds.pages[s], lds.ring + s * STAGE, KV);
+    for (int i = 0; i < np; ++i) {
+      const int after = ::min(ST - 2, np - 1 - i);  // pages issued after this one
+      if (after >= 2) wait_vmcnt<2 * LPT>();
+      else if (after == 1) wait_vmcnt<LPT>();
+      else wait_vmcnt<0>();
+      wait_lds();
+      __builtin_amdgcn_s_barrier();
+      if (i + ST - 1 < np) issue(lds.pages[i + ST - 1], lds.ring + ((i + ST - 1) % ST) * STAGE, KV);
+      body(i, lds.ring + (i % ST) * STAGE);
+    }
+  };
+  const int kr = 16 * (qi >> 2) + (qi & 3);
+  const int koff0 = kr * 128 + ((g ^ tl_kswz(kr)) << 4);
+  const int koff1 = kr * 128 + (((g + 4) ^ tl_kswz(kr)) << 4);
+  auto load_k = [&](const int8_t* st, v4i (&kf)[8]) {
+#pragma unroll
+    for (int blk = 0; blk < 4; ++blk) {
+      kf[2 * blk] = *(const v4i*)(st + koff0 + blk * 512);
+      kf[2 * blk + 1] = *(const v4i*)(st + koff1 + blk * 512);
+    }
+  };
+  // both halves' scores from accumulators z, then fn(st, s0, hf) per half (its
+  // first slot s0); a page that is not there, or that no query row of the wave
+  // sees, is passed over
+  auto halves = [&](const int8_t* stg, int i, const v4i z, auto&& fn) {
+    const int s0 = (p0 + i) * DI_PAGE;
+    if (!work || s0 > wmax || __builtin_amdgcn_readfirstlane(lds.pages[i]) < 0) return;
+    v4i ka[8], kb[8], sa[4], sb[4];
+    load_k(stg, ka);
+    load_k(stg + 64 * 128, kb);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int blk = 0; blk < 4; ++blk) sa[blk] = mfma16(ka[2 * blk], qf0, z);
+#pragma unroll
+    for (int blk = 0; blk < 4; ++blk) sb[blk] = mfma16(kb[2 * blk], qf0, z);
+#pragma unroll
+    for (int blk = 0; blk < 4; ++blk) sa[blk] = mfma16(ka[2 * blk + 1], qf1, sa[blk]);
+#pragma unroll
+    for (int blk = 0; blk < 4; ++blk) sb[blk] = mfma16(kb[2 * blk + 1], qf1, sb[blk]);
+    __builtin_amdgcn_sched_barrier(0);
+    fn(sa, s0, 0);
+    if (s0 + 64 <= wmax) fn(sb, s0 + 64, 1);
+  };
+
+  int32_t mx = NO_SCORE;
+  if constexpr ((PH & PH_MAX) != 0) {
+    pass(std::false_type{}, [&](int i, const int8_t* stg) {
+      halves(stg, i, v4i{0, 0, 0, 0}, [&](const v4i (&st)[4], int s0, int) {
+        if (s0 + 63 <= wlim) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) mx = ::max(mx, st[e >> 2][e & 3]);
+        } else {
+          const uint32_t bits = seen16(limit, s0 + 16 * g);
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            if ((bits >> e) & 1u) mx = ::max(mx, st[e >> 2][e & 3]);
+        }
+      });
+    });
+    mx = max16(mx);
+    if constexpr (PH == PH_MAX) {
+      if (work && g == 0) a.smax[cell(a, w, w.c) + wave * 16 + qi] = mx;
+      return;
+    }
+    if (mx == NO_SCORE) mx = 0;  // nothing seen: max := 0, every p = 0
+  }
+  const int nc = (end + a.chunk - 1) / a.chunk;
+  i64 den = 0;
+  if constexpr (PH == PH_DEN) over_chunks<false>(a, w, nc, ::min(wr0 + qi, R - 1) - r0, &mx, &den);
+  if constexpr (PH == PH_PV) over_chunks<true>(a, w, nc, ::min(wr0 + qi, R - 1) - r0, &mx, &den);
+
+  const bool fast_e = __ballot(tpos >= FAST_T) == 0;
+  const RowExp E = make_rowexp(fast_e ? tpos : 1, mx);
+  // the accumulators of the slow forms start from 0
+  const int32_t c0 = fast_e ? E.c0 : 0;
+  const v4i cinit = v4i{c0, c0, c0, c0};
+  RowSlow sl;
+  if (DI_UNLIKELY(!fast_e)) sl.E = make_exp(tpos);
+  if constexpr ((PH & PH_DEN) != 0) {
+    den = 0;
+    pass(std::false_type{}, [&](int i, const int8_t* stg) {
+      halves(stg, i, cinit, [&](const v4i (&st)[4], int s0, int) {
+        if (DI_LIKELY(fast_e)) {
+          uint32_t sum = 0;
+          if (s0 + 63 <= wlim) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) sum += row_exp(st[e >> 2][e & 3], E);
+          } else {
+            const uint32_t bits = seen16(limit, s0 + 16 * g);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              const uint32_t x = row_exp(st[e >> 2][e & 3], E);
+              sum += (bits >> e) & 1u ? x : 0u;
+            }
+          }
+          den += sum;
+        } else {
+          den = wadd(den, few_den(st, seen16(limit, s0 + 16 * g), false, E, mx, sl.E));
+        }
+      });
+    });
+    den = group4_sum(den);
+    if constexpr (PH == PH_DEN) {
+      if (work && g == 0) a.sden[cell(a, w, w.c) + wave * 16 + qi] = den;
+      return;
+    }
+    den = imax(den, 1);
+  }
+  const bool fast = fast_e && __ballot(den >= FAST_DEN) == 0;
+  const double rp = make_rowp(den);
+  if (DI_UNLIKELY(!fast)) {
+    sl.E = make_exp(tpos);
+    sl.R = make_recip(den);
+  }
+  // (a wave of few rows' exponentials in the fast form and its quotients not: the
+  // slow forms take the scores back from the accumulators)
+  v4i ohi[8], olo[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) ohi[j] = olo[j] = v4i{0, 0, 0, 0};
+  int voff[2];
+#pragma unroll
+  for (int hf = 0; hf < 2; ++hf) voff[hf] = TL_K + qi * 128 + (((4 * hf + g) ^ tl_vswz(qi)) << 4);
+  pass(std::true_type{}, [&](int i, const int8_t* stg) {
+    halves(stg, i, cinit, [&](const v4i (&st)[4], int s0, int hf) {
+      v4i vf[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) vf[j] = *(const v4i*)(stg + voff[hf] + j * 2048);
+      __builtin_amdgcn_sched_barrier(0);
+      v4i phi, plo;
+      const bool full = s0 + 63 <= wlim;
+      if (DI_LIKELY(fast && full)) {
+#pragma unroll
+        for (int blk = 0; blk < 4; ++blk) {
+          uint32_t w4[4];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) w4[r] = row_p128(row_exp(st[blk][r], E), rp);
+          int h, l;
+          pack4(w4, h, l);
+          phi[blk] = h;
+          plo[blk] = l;
+        }
+      } else {
+        const uint32_t bits = seen16(limit, s0 + 16 * g);
+#pragma unroll
+        for (int blk = 0; blk < 4; ++blk) {
+          uint32_t w4[4];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const bool vis = (bits >> (4 * blk + r)) & 1u;
+            if (fast) {
+              const uint32_t x = row_exp(st[blk][r], E);
+              w4[r] = row_p128(vis ? x : 0u, rp);
+            } else {
+              w4[r] = vis ? slow_p128(slow_exp(st[blk][r] - c0, mx, sl.E), sl.R) : 128u;
+            }
+          }
+          int h, l;
+          pack4(w4, h, l);
+          phi[blk] = h;
+          plo[blk] = l;
+        }
+      }
+      pv16(phi, plo, vf, ohi, olo);
+    });
+  });
+  if (!work) return;
+  // lane (qi, g): query rows 4 g + r of the wave, channel 16 j + qi
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const int row = wr0 + 4 * g + r;
+    if (row < R) {
+      const i64 at = ((i64)(w.tok0 + (row >> a.lg)) * a.n_q + (w.kvh << a.lg) +
+                      (row & ((1 << a.lg) - 1))) * 128 + qi;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int x = ohi[j][r] * 256 + olo[j][r];
+        if (a.part) a.part[(i64)w.c * a.N * a.n_q * 128 + at + 16 * j] = x;
+        else a.out[at + 16 * j] = x;
+      }
+    }
+  }
+}
+
+}  // namespace

@@ -1,0 +1,224 @@
+// Attention of packed rows over the paged cache (gfx950): each row has its own
+// number of new tokens (none, one, a draft, a prompt's chunk), their token rows
+// follow each other, and token t of a row at `past` slots sees the row's slots up
+// to past + t. The integers of a query are those of the prefill attention.
+//
+// The rows' lengths are on the device, so a block finds its work itself: the
+// launch is sized by bounds (token rows, rows, slots), a block's unit is a row of
+// at most 16 query rows (tokens x query heads of a kv head) or 64 query rows of a
+// longer one, and every wave finds it by a scan of the rows' lengths, one round
+// trip, with no launch before it and nothing read on the host.
+//
+// DI-Exp is not multiplicative: the row maximum comes before the first
+// exponential, the whole denominator before the first probability. One launch
+// makes all three passes (k_packed_one: short rows, or enough units to fill the
+// chip); else each pass is a launch over chunks of the slots (k_packed_phase),
+// whose maxima, denominators and int32 contexts meet in scratch.
+#include "attn_packed.h"
+
+#include "../../include/detllm_hip.h"
+
+namespace {
+
+// Rows of at most 16 query rows alone, all slots in registers: NW waves, NT
+// 64-slot tiles each.
+template <int NT>
+__global__ __launch_bounds__(512, 2) void k_packed_few(PackedArgs a) {
+  keep_hidden_args();
+  __shared__ FewLds<8> lds;
+  const Work w = find_work(a);
+  if (!w.live) {
+    zero_tail(a, w);
+    return;
+  }
+  report_row(a, w);
+  few_one<8, NT>(a, w, lds);
+}
+
+// All three passes of any rows
+__global__ __launch_bounds__(256, 2) void k_packed_one(PackedArgs a) {
+  keep_hidden_args();
+  __shared__ TileLds lds;
+  const Work w = find_work(a);
+  if (!w.live) {
+    zero_tail(a, w);
+    return;
+  }
+  report_row(a, w);
+  if (w.few && w.len <= FEW_ONE_SLOTS) few_one<4, FEW_ONE_SLOTS / 256>(a, w, lds.few);
+  else tile_body<PH_ALL>(a, w, lds);
+}
+
+// One pass over a chunk. FEW: the launch's rows have at most 16 query rows
+template <int PH, bool FEW>
+__global__ __launch_bounds__(256, FEW ? 4 : 2) void k_packed_phase(PackedArgs a) {
+  keep_hidden_args();
+  const Work w = find_work(a);
+  if (!w.live) {
+    if (PH == PH_PV && a.nch == 1) zero_tail(a, w);
+    return;
+  }
+  if (PH == PH_MAX) report_row(a, w);
+  if constexpr (FEW) {
+    __shared__ FewLds<4> lds;
+    few_phase<PH>(a, w, lds);
+  } else {
+    __shared__ TileLds lds;
+    if (w.few) few_phase<PH>(a, w, lds.few);
+    else tile_body<PH>(a, w, lds);
+  }
+}
+
+// The chunks' contexts of a token added up (one block per token row)
+__global__ __launch_bounds__(256) void k_packed_join(PackedArgs a) {
+  keep_hidden_args();
+  const int tok = blockIdx.x, cols = a.n_q * 128, lane = threadIdx.x & 63;
+  int b = 0;  // rows that end at or before this token
+  int last = 0;
+  for (int b0 = 0; b0 < a.B; b0 += 64) {
+    const int i = b0 + lane;
+    const int e = a.cu[i < a.B ? i + 1 : a.B];
+    b += __popcll(__ballot(i < a.B && e <= tok));
+  }
+  int nc = 0;
+  if (b < a.B) {
+    last = ::max(0, a.cu[b]);
+    nc = (row_limit(a, a.past[b], tok - last) + a.chunk) / a.chunk;  // ceil((limit + 1) / chunk)
+    if (tok < last || tok - last >= a.max_new) nc = 0;
+  }
+  for (int i = 4 * threadIdx.x; i < cols; i += 1024) {
+    v4i sum = v4i{0, 0, 0, 0};
+    const int32_t* p = a.part + (i64)tok * cols + i;
+    for (int c = 0; c < nc; c += 4) {
+      v4i x[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) x[u] = *(const v4i*)(p + (i64)::min(c + u, nc - 1) * a.N * cols);
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (c + u < nc) sum += x[u];
+    }
+    int64_t* o = a.out + (i64)tok * cols + i;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) o[r] = sum[r];
+  }
+}
+
+// How a call is cut, from bounds on its sizes
+struct Plan {
+  bool few;    // every row has at most 16 query rows
+  bool one;    // one launch
+  int units;   // units that the rows can make, and one for the tail
+  int rows;    // query rows of a few-row unit
+  int chunk, nch;
+  i64 scores_at, max_at, den_at, part_at, bytes;
+};
+
+// us a call, one launch against chunks, stand beside the rules (16 query heads,
+// 8 kv heads).
+inline Plan packed_plan(int N, int B, int S, int max_new, int n_q, int n_kv) {
+  Plan p{};
+  const int G = n_q / n_kv;
+  const i64 most = imin(max_new, N);
+  p.few = most * G <= 16;
+  const i64 rows = ::min(B, N);
+  const i64 units = p.few ? rows : imin((i64)N * G / 64 + rows, N);
+  p.units = (int)units + 1;
+  p.rows = (int)imin(16, most * G);
+  const i64 pairs = units * n_kv;
+  p.one = p.few ? S <= FEW_SLOTS : S <= FEW_ONE_SLOTS;
+  p.chunk = S;
+  if (!p.one) {
+    // chunks for about 1024 blocks
+    const i64 want = imax(1, imin((S + 511) / 512, 1024 / imax(1, pairs)));
+    p.chunk = (int)(((S + want - 1) / want + DI_PAGE - 1) / DI_PAGE * DI_PAGE);
+  }
+  p.chunk = ::max(p.chunk, 1);
+  p.nch = ::max(1, (S + p.chunk - 1) / p.chunk);
+  if (p.one) return p;
+  auto room = [&](i64 n) {
+    const i64 at = p.bytes;
+    p.bytes += (n + 15) / 16 * 16;
+    return at;
+  };
+  p.scores_at = room((i64)B * n_kv * p.rows * p.nch * p.chunk * 4);
+  const i64 cells = (i64)p.units * n_kv * p.nch * 64;
+  p.max_at = room(cells * 4);
+  p.den_at = room(cells * 8);
+  p.part_at = room(p.nch > 1 ? (i64)p.nch * N * n_q * 128 * 4 : 0);
+  return p;
+}
+
+inline int packed_check(int N, int B, int S, int max_new, int n_q, int n_kv) {
+  if (N < 0 || B < 1 || S < 1 || max_new < 0 || n_q <= 0 || n_kv <= 0 || n_q % n_kv) return DI_EINVAL;
+  const int G = n_q / n_kv;
+  if (G != 1 && G != 2 && G != 4 && G != 8) return DI_ENOSYS;
+  if (S > PACKED_MAX_S || B > PACKED_MAX_ROWS || (i64)N * n_q > (1 << 24)) return DI_ERANGE;
+  return DI_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int detllm_attn_packed_work(int N, int B, int S, int max_new, int n_q, int n_kv, int64_t* bytes) {
+  if (!bytes) return DI_EINVAL;
+  const int rc = packed_check(N, B, S, max_new, n_q, n_kv);
+  if (rc != DI_OK) return rc;
+  *bytes = packed_plan(N, B, S, max_new, n_q, n_kv).bytes;
+  return DI_OK;
+}
+
+int detllm_attn_packed(const int8_t* q8, const int64_t* tpos, const int8_t* kpool,
+                       const int8_t* vpool, int n_pages, const int32_t* table, int width,
+                       const int32_t* cu, const int32_t* past, int N, int B, int S, int max_new,
+                       int n_q, int n_kv, void* work, int64_t work_bytes, int64_t* out,
+                       int32_t* err, hipStream_t s) {
+  const int rc = packed_check(N, B, S, max_new, n_q, n_kv);
+  if (rc != DI_OK) return rc;
+  if (N == 0) return DI_OK;
+  if (!q8 || !tpos || !kv_ok(kpool, vpool, table, width) || n_pages < 1 || !cu || !past || !out ||
+      S > (i64)width * DI_PAGE)
+    return DI_EINVAL;
+  const Plan p = packed_plan(N, B, S, max_new, n_q, n_kv);
+  if (p.bytes > 0 && (!work || ((uintptr_t)work & 15))) return DI_EINVAL;
+  if (work_bytes < p.bytes) return DI_ERANGE;
+  PackedArgs a{};
+  a.q8 = q8; a.tpos = tpos;
+  a.kv = KVPages{(int8_t*)kpool, (int8_t*)vpool, table, width, n_kv};
+  a.n_pages = n_pages; a.cu = cu; a.past = past; a.N = N; a.B = B; a.S = S;
+  a.n_q = n_q; a.n_kv = n_kv; a.lg = n_q / n_kv == 1 ? 0 : n_q / n_kv == 2 ? 1 : n_q / n_kv == 4 ? 2 : 3;
+  a.max_new = max_new; a.few_rows = p.rows; a.units = p.units; a.chunk = p.chunk; a.nch = p.nch; a.out = out; a.err = err;
+  char* const w = (char*)work;
+  a.scores = (int32_t*)(w + p.scores_at);
+  a.smax = (int32_t*)(w + p.max_at);
+  a.sden = (int64_t*)(w + p.den_at);
+  a.part = p.nch > 1 ? (int32_t*)(w + p.part_at) : nullptr;
+  const i64 blocks = (i64)p.units * p.nch * n_kv;
+  if (blocks > 0x7fffffff) return DI_ERANGE;
+  const dim3 grid((unsigned)blocks);
+  if (p.one) {
+    if (!p.few) hipLaunchKernelGGL(k_packed_one, grid, dim3(256), 0, s, a);
+    else if (S <= 512) hipLaunchKernelGGL(k_packed_few<1>, grid, dim3(512), 0, s, a);
+    else if (S <= 1024) hipLaunchKernelGGL(k_packed_few<2>, grid, dim3(512), 0, s, a);
+    else hipLaunchKernelGGL(k_packed_few<4>, grid, dim3(512), 0, s, a);
+    DI_LAUNCH_CHECK();
+    return DI_OK;
+  }
+#define DI_PHASES(FEW_)                                                              \
+  hipLaunchKernelGGL((k_packed_phase<PH_MAX, FEW_>), grid, dim3(256), 0, s, a);      \
+  DI_LAUNCH_CHECK();                                                                 \
+  hipLaunchKernelGGL((k_packed_phase<PH_DEN, FEW_>), grid, dim3(256), 0, s, a);      \
+  DI_LAUNCH_CHECK();                                                                 \
+  hipLaunchKernelGGL((k_packed_phase<PH_PV, FEW_>), grid, dim3(256), 0, s, a);       \
+  DI_LAUNCH_CHECK()
+  if (p.few) { DI_PHASES(true); }
+  else { DI_PHASES(false); }
+#undef DI_PHASES
+  if (p.nch > 1) {
+    hipLaunchKernelGGL(k_packed_join, dim3(N), dim3(256), 0, s, a);
+    DI_LAUNCH_CHECK();
+  }
+  return DI_OK;
+}
+
+}  // extern "C"

@@ -27,6 +27,7 @@
 #define DI_ERR_TOKEN 1     // token id outside [-vocab, vocab)
 #define DI_ERR_POSITION 2  // position outside [-max_pos, max_pos)
 #define DI_ERR_SLOTS 4     // device slot count beyond the launch's slot bound
+#define DI_ERR_PAGES 8     // free pages too few (or too many) for a packed step
 
 // Slots per page of the paged KV cache.
 #define DI_PAGE 128

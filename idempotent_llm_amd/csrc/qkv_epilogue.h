@@ -52,6 +52,23 @@ struct QKVArgs {
   int32_t* err;  // optional device error word (DI_ERR_POSITION)
 };
 
+// The same for packed token rows (T = 1): row r's K and V go to its own entry of
+// a slot map, page * DI_PAGE + offset (negative or past the pools: not stored),
+// instead of slot base + t of a row's pages.
+struct QKVSlotArgs : QKVArgs {
+  const int64_t* slots;  // [R]
+  i64 n_slots;           // slots of the pools: pages * DI_PAGE
+};
+template <class A>
+constexpr bool kSlotMap = std::is_same_v<A, QKVSlotArgs>;
+
+// The page of row b's slot (-1: not stored); the offset is slot % DI_PAGE
+template <class A>
+__device__ __forceinline__ int page_of(const A& a, int b, i64 slot) {
+  if constexpr (kSlotMap<A>) return slot >= 0 && slot < a.n_slots ? (int)(slot >> 7) : -1;
+  else return a.kv.page(b, slot);
+}
+
 // The static K requantisation's divisor of one channel (model.py:326-329,
 // requant_i8_static with row scale (1, rowk)): den = kq_m << max(rowk - kq_k,
 // 0) (wrapping as torch's shift does; 1 if it is 0, where the reference's
@@ -457,7 +474,8 @@ __device__ __forceinline__ i64 q_head_tpos(const QKVArgs& a, i64 am, i64 ksm, i6
 // (global memory for the standalone kernel, LDS for the fused one), or,
 // with am_out, its quantisation maximum am to *am_out for q_head_tpos
 // later. `in`: qkv_head_load then qkv_head_rope_load of the same (r, slotw).
-__device__ __forceinline__ void qkv_head_compute(const QKVArgs& a, int r, int slotw,
+template <class A>
+__device__ __forceinline__ void qkv_head_compute(const A& a, int r, int slotw,
                                                  const QKVHeadIn& in, int8_t* q8_out,
                                                  int64_t* tpos_out, int8_t* k_lds = nullptr,
                                                  int64_t* am_out = nullptr) {
@@ -480,7 +498,7 @@ __device__ __forceinline__ void qkv_head_compute(const QKVArgs& a, int r, int sl
     const i64 up = imax(wneg(shift), 0), down = imax(shift, 0);
     i64 den = shl(vqm, down);
     if (den == 0) den = 1;  // the reference's division raises there
-    const int pg = a.kv.page(b, slot);
+    const int pg = page_of(a, b, slot);
     int8_t o0, o1;
     // the prefill form's exact fp64 n where the operands allow it
     constexpr i64 WM_LIM = (i64)1 << 21;
@@ -579,7 +597,7 @@ __device__ __forceinline__ void qkv_head_compute(const QKVArgs& a, int r, int sl
     }
   }
   if (!is_q) {
-    const int pg = a.kv.page(b, slot);
+    const int pg = page_of(a, b, slot);
     if (pg >= 0) {
       int8_t* krow = a.kv.krow(pg, h, (int)(slot & (DI_PAGE - 1)));
       krow[c0] = (int8_t)o[0];
@@ -600,9 +618,13 @@ __device__ __forceinline__ void qkv_head_compute(const QKVArgs& a, int r, int sl
   }
 }
 
-__device__ __forceinline__ void qkv_head(const QKVArgs& a, int r, int slotw, int8_t* q8_out,
+template <class A>
+__device__ __forceinline__ void qkv_head(const A& a, int r, int slotw, int8_t* q8_out,
                                          int64_t* tpos_out, int8_t* k_lds = nullptr) {
-  QKVHeadIn in = qkv_head_load(a, r, slotw, qkv_scalars(a, r, slotw, slot_base_of(a)));
+  i64 base;
+  if constexpr (kSlotMap<A>) base = a.slots[r];
+  else base = slot_base_of(a);
+  QKVHeadIn in = qkv_head_load(a, r, slotw, qkv_scalars(a, r, slotw, base));
   qkv_head_rope_load(a, slotw, in);
   qkv_head_compute(a, r, slotw, in, q8_out, tpos_out, k_lds);
   qkv_head_report(a, slotw, in);
@@ -643,8 +665,8 @@ typedef short v4s_u __attribute__((ext_vector_type(4), aligned(2)));  // any int
 // wave (qkv_head: any operands), over what the fast passes stored. After the
 // passes, so that their registers are free. Slow, for what the quantiser never
 // makes: 2048 rows of 32 heads whose gammas pass 2^14 take 93 us, not 25.
-template <int NG>
-__device__ __forceinline__ void qkv_rows_redo(const QKVArgs& a, int R, int r0, int slotw,
+template <int NG, class A>
+__device__ __forceinline__ void qkv_rows_redo(const A& a, int R, int r0, int slotw,
                                               uint32_t bad) {
   __threadfence_block();  // the passes' stores are ahead of these
   const int h = slotw < a.n_q ? slotw : 0;
@@ -662,8 +684,8 @@ __device__ __forceinline__ void qkv_rows_redo(const QKVArgs& a, int R, int r0, i
 // nothing. KIND: the head slot's kind (0 query, 1 key, 2 value), so that each
 // kind holds its own operands only. Returns the passes (bit i) in which some
 // row left the fp64 forms' bounds: what they stored is redone (qkv_rows_redo).
-template <int NG, int KIND>
-__device__ __forceinline__ uint32_t qkv_rows_kind(const QKVArgs& a, int R, int r0, int slotw) {
+template <int NG, int KIND, class A>
+__device__ __forceinline__ uint32_t qkv_rows_kind(const A& a, int R, int r0, int slotw) {
   static_assert(NG == 1 || NG == 2 || NG == 4, "rows per lane");
   const int lane = threadIdx.x & 63, g = lane >> 4, j = lane & 15;
   const int n_heads = a.n_q + 2 * a.n_kv;
@@ -704,7 +726,8 @@ __device__ __forceinline__ uint32_t qkv_rows_kind(const QKVArgs& a, int R, int r
   };
   int32_t p[8];
   load_p(row(0), p);
-  const i64 base = slot_base_of(a);
+  i64 base = 0;
+  if constexpr (!kSlotMap<A>) base = slot_base_of(a);
   uint32_t bad = 0;  // bit i: pass i left the fp64 forms' bounds in some row (wave-uniform)
   float wm[8];
   bool hok = true;  // the head's mantissas are inside qk_head_f64's bounds
@@ -720,8 +743,9 @@ __device__ __forceinline__ uint32_t qkv_rows_kind(const QKVArgs& a, int R, int r
   // page of a row's slot (-1: not stored), its slot
   auto place = [&](int i, i64* slot) {
     const int r = row(i), b = r / a.T, t = r - b * a.T;
-    *slot = base + t;
-    return rl + i < R ? a.kv.page(b, *slot) : -1;
+    if constexpr (kSlotMap<A>) *slot = a.slots[r];
+    else *slot = base + t;
+    return rl + i < R ? page_of(a, b, *slot) : -1;
   };
 
   if constexpr (is_v) {
@@ -766,10 +790,16 @@ __device__ __forceinline__ uint32_t qkv_rows_kind(const QKVArgs& a, int R, int r
     // row that start at a multiple of NG (then they share a page too), else
     // a byte each
     using VWord = std::conditional_t<NG == 4, uint32_t, uint16_t>;
-    const int b0 = row(0) / a.T;
     i64 slot;
     const int pg = place(0, &slot);
-    if (NG > 1 && rl + NG <= R && (rl + NG - 1) / a.T == b0 && (slot & (NG - 1)) == 0) {
+    bool together = NG > 1 && rl + NG <= R;
+    if constexpr (kSlotMap<A>) {
+#pragma unroll
+      for (int i = 1; i < NG; ++i) together = together && a.slots[row(i)] == slot + i;
+    } else {
+      together = together && (rl + NG - 1) / a.T == row(0) / a.T;
+    }
+    if (together && (slot & (NG - 1)) == 0) {
       if (pg >= 0) {
 #pragma unroll
         for (int k = 0; k < 8; ++k)
@@ -924,22 +954,22 @@ __device__ __forceinline__ uint32_t qkv_rows_kind(const QKVArgs& a, int R, int r
 // segment, so that the passes do not hold all of it in scalar registers:
 // three to four waves per SIMD at NG = 1, 2048 rows of 48 heads at NG = 4 36.2
 // -> 35.3 us).
-template <int NG>
-__device__ __forceinline__ void qkv_rows(const QKVArgs& a, int R, int r0, int slotw) {
+template <int NG, class A>
+__device__ __forceinline__ void qkv_rows(const A& a, int R, int r0, int slotw) {
   uint32_t bad;
-  if (slotw < a.n_q) bad = qkv_rows_kind<NG, 0>(a, R, r0, slotw);
-  else if (slotw < a.n_q + a.n_kv) bad = qkv_rows_kind<NG, 1>(a, R, r0, slotw);
-  else bad = qkv_rows_kind<NG, 2>(a, R, r0, slotw);
+  if (slotw < a.n_q) bad = qkv_rows_kind<NG, 0, A>(a, R, r0, slotw);
+  else if (slotw < a.n_q + a.n_kv) bad = qkv_rows_kind<NG, 1, A>(a, R, r0, slotw);
+  else bad = qkv_rows_kind<NG, 2, A>(a, R, r0, slotw);
   if (DI_UNLIKELY(bad != 0)) {
     struct Words {
-      u64 w[sizeof(QKVArgs) / 8];
+      u64 w[sizeof(A) / 8];
     } args;
-    static_assert(sizeof(QKVArgs) % 8 == 0 && std::is_trivially_copyable_v<QKVArgs>);
+    static_assert(sizeof(A) % 8 == 0 && std::is_trivially_copyable_v<A>);
     auto src = (const __attribute__((address_space(4))) u64*)__builtin_amdgcn_kernarg_segment_ptr();
     asm volatile("" : "+s"(src));  // (not the loads made at the kernel's start)
 #pragma unroll
-    for (int i = 0; i < (int)(sizeof(QKVArgs) / 8); ++i) args.w[i] = src[i];
-    qkv_rows_redo<NG>(__builtin_bit_cast(QKVArgs, args), R, r0, slotw, bad);
+    for (int i = 0; i < (int)(sizeof(A) / 8); ++i) args.w[i] = src[i];
+    qkv_rows_redo<NG, A>(__builtin_bit_cast(A, args), R, r0, slotw, bad);
   }
 }
 

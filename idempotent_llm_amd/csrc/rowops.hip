@@ -1108,7 +1108,8 @@ __global__ __launch_bounds__(NT) void k_merge_rowcol(MergeArgs a) {
   merge_rowcol_row<VPT>(a, (int)blockIdx.x - (WARM ? L2WARM_BLOCKS : 0), red);
 }
 
-__global__ __launch_bounds__(RT) void k_qkv_epilogue(QKVArgs a) {
+template <class A>
+__global__ __launch_bounds__(RT) void k_qkv_epilogue(A a) {
   keep_hidden_args();
   const int slotw = blockIdx.y * 4 + (threadIdx.x >> 6);
   if (slotw >= a.n_q + 2 * a.n_kv) return;
@@ -1122,8 +1123,8 @@ __global__ __launch_bounds__(RT) void k_qkv_epilogue(QKVArgs a) {
 // so a block's waves share a head's scale vectors. Waves per SIMD: four, at NG
 // = 2 three (149 VGPRs; four spill 72: 1000 rows of 32 heads 17.9 against 16.9
 // us, 500 13.8 against 10.7).
-template <int NG>
-__global__ __launch_bounds__(RT, NG == 2 ? 3 : 4) void k_qkv_epilogue_rows(QKVArgs a, int R,
+template <int NG, class A>
+__global__ __launch_bounds__(RT, NG == 2 ? 3 : 4) void k_qkv_epilogue_rows(A a, int R,
                                                                            int ngroups) {
   keep_hidden_args();
   const int heads = a.n_q + 2 * a.n_kv;
@@ -1131,7 +1132,7 @@ __global__ __launch_bounds__(RT, NG == 2 ? 3 : 4) void k_qkv_epilogue_rows(QKVAr
   const int wg = __builtin_amdgcn_readfirstlane((int)(blockIdx.x * 4 + (threadIdx.x >> 6)));
   if (wg >= heads * ngroups) return;  // whole waves only
   const int slotw = wg / ngroups, grp = wg - slotw * ngroups;
-  qkv_rows<NG>(a, R, grp * 4 * NG, slotw);
+  qkv_rows<NG, A>(a, R, grp * 4 * NG, slotw);
 }
 
 // Bookkeeping of one graphed decode step before its replay (graphed.py:112-131
@@ -1914,6 +1915,38 @@ static bool rows_wave_launch(int R, int C, hipStream_t s, ResNormArgs& a) {
   return true;
 }
 
+// The Q/K/V epilogue of R token rows
+template <class A>
+static int qkv_epilogue_launch(const A& a, int R, hipStream_t s) {
+  const int heads = a.n_q + 2 * a.n_kv;
+  // the rows layout reads P 16 bytes at a time
+  if (R > 64 && (a.nsplit == 1 || a.split_stride % 4 == 0) && ((uintptr_t)a.P & 15) == 0) {
+    // Rows per lane, by (row, head) pairs: a lane that takes more rows shares
+    // the scale vectors among them, one that takes fewer leaves more waves to
+    // the chip. One row up to 21504 pairs (a round and a third of four waves
+    // per SIMD), two up to 49152 (two rounds of three), then four. us at 1 / 2
+    // / 4 rows per lane: 32 heads 200 rows 7.2 / 7.6 / 14.1, 600 11.5 / 12.9 /
+    // 14.5, 700 13.8 / 13.1 / 17.9, 1000 18.6 / 16.9 / 18.6, 1200 - / 20.2 /
+    // 20.1, 1500 - / 23.1 / 23.5, 2048 - / 27.9 / 25.0; 10 heads 2048 rows 11.9
+    // / 12.2 / 17.7, 3000 17.2 / 16.7 / 19.2, 4096 - / 18.6 / 22.7; 48 heads 400
+    // rows 11.4 / 11.5 / 14.5, 500 14.0 / 12.8 / 18.0, 1000 - / 22.2 / 23.3, 1152
+    // - / 25.3 / 24.0.
+    const i64 pairs = (i64)R * heads;
+    const int ng = pairs < 21504 ? 1 : (pairs < 49152 ? 2 : 4);
+    const int ngroups = (R + 4 * ng - 1) / (4 * ng);
+    const i64 waves = (i64)ngroups * heads;
+    if (waves > 0x7fffffff) return DI_ERANGE;
+    const dim3 grid((unsigned)((waves + 3) / 4));
+    if (ng == 4) hipLaunchKernelGGL((k_qkv_epilogue_rows<4, A>), grid, dim3(RT), 0, s, a, R, ngroups);
+    else if (ng == 2) hipLaunchKernelGGL((k_qkv_epilogue_rows<2, A>), grid, dim3(RT), 0, s, a, R, ngroups);
+    else hipLaunchKernelGGL((k_qkv_epilogue_rows<1, A>), grid, dim3(RT), 0, s, a, R, ngroups);
+  } else {
+    hipLaunchKernelGGL(k_qkv_epilogue<A>, dim3(R, (heads + 3) / 4), dim3(RT), 0, s, a);
+  }
+  DI_LAUNCH_CHECK();
+  return DI_OK;
+}
+
 extern "C" {
 
 // ---------------------------------------------------------------- model path
@@ -2231,34 +2264,34 @@ int detllm_qkv_epilogue(const int32_t* P, int nsplit, int64_t split_stride, int 
   a.sin_t = sin_t; a.max_pos = max_pos; a.q8 = q8; a.tpos = tpos; a.dbg = dbg;
   a.kv = KVPages{kpool, vpool, table, width, n_kv}; a.slot_base_dev = slot_base_dev;
   a.slot_base = slot_base; a.kq_est = kq_est; a.err = err;
-  const int heads = n_q + 2 * n_kv;
-  const int R = B * T;
-  // the rows layout reads P 16 bytes at a time
-  if (R > 64 && (nsplit == 1 || split_stride % 4 == 0) && ((uintptr_t)P & 15) == 0) {
-    // Rows per lane, by (row, head) pairs: a lane that takes more rows shares
-    // the scale vectors among them, one that takes fewer leaves more waves to
-    // the chip. One row up to 21504 pairs (a round and a third of four waves
-    // per SIMD), two up to 49152 (two rounds of three), then four. us at 1 / 2
-    // / 4 rows per lane: 32 heads 200 rows 7.2 / 7.6 / 14.1, 600 11.5 / 12.9 /
-    // 14.5, 700 13.8 / 13.1 / 17.9, 1000 18.6 / 16.9 / 18.6, 1200 - / 20.2 /
-    // 20.1, 1500 - / 23.1 / 23.5, 2048 - / 27.9 / 25.0; 10 heads 2048 rows 11.9
-    // / 12.2 / 17.7, 3000 17.2 / 16.7 / 19.2, 4096 - / 18.6 / 22.7; 48 heads 400
-    // rows 11.4 / 11.5 / 14.5, 500 14.0 / 12.8 / 18.0, 1000 - / 22.2 / 23.3, 1152
-    // - / 25.3 / 24.0.
-    const i64 pairs = (i64)R * heads;
-    const int ng = pairs < 21504 ? 1 : (pairs < 49152 ? 2 : 4);
-    const int ngroups = (R + 4 * ng - 1) / (4 * ng);
-    const i64 waves = (i64)ngroups * heads;
-    if (waves > 0x7fffffff) return DI_ERANGE;
-    const dim3 grid((unsigned)((waves + 3) / 4));
-    if (ng == 4) hipLaunchKernelGGL(k_qkv_epilogue_rows<4>, grid, dim3(RT), 0, s, a, R, ngroups);
-    else if (ng == 2) hipLaunchKernelGGL(k_qkv_epilogue_rows<2>, grid, dim3(RT), 0, s, a, R, ngroups);
-    else hipLaunchKernelGGL(k_qkv_epilogue_rows<1>, grid, dim3(RT), 0, s, a, R, ngroups);
-  } else {
-    hipLaunchKernelGGL(k_qkv_epilogue, dim3(R, (heads + 3) / 4), dim3(RT), 0, s, a);
-  }
-  DI_LAUNCH_CHECK();
-  return DI_OK;
+  return qkv_epilogue_launch(a, B * T, s);
+}
+
+int detllm_qkv_epilogue_packed(
+    const int32_t* P, int nsplit, int64_t split_stride, int N, int n_q, int n_kv,
+    const int64_t* xm, const int64_t* xk, const int64_t* positions, const int64_t* slots,
+    const int64_t* q_m, int64_t q_k, const int64_t* k_m, int64_t k_k, const int64_t* v_m,
+    int64_t v_k, const int64_t* q_norm_m, int64_t q_norm_k, const int64_t* k_norm_m,
+    int64_t k_norm_k, const int64_t* qs_m, int64_t qs_k, const int64_t* kq_m, const int64_t* kq_k,
+    const int64_t* ks_m, const int64_t* ks_k, const int64_t* vq_m, const int64_t* vq_k,
+    const int16_t* cos_t, const int16_t* sin_t, int64_t max_pos, int8_t* q8, int64_t* tpos,
+    int8_t* kpool, int8_t* vpool, int n_pages, const int64_t* kq_est, int32_t* err,
+    hipStream_t s) {
+  if (N <= 0) return DI_OK;
+  if (n_q <= 0 || n_kv <= 0 || n_q % n_kv != 0 || nsplit < 1 || max_pos <= 0 || !kpool || !vpool ||
+      n_pages < 1 || !P || !positions || !slots || !q8 || !tpos)
+    return DI_EINVAL;
+  if ((i64)N * (n_q + 2 * n_kv) > 0x7fffffff) return DI_ERANGE;
+  QKVSlotArgs a{};
+  a.T = 1; a.n_q = n_q; a.n_kv = n_kv; a.P = P; a.nsplit = nsplit; a.split_stride = split_stride;
+  a.xm = xm; a.xk = xk; a.positions = positions; a.q_m = q_m; a.k_m = k_m; a.v_m = v_m;
+  a.q_k = q_k; a.k_k = k_k; a.v_k = v_k; a.q_norm_m = q_norm_m; a.k_norm_m = k_norm_m;
+  a.q_norm_k = q_norm_k; a.k_norm_k = k_norm_k; a.qs_m = qs_m; a.qs_k = qs_k; a.kq_m = kq_m;
+  a.kq_k = kq_k; a.ks_m = ks_m; a.ks_k = ks_k; a.vq_m = vq_m; a.vq_k = vq_k; a.cos_t = cos_t;
+  a.sin_t = sin_t; a.max_pos = max_pos; a.q8 = q8; a.tpos = tpos;
+  a.kv = KVPages{kpool, vpool, nullptr, 0, n_kv}; a.kq_est = kq_est; a.err = err;
+  a.slots = slots; a.n_slots = (i64)n_pages * DI_PAGE;
+  return qkv_epilogue_launch(a, N, s);
 }
 
 // ---------------------------------------------------------------- op level

@@ -147,6 +147,9 @@ const Entry ENTRIES[] = {
     DI_ENTRY(detllm_attn_decode_acc), DI_ENTRY(detllm_kv_select_work),
     DI_ENTRY(detllm_kv_select), DI_ENTRY(detllm_kv_compact),
     DI_ENTRY(detllm_attn_decode_shared_work), DI_ENTRY(detllm_attn_decode_shared),
+    DI_ENTRY(detllm_packed_plan_work), DI_ENTRY(detllm_packed_plan),
+    DI_ENTRY(detllm_qkv_epilogue_packed), DI_ENTRY(detllm_attn_packed_work),
+    DI_ENTRY(detllm_attn_packed), DI_ENTRY(detllm_lora_add),
 };
 #undef DI_ENTRY
 
@@ -711,9 +714,188 @@ void op_kv_compact(at::TensorList kpools, at::TensorList vpools, const Tensor& t
   }
 }
 
+// ------------------------------------------------------------ packed steps
+
+// t is a contiguous vector or matrix of `sizes` on like's device
+void check_is(const char* op, const char* name, const Tensor& t, at::ScalarType dt,
+              at::IntArrayRef sizes, const Tensor& like) {
+  DI_CHECK(t.scalar_type() == dt && t.sizes() == sizes && t.is_contiguous(), op, "expected ", name,
+           " as contiguous ", dt, " ", sizes, ", got ", t.scalar_type(), " ", t.sizes());
+  DI_CHECK(t.device() == like.device(), op, "operands on ", like.device(), " and ", t.device());
+}
+void check_pools(const char* op, const Tensor& kpool, const Tensor& vpool, int64_t n_kv,
+                 const Tensor& like) {
+  rank(kpool, 4, op);
+  DI_CHECK(kpool.size(0) > 0 && kpool.size(0) <= INT32_MAX / 128, op, "no pages, or too many");
+  check_is(op, "the K pool", kpool, at::kChar, {kpool.size(0), n_kv, 128, 128}, like);
+  check_is(op, "the V pool", vpool, at::kChar, {kpool.size(0), n_kv, 128, 128}, like);
+}
+
+std::tuple<Tensor, Tensor, Tensor, Tensor> op_packed_plan(const Tensor& table, const Tensor& free,
+                                                          const Tensor& n_free, const Tensor& past,
+                                                          const Tensor& fresh, int64_t N,
+                                                          const Tensor& err) {
+  constexpr const char* op = "packed_plan";
+  rank(table, 2, op);
+  rank(free, 1, op);
+  const int64_t B = table.size(0), width = table.size(1);
+  DI_CHECK(B >= 1 && B <= 2048 && width >= 1 && width <= 1024, op, "a table of ", table.sizes(),
+           " (at most 2048 rows of 1024 pages)");
+  DI_CHECK(N >= 0 && N <= INT32_MAX && free.size(0) <= INT32_MAX, op, N, " token rows, ",
+           free.size(0), " pages");
+  check_is(op, "the table", table, at::kInt, {B, width}, table);
+  check_is(op, "the free list", free, at::kInt, {free.size(0)}, table);
+  check_is(op, "its length", n_free, at::kInt, {1}, table);
+  check_is(op, "past", past, at::kInt, {B}, table);
+  check_is(op, "new", fresh, at::kInt, {B}, table);
+  check_is(op, "err", err, at::kInt, {1}, table);
+  int64_t bytes = 0;
+  check(detllm_packed_plan_work((int)B, (int)N, &bytes), "detllm_packed_plan_work");
+  const c10::DeviceGuard guard(table.device());
+  Tensor cu = empty({B + 1}, at::kInt, table), row = empty({N}, at::kInt, table);
+  Tensor pos = empty({N}, at::kLong, table), slot = empty({N}, at::kLong, table);
+  const Tensor work = scratch(bytes, table);
+  DI_RUN(detllm_packed_plan, ptr<int32_t>(table), (int)width, ptr<int32_t>(free),
+         (int)free.size(0), ptr<int32_t>(n_free), ptr<int32_t>(past), ptr<int32_t>(fresh), (int)B,
+         (int)N, ptr<int32_t>(cu), ptr<int32_t>(row), ptr<int64_t>(pos), ptr<int64_t>(slot),
+         work.data_ptr(), bytes, ptr<int32_t>(err));
+  for (const Tensor* t : {&table, &free, &n_free, &err}) mutated(*t);
+  return {cu, row, pos, slot};
+}
+
+T2 op_qkv_epilogue_packed(const Tensor& P, int64_t n_q, int64_t n_kv, const Tensor& xm,
+                          const Tensor& xk, const Tensor& positions, const Tensor& slots,
+                          const Tensor& q_m, int64_t q_k, const Tensor& k_m, int64_t k_k,
+                          const Tensor& v_m, int64_t v_k, const Tensor& q_norm_m, int64_t q_norm_k,
+                          const Tensor& k_norm_m, int64_t k_norm_k, const Tensor& qs_m,
+                          int64_t qs_k, const Tensor& kq_m, const Tensor& kq_k, const Tensor& ks_m,
+                          const Tensor& ks_k, const Tensor& vq_m, const Tensor& vq_k,
+                          const Tensor& cos_t, const Tensor& sin_t, const Tensor& kpool,
+                          const Tensor& vpool, const Tensor& err) {
+  constexpr const char* op = "qkv_epilogue_packed";
+  rank(P, 3, op);
+  rank(cos_t, 2, op);
+  DI_CHECK(n_q > 0 && n_kv > 0 && n_q % n_kv == 0 && n_q <= (1 << 16), op, n_q,
+           " query heads over ", n_kv, " kv heads");
+  const int64_t ns = P.size(0), N = P.size(1), C = (n_q + 2 * n_kv) * 128;
+  DI_CHECK(ns >= 1 && ns <= INT32_MAX && N * (n_q + 2 * n_kv) <= INT32_MAX, op, "a product ",
+           P.sizes());
+  const Tensor Pc = P.contiguous();
+  check_is(op, "the product", Pc, at::kInt, {ns, N, C}, P);
+  const int64_t maxp = cos_t.size(0);
+  DI_CHECK(maxp > 0, op, "rotation tables without rows");
+  struct {
+    const char* name;
+    const Tensor& t;
+    int64_t n;
+  } vecs[] = {{"xm", xm, N},           {"xk", xk, N},
+              {"positions", positions, N}, {"slots", slots, N},
+              {"q_m", q_m, n_q * 128}, {"k_m", k_m, n_kv * 128},
+              {"v_m", v_m, n_kv * 128}, {"q_norm_m", q_norm_m, 128},
+              {"k_norm_m", k_norm_m, 128}, {"qs_m", qs_m, n_kv * 128},
+              {"kq_m", kq_m, n_kv * 128}, {"kq_k", kq_k, n_kv * 128},
+              {"ks_m", ks_m, n_kv},    {"ks_k", ks_k, n_kv},
+              {"vq_m", vq_m, n_kv},    {"vq_k", vq_k, n_kv}};
+  for (const auto& v : vecs) check_is(op, v.name, v.t, at::kLong, {v.n}, P);
+  check_is(op, "cos_t", cos_t, at::kShort, {maxp, 128}, P);
+  check_is(op, "sin_t", sin_t, at::kShort, {maxp, 128}, P);
+  check_pools(op, kpool, vpool, n_kv, P);
+  check_is(op, "err", err, at::kInt, {1}, P);
+  const c10::DeviceGuard guard(P.device());
+  Tensor q8 = empty({N, n_q, 128}, at::kChar, P), tpos = empty({N, n_q}, at::kLong, P);
+  DI_RUN(detllm_qkv_epilogue_packed, ptr<int32_t>(Pc), (int)ns, N * C, (int)N, (int)n_q, (int)n_kv,
+         i64(xm), i64(xk), i64(positions), i64(slots), i64(q_m), q_k, i64(k_m), k_k, i64(v_m), v_k,
+         i64(q_norm_m), q_norm_k, i64(k_norm_m), k_norm_k, i64(qs_m), qs_k, i64(kq_m), i64(kq_k),
+         i64(ks_m), i64(ks_k), i64(vq_m), i64(vq_k), ptr<int16_t>(cos_t), ptr<int16_t>(sin_t), maxp,
+         ptr<int8_t>(q8), ptr<int64_t>(tpos), ptr<int8_t>(kpool), ptr<int8_t>(vpool),
+         (int)kpool.size(0), nullptr, ptr<int32_t>(err));
+  for (const Tensor* t : {&kpool, &vpool, &err}) mutated(*t);
+  return {q8, tpos};
+}
+
+Tensor op_attn_packed(const Tensor& q8, const Tensor& tpos, const Tensor& kpool,
+                      const Tensor& vpool, const Tensor& table, const Tensor& cu,
+                      const Tensor& past, int64_t S, int64_t max_new, const Tensor& err) {
+  constexpr const char* op = "attn_packed";
+  rank(q8, 3, op);
+  rank(kpool, 4, op);
+  rank(table, 2, op);
+  const int64_t N = q8.size(0), n_q = q8.size(1), n_kv = kpool.size(1), B = table.size(0);
+  DI_CHECK(n_kv > 0 && n_q > 0 && n_q % n_kv == 0 &&
+               (n_q / n_kv == 1 || n_q / n_kv == 2 || n_q / n_kv == 4 || n_q / n_kv == 8),
+           op, n_q, " query heads over ", n_kv, " kv heads (1, 2, 4 or 8 each)");
+  DI_CHECK(q8.scalar_type() == at::kChar && q8.size(2) == 128, op,
+           "expected int8 queries of 128 channels, got ", q8.scalar_type(), " ", q8.sizes());
+  DI_CHECK(N * n_q <= (1 << 24) && B >= 1 && B <= 65536, op, N, " token rows of ", B, " rows");
+  DI_CHECK(S >= 1 && S <= 131071 && S <= table.size(1) * 128 && max_new >= 0, op, S,
+           " slots over a table of ", table.size(1), " pages, ", max_new, " new tokens");
+  const Tensor qc = q8.contiguous(), tc = tpos.contiguous();
+  check_is(op, "tpos", tc, at::kLong, {N, n_q}, q8);
+  check_pools(op, kpool, vpool, n_kv, q8);
+  check_is(op, "the table", table, at::kInt, {B, table.size(1)}, q8);
+  DI_CHECK(table.size(1) <= (1 << 24), op, "a table of ", table.size(1), " pages");
+  check_is(op, "cu", cu, at::kInt, {B + 1}, q8);
+  check_is(op, "past", past, at::kInt, {B}, q8);
+  check_is(op, "err", err, at::kInt, {1}, q8);
+  const int most = as_i32(max_new);
+  int64_t bytes = 0;
+  check(detllm_attn_packed_work((int)N, (int)B, (int)S, most, (int)n_q, (int)n_kv, &bytes),
+        "detllm_attn_packed_work");
+  const c10::DeviceGuard guard(q8.device());
+  Tensor out = empty({N, n_q * 128}, at::kLong, q8);
+  const Tensor work = scratch(bytes, q8);
+  DI_RUN(detllm_attn_packed, ptr<int8_t>(qc), i64(tc), ptr<int8_t>(kpool), ptr<int8_t>(vpool),
+         (int)kpool.size(0), ptr<int32_t>(table), (int)table.size(1), ptr<int32_t>(cu),
+         ptr<int32_t>(past), (int)N, (int)B, (int)S, most, (int)n_q, (int)n_kv, work.data_ptr(),
+         bytes, ptr<int64_t>(out), ptr<int32_t>(err));
+  mutated(err);
+  return out;
+}
+
+Tensor op_lora_gemm(const Tensor& x8, const Tensor& w, const Tensor& a8, const Tensor& b8,
+                    const Tensor& bm, const Tensor& bk, const Tensor& adapter) {
+  constexpr const char* op = "lora_gemm";
+  rank(x8, 2, op);
+  rank(w, 2, op);
+  rank(a8, 3, op);
+  const int64_t N = x8.size(0), K = x8.size(1), C = w.size(0), n_ad = a8.size(0), r = a8.size(1);
+  DI_CHECK(K >= 16 && K % 16 == 0 && K <= 65536 && r >= 16 && r % 16 == 0 && r <= 128, op,
+           "K of ", K, " (a multiple of 16 up to 65536), rank ", r, " (one up to 128)");
+  DI_CHECK(N <= (1 << 20) && C >= 1 && C <= (1 << 24) && n_ad >= 1 && n_ad <= INT32_MAX, op, N,
+           " token rows, ", C, " columns, ", n_ad, " adapters");
+  auto aligned = [](const Tensor& t) {   // (the kernels load 16 bytes at a time)
+    const Tensor c = t.contiguous();
+    return (reinterpret_cast<uintptr_t>(c.data_ptr()) & 15) == 0 ? c : c.clone();
+  };
+  const Tensor xc = aligned(x8), wc = aligned(w), ac = aligned(a8), bc = aligned(b8);
+  check_is(op, "x8", xc, at::kChar, {N, K}, x8);
+  check_is(op, "w", wc, at::kChar, {C, K}, x8);
+  check_is(op, "a8", ac, at::kChar, {n_ad, r, K}, x8);
+  check_is(op, "b8", bc, at::kChar, {n_ad, C, r}, x8);
+  check_is(op, "bm", bm, at::kLong, {n_ad, C}, x8);
+  check_is(op, "bk", bk, at::kLong, {n_ad}, x8);
+  check_is(op, "adapter", adapter, at::kInt, {N}, x8);
+  const c10::DeviceGuard guard(x8.device());
+  Tensor out = empty({N, C}, at::kInt, x8);
+  if (N == 0) return out;
+  if (N <= 64)
+    DI_RUN(detllm_igemv_nt, ptr<int8_t>(xc), ptr<int8_t>(wc), ptr<int32_t>(out), (int)N, (int)C,
+           (int)K, 1, N * C);
+  else
+    DI_RUN(detllm_igemm_nt, ptr<int8_t>(xc), ptr<int8_t>(wc), ptr<int32_t>(out), (int)N, (int)C,
+           (int)K, 1, N * K, C * K, N * C);
+  DI_RUN(detllm_lora_add, ptr<int32_t>(out), ptr<int8_t>(xc), ptr<int8_t>(ac), ptr<int8_t>(bc),
+         i64(bm), i64(bk), ptr<int32_t>(adapter), (int)N, (int)K, (int)C, (int)r, (int)n_ad);
+  return out;
+}
+
 }  // namespace
 
 TORCH_LIBRARY_IMPL(detllm_rocm, CUDA, m) {
+  m.impl("packed_plan", &op_packed_plan);
+  m.impl("qkv_epilogue_packed", &op_qkv_epilogue_packed);
+  m.impl("attn_packed", &op_attn_packed);
+  m.impl("lora_gemm", &op_lora_gemm);
   m.impl("attn_window_prefill", &op_attn_window_prefill);
   m.impl("attn_window_decode", &op_attn_window_decode);
   m.impl("attn_prefill_acc", &op_attn_prefill_acc);

@@ -39,12 +39,15 @@ OPS = ("int_gemm", "isqrt_i64", "ilog2_i64", "greedy_pick", "embed_normq", "norm
 LONG_OPS = ("attn_window_prefill", "attn_window_decode", "attn_prefill_acc", "attn_decode_acc",
             "attn_decode_shared", "kv_select", "kv_compact")
 
+# The operators of packed steps (no counterpart in the reference)
+PACKED_OPS = ("packed_plan", "qkv_epilogue_packed", "attn_packed", "lora_gemm")
+
 
 def _op(schema):
     """Define one operator; the decorated function is its fake (shapes and
     integer dtypes), the result the operator itself."""
     name = schema.split("(", 1)[0]
-    assert name in OPS + LONG_OPS
+    assert name in OPS + LONG_OPS + PACKED_OPS
     torch.library.define(f"{NS}::{name}", schema[len(name):], tags=(torch.Tag.pt2_compliant_tag,))
 
     def wrap(fake):
@@ -246,6 +249,62 @@ def kv_compact(kpools, vpools, table, dst, keep):
     is in dst twice."""
 
 
+# ----------------------------------------------------------- packed steps
+#
+# Rows of any lengths in one step without padding: row b has past[b] filled slots
+# and new tokens whose token rows follow each other (row b's at cu[b] ..
+# cu[b + 1] - 1); token t of row b has position and slot past[b] + t. Operands that
+# do not fit raise ValueError before any launch; lengths are on the device, and
+# those outside the bounds that a call is given set bits of err (_lib.ERR_SLOTS,
+# ERR_PAGES), which the host raises from at its next check.
+
+@_op("packed_plan(Tensor(a0!) table, Tensor(a1!) free, Tensor(a2!) n_free, Tensor past, "
+     "Tensor new, SymInt N, Tensor(a6!) err) -> (Tensor, Tensor, Tensor, Tensor)")
+def packed_plan(table, free, n_free, past, new, N, err):
+    """A step's bookkeeping for N token rows: pages of table [B, width] mapped
+    from (and given back to) the first n_free [1] of free, in place, so that row b
+    has ceil((past + new) / 128); surplus pages first, to the list's end, then
+    missing ones from it, row by row, all of them or (err bit 8) none. A row's
+    mapped pages come first in its table row. -> (cu [B + 1] int32, and per token
+    row: row [N] int32 (-1 behind the last), position [N] int64 (0), slot [N] int64
+    page * 128 + position % 128 (-1))."""
+    return (past.new_empty(past.shape[0] + 1), past.new_empty(N), past.new_empty(N, dtype=I64),
+            past.new_empty(N, dtype=I64))
+
+
+@_op("qkv_epilogue_packed(Tensor P, SymInt n_q, SymInt n_kv, Tensor xm, Tensor xk, "
+     "Tensor positions, Tensor slots, Tensor q_m, SymInt q_k, Tensor k_m, SymInt k_k, Tensor v_m, "
+     "SymInt v_k, Tensor q_norm_m, SymInt q_norm_k, Tensor k_norm_m, SymInt k_norm_k, Tensor qs_m, "
+     "SymInt qs_k, Tensor kq_m, Tensor kq_k, Tensor ks_m, Tensor ks_k, Tensor vq_m, Tensor vq_k, "
+     "Tensor cos_t, Tensor sin_t, Tensor(a27!) kpool, Tensor(a28!) vpool, Tensor(a29!) err) "
+     "-> (Tensor, Tensor)")
+def qkv_epilogue_packed(P, n_q, n_kv, *rest):
+    """qkv_epilogue of packed token rows: P int32 [nsplit, N, (n_q + 2 n_kv) * 128],
+    positions and slots [N]; K and V of token row i to slot slots[i] of the pools
+    (outside them: not stored; no slot twice). -> (q8 [N, n_q, 128], tpos [N, n_q])."""
+    N = P.shape[1]
+    return P.new_empty(N, n_q, 128, dtype=torch.int8), P.new_empty(N, n_q, dtype=I64)
+
+
+@_op("attn_packed(Tensor q8, Tensor tpos, Tensor kpool, Tensor vpool, Tensor table, Tensor cu, "
+     "Tensor past, SymInt S, SymInt max_new, Tensor(a9!) err) -> Tensor")
+def attn_packed(q8, tpos, kpool, vpool, table, cu, past, S, max_new, err):
+    """Attention of packed token rows over the cache: q8 [N, n_q, 128], tpos
+    [N, n_q], cu [B + 1] and past [B] int32; no row has more than S slots (its new
+    ones counted) or max_new tokens. Slots of pages that are not mapped are not
+    seen. -> exact int64 contexts [N, n_q * 128], 0 behind the last row's tokens."""
+    return q8.new_empty(q8.shape[0], q8.shape[1] * 128, dtype=I64)
+
+
+@_op("lora_gemm(Tensor x8, Tensor w, Tensor a8, Tensor b8, Tensor bm, Tensor bk, Tensor adapter) "
+     "-> Tensor")
+def lora_gemm(x8, w, a8, b8, bm, bk, adapter):
+    """x8 [N, K] int8 . w [C, K]^T and, for token rows with adapter[i] in [0, n_ad),
+    its low-rank change (detllm_lora_add): a8 [n_ad, rank, K], b8 [n_ad, C, rank]
+    int8, bm [n_ad, C], bk [n_ad] int64; K and rank multiples of 16. -> int32 [N, C]."""
+    return x8.new_empty(x8.shape[0], w.shape[0], dtype=torch.int32)
+
+
 # Loading the native binding registers the kernels. Where it cannot be loaded
 # (not built, or built for another torch), the import goes on and a call of an
 # operator raises, as the other entries do; a call after it has been built
@@ -271,7 +330,7 @@ def _load_kernels():
 def _register_stand_ins():
     global _stand_ins
     _stand_ins = torch.library.Library(NS, "IMPL")
-    for name in OPS + LONG_OPS:
+    for name in OPS + LONG_OPS + PACKED_OPS:
         def call_again(keyset, *args, _op=getattr(torch.ops.detllm_rocm, name).default, **kwargs):
             _load_kernels()
             return _op.redispatch(keyset, *args, **kwargs)

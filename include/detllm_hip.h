@@ -24,7 +24,8 @@
  *     [-vocab, vocab)), bit 2 (position outside [-max_pos, max_pos)), and a
  *     device slot count above a launch's slot bound bit 4; the kernel then
  *     reads row 0 / scans the bounded slots, and the host raises from the
- *     word at its next check (negative indices wrap as in torch).
+ *     word at its next check (negative indices wrap as in torch). Too few free
+ *     pages for a packed step set bit 8.
  *
  * Reference interfaces each entry replaces are cited as file:line in
  * rishabh135/idempotent_llm. The reference has no FFI: its boundary is the
@@ -460,6 +461,69 @@ int detllm_attn_decode_shared(const int8_t* q8, const int64_t* tpos, const int8_
                               const uint8_t* valid, int64_t valid_stride, int B, int S, int n_q,
                               int n_kv, const int64_t* s_dev, int shared, void* work,
                               int64_t work_bytes, int64_t* out, int32_t* err, hipStream_t s);
+
+/* ---- packed steps: no counterpart in the reference. Rows of any lengths share a
+ * step without padding: row b has past[b] filled slots and new tokens, the token
+ * rows of all follow each other (row b's at cu[b] .. cu[b + 1] - 1, int32), and
+ * token t of row b has position and slot past[b] + t. The integers are those of
+ * the padded forms. Lengths stay on the device; N (token rows), S (slots of a row)
+ * and max_new (new tokens of a row) are bounds that size a launch. Values outside
+ * them set bit 4 of *err; nothing is read or written out of range. */
+
+/* The step's bookkeeping: cu [B + 1] from fresh [B] (new tokens), and of each of
+ * the N token rows its row, position and slot (page * 128 + position % 128; behind
+ * the last row's -1, 0 and -1). A row needs ceil((past + fresh) / 128) pages and has
+ * the mapped ones (>= 0) that come first in its table row. Surplus pages go to the
+ * end of the free list free_pages [cap], of which the first *n_free are free (-1 in the
+ * table), missing ones are then taken from its end, both row by row; where they
+ * do not suffice, none is taken (bit 8 of *err) and those slots are -1. past = fresh =
+ * 0 gives a row's pages back. A row past the table (or 131071 slots, or negative)
+ * keeps its pages and has no tokens (bit 4); token rows from N on are not written (bit
+ * 4). A page is in one row's table or free once. B <= 2048, width <= 1024. */
+int detllm_packed_plan_work(int B, int N, int64_t* bytes);
+int detllm_packed_plan(int32_t* table, int width, int32_t* free_pages, int cap, int32_t* n_free,
+                       const int32_t* past, const int32_t* fresh, int B, int N, int32_t* cu,
+                       int32_t* row, int64_t* pos, int64_t* slot, void* work, int64_t work_bytes,
+                       int32_t* err, hipStream_t s);
+
+/* detllm_qkv_epilogue of N packed token rows: token row i's K and V go to
+ * slots[i] of the pools of n_pages pages (negative or past them: not stored; no slot
+ * twice), its queries to q8 [N][n_q][128] and tpos [N][n_q]. */
+int detllm_qkv_epilogue_packed(
+    const int32_t* P, int nsplit, int64_t split_stride, int N, int n_q, int n_kv,
+    const int64_t* xm, const int64_t* xk, const int64_t* positions, const int64_t* slots,
+    const int64_t* q_m, int64_t q_k, const int64_t* k_m, int64_t k_k, const int64_t* v_m,
+    int64_t v_k, const int64_t* q_norm_m, int64_t q_norm_k, const int64_t* k_norm_m,
+    int64_t k_norm_k, const int64_t* qs_m, int64_t qs_k, const int64_t* kq_m, const int64_t* kq_k,
+    const int64_t* ks_m, const int64_t* ks_k, const int64_t* vq_m, const int64_t* vq_k,
+    const int16_t* cos_t, const int16_t* sin_t, int64_t max_pos, int8_t* q8, int64_t* tpos,
+    int8_t* kpool, int8_t* vpool, int n_pages, const int64_t* kq_est, int32_t* err, hipStream_t s);
+
+/* Attention of packed token rows: token t of row b sees the slots s <= past[b] + t
+ * of the pages that its table row maps (ids outside [0, n_pages) are not mapped).
+ * q8 [N][n_q][128], tpos [N][n_q] (detllm_qkv_epilogue_packed), out [N][n_q * 128];
+ * rows of out behind the last row's tokens become 0. A row's slots past S are not
+ * seen; its tokens past max_new are not computed (their rows of out are
+ * unspecified; bit 4 for both). n_q / n_kv is 1, 2, 4 or 8, S at most 131071 and
+ * width * 128, N n_q at most 2^24, B at most 65536. */
+int detllm_attn_packed_work(int N, int B, int S, int max_new, int n_q, int n_kv, int64_t* bytes);
+int detllm_attn_packed(const int8_t* q8, const int64_t* tpos, const int8_t* kpool,
+                       const int8_t* vpool, int n_pages, const int32_t* table, int width,
+                       const int32_t* cu, const int32_t* past, int N, int B, int S, int max_new,
+                       int n_q, int n_kv, void* work, int64_t work_bytes, int64_t* out,
+                       int32_t* err, hipStream_t s);
+
+/* Low-rank adapters of N token rows beside the product P [N][C] of x8 [N][K], in
+ * place (one partial of it): adapter[i] in [0, n_ad) names token row i's, any other
+ * value none (its row of P is left as it is). Per row, with a8 [n_ad][rank][K], b8
+ * [n_ad][C][rank], bm [n_ad][C], bk [n_ad]: u = a8 x8; h = max(ilog2(max(|u|, 1)) - 12,
+ * 0); w = rshift_round(u, h) (dyadic.py:108-120 at 13 bits); v = b8 w; P[c] +=
+ * rshift_round(v[c] bm[c], bk - h), a left shift where bk < h, int64 and then int32
+ * (wrapping). rank a multiple of 16 up to 128 (zeros fill it up), K one up to 65536;
+ * x8, a8 and b8 16-byte aligned. */
+int detllm_lora_add(int32_t* P, const int8_t* x8, const int8_t* a8, const int8_t* b8,
+                    const int64_t* bm, const int64_t* bk, const int32_t* adapter, int N, int K,
+                    int C, int rank, int n_ad, hipStream_t s);
 
 /* Per-step bookkeeping of the graph-captured decode (src/detllm/graphed.py:
  * 112-131: the validity flag of the step's slot, the device scalars holding
