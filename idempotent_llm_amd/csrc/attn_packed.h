@@ -24,6 +24,7 @@ struct PackedArgs {
   int lg;        // log2 of the query heads per kv head
   int few_rows;  // query rows of a few-row unit at most (its rows of scores)
   int units, chunk, nch;
+  int step;      // blocks per kv head
   int32_t* scores;  // few-row units: [B][n_kv][few_rows][nch * chunk]
   int32_t* smax;    // [units][n_kv][nch][64]: maxima of the visible scores
   int64_t* sden;    // the same of partial denominators
@@ -35,16 +36,13 @@ struct PackedArgs {
 // Never a score: |q . k| <= 2^21
 constexpr int32_t NO_SCORE = INT32_MIN;
 
-// What a block works on
+// What a block works on: a chunk of a unit, for a kv head
 struct Work {
-  bool live;  // else: no such unit (spare: its number among those, of `spares`)
   bool few;   // the row has at most 16 query rows
   bool bad;   // the row's slots or tokens are past the launch's bounds
   int b, tile, unit, kvh, c;
   int tok0, T, past;  // the row's first token row, its tokens and filled slots
   int len;            // slots that its tokens see (past + T, bounded)
-  int ntok;           // token rows of all rows
-  int spare, spares;
 };
 
 // Last slot that token t of a row at `past` sees
@@ -67,55 +65,74 @@ __device__ __forceinline__ int wave_scan(int v) {
 // Every LDS read of the wave done (before a barrier that frees what it read)
 __device__ __forceinline__ void wait_lds() { __builtin_amdgcn_s_waitcnt(0xC07F); }
 
-// The unit of this block, found by every wave for itself. Blocks: kv heads
-// fastest (with 8 of them a head's blocks share an XCD, so its L2 holds their K
-// and V), then chunks, then units from the last row's last tile on (the tiles of
-// a prompt that see most go first).
-__device__ __forceinline__ Work find_work(const PackedArgs& a) {
-  Work w{};
-  const int lane = threadIdx.x & 63;
-  const int bid = blockIdx.x;
-  w.kvh = bid % a.n_kv;
-  const int rest = bid / a.n_kv;
-  w.c = rest % a.nch;
-  const int want = a.units - 1 - rest / a.nch;
-  w.unit = want;
-  w.ntok = ::min(::max(a.cu[a.B], 0), a.N);
-  int base = 0;
-  for (int b0 = 0; b0 < a.B; b0 += 64) {
-    const int b = b0 + lane, bc = ::min(b, a.B - 1);
-    const int past = a.past[bc];
+// The rows' work, found by every wave for itself: lane l holds row b0 + l of 64.
+// A row's items are its units times its chunks.
+struct Rows {
+  int tok0, T, past, over, units, nc;  // the lane's row
+  int items, units_to, items_to;       // its items; units and items up to and with it
+  __device__ __forceinline__ void load(const PackedArgs& a, int b0) {
+    const int b = b0 + (int)(threadIdx.x & 63), bc = ::min(b, a.B - 1);
+    past = a.past[bc];
     const int c0 = ::min(::max(a.cu[bc], 0), a.N), c1 = ::min(::max(a.cu[bc + 1], c0), a.N);
-    const int T = b < a.B ? ::min(c1 - c0, a.max_new) : 0;
+    tok0 = c0;
+    over = c1 - c0 > a.max_new;
+    T = b < a.B ? ::min(c1 - c0, a.max_new) : 0;
     const i64 R = (i64)T << a.lg;
-    const int n = R <= 16 ? (T > 0 ? 1 : 0) : (int)((R + 63) >> 6);
-    const int over = c1 - c0 > a.max_new;
-    const int incl = wave_scan(n);
-    const int tot = __builtin_amdgcn_readlane(incl, 63);
-    if (!w.live && want < base + tot) {
-      const int l = __ffsll((unsigned long long)__ballot(base + incl > want)) - 1;
-      w.live = true;
-      w.b = b0 + l;
-      w.tile = want - base - (__builtin_amdgcn_readlane(incl, l) - __builtin_amdgcn_readlane(n, l));
-      w.tok0 = __builtin_amdgcn_readlane(c0, l);
-      w.T = __builtin_amdgcn_readlane(T, l);
-      w.bad = __builtin_amdgcn_readlane(over, l) != 0;
-      w.past = __builtin_amdgcn_readlane(past, l);
-    }
-    base += tot;
+    units = R <= 16 ? (T > 0 ? 1 : 0) : (int)((R + 63) >> 6);
+    nc = (row_limit(a, past, T - 1) + a.chunk) / a.chunk;
+    items = units * nc;
+    units_to = wave_scan(units);
+    items_to = wave_scan(items);
   }
-  if (!w.live) {
-    w.spare = want - base;
-    w.spares = a.units - base;
+};
+
+// Items from the last row's last unit on (the tiles of a prompt that see most go
+// first), kv heads fastest (with 8 of them a head's blocks share an XCD, so its L2
+// holds their K and V). A block takes item j, j + a.step, ...
+struct Finder {
+  Rows r;     // of the first 64 rows (all of most batches)
+  int total;  // items
+  int ntok;   // token rows of all rows
+  __device__ __forceinline__ explicit Finder(const PackedArgs& a) {
+    ntok = ::min(::max(a.cu[a.B], 0), a.N);
+    r.load(a, 0);
+    total = __builtin_amdgcn_readlane(r.items_to, 63);
+    for (int b0 = 64; b0 < a.B; b0 += 64) {
+      Rows x;
+      x.load(a, b0);
+      total += __builtin_amdgcn_readlane(x.items_to, 63);
+    }
+  }
+  __device__ __forceinline__ Work find(const PackedArgs& a, int kvh, int item) const {
+    Work w{};
+    w.kvh = kvh;
+    Rows x = r;
+    int items = 0, units = 0, b0 = 0;
+    for (;;) {
+      const int tot = __builtin_amdgcn_readlane(x.items_to, 63);
+      if (item < items + tot || b0 + 64 >= a.B) break;
+      items += tot;
+      units += __builtin_amdgcn_readlane(x.units_to, 63);
+      b0 += 64;
+      x.load(a, b0);
+    }
+    const int l = __ffsll((unsigned long long)__ballot(items + x.items_to > item)) - 1;
+    auto of = [&](int v) { return __builtin_amdgcn_readlane(v, l); };
+    const int nc = of(x.nc), at = item - items - (of(x.items_to) - of(x.items));
+    w.b = b0 + l;
+    w.tile = at / nc;
+    w.c = at - w.tile * nc;
+    w.unit = units + of(x.units_to) - of(x.units) + w.tile;
+    w.tok0 = of(x.tok0);
+    w.T = of(x.T);
+    const int past = of(x.past);
+    w.bad = of(x.over) != 0 || past < 0 || (i64)past + w.T > (i64)a.S;
+    w.past = ::max(past, 0);
+    w.len = row_limit(a, w.past, w.T - 1) + 1;
+    w.few = (w.T << a.lg) <= 16;
     return w;
   }
-  const i64 end = (i64)w.past + w.T;
-  w.bad = w.bad || w.past < 0 || end > (i64)a.S;
-  w.past = ::max(w.past, 0);
-  w.len = row_limit(a, w.past, w.T - 1) + 1;
-  w.few = (w.T << a.lg) <= 16;
-  return w;
-}
+};
 
 // Slots outside the launch's bound: DI_ERR_SLOTS, once a row
 __device__ __forceinline__ void report_row(const PackedArgs& a, const Work& w) {
@@ -123,13 +140,12 @@ __device__ __forceinline__ void report_row(const PackedArgs& a, const Work& w) {
     atomicOr(a.err, DI_ERR_SLOTS);
 }
 
-// Token rows behind the last row's: zeros, shared among the blocks without a unit
-__device__ __forceinline__ void zero_tail(const PackedArgs& a, const Work& w) {
-  if (w.c != 0) return;
+// Token rows behind the last row's: zeros, shared among the blocks
+__device__ __forceinline__ void zero_tail(const PackedArgs& a, int ntok, int kvh, int j) {
   const int cols = 128 << a.lg;
-  for (int tok = w.ntok + w.spare; tok < a.N; tok += w.spares) {
-    int64_t* o = a.out + ((i64)tok * a.n_kv + w.kvh) * cols;
-    for (int i = threadIdx.x; i < cols; i += blockDim.x) o[i] = 0;
+  for (int tok = ntok + j; tok < a.N; tok += a.step) {
+    int64_t* o = a.out + ((i64)tok * a.n_kv + kvh) * cols;
+    for (int i = threadIdx.x; i < cols; i += 256) o[i] = 0;
   }
 }
 
@@ -185,17 +201,67 @@ __device__ __forceinline__ uint32_t row_exp(int32_t F, const RowExp& E) {
   const float sp = __builtin_bit_cast(float, F) - 12582912.0f;
   const float x = __builtin_amdgcn_fmed3f(__builtin_fmaf(sp, -E.a, E.b), 0.0f, 1.0f);
   const uint32_t y = __builtin_bit_cast(uint32_t, __builtin_fmaf(x, 31.0f, 8388608.0f));
-  const uint32_t m = mad_u24(y, E.t, (uint32_t)F) & 0x3FFFFFu;
-  return m >> (y & 31u);
+  return (mad_u24(y, E.t, (uint32_t)F) & 0x3FFFFFu) >> (y & 31u);
+}
+// Of 16 scores, eight at a time, step by step: each step waits for the one before,
+// so eight chains run side by side
+__device__ __forceinline__ void row_exps(const v4i (&st)[4], const RowExp& E, uint32_t (&e)[16]) {
+#pragma unroll
+  for (int h = 0; h < 16; h += 8) {
+    int32_t F[8];
+    float x[8];
+    uint32_t m[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) F[i] = st[(h + i) >> 2][i & 3];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = __builtin_bit_cast(float, F[i]) - 12582912.0f;
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      x[i] = __builtin_amdgcn_fmed3f(__builtin_fmaf(x[i], -E.a, E.b), 0.0f, 1.0f);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = __builtin_fmaf(x[i], 31.0f, 8388608.0f);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      m[i] = mad_u24(__builtin_bit_cast(uint32_t, x[i]), E.t, (uint32_t)F[i]);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m[i] &= 0x3FFFFFu;
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) e[h + i] = m[i] >> (__builtin_bit_cast(uint32_t, x[i]) & 31u);
+  }
 }
 
 __device__ __forceinline__ double make_rowp(i64 den) {
   const double r = 16384.0 / (double)den;
   return fma(r, 0x1p-50, r);
 }
-__device__ __forceinline__ uint32_t row_p128(uint32_t e, double r) {  // p + 128
-  const double y = fma((double)e, r, 0x1p52 + 128.0);
-  return (uint32_t)__builtin_bit_cast(u64, y);
+// The P operands of 16 exponentials
+__device__ __forceinline__ void pack4(const uint32_t (&w)[4], int& hi, int& lo);
+__device__ __forceinline__ void row_probs(const uint32_t (&e)[16], double r, v4i& phi, v4i& plo) {
+#pragma unroll
+  for (int h = 0; h < 16; h += 8) {
+    double d[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) d[i] = (double)e[h + i];
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) d[i] = fma(d[i], r, 0x1p52 + 128.0);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      uint32_t w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = (uint32_t)__builtin_bit_cast(u64, d[4 * q + i]);
+      int a, b;
+      pack4(w, a, b);
+      phi[(h >> 2) + q] = a;
+      plo[(h >> 2) + q] = b;
+    }
+  }
 }
 // Four words p + 128 as the operands' bytes
 __device__ __forceinline__ void pack4(const uint32_t (&w)[4], int& hi, int& lo) {
@@ -206,15 +272,60 @@ __device__ __forceinline__ void pack4(const uint32_t (&w)[4], int& hi, int& lo) 
 }
 
 // The integer forms
-struct RowSlow {
-  ExpR E;
-  Recip R;
-};
 __device__ __forceinline__ i64 slow_exp(int32_t st, int32_t mx, const ExpR& E) {
   return di_exp_neg((u64)(uint32_t)(mx - st), E);
 }
 __device__ __forceinline__ uint32_t slow_p128(i64 e, const Recip& R) {
   return (uint32_t)to_i32(rhad_r(shl(e, 14), R)) + 128u;
+}
+
+// 16 values of a lane that a loop reads and writes at a number of its own: a
+// vector, or LDS (a wave's [16][64] words)
+typedef int v16i __attribute__((ext_vector_type(16)));
+struct InRegs {
+  v16i x;
+  __device__ __forceinline__ int get(int i) const { return x[i]; }
+  __device__ __forceinline__ void put(int i, int v) { x[i] = v; }
+};
+struct InLds {
+  int32_t* p;
+  __device__ __forceinline__ int get(int i) const { return p[i * 64 + (threadIdx.x & 63)]; }
+  __device__ __forceinline__ void put(int i, int v) { p[i * 64 + (threadIdx.x & 63)] = v; }
+};
+// In the integer forms, a score after the other: the sum of 16 exponentials, and
+// their P operands (small code and few registers, for what is hardly ever met)
+template <class Mem>
+__device__ __forceinline__ i64 slow_den(const v4i (&st)[4], int32_t off, uint32_t bits, int32_t mx,
+                                        i64 tpos, Mem m) {
+  const ExpR E = make_exp(tpos);
+#pragma unroll
+  for (int i = 0; i < 16; ++i) m.put(i, st[i >> 2][i & 3] - off);
+  i64 den = 0;
+#pragma unroll 1
+  for (int i = 0; i < 16; ++i)
+    if ((bits >> i) & 1u) den = wadd(den, slow_exp(m.get(i), mx, E));
+  return den;
+}
+template <class Mem>
+__device__ __forceinline__ void slow_probs(const v4i (&st)[4], int32_t off, uint32_t bits,
+                                           int32_t mx, i64 tpos, i64 den, v4i& phi, v4i& plo,
+                                           Mem m) {
+#pragma unroll
+  for (int i = 0; i < 16; ++i) m.put(i, st[i >> 2][i & 3] - off);
+  const ExpR E = make_exp(tpos);
+  const Recip R = make_recip(den);
+#pragma unroll 1
+  for (int i = 0; i < 16; ++i)
+    m.put(i, (bits >> i) & 1u ? (int)slow_p128(slow_exp(m.get(i), mx, E), R) : 128);
+#pragma unroll
+  for (int b = 0; b < 4; ++b) {
+    const uint32_t w4[4] = {(uint32_t)m.get(4 * b), (uint32_t)m.get(4 * b + 1),
+                            (uint32_t)m.get(4 * b + 2), (uint32_t)m.get(4 * b + 3)};
+    int a, c;
+    pack4(w4, a, c);
+    phi[b] = a;
+    plo[b] = c;
+  }
 }
 
 __device__ __forceinline__ int max16(int v) {  // over the lanes of one query row
@@ -231,13 +342,16 @@ __device__ __forceinline__ int max16(int v) {  // over the lanes of one query ro
 // its bytes of the P operand. Each byte of K and V is read once; what bounds it
 // is HBM, or, for short rows, one chain of loads and three block reductions. The
 // arithmetic of the query rows that are not there (14 of 16 at one token and two
-// heads) is 5 cycles a slot and CU against the 31 that its 256 bytes take.
+// heads) is 5 cycles a slot and CU against the 31 that its 256 bytes take. Up to 8
+// query rows (R8), a lane works for row qi % 8: the P operand has the high bytes in
+// rows 0 to 7 and the low bytes in rows 8 to 15, one MFMA and half the accumulators.
 
 template <int NW>
 struct FewLds {
   int32_t mx[NW][16];
   int64_t den[NW][16];
   int32_t ctx[16][128];
+  int32_t slow[NW][16 * 64];
 };
 
 struct FewRow {
@@ -247,8 +361,9 @@ struct FewRow {
   v4i q0, q1;
 };
 
+template <bool R8>
 __device__ __forceinline__ FewRow few_row(const PackedArgs& a, const Work& w) {
-  const int lane = threadIdx.x & 63, qi = lane & 15, g4 = lane >> 4;
+  const int lane = threadIdx.x & 63, qi = R8 ? lane & 7 : lane & 15, g4 = lane >> 4;
   FewRow r;
   const int t = qi >> a.lg, g = qi & ((1 << a.lg) - 1);
   r.on = qi < (w.T << a.lg);
@@ -303,65 +418,74 @@ __device__ __forceinline__ void pv16(const v4i& phi, const v4i& plo, const v4i (
     lo[j] = mfma16(plo, v[j], lo[j]);
   }
 }
-
-// The tile's operands from its 16 scores a lane; `bits` of them are seen
-__device__ __forceinline__ void few_probs(const v4i (&st)[4], uint32_t bits, bool fast,
-                                          const RowExp& E, double rp, int32_t mx, const RowSlow& sl,
-                                          v4i& phi, v4i& plo) {
+template <bool R8>
+struct FewAcc {
+  v4i hi[8], lo[R8 ? 1 : 8];
+  __device__ __forceinline__ void clear() {
 #pragma unroll
-  for (int blk = 0; blk < 4; ++blk) {
-    uint32_t w4[4];
+    for (int j = 0; j < 8; ++j) hi[j] = v4i{0, 0, 0, 0};
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const bool vis = (bits >> (4 * blk + r)) & 1u;
-      if (fast) {
-        const uint32_t e = row_exp(st[blk][r] + E.c0, E);
-        w4[r] = row_p128(vis ? e : 0u, rp);
-      } else {
-        w4[r] = vis ? slow_p128(slow_exp(st[blk][r], mx, sl.E), sl.R) : 128u;
-      }
-    }
-    int h, l;
-    pack4(w4, h, l);
-    phi[blk] = h;
-    plo[blk] = l;
+    for (int j = 0; j < (R8 ? 1 : 8); ++j) lo[j] = v4i{0, 0, 0, 0};
   }
+  __device__ __forceinline__ void add(const v4i& phi, const v4i& plo, const v4i (&v)[8]) {
+    if constexpr (R8) {
+      const v4i p = (threadIdx.x & 8) ? plo : phi;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) hi[j] = mfma16(p, v[j], hi[j]);
+    } else {
+      pv16(phi, plo, v, hi, lo);
+    }
+  }
+};
+
+// The tile's operands from its 16 scores a lane (raw; `bits` of them are seen)
+__device__ __forceinline__ void few_probs(const v4i (&st)[4], uint32_t bits, bool fast,
+                                          const RowExp& E, double rp, int32_t mx, i64 tpos, i64 den,
+                                          v4i& phi, v4i& plo, InLds m) {
+  if (DI_UNLIKELY(!fast)) {
+    slow_probs(st, 0, bits, mx, tpos, den, phi, plo, m);
+    return;
+  }
+  v4i f[4];
+#pragma unroll
+  for (int b = 0; b < 4; ++b) f[b] = st[b] + E.c0;
+  uint32_t e[16];
+  row_exps(f, E, e);
+#pragma unroll
+  for (int i = 0; i < 16; ++i) e[i] = (bits >> i) & 1u ? e[i] : 0u;
+  row_probs(e, rp, phi, plo);
 }
 __device__ __forceinline__ i64 few_den(const v4i (&st)[4], uint32_t bits, bool fast, const RowExp& E,
-                                       int32_t mx, const ExpR& Es) {
-  i64 den = 0;
-  if (fast) {
-    uint32_t sum = 0;
+                                       int32_t mx, i64 tpos, InLds m) {
+  if (DI_UNLIKELY(!fast)) return slow_den(st, 0, bits, mx, tpos, m);
+  v4i f[4];
 #pragma unroll
-    for (int blk = 0; blk < 4; ++blk)
+  for (int b = 0; b < 4; ++b) f[b] = st[b] + E.c0;
+  uint32_t e[16], sum = 0;
+  row_exps(f, E, e);
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const uint32_t e = row_exp(st[blk][r] + E.c0, E);
-        sum += (bits >> (4 * blk + r)) & 1u ? e : 0u;
-      }
-    return sum;
-  }
-#pragma unroll
-  for (int blk = 0; blk < 4; ++blk)
-#pragma unroll
-    for (int r = 0; r < 4; ++r)
-      if ((bits >> (4 * blk + r)) & 1u) den = wadd(den, slow_exp(st[blk][r], mx, Es));
-  return den;
+  for (int i = 0; i < 16; ++i) sum += (bits >> i) & 1u ? e[i] : 0u;
+  return sum;
 }
 
-// The waves' contexts (accumulators of query row 4 g4 + r, channel 16 j + qi) added
-// up in LDS, then written: to out, or to a chunk's part
-template <int NW>
+// The waves' contexts (accumulators of operand row 4 g4 + r, channel 16 j + qi)
+// added up in LDS, then written: to out, or to a chunk's part
+template <int NW, bool R8>
 __device__ __forceinline__ void few_store(const PackedArgs& a, const Work& w, FewLds<NW>& lds,
-                                          const v4i (&hi)[8], const v4i (&lo)[8], bool any) {
+                                          const FewAcc<R8>& c, bool any) {
   const int lane = threadIdx.x & 63, qi = lane & 15, g4 = lane >> 4;
   const int R = w.T << a.lg;
   if (any) {
 #pragma unroll
     for (int j = 0; j < 8; ++j)
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
-        if (4 * g4 + r < R) atomicAdd(&lds.ctx[4 * g4 + r][16 * j + qi], hi[j][r] * 256 + lo[j][r]);
+      for (int r = 0; r < 4; ++r) {
+        const int row = R8 ? (4 * g4 + r) & 7 : 4 * g4 + r;
+        int x;
+        if constexpr (R8) x = g4 < 2 ? c.hi[j][r] * 256 : c.hi[j][r];
+        else x = c.hi[j][r] * 256 + c.lo[j][r];
+        if (row < R) atomicAdd(&lds.ctx[row][16 * j + qi], x);
+      }
   }
   __syncthreads();
   for (int i = threadIdx.x; i < R * 128; i += NW * 64) {
@@ -374,7 +498,7 @@ __device__ __forceinline__ void few_store(const PackedArgs& a, const Work& w, Fe
 }
 
 // A whole row of at most 64 NW NT slots: tile i of wave v is tile i NW + v
-template <int NW, int NT>
+template <int NW, int NT, bool R8>
 __device__ __forceinline__ void few_one(const PackedArgs& a, const Work& w, FewLds<NW>& lds) {
   const int lane = threadIdx.x & 63, qi = lane & 15, g4 = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
@@ -385,7 +509,7 @@ __device__ __forceinline__ void few_one(const PackedArgs& a, const Work& w, FewL
     const int it = i * NW + wave;
     pg[i] = it < ntiles ? packed_page(a, w.b, it >> 1) : -1;
   }
-  const FewRow row = few_row(a, w);
+  const FewRow row = few_row<R8>(a, w);
   for (int i = threadIdx.x; i < 16 * 128; i += NW * 64) ((int32_t*)lds.ctx)[i] = 0;
   v4i st[NT][4];
   {
@@ -423,12 +547,10 @@ __device__ __forceinline__ void few_one(const PackedArgs& a, const Work& w, FewL
   if (mx == NO_SCORE) mx = 0;  // nothing seen: max := 0, every p = 0
   const bool fast_e = __ballot(row.tpos >= FAST_T) == 0;
   const RowExp E = make_rowexp(row.tpos, mx);
-  RowSlow sl;
-  if (!fast_e) sl.E = make_exp(row.tpos);
   i64 den = 0;
 #pragma unroll
   for (int i = 0; i < NT; ++i)
-    if (i * NW + wave < ntiles) den = wadd(den, few_den(st[i], bits(i), fast_e, E, mx, sl.E));
+    if (i * NW + wave < ntiles) den = wadd(den, few_den(st[i], bits(i), fast_e, E, mx, row.tpos, {lds.slow[wave]}));
   den = group4_sum(den);
   if (g4 == 0) lds.den[wave][qi] = den;
   __syncthreads();
@@ -438,24 +560,19 @@ __device__ __forceinline__ void few_one(const PackedArgs& a, const Work& w, FewL
   den = imax(den, 1);
   const bool fast = fast_e && __ballot(den >= FAST_DEN) == 0;
   const double rp = make_rowp(den);
-  if (!fast) {
-    sl.E = make_exp(row.tpos);
-    sl.R = make_recip(den);
-  }
-  v4i hi[8], lo[8];
-#pragma unroll
-  for (int j = 0; j < 8; ++j) hi[j] = lo[j] = v4i{0, 0, 0, 0};
+  FewAcc<R8> acc;
+  acc.clear();
 #pragma unroll
   for (int i = 0; i < NT; ++i) {
     const int it = i * NW + wave;
     if (it < ntiles) {
       v4i v[8], phi, plo;
       if (i > 0) few_v(a, pg[i], w.kvh, it & 1, v);
-      few_probs(st[i], bits(i), fast, E, rp, mx, sl, phi, plo);
-      pv16(phi, plo, i > 0 ? v : v0, hi, lo);
+      few_probs(st[i], bits(i), fast, E, rp, mx, row.tpos, den, phi, plo, {lds.slow[wave]});
+      acc.add(phi, plo, i > 0 ? v : v0);
     }
   }
-  few_store<NW>(a, w, lds, hi, lo, wave < ntiles);
+  few_store<NW, R8>(a, w, lds, acc, wave < ntiles);
 }
 
 // The place of a unit's chunk in smax and sden
@@ -492,7 +609,7 @@ __device__ __forceinline__ void over_chunks(const PackedArgs& a, const Work& w, 
 }
 
 // One pass over chunk w.c of a few-row unit, four waves
-template <int PH>
+template <int PH, bool R8 = false>
 __device__ __forceinline__ void few_phase(const PackedArgs& a, const Work& w, FewLds<4>& lds) {
   const int lane = threadIdx.x & 63, qi = lane & 15, g4 = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
@@ -503,7 +620,7 @@ __device__ __forceinline__ void few_phase(const PackedArgs& a, const Work& w, Fe
   int32_t* const sc = a.scores + (((i64)w.b * a.n_kv + w.kvh) * a.few_rows) * pitch;
   const int t0 = lo_s / 64, t1 = (hi_s + 63) / 64;
   if constexpr (PH == PH_MAX) {
-    const FewRow row = few_row(a, w);
+    const FewRow row = few_row<false>(a, w);
     int mx = NO_SCORE;
     // two tiles of K in flight a wave
     for (int it = t0 + wave; it < t1; it += 8) {
@@ -582,11 +699,13 @@ __device__ __forceinline__ void few_phase(const PackedArgs& a, const Work& w, Fe
       if (lane == 0) a.sden[cell(a, w, w.c) + r] = den;
     }
   } else {
-    const FewRow row = few_row(a, w);
+    const FewRow row = few_row<R8>(a, w);
+    const int ri = R8 ? qi & 7 : qi;  // the lane's query row
+    const int32_t* src = sc + (row.on ? ri : 0) * pitch + 16 * g4;
     for (int i = threadIdx.x; i < 16 * 128; i += 256) ((int32_t*)lds.ctx)[i] = 0;
     int32_t mx;
     i64 den;
-    over_chunks<true>(a, w, nc, qi, &mx, &den);
+    over_chunks<true>(a, w, nc, ri, &mx, &den);
     if (!row.on) {
       mx = 0;
       den = 1;
@@ -594,41 +713,23 @@ __device__ __forceinline__ void few_phase(const PackedArgs& a, const Work& w, Fe
     const bool fast = __ballot(row.tpos >= FAST_T || den >= FAST_DEN) == 0;
     const RowExp E = make_rowexp(row.tpos, mx);
     const double rp = make_rowp(den);
-    RowSlow sl;
-    if (!fast) {
-      sl.E = make_exp(row.tpos);
-      sl.R = make_recip(den);
-    }
-    v4i hi[8], lo[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) hi[j] = lo[j] = v4i{0, 0, 0, 0};
+    FewAcc<R8> acc;
+    acc.clear();
     __syncthreads();  // ctx is zero
-    const int32_t* src = sc + (row.on ? qi : 0) * pitch + 16 * g4;
-    for (int it = t0 + wave; it < t1; it += 8) {
-      v4i v[2][8], st[2][4];
-      int pg[2];
+    for (int it = t0 + wave; it < t1; it += 4) {
+      v4i v[8], st[4];
+      const int pg = __builtin_amdgcn_readfirstlane(packed_page(a, w.b, it >> 1));
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
-        pg[u] = __builtin_amdgcn_readfirstlane(it + 4 * u < t1 ? packed_page(a, w.b, (it + 4 * u) >> 1) : -1);
+      for (int blk = 0; blk < 4; ++blk) st[blk] = *(const v4i*)(src + it * 64 + 4 * blk);
+      few_v(a, pg, w.kvh, it & 1, v);
+      uint32_t bb = 0;
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const int x = it + 4 * u < t1 ? it + 4 * u : it;
-#pragma unroll
-        for (int blk = 0; blk < 4; ++blk) st[u][blk] = *(const v4i*)(src + x * 64 + 4 * blk);
-        few_v(a, pg[u], w.kvh, (it + 4 * u) & 1, v[u]);
-      }
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-        if (it + 4 * u < t1) {
-          uint32_t bb = 0;
-#pragma unroll
-          for (int e = 0; e < 16; ++e) bb |= (st[u][e >> 2][e & 3] != NO_SCORE ? 1u : 0u) << e;
-          v4i phi, plo;
-          few_probs(st[u], row.on ? bb : 0u, fast, E, rp, mx, sl, phi, plo);
-          pv16(phi, plo, v[u], hi, lo);
-        }
+      for (int e = 0; e < 16; ++e) bb |= (st[e >> 2][e & 3] != NO_SCORE ? 1u : 0u) << e;
+      v4i phi, plo;
+      few_probs(st, row.on ? bb : 0u, fast, E, rp, mx, row.tpos, den, phi, plo, {lds.slow[wave]});
+      acc.add(phi, plo, v);
     }
-    few_store<4>(a, w, lds, hi, lo, true);
+    few_store<4, R8>(a, w, lds, acc, true);
   }
 }
 
@@ -811,29 +912,25 @@ __device__ __forceinline__ void tile_body(const PackedArgs& a, const Work& w, Ti
   // the accumulators of the slow forms start from 0
   const int32_t c0 = fast_e ? E.c0 : 0;
   const v4i cinit = v4i{c0, c0, c0, c0};
-  RowSlow sl;
-  if (DI_UNLIKELY(!fast_e)) sl.E = make_exp(tpos);
   if constexpr ((PH & PH_DEN) != 0) {
     den = 0;
     pass(std::false_type{}, [&](int i, const int8_t* stg) {
       halves(stg, i, cinit, [&](const v4i (&st)[4], int s0, int) {
-        if (DI_LIKELY(fast_e)) {
-          uint32_t sum = 0;
-          if (s0 + 63 <= wlim) {
-#pragma unroll
-            for (int e = 0; e < 16; ++e) sum += row_exp(st[e >> 2][e & 3], E);
-          } else {
-            const uint32_t bits = seen16(limit, s0 + 16 * g);
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              const uint32_t x = row_exp(st[e >> 2][e & 3], E);
-              sum += (bits >> e) & 1u ? x : 0u;
-            }
-          }
-          den += sum;
-        } else {
-          den = wadd(den, few_den(st, seen16(limit, s0 + 16 * g), false, E, mx, sl.E));
+        const uint32_t bits = seen16(limit, s0 + 16 * g);
+        if (DI_UNLIKELY(!fast_e)) {
+          den = wadd(den, slow_den(st, 0, bits, mx, tpos, InRegs{}));
+          return;
         }
+        uint32_t e[16], sum = 0;
+        row_exps(st, E, e);
+        if (s0 + 63 <= wlim) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) sum += e[i];
+        } else {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) sum += (bits >> i) & 1u ? e[i] : 0u;
+        }
+        den += sum;
       });
     });
     den = group4_sum(den);
@@ -845,12 +942,6 @@ __device__ __forceinline__ void tile_body(const PackedArgs& a, const Work& w, Ti
   }
   const bool fast = fast_e && __ballot(den >= FAST_DEN) == 0;
   const double rp = make_rowp(den);
-  if (DI_UNLIKELY(!fast)) {
-    sl.E = make_exp(tpos);
-    sl.R = make_recip(den);
-  }
-  // (a wave of few rows' exponentials in the fast form and its quotients not: the
-  // slow forms take the scores back from the accumulators)
   v4i ohi[8], olo[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) ohi[j] = olo[j] = v4i{0, 0, 0, 0};
@@ -864,38 +955,18 @@ __device__ __forceinline__ void tile_body(const PackedArgs& a, const Work& w, Ti
       for (int j = 0; j < 8; ++j) vf[j] = *(const v4i*)(stg + voff[hf] + j * 2048);
       __builtin_amdgcn_sched_barrier(0);
       v4i phi, plo;
-      const bool full = s0 + 63 <= wlim;
-      if (DI_LIKELY(fast && full)) {
-#pragma unroll
-        for (int blk = 0; blk < 4; ++blk) {
-          uint32_t w4[4];
-#pragma unroll
-          for (int r = 0; r < 4; ++r) w4[r] = row_p128(row_exp(st[blk][r], E), rp);
-          int h, l;
-          pack4(w4, h, l);
-          phi[blk] = h;
-          plo[blk] = l;
-        }
+      if (DI_UNLIKELY(!fast)) {
+        // (c0: scores that came with an offset are taken back)
+        slow_probs(st, c0, seen16(limit, s0 + 16 * g), mx, tpos, den, phi, plo, InRegs{});
       } else {
-        const uint32_t bits = seen16(limit, s0 + 16 * g);
+        uint32_t e[16];
+        row_exps(st, E, e);
+        if (s0 + 63 > wlim) {
+          const uint32_t bits = seen16(limit, s0 + 16 * g);
 #pragma unroll
-        for (int blk = 0; blk < 4; ++blk) {
-          uint32_t w4[4];
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const bool vis = (bits >> (4 * blk + r)) & 1u;
-            if (fast) {
-              const uint32_t x = row_exp(st[blk][r], E);
-              w4[r] = row_p128(vis ? x : 0u, rp);
-            } else {
-              w4[r] = vis ? slow_p128(slow_exp(st[blk][r] - c0, mx, sl.E), sl.R) : 128u;
-            }
-          }
-          int h, l;
-          pack4(w4, h, l);
-          phi[blk] = h;
-          plo[blk] = l;
+          for (int i = 0; i < 16; ++i) e[i] = (bits >> i) & 1u ? e[i] : 0u;
         }
+        row_probs(e, rp, phi, plo);
       }
       pv16(phi, plo, vf, ohi, olo);
     });

@@ -22,51 +22,56 @@ namespace {
 
 // Rows of at most 16 query rows alone, all slots in registers: NW waves, NT
 // 64-slot tiles each.
-template <int NT>
+template <int NT, bool R8>
 __global__ __launch_bounds__(512, 2) void k_packed_few(PackedArgs a) {
   keep_hidden_args();
   __shared__ FewLds<8> lds;
-  const Work w = find_work(a);
-  if (!w.live) {
-    zero_tail(a, w);
-    return;
+  const Finder f(a);
+  const int kvh = blockIdx.x % a.n_kv, j = blockIdx.x / a.n_kv;
+  if (j < f.total) {
+    const Work w = f.find(a, kvh, f.total - 1 - j);
+    report_row(a, w);
+    few_one<8, NT, R8>(a, w, lds);
   }
-  report_row(a, w);
-  few_one<8, NT>(a, w, lds);
+  if (threadIdx.x < 256) zero_tail(a, f.ntok, kvh, j);
 }
 
 // All three passes of any rows
 __global__ __launch_bounds__(256, 2) void k_packed_one(PackedArgs a) {
   keep_hidden_args();
   __shared__ TileLds lds;
-  const Work w = find_work(a);
-  if (!w.live) {
-    zero_tail(a, w);
-    return;
+  const Finder f(a);
+  const int kvh = blockIdx.x % a.n_kv, j = blockIdx.x / a.n_kv;
+  if (j < f.total) {
+    const Work w = f.find(a, kvh, f.total - 1 - j);
+    report_row(a, w);
+    if (w.few && w.len <= FEW_ONE_SLOTS) few_one<4, FEW_ONE_SLOTS / 256, false>(a, w, lds.few);
+    else tile_body<PH_ALL>(a, w, lds);
   }
-  report_row(a, w);
-  if (w.few && w.len <= FEW_ONE_SLOTS) few_one<4, FEW_ONE_SLOTS / 256>(a, w, lds.few);
-  else tile_body<PH_ALL>(a, w, lds);
+  zero_tail(a, f.ntok, kvh, j);
 }
 
-// One pass over a chunk. FEW: the launch's rows have at most 16 query rows
-template <int PH, bool FEW>
-__global__ __launch_bounds__(256, FEW ? 4 : 2) void k_packed_phase(PackedArgs a) {
+// One pass over chunks. FEW: the launch's rows have at most FEW (8 or 16) query rows
+template <int PH, int FEW>
+__global__ __launch_bounds__(256, FEW == 0 ? 2 : PH == PH_PV ? 3 : 4) void k_packed_phase(PackedArgs a) {
   keep_hidden_args();
-  const Work w = find_work(a);
-  if (!w.live) {
-    if (PH == PH_PV && a.nch == 1) zero_tail(a, w);
-    return;
+  const Finder f(a);
+  const int kvh = blockIdx.x % a.n_kv, j0 = blockIdx.x / a.n_kv;
+  for (int j = j0; j < f.total; j += a.step) {
+    const Work w = f.find(a, kvh, f.total - 1 - j);
+    if (PH == PH_MAX) report_row(a, w);
+    if (j != j0) __syncthreads();  // the item before is done with LDS
+    if constexpr (FEW != 0) {
+      __shared__ FewLds<4> lds;
+      few_phase<PH, FEW == 8>(a, w, lds);
+    } else {
+      __shared__ TileLds lds;
+      if (w.few && (w.T << a.lg) <= 8) few_phase<PH, true>(a, w, lds.few);
+      else if (w.few) few_phase<PH, false>(a, w, lds.few);
+      else tile_body<PH>(a, w, lds);
+    }
   }
-  if (PH == PH_MAX) report_row(a, w);
-  if constexpr (FEW) {
-    __shared__ FewLds<4> lds;
-    few_phase<PH>(a, w, lds);
-  } else {
-    __shared__ TileLds lds;
-    if (w.few) few_phase<PH>(a, w, lds.few);
-    else tile_body<PH>(a, w, lds);
-  }
+  if (PH == PH_PV && a.nch == 1) zero_tail(a, f.ntok, kvh, j0);
 }
 
 // The chunks' contexts of a token added up (one block per token row)
@@ -107,7 +112,8 @@ __global__ __launch_bounds__(256) void k_packed_join(PackedArgs a) {
 struct Plan {
   bool few;    // every row has at most 16 query rows
   bool one;    // one launch
-  int units;   // units that the rows can make, and one for the tail
+  int units;   // units that the rows can make
+  int step;    // blocks per kv head
   int rows;    // query rows of a few-row unit
   int chunk, nch;
   i64 scores_at, max_at, den_at, part_at, bytes;
@@ -122,18 +128,20 @@ inline Plan packed_plan(int N, int B, int S, int max_new, int n_q, int n_kv) {
   p.few = most * G <= 16;
   const i64 rows = ::min(B, N);
   const i64 units = p.few ? rows : imin((i64)N * G / 64 + rows, N);
-  p.units = (int)units + 1;
+  p.units = (int)imax(1, units);
   p.rows = (int)imin(16, most * G);
   const i64 pairs = units * n_kv;
   p.one = p.few ? S <= FEW_SLOTS : S <= FEW_ONE_SLOTS;
   p.chunk = S;
   if (!p.one) {
-    // chunks for about 1024 blocks
-    const i64 want = imax(1, imin((S + 511) / 512, 1024 / imax(1, pairs)));
+    // few-row units: chunks of 512 slots; 64 query rows: chunks for about 1024 blocks
+    const i64 want = p.few ? (S + 511) / 512 : imax(1, imin((S + 511) / 512, 1024 / imax(1, pairs)));
     p.chunk = (int)(((S + want - 1) / want + DI_PAGE - 1) / DI_PAGE * DI_PAGE);
   }
   p.chunk = ::max(p.chunk, 1);
   p.nch = ::max(1, (S + p.chunk - 1) / p.chunk);
+  p.step = p.units * p.nch;
+  if (!p.one) p.step = (int)imin(p.step, imax(1, 2048 / n_kv));
   if (p.one) return p;
   auto room = [&](i64 n) {
     const i64 at = p.bytes;
@@ -187,20 +195,26 @@ int detllm_attn_packed(const int8_t* q8, const int64_t* tpos, const int8_t* kpoo
   a.kv = KVPages{(int8_t*)kpool, (int8_t*)vpool, table, width, n_kv};
   a.n_pages = n_pages; a.cu = cu; a.past = past; a.N = N; a.B = B; a.S = S;
   a.n_q = n_q; a.n_kv = n_kv; a.lg = n_q / n_kv == 1 ? 0 : n_q / n_kv == 2 ? 1 : n_q / n_kv == 4 ? 2 : 3;
-  a.max_new = max_new; a.few_rows = p.rows; a.units = p.units; a.chunk = p.chunk; a.nch = p.nch; a.out = out; a.err = err;
+  a.max_new = max_new; a.few_rows = p.rows; a.units = p.units; a.step = p.step; a.chunk = p.chunk; a.nch = p.nch; a.out = out; a.err = err;
   char* const w = (char*)work;
   a.scores = (int32_t*)(w + p.scores_at);
   a.smax = (int32_t*)(w + p.max_at);
   a.sden = (int64_t*)(w + p.den_at);
   a.part = p.nch > 1 ? (int32_t*)(w + p.part_at) : nullptr;
-  const i64 blocks = (i64)p.units * p.nch * n_kv;
+  const i64 blocks = (i64)p.step * n_kv;
   if (blocks > 0x7fffffff) return DI_ERANGE;
   const dim3 grid((unsigned)blocks);
   if (p.one) {
     if (!p.few) hipLaunchKernelGGL(k_packed_one, grid, dim3(256), 0, s, a);
-    else if (S <= 512) hipLaunchKernelGGL(k_packed_few<1>, grid, dim3(512), 0, s, a);
-    else if (S <= 1024) hipLaunchKernelGGL(k_packed_few<2>, grid, dim3(512), 0, s, a);
-    else hipLaunchKernelGGL(k_packed_few<4>, grid, dim3(512), 0, s, a);
+    else if (p.rows <= 8) {
+      if (S <= 512) hipLaunchKernelGGL((k_packed_few<1, true>), grid, dim3(512), 0, s, a);
+      else if (S <= 1024) hipLaunchKernelGGL((k_packed_few<2, true>), grid, dim3(512), 0, s, a);
+      else hipLaunchKernelGGL((k_packed_few<4, true>), grid, dim3(512), 0, s, a);
+    } else {
+      if (S <= 512) hipLaunchKernelGGL((k_packed_few<1, false>), grid, dim3(512), 0, s, a);
+      else if (S <= 1024) hipLaunchKernelGGL((k_packed_few<2, false>), grid, dim3(512), 0, s, a);
+      else hipLaunchKernelGGL((k_packed_few<4, false>), grid, dim3(512), 0, s, a);
+    }
     DI_LAUNCH_CHECK();
     return DI_OK;
   }
@@ -211,8 +225,9 @@ int detllm_attn_packed(const int8_t* q8, const int64_t* tpos, const int8_t* kpoo
   DI_LAUNCH_CHECK();                                                                 \
   hipLaunchKernelGGL((k_packed_phase<PH_PV, FEW_>), grid, dim3(256), 0, s, a);       \
   DI_LAUNCH_CHECK()
-  if (p.few) { DI_PHASES(true); }
-  else { DI_PHASES(false); }
+  if (p.few && p.rows <= 8) { DI_PHASES(8); }
+  else if (p.few) { DI_PHASES(16); }
+  else { DI_PHASES(0); }
 #undef DI_PHASES
   if (p.nch > 1) {
     hipLaunchKernelGGL(k_packed_join, dim3(N), dim3(256), 0, s, a);
