@@ -8,7 +8,7 @@ namespace {
 constexpr int PACKED_MAX_S = 131071;    // int32 accumulators: 128 * 128 * S < 2^31
 constexpr int PACKED_MAX_ROWS = 65536;  // rows of a batch
 constexpr int FEW_SLOTS = 2048;         // slots of a few-row unit in a block of eight waves
-constexpr int FEW_ONE_SLOTS = 1024;     // and of four
+constexpr int FEW_ONE_SLOTS = 512;      // and of four
 
 // Passes
 constexpr int PH_MAX = 1, PH_DEN = 2, PH_PV = 4, PH_ALL = 7;
@@ -90,10 +90,10 @@ struct Rows {
 // first), kv heads fastest (with 8 of them a head's blocks share an XCD, so its L2
 // holds their K and V). A block takes item j, j + a.step, ...
 struct Finder {
-  Rows r;     // of the first 64 rows (all of most batches)
   int total;  // items
   int ntok;   // token rows of all rows
-  __device__ __forceinline__ explicit Finder(const PackedArgs& a) {
+  // r: the first 64 rows (all of most batches)
+  __device__ __forceinline__ Finder(const PackedArgs& a, Rows& r) {
     ntok = ::min(::max(a.cu[a.B], 0), a.N);
     r.load(a, 0);
     total = __builtin_amdgcn_readlane(r.items_to, 63);
@@ -103,10 +103,11 @@ struct Finder {
       total += __builtin_amdgcn_readlane(x.items_to, 63);
     }
   }
-  __device__ __forceinline__ Work find(const PackedArgs& a, int kvh, int item) const {
+  // item j of kv head kvh; x: the first 64 rows
+  __device__ __forceinline__ Work find(const PackedArgs& a, Rows x, int kvh, int j) const {
     Work w{};
     w.kvh = kvh;
-    Rows x = r;
+    const int item = total - 1 - j;
     int items = 0, units = 0, b0 = 0;
     for (;;) {
       const int tot = __builtin_amdgcn_readlane(x.items_to, 63);
@@ -390,11 +391,12 @@ __device__ __forceinline__ void few_k(const PackedArgs& a, int pg, int kvh, int 
   }
 }
 // V operands: channel 16 j + qi, slots 16 g4 .. + 15 of the half
+template <int J0 = 0, int J1 = 8>
 __device__ __forceinline__ void few_v(const PackedArgs& a, int pg, int kvh, int hf, v4i (&v)[8]) {
   const int lane = threadIdx.x & 63, qi = lane & 15, g4 = lane >> 4;
   const int8_t* p = a.kv.vchan(::max(pg, 0), kvh, qi) + hf * 64 + g4 * 16;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) v[j] = *(const v4i*)(p + j * 16 * DI_PAGE);
+  for (int j = J0; j < J1; ++j) v[j] = *(const v4i*)(p + j * 16 * DI_PAGE);
 }
 __device__ __forceinline__ void few_scores(const v4i (&k)[8], const FewRow& r, v4i (&st)[4]) {
   const v4i z = v4i{0, 0, 0, 0};
@@ -608,9 +610,9 @@ __device__ __forceinline__ void over_chunks(const PackedArgs& a, const Work& w, 
   if (DEN) *den = imax(group4_sum(d), 1);
 }
 
-// One pass over chunk w.c of a few-row unit, four waves
-template <int PH, bool R8 = false>
-__device__ __forceinline__ void few_phase(const PackedArgs& a, const Work& w, FewLds<4>& lds) {
+// One pass over chunk w.c of a few-row unit, NW waves
+template <int PH, int NW, bool R8>
+__device__ __forceinline__ void few_phase(const PackedArgs& a, const Work& w, FewLds<NW>& lds) {
   const int lane = threadIdx.x & 63, qi = lane & 15, g4 = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const int lo_s = w.c * a.chunk, hi_s = ::min(w.len, lo_s + a.chunk);
@@ -623,17 +625,17 @@ __device__ __forceinline__ void few_phase(const PackedArgs& a, const Work& w, Fe
     const FewRow row = few_row<false>(a, w);
     int mx = NO_SCORE;
     // two tiles of K in flight a wave
-    for (int it = t0 + wave; it < t1; it += 8) {
+    for (int it = t0 + wave; it < t1; it += 2 * NW) {
       v4i k[2][8];
       int pg[2];
 #pragma unroll
       for (int u = 0; u < 2; ++u)
-        pg[u] = __builtin_amdgcn_readfirstlane(it + 4 * u < t1 ? packed_page(a, w.b, (it + 4 * u) >> 1) : -1);
+        pg[u] = __builtin_amdgcn_readfirstlane(it + NW * u < t1 ? packed_page(a, w.b, (it + NW * u) >> 1) : -1);
 #pragma unroll
-      for (int u = 0; u < 2; ++u) few_k(a, pg[u], w.kvh, (it + 4 * u) & 1, k[u]);
+      for (int u = 0; u < 2; ++u) few_k(a, pg[u], w.kvh, (it + NW * u) & 1, k[u]);
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        const int x = it + 4 * u;
+        const int x = it + NW * u;
         if (x < t1) {
           v4i st[4];
           few_scores(k[u], row, st);
@@ -657,12 +659,12 @@ __device__ __forceinline__ void few_phase(const PackedArgs& a, const Work& w, Fe
     __syncthreads();
     if (threadIdx.x < 16) {
 #pragma unroll
-      for (int v = 0; v < 4; ++v) mx = ::max(mx, lds.mx[v][qi]);
+      for (int v = 0; v < NW; ++v) mx = ::max(mx, lds.mx[v][qi]);
       a.smax[cell(a, w, w.c) + qi] = mx;
     }
   } else if constexpr (PH == PH_DEN) {
     // a query row a wave, four slots a lane and load (chunks end on whole tiles)
-    for (int r = wave; r < R; r += 4) {
+    for (int r = wave; r < R; r += NW) {
       int m = NO_SCORE;
       for (int c = lane; c < nc; c += 64) m = ::max(m, a.smax[cell(a, w, c) + r]);
 #pragma unroll
@@ -702,7 +704,7 @@ __device__ __forceinline__ void few_phase(const PackedArgs& a, const Work& w, Fe
     const FewRow row = few_row<R8>(a, w);
     const int ri = R8 ? qi & 7 : qi;  // the lane's query row
     const int32_t* src = sc + (row.on ? ri : 0) * pitch + 16 * g4;
-    for (int i = threadIdx.x; i < 16 * 128; i += 256) ((int32_t*)lds.ctx)[i] = 0;
+    for (int i = threadIdx.x; i < 16 * 128; i += NW * 64) ((int32_t*)lds.ctx)[i] = 0;
     int32_t mx;
     i64 den;
     over_chunks<true>(a, w, nc, ri, &mx, &den);
@@ -716,48 +718,63 @@ __device__ __forceinline__ void few_phase(const PackedArgs& a, const Work& w, Fe
     FewAcc<R8> acc;
     acc.clear();
     __syncthreads();  // ctx is zero
-    for (int it = t0 + wave; it < t1; it += 4) {
+    for (int it = t0 + wave; it < t1; it += NW) {
       v4i v[8], st[4];
       const int pg = __builtin_amdgcn_readfirstlane(packed_page(a, w.b, it >> 1));
 #pragma unroll
       for (int blk = 0; blk < 4; ++blk) st[blk] = *(const v4i*)(src + it * 64 + 4 * blk);
-      few_v(a, pg, w.kvh, it & 1, v);
+      // (with twice the accumulators, half of V waits until the scores' registers are free)
+      few_v<0, R8 ? 8 : 4>(a, pg, w.kvh, it & 1, v);
       uint32_t bb = 0;
 #pragma unroll
       for (int e = 0; e < 16; ++e) bb |= (st[e >> 2][e & 3] != NO_SCORE ? 1u : 0u) << e;
       v4i phi, plo;
       few_probs(st, row.on ? bb : 0u, fast, E, rp, mx, row.tpos, den, phi, plo, {lds.slow[wave]});
+      if constexpr (!R8) {
+        __builtin_amdgcn_sched_barrier(0);
+        few_v<4, 8>(a, pg, w.kvh, it & 1, v);
+      }
       acc.add(phi, plo, v);
     }
-    few_store<4, R8>(a, w, lds, acc, true);
+    few_store<NW, R8>(a, w, lds, acc, true);
   }
 }
 
 // ------------------------------------------------------------- 64 query rows
 //
 // Four waves of 16 query rows (row i: token i / G, head i % G of the kv head, so K
-// and V are read once for the kv head's query heads); key pages reach LDS by
-// direct-to-LDS loads, a 64 KB ring of them ahead of the pass, one barrier per
-// page, their 16-byte chunks swizzled against bank conflicts.
+// and V are read once for the kv head's query heads). Keys reach LDS by
+// direct-to-LDS loads, 16 KB a stage: a page of K in the first two passes, half a
+// page of K and V in the third; one barrier a stage, 16-byte chunks swizzled
+// against bank conflicts.
+//
+// What bounds it: a stage arrives about a microsecond after it is asked for, so a
+// CU needs some 100 KB on their way (three blocks, two of three stages each: with
+// one of two 32 KB stages ahead, the loads alone of the third pass over 2500 slots
+// took 26 of its 39 us); and a SIMD takes an instruction of one wave every five
+// cycles, while most operations of an exponential last two, so it wants three
+// waves (168 registers a lane; scratch memory for spills would cost a launch
+// 8 us by itself).
 
-constexpr int TL_K = 128 * 128;       // K page: 128 slot rows of 128 B
-constexpr int TL_V = 128 * 128;       // V page: 128 channel rows of 128 B
-constexpr int TL_RING = 64 * 1024;
-constexpr int TL_RESIDENT = TL_RING / (TL_K + TL_V);  // pages that stay for all three passes
-constexpr int TL_PAGES = 1024;        // pages of the longest row
+constexpr int TL_NT = 256;
+constexpr int TL_STAGE = 16 * 1024;
+constexpr int TL_STAGES = 3;
+constexpr int TL_HALF = 8 * 1024;  // K's part of a half-page stage: 64 slot rows of 128 B
+constexpr int TL_PAGES = 1024;     // pages of the longest row
 
 struct TileLds {
   union {
-    __attribute__((aligned(1024))) int8_t ring[TL_RING];
+    __attribute__((aligned(1024))) int8_t ring[TL_STAGES * TL_STAGE];
     FewLds<4> few;
   };
   int32_t pages[TL_PAGES];
 };
 
 // Physical chunk = logical ^ swizzle, so that the operand reads below take LDS's
-// full rate: bits 0, 1 and 4 of a K row, the low 3 bits of a V row
+// full rate. K (rows of 8 chunks): bits 0, 1 and 4 of the row. V half pages (channel
+// rows of 4 chunks, two to 128 bytes): bits 1 and 2 of the channel.
 __device__ __forceinline__ int tl_kswz(int row) { return (row & 3) | ((row >> 2) & 4); }
-__device__ __forceinline__ int tl_vswz(int d) { return d & 7; }
+__device__ __forceinline__ int tl_vswz(int d) { return (d >> 1) & 3; }
 
 template <int PH>
 __device__ __forceinline__ void tile_body(const PackedArgs& a, const Work& w, TileLds& lds) {
@@ -772,6 +789,7 @@ __device__ __forceinline__ void tile_body(const PackedArgs& a, const Work& w, Ti
   const int hi_s = PH == PH_ALL ? end : ::min(end, lo_s + a.chunk);
   if (lo_s >= hi_s) return;
   const int p0 = lo_s / DI_PAGE, np = (hi_s + DI_PAGE - 1) / DI_PAGE - p0;
+  const int nh = (hi_s + 63) / 64 - 2 * p0;  // half pages
   const int wr0 = r0 + wave * 16;          // the wave's first query row
   const bool work = wr0 < R;               // (waves without one only load)
   const int qr = ::min(wr0 + qi, R - 1);   // the lane's (rows past the last: the last, not stored)
@@ -784,116 +802,104 @@ __device__ __forceinline__ void tile_body(const PackedArgs& a, const Work& w, Ti
   const v4i qf1 = *(const v4i*)(a.q8 + qrow * 128 + 64 + g * 16);
   const i64 tpos = a.tpos[qrow];
 
-  int koffl[4], voffl[4];
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int row = (wave * 4 + j) * 8 + (lane >> 3);
-    koffl[j] = row * 128 + ((lane & 7) ^ tl_kswz(row)) * 16;
-    voffl[j] = row * DI_PAGE + ((lane & 7) ^ tl_vswz(row)) * 16;
-  }
-  // a page that is not there: a view of no bytes, whose loads read 0
-  auto issue = [&](int page, int8_t* st, bool with_v) {
+  // Load j of a wave brings 1 KB: K rows 8 (4 wave + j) .. + 7 of a page, or 8 (2
+  // wave + j) .. of a half; V: channels 16 (2 wave + j) .. + 15, 64 bytes each
+  auto rsrc = [&](const int8_t* p, int page) {
+    // (a page that is not there: a view of no bytes, whose loads read 0)
+    return __builtin_amdgcn_make_buffer_rsrc((void*)p, (short)0, page < 0 ? 0 : DI_PAGE * 128,
+                                             0x00020000);
+  };
+  auto k_off = [&](int row) { return row * 128 + ((lane & 7) ^ tl_kswz(row)) * 16; };
+  auto issue_page = [&](int page, int8_t* st) {
     const int pg = __builtin_amdgcn_readfirstlane(page);
-    const int pgc = pg < 0 ? 0 : pg, n = pg < 0 ? 0 : DI_PAGE * 128;
-    const __amdgpu_buffer_rsrc_t krs = __builtin_amdgcn_make_buffer_rsrc(
-        (void*)a.kv.krow(pgc, w.kvh, 0), (short)0, n, 0x00020000);
+    const auto krs = rsrc(a.kv.krow(::max(pg, 0), w.kvh, 0), pg);
 #pragma unroll
     for (int j = 0; j < 4; ++j)
       __builtin_amdgcn_raw_ptr_buffer_load_lds(krs, (lds_ptr_t)(st + (wave * 4 + j) * 1024), 16,
-                                               koffl[j], 0, 0, 0);
-    if (with_v) {
-      const __amdgpu_buffer_rsrc_t vrs = __builtin_amdgcn_make_buffer_rsrc(
-          (void*)a.kv.vchan(pgc, w.kvh, 0), (short)0, n, 0x00020000);
+                                               k_off((wave * 4 + j) * 8 + (lane >> 3)), 0, 0, 0);
+  };
+  auto issue_half = [&](int page, int hf, int8_t* st) {
+    const int pg = __builtin_amdgcn_readfirstlane(page);
+    const auto krs = rsrc(a.kv.krow(::max(pg, 0), w.kvh, 0), pg);
+    const auto vrs = rsrc(a.kv.vchan(::max(pg, 0), w.kvh, 0), pg);
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(
-            vrs, (lds_ptr_t)(st + TL_K + (wave * 4 + j) * 1024), 16, voffl[j], 0, 0, 0);
+    for (int j = 0; j < 2; ++j) {
+      const int at = wave * 2 + j;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(krs, (lds_ptr_t)(st + at * 1024), 16,
+                                               k_off(at * 8 + (lane >> 3)), hf * TL_HALF, 0, 0);
+      const int d = at * 16 + (lane >> 2);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(
+          vrs, (lds_ptr_t)(st + TL_HALF + at * 1024), 16,
+          d * DI_PAGE + ((lane & 3) ^ tl_vswz(d)) * 16, hf * 64, 0, 0);
     }
   };
-  const bool resident = PH == PH_ALL && np <= TL_RESIDENT;
-  for (int i = tid; i < np; i += 256) lds.pages[i] = packed_page(a, w.b, p0 + i);
-  if (resident)
-    for (int i = 0; i < np; ++i)
-      issue(packed_page(a, w.b, p0 + i), lds.ring + i * (TL_K + TL_V), true);
-  wait_vmcnt<0>();  // queries, page ids; a resident tile's pages
+  for (int i = tid; i < np; i += TL_NT) lds.pages[i] = packed_page(a, w.b, p0 + i);
+  wait_vmcnt<0>();  // queries, page ids
   __syncthreads();
 
-  // One pass over the pages; body(i, stage) runs with page i in LDS. Each wave
-  // waits for its own loads of the page (they complete in order), then one
-  // barrier publishes every wave's part and frees the stage that the next issue
-  // overwrites.
-  auto pass = [&](auto kv, auto&& body) {
-    constexpr bool KV = decltype(kv)::value;
-    constexpr int STAGE = KV ? TL_K + TL_V : TL_K;
-    constexpr int ST = TL_RING / STAGE;
-    constexpr int LPT = KV ? 8 : 4;  // loads per page and wave
-    if (resident) {
-      for (int i = 0; i < np; ++i) body(i, lds.ring + i * (TL_K + TL_V));
-      return;
-    }
+  // One pass over n stages; issue(i, stage), body(i, stage). Each wave waits for
+  // its own loads of a stage (four, and they complete in order), then one barrier
+  // publishes every wave's part and frees the stage that the next issue overwrites.
+  auto pass = [&](int n, auto&& issue, auto&& body) {
     wait_lds();
     __builtin_amdgcn_s_barrier();  // the pass before is done with the ring
 #pragma unroll
-    for (int s = 0; s < ST - 1; ++s)
-      if (s < np) issue(lds.pages[s], lds.ring + s * STAGE, KV);
-    for (int i = 0; i < np; ++i) {
-      const int after = ::min(ST - 2, np - 1 - i);  // pages issued after this one
-      if (after >= 2) wait_vmcnt<2 * LPT>();
-      else if (after == 1) wait_vmcnt<LPT>();
+    for (int s = 0; s < TL_STAGES - 1; ++s)
+      if (s < n) issue(s, lds.ring + s * TL_STAGE);
+    int at = 0;  // the stage of i
+    for (int i = 0; i < n; ++i) {
+      if (i + 1 < n) wait_vmcnt<4>();
       else wait_vmcnt<0>();
       wait_lds();
       __builtin_amdgcn_s_barrier();
-      if (i + ST - 1 < np) issue(lds.pages[i + ST - 1], lds.ring + ((i + ST - 1) % ST) * STAGE, KV);
-      body(i, lds.ring + (i % ST) * STAGE);
+      const int next = at == 0 ? TL_STAGES - 1 : at - 1;
+      if (i + TL_STAGES - 1 < n) issue(i + TL_STAGES - 1, lds.ring + next * TL_STAGE);
+      body(i, lds.ring + at * TL_STAGE);
+      at = at + 1 == TL_STAGES ? 0 : at + 1;
     }
   };
+  auto k_pages = [&](int i, int8_t* st) { issue_page(lds.pages[i], st); };
+  auto kv_halves = [&](int i, int8_t* st) { issue_half(lds.pages[i >> 1], i & 1, st); };
   const int kr = 16 * (qi >> 2) + (qi & 3);
   const int koff0 = kr * 128 + ((g ^ tl_kswz(kr)) << 4);
   const int koff1 = kr * 128 + (((g + 4) ^ tl_kswz(kr)) << 4);
-  auto load_k = [&](const int8_t* st, v4i (&kf)[8]) {
+  // half page i (its K rows at `keys`): its scores from accumulators z, then fn(st,
+  // s0) (its first slot s0); one that is not there, or that no query row of the
+  // wave sees, is passed over
+  auto half = [&](const int8_t* keys, int i, const v4i z, auto&& fn) {
+    const int s0 = p0 * DI_PAGE + i * 64;
+    if (!work || s0 > wmax || __builtin_amdgcn_readfirstlane(lds.pages[i >> 1]) < 0) return;
+    v4i kf[8], st[4];
 #pragma unroll
     for (int blk = 0; blk < 4; ++blk) {
-      kf[2 * blk] = *(const v4i*)(st + koff0 + blk * 512);
-      kf[2 * blk + 1] = *(const v4i*)(st + koff1 + blk * 512);
+      kf[2 * blk] = *(const v4i*)(keys + koff0 + blk * 512);
+      kf[2 * blk + 1] = *(const v4i*)(keys + koff1 + blk * 512);
     }
+#pragma unroll
+    for (int blk = 0; blk < 4; ++blk) st[blk] = mfma16(kf[2 * blk], qf0, z);
+#pragma unroll
+    for (int blk = 0; blk < 4; ++blk) st[blk] = mfma16(kf[2 * blk + 1], qf1, st[blk]);
+    fn(st, s0);
   };
-  // both halves' scores from accumulators z, then fn(st, s0, hf) per half (its
-  // first slot s0); a page that is not there, or that no query row of the wave
-  // sees, is passed over
-  auto halves = [&](const int8_t* stg, int i, const v4i z, auto&& fn) {
-    const int s0 = (p0 + i) * DI_PAGE;
-    if (!work || s0 > wmax || __builtin_amdgcn_readfirstlane(lds.pages[i]) < 0) return;
-    v4i ka[8], kb[8], sa[4], sb[4];
-    load_k(stg, ka);
-    load_k(stg + 64 * 128, kb);
-    __builtin_amdgcn_sched_barrier(0);
+  auto k_pass = [&](const v4i z, auto&& fn) {
+    pass(np, k_pages, [&](int i, const int8_t* st) {
 #pragma unroll
-    for (int blk = 0; blk < 4; ++blk) sa[blk] = mfma16(ka[2 * blk], qf0, z);
-#pragma unroll
-    for (int blk = 0; blk < 4; ++blk) sb[blk] = mfma16(kb[2 * blk], qf0, z);
-#pragma unroll
-    for (int blk = 0; blk < 4; ++blk) sa[blk] = mfma16(ka[2 * blk + 1], qf1, sa[blk]);
-#pragma unroll
-    for (int blk = 0; blk < 4; ++blk) sb[blk] = mfma16(kb[2 * blk + 1], qf1, sb[blk]);
-    __builtin_amdgcn_sched_barrier(0);
-    fn(sa, s0, 0);
-    if (s0 + 64 <= wmax) fn(sb, s0 + 64, 1);
+      for (int h = 0; h < 2; ++h) half(st + h * TL_HALF, 2 * i + h, z, fn);
+    });
   };
 
   int32_t mx = NO_SCORE;
   if constexpr ((PH & PH_MAX) != 0) {
-    pass(std::false_type{}, [&](int i, const int8_t* stg) {
-      halves(stg, i, v4i{0, 0, 0, 0}, [&](const v4i (&st)[4], int s0, int) {
-        if (s0 + 63 <= wlim) {
+    k_pass(v4i{0, 0, 0, 0}, [&](const v4i (&st)[4], int s0) {
+      if (s0 + 63 <= wlim) {
 #pragma unroll
-          for (int e = 0; e < 16; ++e) mx = ::max(mx, st[e >> 2][e & 3]);
-        } else {
-          const uint32_t bits = seen16(limit, s0 + 16 * g);
+        for (int e = 0; e < 16; ++e) mx = ::max(mx, st[e >> 2][e & 3]);
+      } else {
+        const uint32_t bits = seen16(limit, s0 + 16 * g);
 #pragma unroll
-          for (int e = 0; e < 16; ++e)
-            if ((bits >> e) & 1u) mx = ::max(mx, st[e >> 2][e & 3]);
-        }
-      });
+        for (int e = 0; e < 16; ++e)
+          if ((bits >> e) & 1u) mx = ::max(mx, st[e >> 2][e & 3]);
+      }
     });
     mx = max16(mx);
     if constexpr (PH == PH_MAX) {
@@ -904,8 +910,8 @@ __device__ __forceinline__ void tile_body(const PackedArgs& a, const Work& w, Ti
   }
   const int nc = (end + a.chunk - 1) / a.chunk;
   i64 den = 0;
-  if constexpr (PH == PH_DEN) over_chunks<false>(a, w, nc, ::min(wr0 + qi, R - 1) - r0, &mx, &den);
-  if constexpr (PH == PH_PV) over_chunks<true>(a, w, nc, ::min(wr0 + qi, R - 1) - r0, &mx, &den);
+  if constexpr (PH == PH_DEN) over_chunks<false>(a, w, nc, qr - r0, &mx, &den);
+  if constexpr (PH == PH_PV) over_chunks<true>(a, w, nc, qr - r0, &mx, &den);
 
   const bool fast_e = __ballot(tpos >= FAST_T) == 0;
   const RowExp E = make_rowexp(fast_e ? tpos : 1, mx);
@@ -914,25 +920,26 @@ __device__ __forceinline__ void tile_body(const PackedArgs& a, const Work& w, Ti
   const v4i cinit = v4i{c0, c0, c0, c0};
   if constexpr ((PH & PH_DEN) != 0) {
     den = 0;
-    pass(std::false_type{}, [&](int i, const int8_t* stg) {
-      halves(stg, i, cinit, [&](const v4i (&st)[4], int s0, int) {
-        const uint32_t bits = seen16(limit, s0 + 16 * g);
-        if (DI_UNLIKELY(!fast_e)) {
-          den = wadd(den, slow_den(st, 0, bits, mx, tpos, InRegs{}));
-          return;
-        }
+    // (the slow forms in a loop of their own: what they hold does not weigh on the other)
+    if (DI_LIKELY(fast_e)) {
+      k_pass(cinit, [&](const v4i (&st)[4], int s0) {
         uint32_t e[16], sum = 0;
         row_exps(st, E, e);
         if (s0 + 63 <= wlim) {
 #pragma unroll
           for (int i = 0; i < 16; ++i) sum += e[i];
         } else {
+          const uint32_t bits = seen16(limit, s0 + 16 * g);
 #pragma unroll
           for (int i = 0; i < 16; ++i) sum += (bits >> i) & 1u ? e[i] : 0u;
         }
         den += sum;
       });
-    });
+    } else {
+      k_pass(cinit, [&](const v4i (&st)[4], int s0) {
+        den = wadd(den, slow_den(st, 0, seen16(limit, s0 + 16 * g), mx, tpos, InRegs{}));
+      });
+    }
     den = group4_sum(den);
     if constexpr (PH == PH_DEN) {
       if (work && g == 0) a.sden[cell(a, w, w.c) + wave * 16 + qi] = den;
@@ -945,20 +952,19 @@ __device__ __forceinline__ void tile_body(const PackedArgs& a, const Work& w, Ti
   v4i ohi[8], olo[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) ohi[j] = olo[j] = v4i{0, 0, 0, 0};
-  int voff[2];
+  // V operand of a half page: channel 16 j + qi, slots 16 g .. + 15 (the swizzle of
+  // channel 16 j + qi does not depend on j)
+  const int voff = TL_HALF + qi * 64 + ((g ^ tl_vswz(qi)) << 4);
+  auto pv = [&](const int8_t* stg, const v4i& phi, const v4i& plo) {
+    v4i vf[8];
 #pragma unroll
-  for (int hf = 0; hf < 2; ++hf) voff[hf] = TL_K + qi * 128 + (((4 * hf + g) ^ tl_vswz(qi)) << 4);
-  pass(std::true_type{}, [&](int i, const int8_t* stg) {
-    halves(stg, i, cinit, [&](const v4i (&st)[4], int s0, int hf) {
-      v4i vf[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) vf[j] = *(const v4i*)(stg + voff[hf] + j * 2048);
-      __builtin_amdgcn_sched_barrier(0);
-      v4i phi, plo;
-      if (DI_UNLIKELY(!fast)) {
-        // (c0: scores that came with an offset are taken back)
-        slow_probs(st, c0, seen16(limit, s0 + 16 * g), mx, tpos, den, phi, plo, InRegs{});
-      } else {
+    for (int j = 0; j < 8; ++j) vf[j] = *(const v4i*)(stg + voff + j * 1024);
+    pv16(phi, plo, vf, ohi, olo);
+  };
+  if (DI_LIKELY(fast)) {
+    pass(nh, kv_halves, [&](int i, const int8_t* stg) {
+      half(stg, i, cinit, [&](const v4i (&st)[4], int s0) {
+        v4i phi, plo;
         uint32_t e[16];
         row_exps(st, E, e);
         if (s0 + 63 > wlim) {
@@ -967,10 +973,19 @@ __device__ __forceinline__ void tile_body(const PackedArgs& a, const Work& w, Ti
           for (int i = 0; i < 16; ++i) e[i] = (bits >> i) & 1u ? e[i] : 0u;
         }
         row_probs(e, rp, phi, plo);
-      }
-      pv16(phi, plo, vf, ohi, olo);
+        pv(stg, phi, plo);
+      });
     });
-  });
+  } else {
+    pass(nh, kv_halves, [&](int i, const int8_t* stg) {
+      half(stg, i, cinit, [&](const v4i (&st)[4], int s0) {
+        v4i phi, plo;
+        // (c0: scores that came with an offset are taken back)
+        slow_probs(st, c0, seen16(limit, s0 + 16 * g), mx, tpos, den, phi, plo, InRegs{});
+        pv(stg, phi, plo);
+      });
+    });
+  }
   if (!work) return;
   // lane (qi, g): query rows 4 g + r of the wave, channel 16 j + qi
 #pragma unroll

@@ -26,10 +26,11 @@ template <int NT, bool R8>
 __global__ __launch_bounds__(512, 2) void k_packed_few(PackedArgs a) {
   keep_hidden_args();
   __shared__ FewLds<8> lds;
-  const Finder f(a);
+  Rows rows;
+  const Finder f(a, rows);
   const int kvh = blockIdx.x % a.n_kv, j = blockIdx.x / a.n_kv;
   if (j < f.total) {
-    const Work w = f.find(a, kvh, f.total - 1 - j);
+    const Work w = f.find(a, rows, kvh, j);
     report_row(a, w);
     few_one<8, NT, R8>(a, w, lds);
   }
@@ -37,13 +38,14 @@ __global__ __launch_bounds__(512, 2) void k_packed_few(PackedArgs a) {
 }
 
 // All three passes of any rows
-__global__ __launch_bounds__(256, 2) void k_packed_one(PackedArgs a) {
+__global__ __launch_bounds__(TL_NT, 3) void k_packed_one(PackedArgs a) {
   keep_hidden_args();
   __shared__ TileLds lds;
-  const Finder f(a);
+  Rows rows;
+  const Finder f(a, rows);
   const int kvh = blockIdx.x % a.n_kv, j = blockIdx.x / a.n_kv;
   if (j < f.total) {
-    const Work w = f.find(a, kvh, f.total - 1 - j);
+    const Work w = f.find(a, rows, kvh, j);
     report_row(a, w);
     if (w.few && w.len <= FEW_ONE_SLOTS) few_one<4, FEW_ONE_SLOTS / 256, false>(a, w, lds.few);
     else tile_body<PH_ALL>(a, w, lds);
@@ -53,21 +55,25 @@ __global__ __launch_bounds__(256, 2) void k_packed_one(PackedArgs a) {
 
 // One pass over chunks. FEW: the launch's rows have at most FEW (8 or 16) query rows
 template <int PH, int FEW>
-__global__ __launch_bounds__(256, FEW == 0 ? 2 : PH == PH_PV ? 3 : 4) void k_packed_phase(PackedArgs a) {
+__global__ __launch_bounds__(256, FEW == 0 || PH == PH_PV ? 3 : 4) void k_packed_phase(PackedArgs a) {
   keep_hidden_args();
-  const Finder f(a);
+  Rows rows;
+  const Finder f(a, rows);
   const int kvh = blockIdx.x % a.n_kv, j0 = blockIdx.x / a.n_kv;
   for (int j = j0; j < f.total; j += a.step) {
-    const Work w = f.find(a, kvh, f.total - 1 - j);
+    if (j != j0) {
+      rows.load(a, 0);  // (again, or its registers are held all along)
+      __syncthreads();  // the item before is done with LDS
+    }
+    const Work w = f.find(a, rows, kvh, j);
     if (PH == PH_MAX) report_row(a, w);
-    if (j != j0) __syncthreads();  // the item before is done with LDS
     if constexpr (FEW != 0) {
       __shared__ FewLds<4> lds;
-      few_phase<PH, FEW == 8>(a, w, lds);
+      few_phase<PH, 4, FEW == 8>(a, w, lds);
     } else {
       __shared__ TileLds lds;
-      if (w.few && (w.T << a.lg) <= 8) few_phase<PH, true>(a, w, lds.few);
-      else if (w.few) few_phase<PH, false>(a, w, lds.few);
+      if (w.few && (w.T << a.lg) <= 8) few_phase<PH, 4, true>(a, w, lds.few);
+      else if (w.few) few_phase<PH, 4, false>(a, w, lds.few);
       else tile_body<PH>(a, w, lds);
     }
   }
@@ -131,7 +137,7 @@ inline Plan packed_plan(int N, int B, int S, int max_new, int n_q, int n_kv) {
   p.units = (int)imax(1, units);
   p.rows = (int)imin(16, most * G);
   const i64 pairs = units * n_kv;
-  p.one = p.few ? S <= FEW_SLOTS : S <= FEW_ONE_SLOTS;
+  p.one = p.few ? S <= FEW_SLOTS : S <= FEW_ONE_SLOTS || pairs >= 384;
   p.chunk = S;
   if (!p.one) {
     // few-row units: chunks of 512 slots; 64 query rows: chunks for about 1024 blocks
@@ -205,7 +211,7 @@ int detllm_attn_packed(const int8_t* q8, const int64_t* tpos, const int8_t* kpoo
   if (blocks > 0x7fffffff) return DI_ERANGE;
   const dim3 grid((unsigned)blocks);
   if (p.one) {
-    if (!p.few) hipLaunchKernelGGL(k_packed_one, grid, dim3(256), 0, s, a);
+    if (!p.few) hipLaunchKernelGGL(k_packed_one, grid, dim3(TL_NT), 0, s, a);
     else if (p.rows <= 8) {
       if (S <= 512) hipLaunchKernelGGL((k_packed_few<1, true>), grid, dim3(512), 0, s, a);
       else if (S <= 1024) hipLaunchKernelGGL((k_packed_few<2, true>), grid, dim3(512), 0, s, a);
