@@ -8,7 +8,7 @@ namespace {
 constexpr int PACKED_MAX_S = 131071;    // int32 accumulators: 128 * 128 * S < 2^31
 constexpr int PACKED_MAX_ROWS = 65536;  // rows of a batch
 constexpr int FEW_SLOTS = 2048;         // slots of a few-row unit in a block of eight waves
-constexpr int FEW_ONE_SLOTS = 512;      // and of four
+constexpr int FEW_ONE_SLOTS = 512;      // and beside tiles
 
 // Passes
 constexpr int PH_MAX = 1, PH_DEN = 2, PH_PV = 4, PH_ALL = 7;
@@ -49,6 +49,14 @@ struct Work {
 __device__ __forceinline__ int row_limit(const PackedArgs& a, int past, int t) {
   const i64 l = (i64)::max(past, 0) + t;
   return (int)imin(l, (i64)a.S - 1);
+}
+
+// threadIdx.x as a value of its own: what follows from it is made anew for each item
+// of a block, not held in registers across them
+__device__ __forceinline__ int thread_now() {
+  int t = threadIdx.x;
+  asm volatile("" : "+v"(t));
+  return t;
 }
 
 // Inclusive sum over the lanes: within rows of 16 (row shifts by 1, 2, 4, 8),
@@ -178,7 +186,7 @@ __device__ __forceinline__ int packed_page(const PackedArgs& a, int b, int j) {
 // halves up (for odd den there are none). In double, r = fl(2^14 / den) (1 + 2^-50)
 // and fma(e, r, 2^52 + 128) rounds e r once, to an integer: a half goes up, since
 // r exceeds 2^14 / den by 2^-51 of it at least, and another value is 1 / (2 den) from the
-// next half, more than the 2^14 2^-49 that r adds, for den < 2^34. The low word
+// next half, more than the 2^14 2^-49 that r adds, as den <= S t < 2^34. The low word
 // is p + 128: its second byte H and its first L give p = 256 H + (L - 128), and
 // L - 128 as a byte is L ^ 0x80, so the bytes are two int8 operands.
 struct RowExp {
@@ -187,7 +195,6 @@ struct RowExp {
   int32_t c0;  // the accumulators' start
 };
 constexpr i64 FAST_T = (i64)1 << 17;
-constexpr i64 FAST_DEN = (i64)1 << 34;
 
 __device__ __forceinline__ RowExp make_rowexp(i64 t, int32_t mx) {
   RowExp E;
@@ -272,12 +279,18 @@ __device__ __forceinline__ void pack4(const uint32_t (&w)[4], int& hi, int& lo) 
   hi = (int)__builtin_amdgcn_perm(b, a, 0x07060302u);
 }
 
-// The integer forms
-__device__ __forceinline__ i64 slow_exp(int32_t st, int32_t mx, const ExpR& E) {
-  return di_exp_neg((u64)(uint32_t)(mx - st), E);
+// Any tpos (from 2^17 on, a few instructions a value do not matter): q as in
+// dexp_est, whose bound holds for every t >= 1 with n <= 2^22 (from t = 2^23 on n / t
+// is at most a half), the rest in 64 bits. The sums that wrap wrap as the
+// reference's do.
+__device__ __forceinline__ i64 slow_exp(int32_t st, int32_t mx, i64 t) {
+  const uint32_t n = (uint32_t)(mx - st);
+  const uint32_t q1 = (uint32_t)fma((double)n, 1.0 / (double)t, 1.0 + 0x1p-26);
+  const u64 m = (u64)q1 * (u64)t + (u64)t - n;
+  return q1 < 64u ? (i64)(m >> q1) : 0;
 }
-__device__ __forceinline__ uint32_t slow_p128(i64 e, const Recip& R) {
-  return (uint32_t)to_i32(rhad_r(shl(e, 14), R)) + 128u;
+__device__ __forceinline__ uint32_t slow_p128(i64 e, i64 den) {
+  return (uint32_t)to_i32(rhad(shl(e, 14), den)) + 128u;
 }
 
 // 16 values of a lane that a loop reads and writes at a number of its own: a
@@ -298,13 +311,12 @@ struct InLds {
 template <class Mem>
 __device__ __forceinline__ i64 slow_den(const v4i (&st)[4], int32_t off, uint32_t bits, int32_t mx,
                                         i64 tpos, Mem m) {
-  const ExpR E = make_exp(tpos);
 #pragma unroll
   for (int i = 0; i < 16; ++i) m.put(i, st[i >> 2][i & 3] - off);
   i64 den = 0;
 #pragma unroll 1
   for (int i = 0; i < 16; ++i)
-    if ((bits >> i) & 1u) den = wadd(den, slow_exp(m.get(i), mx, E));
+    if ((bits >> i) & 1u) den = wadd(den, slow_exp(m.get(i), mx, tpos));
   return den;
 }
 template <class Mem>
@@ -313,11 +325,9 @@ __device__ __forceinline__ void slow_probs(const v4i (&st)[4], int32_t off, uint
                                            Mem m) {
 #pragma unroll
   for (int i = 0; i < 16; ++i) m.put(i, st[i >> 2][i & 3] - off);
-  const ExpR E = make_exp(tpos);
-  const Recip R = make_recip(den);
 #pragma unroll 1
   for (int i = 0; i < 16; ++i)
-    m.put(i, (bits >> i) & 1u ? (int)slow_p128(slow_exp(m.get(i), mx, E), R) : 128);
+    m.put(i, (bits >> i) & 1u ? (int)slow_p128(slow_exp(m.get(i), mx, tpos), den) : 128);
 #pragma unroll
   for (int b = 0; b < 4; ++b) {
     const uint32_t w4[4] = {(uint32_t)m.get(4 * b), (uint32_t)m.get(4 * b + 1),
@@ -364,7 +374,7 @@ struct FewRow {
 
 template <bool R8>
 __device__ __forceinline__ FewRow few_row(const PackedArgs& a, const Work& w) {
-  const int lane = threadIdx.x & 63, qi = R8 ? lane & 7 : lane & 15, g4 = lane >> 4;
+  const int lane = thread_now() & 63, qi = R8 ? lane & 7 : lane & 15, g4 = lane >> 4;
   FewRow r;
   const int t = qi >> a.lg, g = qi & ((1 << a.lg) - 1);
   r.on = qi < (w.T << a.lg);
@@ -382,7 +392,7 @@ __device__ __forceinline__ FewRow few_row(const PackedArgs& a, const Work& w) {
 
 // K operands of the 64-slot half hf of a page (a page that is not there reads page 0)
 __device__ __forceinline__ void few_k(const PackedArgs& a, int pg, int kvh, int hf, v4i (&k)[8]) {
-  const int lane = threadIdx.x & 63, qi = lane & 15, g4 = lane >> 4;
+  const int lane = thread_now() & 63, qi = lane & 15, g4 = lane >> 4;
   const int8_t* p = a.kv.krow(::max(pg, 0), kvh, hf * 64 + 16 * (qi >> 2) + (qi & 3)) + g4 * 16;
 #pragma unroll
   for (int blk = 0; blk < 4; ++blk) {
@@ -393,7 +403,7 @@ __device__ __forceinline__ void few_k(const PackedArgs& a, int pg, int kvh, int 
 // V operands: channel 16 j + qi, slots 16 g4 .. + 15 of the half
 template <int J0 = 0, int J1 = 8>
 __device__ __forceinline__ void few_v(const PackedArgs& a, int pg, int kvh, int hf, v4i (&v)[8]) {
-  const int lane = threadIdx.x & 63, qi = lane & 15, g4 = lane >> 4;
+  const int lane = thread_now() & 63, qi = lane & 15, g4 = lane >> 4;
   const int8_t* p = a.kv.vchan(::max(pg, 0), kvh, qi) + hf * 64 + g4 * 16;
 #pragma unroll
   for (int j = J0; j < J1; ++j) v[j] = *(const v4i*)(p + j * 16 * DI_PAGE);
@@ -429,13 +439,19 @@ struct FewAcc {
 #pragma unroll
     for (int j = 0; j < (R8 ? 1 : 8); ++j) lo[j] = v4i{0, 0, 0, 0};
   }
+  // channel blocks [J0, J1)
+  template <int J0 = 0, int J1 = 8>
   __device__ __forceinline__ void add(const v4i& phi, const v4i& plo, const v4i (&v)[8]) {
     if constexpr (R8) {
       const v4i p = (threadIdx.x & 8) ? plo : phi;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) hi[j] = mfma16(p, v[j], hi[j]);
+      for (int j = J0; j < J1; ++j) hi[j] = mfma16(p, v[j], hi[j]);
     } else {
-      pv16(phi, plo, v, hi, lo);
+#pragma unroll
+      for (int j = J0; j < J1; ++j) {
+        hi[j] = mfma16(phi, v[j], hi[j]);
+        lo[j] = mfma16(plo, v[j], lo[j]);
+      }
     }
   }
 };
@@ -471,11 +487,13 @@ __device__ __forceinline__ i64 few_den(const v4i (&st)[4], uint32_t bits, bool f
 }
 
 // The waves' contexts (accumulators of operand row 4 g4 + r, channel 16 j + qi)
-// added up in LDS, then written: to out, or to a chunk's part
+// added up in LDS, then written: to out, to a chunk's part, or (where the launch has
+// only few-row units) added to out, which the first pass cleared: integers, so in
+// any order
 template <int NW, bool R8>
 __device__ __forceinline__ void few_store(const PackedArgs& a, const Work& w, FewLds<NW>& lds,
                                           const FewAcc<R8>& c, bool any) {
-  const int lane = threadIdx.x & 63, qi = lane & 15, g4 = lane >> 4;
+  const int lane = thread_now() & 63, qi = lane & 15, g4 = lane >> 4;
   const int R = w.T << a.lg;
   if (any) {
 #pragma unroll
@@ -495,6 +513,7 @@ __device__ __forceinline__ void few_store(const PackedArgs& a, const Work& w, Fe
     const i64 at = ((i64)(w.tok0 + t) * a.n_q + (w.kvh << a.lg) + g) * 128 + (i & 127);
     const int x = lds.ctx[row][i & 127];
     if (a.part) a.part[(i64)w.c * a.N * a.n_q * 128 + at] = x;
+    else if (a.nch > 1) atomicAdd((unsigned long long*)&a.out[at], (unsigned long long)(i64)x);
     else a.out[at] = x;
   }
 }
@@ -547,12 +566,12 @@ __device__ __forceinline__ void few_one(const PackedArgs& a, const Work& w, FewL
 #pragma unroll
   for (int v = 0; v < NW; ++v) mx = ::max(mx, lds.mx[v][qi]);
   if (mx == NO_SCORE) mx = 0;  // nothing seen: max := 0, every p = 0
-  const bool fast_e = __ballot(row.tpos >= FAST_T) == 0;
+  const bool fast = __ballot(row.tpos >= FAST_T) == 0;
   const RowExp E = make_rowexp(row.tpos, mx);
   i64 den = 0;
 #pragma unroll
   for (int i = 0; i < NT; ++i)
-    if (i * NW + wave < ntiles) den = wadd(den, few_den(st[i], bits(i), fast_e, E, mx, row.tpos, {lds.slow[wave]}));
+    if (i * NW + wave < ntiles) den = wadd(den, few_den(st[i], bits(i), fast, E, mx, row.tpos, {lds.slow[wave]}));
   den = group4_sum(den);
   if (g4 == 0) lds.den[wave][qi] = den;
   __syncthreads();
@@ -560,7 +579,6 @@ __device__ __forceinline__ void few_one(const PackedArgs& a, const Work& w, FewL
 #pragma unroll
   for (int v = 0; v < NW; ++v) den = wadd(den, lds.den[v][qi]);
   den = imax(den, 1);
-  const bool fast = fast_e && __ballot(den >= FAST_DEN) == 0;
   const double rp = make_rowp(den);
   FewAcc<R8> acc;
   acc.clear();
@@ -613,8 +631,8 @@ __device__ __forceinline__ void over_chunks(const PackedArgs& a, const Work& w, 
 // One pass over chunk w.c of a few-row unit, NW waves
 template <int PH, int NW, bool R8>
 __device__ __forceinline__ void few_phase(const PackedArgs& a, const Work& w, FewLds<NW>& lds) {
-  const int lane = threadIdx.x & 63, qi = lane & 15, g4 = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const int tid = thread_now(), lane = tid & 63, qi = lane & 15, g4 = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lo_s = w.c * a.chunk, hi_s = ::min(w.len, lo_s + a.chunk);
   if (lo_s >= hi_s) return;
   const int R = w.T << a.lg, nc = (w.len + a.chunk - 1) / a.chunk;
@@ -622,6 +640,10 @@ __device__ __forceinline__ void few_phase(const PackedArgs& a, const Work& w, Fe
   int32_t* const sc = a.scores + (((i64)w.b * a.n_kv + w.kvh) * a.few_rows) * pitch;
   const int t0 = lo_s / 64, t1 = (hi_s + 63) / 64;
   if constexpr (PH == PH_MAX) {
+    if (w.c == 0 && !a.part && a.nch > 1)
+      for (int i = threadIdx.x; i < R * 128; i += NW * 64)
+        a.out[((i64)(w.tok0 + (i >> 7 >> a.lg)) * a.n_q + (w.kvh << a.lg) +
+               ((i >> 7) & ((1 << a.lg) - 1))) * 128 + (i & 127)] = 0;
     const FewRow row = few_row<false>(a, w);
     int mx = NO_SCORE;
     // two tiles of K in flight a wave
@@ -674,8 +696,6 @@ __device__ __forceinline__ void few_phase(const PackedArgs& a, const Work& w, Fe
       const i64 tpos = a.tpos[(i64)(w.tok0 + t) * a.n_q + (w.kvh << a.lg) + g];
       const bool fast = tpos < FAST_T;  // (one row: uniform)
       const RowExp E = make_rowexp(fast ? tpos : 1, mx);
-      ExpR Es{};
-      if (!fast) Es = make_exp(tpos);
       const int32_t* src = sc + r * pitch;
       i64 den = 0;
       for (int s0 = lo_s + 4 * lane; s0 < t1 * 64; s0 += 1024) {
@@ -692,7 +712,7 @@ __device__ __forceinline__ void few_phase(const PackedArgs& a, const Work& w, Fe
                 const uint32_t e = row_exp(v + E.c0, E);
                 den += v == NO_SCORE ? 0u : e;
               } else if (v != NO_SCORE) {
-                den = wadd(den, slow_exp(v, mx, Es));
+                den = wadd(den, slow_exp(v, mx, tpos));
               }
             }
           }
@@ -712,7 +732,7 @@ __device__ __forceinline__ void few_phase(const PackedArgs& a, const Work& w, Fe
       mx = 0;
       den = 1;
     }
-    const bool fast = __ballot(row.tpos >= FAST_T || den >= FAST_DEN) == 0;
+    const bool fast = __ballot(row.tpos >= FAST_T) == 0;
     const RowExp E = make_rowexp(row.tpos, mx);
     const double rp = make_rowp(den);
     FewAcc<R8> acc;
@@ -723,18 +743,22 @@ __device__ __forceinline__ void few_phase(const PackedArgs& a, const Work& w, Fe
       const int pg = __builtin_amdgcn_readfirstlane(packed_page(a, w.b, it >> 1));
 #pragma unroll
       for (int blk = 0; blk < 4; ++blk) st[blk] = *(const v4i*)(src + it * 64 + 4 * blk);
-      // (with twice the accumulators, half of V waits until the scores' registers are free)
-      few_v<0, R8 ? 8 : 4>(a, pg, w.kvh, it & 1, v);
+      // (half of V waits until the scores' registers are free)
+      few_v<0, 4>(a, pg, w.kvh, it & 1, v);
       uint32_t bb = 0;
 #pragma unroll
       for (int e = 0; e < 16; ++e) bb |= (st[e >> 2][e & 3] != NO_SCORE ? 1u : 0u) << e;
       v4i phi, plo;
       few_probs(st, row.on ? bb : 0u, fast, E, rp, mx, row.tpos, den, phi, plo, {lds.slow[wave]});
-      if constexpr (!R8) {
-        __builtin_amdgcn_sched_barrier(0);
+      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (R8) {
         few_v<4, 8>(a, pg, w.kvh, it & 1, v);
+        acc.add(phi, plo, v);
+      } else {
+        acc.template add<0, 4>(phi, plo, v);
+        few_v<4, 8>(a, pg, w.kvh, it & 1, v);
+        acc.template add<4, 8>(phi, plo, v);
       }
-      acc.add(phi, plo, v);
     }
     few_store<NW, R8>(a, w, lds, acc, true);
   }
@@ -744,41 +768,52 @@ __device__ __forceinline__ void few_phase(const PackedArgs& a, const Work& w, Fe
 //
 // Four waves of 16 query rows (row i: token i / G, head i % G of the kv head, so K
 // and V are read once for the kv head's query heads). Keys reach LDS by
-// direct-to-LDS loads, 16 KB a stage: a page of K in the first two passes, half a
-// page of K and V in the third; one barrier a stage, 16-byte chunks swizzled
-// against bank conflicts.
+// direct-to-LDS loads into a ring of three 16 KB steps: a page of K in the first two
+// passes, half a page of K and V in the third; one barrier a step, 16-byte chunks
+// swizzled against bank conflicts.
 //
-// What bounds it: a stage arrives about a microsecond after it is asked for, so a
-// CU needs some 100 KB on their way (three blocks, two of three stages each: with
-// one of two 32 KB stages ahead, the loads alone of the third pass over 2500 slots
-// took 26 of its 39 us); and a SIMD takes an instruction of one wave every five
-// cycles, while most operations of an exponential last two, so it wants three
-// waves (168 registers a lane; scratch memory for spills would cost a launch
-// 8 us by itself).
+// What bounds it is issue. Alone on a SIMD a wave takes some 240, 670 and 1520
+// cycles for a half page's three passes, two side by side 170, 460 and 1050, so a
+// prompt of 2500 tokens (632 tiles of up to 40 half pages, 75 us) is bound by its last
+// tiles' own chains; its loads alone take 30 us. Three blocks a CU (168 registers a lane,
+// none spilled: scratch memory cost a launch 8 us by itself, and two waves more a
+// SIMD at 128 registers did not make up for it).
 
-constexpr int TL_NT = 256;
-constexpr int TL_STAGE = 16 * 1024;
-constexpr int TL_STAGES = 3;
-constexpr int TL_HALF = 8 * 1024;  // K's part of a half-page stage: 64 slot rows of 128 B
-constexpr int TL_PAGES = 1024;     // pages of the longest row
+constexpr int TL_HALF = 8 * 1024;   // 64 slot rows of K, or 64 slots of V's 128 channels
+constexpr int TL_PAGE = 16 * 1024;  // a page of K, or of V
 
-struct TileLds {
-  union {
-    __attribute__((aligned(1024))) int8_t ring[TL_STAGES * TL_STAGE];
-    FewLds<4> few;
-  };
-  int32_t pages[TL_PAGES];
+constexpr int TL_STEPS = 3;
+
+union TileLds {
+  __attribute__((aligned(1024))) int8_t ring[TL_STEPS * TL_PAGE];
+  FewLds<4> few;
 };
 
 // Physical chunk = logical ^ swizzle, so that the operand reads below take LDS's
-// full rate. K (rows of 8 chunks): bits 0, 1 and 4 of the row. V half pages (channel
-// rows of 4 chunks, two to 128 bytes): bits 1 and 2 of the channel.
+// full rate (eight lanes at a time over 128 bytes). K (rows of 8 chunks): bits 0, 1
+// and 4 of the row. Half pages of V (channel rows of 4 chunks): bits 1 and 2 of the
+// channel.
 __device__ __forceinline__ int tl_kswz(int row) { return (row & 3) | ((row >> 2) & 4); }
 __device__ __forceinline__ int tl_vswz(int d) { return (d >> 1) & 3; }
 
+// The page ids of a row's pages from p on, 64 of them in the lanes of a register,
+// the next 64 when they come up
+struct PageIds {
+  int v, base;
+  __device__ __forceinline__ void load(const PackedArgs& a, int b, int p) {
+    base = p;
+    v = packed_page(a, b, p + (int)(threadIdx.x & 63));
+    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt 0: here, not at every use
+  }
+  __device__ __forceinline__ int get(const PackedArgs& a, int b, int p) {
+    if (DI_UNLIKELY(p - base >= 64 || p < base)) load(a, b, p);
+    return __builtin_amdgcn_readlane(v, p - base);
+  }
+};
+
 template <int PH>
 __device__ __forceinline__ void tile_body(const PackedArgs& a, const Work& w, TileLds& lds) {
-  const int tid = threadIdx.x, lane = tid & 63, qi = lane & 15, g = lane >> 4;
+  const int tid = thread_now(), lane = tid & 63, qi = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int R = w.T << a.lg;             // the row's query rows
   const int r0 = w.tile * 64;            // the tile's first
@@ -789,103 +824,123 @@ __device__ __forceinline__ void tile_body(const PackedArgs& a, const Work& w, Ti
   const int hi_s = PH == PH_ALL ? end : ::min(end, lo_s + a.chunk);
   if (lo_s >= hi_s) return;
   const int p0 = lo_s / DI_PAGE, np = (hi_s + DI_PAGE - 1) / DI_PAGE - p0;
-  const int nh = (hi_s + 63) / 64 - 2 * p0;  // half pages
-  const int wr0 = r0 + wave * 16;          // the wave's first query row
+  PageIds ids;
+  ids.load(a, w.b, p0);
+  const int wr0 = r0 + wave * 16;            // the wave's first query row
   const bool work = wr0 < R;               // (waves without one only load)
   const int qr = ::min(wr0 + qi, R - 1);   // the lane's (rows past the last: the last, not stored)
-  const int t = qr >> a.lg;
-  const int limit = row_limit(a, w.past, t);
+  const int limit = row_limit(a, w.past, qr >> a.lg);
   const int wlim = row_limit(a, w.past, ::min(wr0, R - 1) >> a.lg);        // the wave's smallest
   const int wmax = row_limit(a, w.past, ::min(wr0 + 15, R - 1) >> a.lg);   // and largest limit
-  const i64 qrow = (i64)(w.tok0 + t) * a.n_q + (w.kvh << a.lg) + (qr & ((1 << a.lg) - 1));
+  // the half pages that the wave sees: [0, nsee)
+  const int nsee = work && wmax >= lo_s ? (wmax - p0 * DI_PAGE) / 64 + 1 : 0;
+
+  u64 there = 0;  // of the last 64 pages asked for, those that are mapped
+  auto page_of = [&](int i) {
+    const int pg = ids.get(a, w.b, p0 + i);
+    const u64 bit = 1ull << (i & 63);
+    there = pg < 0 ? there & ~bit : there | bit;
+    return pg;
+  };
+  // (a page that is not there: a view of no bytes, whose loads read 0)
+  auto view = [&](const int8_t* pool, int pg) {
+    return __builtin_amdgcn_make_buffer_rsrc(
+        (void*)(pool + ((i64)::max(pg, 0) * a.n_kv + w.kvh) * TL_PAGE), (short)0,
+        pg < 0 ? 0 : TL_PAGE, 0x00020000);
+  };
+  auto k_off = [&](int row) { return row * 128 + ((lane & 7) ^ tl_kswz(row)) * 16; };
+  // a page of K to `to`: each load of a wave brings 8 rows, 1 KB
+  auto issue_k = [&](int i, int8_t* to) {
+    const auto rs = view(a.kv.k, page_of(i));
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int at = wave * 4 + j;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr_t)(to + at * 1024), 16,
+                                               k_off(at * 8 + (lane >> 3)), 0, 0, 0);
+    }
+  };
+  // half hf of page i, K then V, to `to`: of each, a wave's two loads bring 1 KB, 8
+  // rows of K or 16 channels of V
+  auto issue_kv = [&](int i, int hf, int8_t* to) {
+    const int pg = page_of(i);
+    const auto ks = view(a.kv.k, pg), vs = view(a.kv.v, pg);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int at = wave * 2 + j, d = at * 16 + (lane >> 2);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(ks, (lds_ptr_t)(to + at * 1024), 16,
+                                               k_off(at * 8 + (lane >> 3)), hf * TL_HALF, 0, 0);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(vs, (lds_ptr_t)(to + TL_HALF + at * 1024), 16,
+                                               d * DI_PAGE + ((lane & 3) ^ tl_vswz(d)) * 16,
+                                               hf * 64, 0, 0);
+    }
+  };
+  const i64 qrow = (i64)(w.tok0 + (qr >> a.lg)) * a.n_q + (w.kvh << a.lg) + (qr & ((1 << a.lg) - 1));
   const v4i qf0 = *(const v4i*)(a.q8 + qrow * 128 + g * 16);
   const v4i qf1 = *(const v4i*)(a.q8 + qrow * 128 + 64 + g * 16);
   const i64 tpos = a.tpos[qrow];
-
-  // Load j of a wave brings 1 KB: K rows 8 (4 wave + j) .. + 7 of a page, or 8 (2
-  // wave + j) .. of a half; V: channels 16 (2 wave + j) .. + 15, 64 bytes each
-  auto rsrc = [&](const int8_t* p, int page) {
-    // (a page that is not there: a view of no bytes, whose loads read 0)
-    return __builtin_amdgcn_make_buffer_rsrc((void*)p, (short)0, page < 0 ? 0 : DI_PAGE * 128,
-                                             0x00020000);
-  };
-  auto k_off = [&](int row) { return row * 128 + ((lane & 7) ^ tl_kswz(row)) * 16; };
-  auto issue_page = [&](int page, int8_t* st) {
-    const int pg = __builtin_amdgcn_readfirstlane(page);
-    const auto krs = rsrc(a.kv.krow(::max(pg, 0), w.kvh, 0), pg);
+  // one page stays for all three passes
+  const bool resident = PH == PH_ALL && np == 1;
+  if (resident)
+    for (int h = 0; h < 2; ++h) issue_kv(0, h, lds.ring + h * TL_PAGE);
+  wait_vmcnt<0>();  // (queries, before the ring's loads count)
+  if (resident) __syncthreads();
+  const int kr = 16 * (qi >> 2) + (qi & 3);
+  const int k0 = kr * 128 + ((g ^ tl_kswz(kr)) << 4);
+  const int k1 = kr * 128 + (((g + 4) ^ tl_kswz(kr)) << 4);
+  // half page i is there, and some query row of the wave sees it
+  auto seen = [&](int i) { return i < nsee && ((there >> ((i >> 1) & 63)) & 1) != 0; };
+  // its K operands (its K rows at p), and the wave's scores from accumulators z
+  auto load_k = [&](const int8_t* p, v4i (&kf)[8]) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(krs, (lds_ptr_t)(st + (wave * 4 + j) * 1024), 16,
-                                               k_off((wave * 4 + j) * 8 + (lane >> 3)), 0, 0, 0);
-  };
-  auto issue_half = [&](int page, int hf, int8_t* st) {
-    const int pg = __builtin_amdgcn_readfirstlane(page);
-    const auto krs = rsrc(a.kv.krow(::max(pg, 0), w.kvh, 0), pg);
-    const auto vrs = rsrc(a.kv.vchan(::max(pg, 0), w.kvh, 0), pg);
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int at = wave * 2 + j;
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(krs, (lds_ptr_t)(st + at * 1024), 16,
-                                               k_off(at * 8 + (lane >> 3)), hf * TL_HALF, 0, 0);
-      const int d = at * 16 + (lane >> 2);
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(
-          vrs, (lds_ptr_t)(st + TL_HALF + at * 1024), 16,
-          d * DI_PAGE + ((lane & 3) ^ tl_vswz(d)) * 16, hf * 64, 0, 0);
+    for (int b = 0; b < 4; ++b) {
+      kf[2 * b] = *(const v4i*)(p + k0 + b * 512);
+      kf[2 * b + 1] = *(const v4i*)(p + k1 + b * 512);
     }
   };
-  for (int i = tid; i < np; i += TL_NT) lds.pages[i] = packed_page(a, w.b, p0 + i);
-  wait_vmcnt<0>();  // queries, page ids
-  __syncthreads();
-
-  // One pass over n stages; issue(i, stage), body(i, stage). Each wave waits for
-  // its own loads of a stage (four, and they complete in order), then one barrier
-  // publishes every wave's part and frees the stage that the next issue overwrites.
+  auto scores = [&](const v4i (&kf)[8], const v4i z, v4i (&st)[4]) {
+#pragma unroll
+    for (int b = 0; b < 4; ++b) st[b] = mfma16(kf[2 * b], qf0, z);
+#pragma unroll
+    for (int b = 0; b < 4; ++b) st[b] = mfma16(kf[2 * b + 1], qf1, st[b]);
+  };
+  // n steps of four loads a wave: issue(i, where). A wave waits for its own loads of
+  // a step (they complete in order), then a barrier publishes every wave's
+  // part and frees what the next issue overwrites; body(i, where) with it in LDS.
   auto pass = [&](int n, auto&& issue, auto&& body) {
     wait_lds();
     __builtin_amdgcn_s_barrier();  // the pass before is done with the ring
 #pragma unroll
-    for (int s = 0; s < TL_STAGES - 1; ++s)
-      if (s < n) issue(s, lds.ring + s * TL_STAGE);
-    int at = 0;  // the stage of i
+    for (int i = 0; i < TL_STEPS - 1; ++i)
+      if (i < n) issue(i, lds.ring + i * TL_PAGE);
+    int at = 0;  // the place of step i
     for (int i = 0; i < n; ++i) {
       if (i + 1 < n) wait_vmcnt<4>();
       else wait_vmcnt<0>();
       wait_lds();
       __builtin_amdgcn_s_barrier();
-      const int next = at == 0 ? TL_STAGES - 1 : at - 1;
-      if (i + TL_STAGES - 1 < n) issue(i + TL_STAGES - 1, lds.ring + next * TL_STAGE);
-      body(i, lds.ring + at * TL_STAGE);
-      at = at + 1 == TL_STAGES ? 0 : at + 1;
+      if (i + TL_STEPS - 1 < n)
+        issue(i + TL_STEPS - 1, lds.ring + (at == 0 ? TL_STEPS - 1 : at - 1) * TL_PAGE);
+      body(i, lds.ring + at * TL_PAGE);
+      at = at + 1 == TL_STEPS ? 0 : at + 1;
     }
   };
-  auto k_pages = [&](int i, int8_t* st) { issue_page(lds.pages[i], st); };
-  auto kv_halves = [&](int i, int8_t* st) { issue_half(lds.pages[i >> 1], i & 1, st); };
-  const int kr = 16 * (qi >> 2) + (qi & 3);
-  const int koff0 = kr * 128 + ((g ^ tl_kswz(kr)) << 4);
-  const int koff1 = kr * 128 + (((g + 4) ^ tl_kswz(kr)) << 4);
-  // half page i (its K rows at `keys`): its scores from accumulators z, then fn(st,
-  // s0) (its first slot s0); one that is not there, or that no query row of the
-  // wave sees, is passed over
-  auto half = [&](const int8_t* keys, int i, const v4i z, auto&& fn) {
-    const int s0 = p0 * DI_PAGE + i * 64;
-    if (!work || s0 > wmax || __builtin_amdgcn_readfirstlane(lds.pages[i >> 1]) < 0) return;
-    v4i kf[8], st[4];
-#pragma unroll
-    for (int blk = 0; blk < 4; ++blk) {
-      kf[2 * blk] = *(const v4i*)(keys + koff0 + blk * 512);
-      kf[2 * blk + 1] = *(const v4i*)(keys + koff1 + blk * 512);
-    }
-#pragma unroll
-    for (int blk = 0; blk < 4; ++blk) st[blk] = mfma16(kf[2 * blk], qf0, z);
-#pragma unroll
-    for (int blk = 0; blk < 4; ++blk) st[blk] = mfma16(kf[2 * blk + 1], qf1, st[blk]);
-    fn(st, s0);
-  };
+  auto first_slot = [&](int i) { return p0 * DI_PAGE + i * 64; };
   auto k_pass = [&](const v4i z, auto&& fn) {
-    pass(np, k_pages, [&](int i, const int8_t* st) {
+    auto one = [&](int i, const int8_t* p) {
+      if (!seen(i)) return;
+      v4i kf[8], st[4];
+      load_k(p, kf);
+      scores(kf, z, st);
+      fn(st, first_slot(i));
+    };
+    if (resident) {
+      for (int i = 0; i < 2; ++i) one(i, lds.ring + i * TL_PAGE);
+    } else {
+      pass(np, issue_k, [&](int i, const int8_t* p) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h) half(st + h * TL_HALF, 2 * i + h, z, fn);
-    });
+        for (int h = 0; h < 2; ++h) one(2 * i + h, p + h * TL_HALF);
+      });
+    }
   };
 
   int32_t mx = NO_SCORE;
@@ -913,15 +968,15 @@ __device__ __forceinline__ void tile_body(const PackedArgs& a, const Work& w, Ti
   if constexpr (PH == PH_DEN) over_chunks<false>(a, w, nc, qr - r0, &mx, &den);
   if constexpr (PH == PH_PV) over_chunks<true>(a, w, nc, qr - r0, &mx, &den);
 
-  const bool fast_e = __ballot(tpos >= FAST_T) == 0;
-  const RowExp E = make_rowexp(fast_e ? tpos : 1, mx);
+  const bool fast = __ballot(tpos >= FAST_T) == 0;
+  const RowExp E = make_rowexp(fast ? tpos : 1, mx);
   // the accumulators of the slow forms start from 0
-  const int32_t c0 = fast_e ? E.c0 : 0;
+  const int32_t c0 = fast ? E.c0 : 0;
   const v4i cinit = v4i{c0, c0, c0, c0};
   if constexpr ((PH & PH_DEN) != 0) {
     den = 0;
     // (the slow forms in a loop of their own: what they hold does not weigh on the other)
-    if (DI_LIKELY(fast_e)) {
+    if (DI_LIKELY(fast)) {
       k_pass(cinit, [&](const v4i (&st)[4], int s0) {
         uint32_t e[16], sum = 0;
         row_exps(st, E, e);
@@ -947,45 +1002,52 @@ __device__ __forceinline__ void tile_body(const PackedArgs& a, const Work& w, Ti
     }
     den = imax(den, 1);
   }
-  const bool fast = fast_e && __ballot(den >= FAST_DEN) == 0;
   const double rp = make_rowp(den);
   v4i ohi[8], olo[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) ohi[j] = olo[j] = v4i{0, 0, 0, 0};
   // V operand of a half page: channel 16 j + qi, slots 16 g .. + 15 (the swizzle of
   // channel 16 j + qi does not depend on j)
-  const int voff = TL_HALF + qi * 64 + ((g ^ tl_vswz(qi)) << 4);
-  auto pv = [&](const int8_t* stg, const v4i& phi, const v4i& plo) {
-    v4i vf[8];
+  const int v0 = TL_HALF + qi * 64 + ((g ^ tl_vswz(qi)) << 4);
+  auto kv_pass = [&](auto&& probs) {
+    auto add = [&](int i, const int8_t* p, const v4i (&st)[4]) {
+      v4i phi, plo, vf[8];
+      probs(st, first_slot(i), phi, plo);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) vf[j] = *(const v4i*)(stg + voff + j * 1024);
-    pv16(phi, plo, vf, ohi, olo);
+      for (int j = 0; j < 8; ++j) vf[j] = *(const v4i*)(p + v0 + j * 1024);
+      pv16(phi, plo, vf, ohi, olo);
+    };
+    auto one = [&](int i, const int8_t* p) {
+      if (!seen(i)) return;
+      v4i kf[8], st[4];
+      load_k(p, kf);
+      scores(kf, cinit, st);
+      add(i, p, st);
+    };
+    if (resident) {
+      for (int i = 0; i < 2; ++i) one(i, lds.ring + i * TL_PAGE);
+    } else {
+      pass(2 * np, [&](int i, int8_t* to) { issue_kv(i >> 1, i & 1, to); }, one);
+    }
   };
   if (DI_LIKELY(fast)) {
-    pass(nh, kv_halves, [&](int i, const int8_t* stg) {
-      half(stg, i, cinit, [&](const v4i (&st)[4], int s0) {
-        v4i phi, plo;
-        uint32_t e[16];
-        row_exps(st, E, e);
-        if (s0 + 63 > wlim) {
-          const uint32_t bits = seen16(limit, s0 + 16 * g);
+    kv_pass([&](const v4i (&st)[4], int s0, v4i& phi, v4i& plo) {
+      uint32_t e[16];
+      row_exps(st, E, e);
+      if (s0 + 63 > wlim) {
+        const uint32_t bits = seen16(limit, s0 + 16 * g);
 #pragma unroll
-          for (int i = 0; i < 16; ++i) e[i] = (bits >> i) & 1u ? e[i] : 0u;
-        }
-        row_probs(e, rp, phi, plo);
-        pv(stg, phi, plo);
-      });
+        for (int i = 0; i < 16; ++i) e[i] = (bits >> i) & 1u ? e[i] : 0u;
+      }
+      row_probs(e, rp, phi, plo);
     });
   } else {
-    pass(nh, kv_halves, [&](int i, const int8_t* stg) {
-      half(stg, i, cinit, [&](const v4i (&st)[4], int s0) {
-        v4i phi, plo;
-        // (c0: scores that came with an offset are taken back)
-        slow_probs(st, c0, seen16(limit, s0 + 16 * g), mx, tpos, den, phi, plo, InRegs{});
-        pv(stg, phi, plo);
-      });
+    kv_pass([&](const v4i (&st)[4], int s0, v4i& phi, v4i& plo) {
+      slow_probs(st, 0, seen16(limit, s0 + 16 * g), mx, tpos, den, phi, plo, InRegs{});
     });
   }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) ohi[j] = ohi[j] * 256 + olo[j];
   if (!work) return;
   // lane (qi, g): query rows 4 g + r of the wave, channel 16 j + qi
 #pragma unroll
@@ -996,9 +1058,8 @@ __device__ __forceinline__ void tile_body(const PackedArgs& a, const Work& w, Ti
                       (row & ((1 << a.lg) - 1))) * 128 + qi;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const int x = ohi[j][r] * 256 + olo[j][r];
-        if (a.part) a.part[(i64)w.c * a.N * a.n_q * 128 + at + 16 * j] = x;
-        else a.out[at + 16 * j] = x;
+        if (a.part) a.part[(i64)w.c * a.N * a.n_q * 128 + at + 16 * j] = ohi[j][r];
+        else a.out[at + 16 * j] = ohi[j][r];
       }
     }
   }

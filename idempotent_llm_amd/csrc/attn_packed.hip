@@ -38,7 +38,7 @@ __global__ __launch_bounds__(512, 2) void k_packed_few(PackedArgs a) {
 }
 
 // All three passes of any rows
-__global__ __launch_bounds__(TL_NT, 3) void k_packed_one(PackedArgs a) {
+__global__ __launch_bounds__(256, 3) void k_packed_one(PackedArgs a) {
   keep_hidden_args();
   __shared__ TileLds lds;
   Rows rows;
@@ -50,7 +50,7 @@ __global__ __launch_bounds__(TL_NT, 3) void k_packed_one(PackedArgs a) {
     if (w.few && w.len <= FEW_ONE_SLOTS) few_one<4, FEW_ONE_SLOTS / 256, false>(a, w, lds.few);
     else tile_body<PH_ALL>(a, w, lds);
   }
-  zero_tail(a, f.ntok, kvh, j);
+  if (threadIdx.x < 256) zero_tail(a, f.ntok, kvh, j);
 }
 
 // One pass over chunks. FEW: the launch's rows have at most FEW (8 or 16) query rows
@@ -77,7 +77,7 @@ __global__ __launch_bounds__(256, FEW == 0 || PH == PH_PV ? 3 : 4) void k_packed
       else tile_body<PH>(a, w, lds);
     }
   }
-  if (PH == PH_PV && a.nch == 1) zero_tail(a, f.ntok, kvh, j0);
+  if (PH == PH_PV && !a.part) zero_tail(a, f.ntok, kvh, j0);
 }
 
 // The chunks' contexts of a token added up (one block per token row)
@@ -158,7 +158,7 @@ inline Plan packed_plan(int N, int B, int S, int max_new, int n_q, int n_kv) {
   const i64 cells = (i64)p.units * n_kv * p.nch * 64;
   p.max_at = room(cells * 4);
   p.den_at = room(cells * 8);
-  p.part_at = room(p.nch > 1 ? (i64)p.nch * N * n_q * 128 * 4 : 0);
+  p.part_at = room(p.nch > 1 && !p.few ? (i64)p.nch * N * n_q * 128 * 4 : 0);
   return p;
 }
 
@@ -206,12 +206,12 @@ int detllm_attn_packed(const int8_t* q8, const int64_t* tpos, const int8_t* kpoo
   a.scores = (int32_t*)(w + p.scores_at);
   a.smax = (int32_t*)(w + p.max_at);
   a.sden = (int64_t*)(w + p.den_at);
-  a.part = p.nch > 1 ? (int32_t*)(w + p.part_at) : nullptr;
+  a.part = p.nch > 1 && !p.few ? (int32_t*)(w + p.part_at) : nullptr;
   const i64 blocks = (i64)p.step * n_kv;
   if (blocks > 0x7fffffff) return DI_ERANGE;
   const dim3 grid((unsigned)blocks);
   if (p.one) {
-    if (!p.few) hipLaunchKernelGGL(k_packed_one, grid, dim3(TL_NT), 0, s, a);
+    if (!p.few) hipLaunchKernelGGL(k_packed_one, grid, dim3(256), 0, s, a);
     else if (p.rows <= 8) {
       if (S <= 512) hipLaunchKernelGGL((k_packed_few<1, true>), grid, dim3(512), 0, s, a);
       else if (S <= 1024) hipLaunchKernelGGL((k_packed_few<2, true>), grid, dim3(512), 0, s, a);
@@ -235,7 +235,7 @@ int detllm_attn_packed(const int8_t* q8, const int64_t* tpos, const int8_t* kpoo
   else if (p.few) { DI_PHASES(16); }
   else { DI_PHASES(0); }
 #undef DI_PHASES
-  if (p.nch > 1) {
+  if (a.part) {
     hipLaunchKernelGGL(k_packed_join, dim3(N), dim3(256), 0, s, a);
     DI_LAUNCH_CHECK();
   }
