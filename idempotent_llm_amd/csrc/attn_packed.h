@@ -39,7 +39,7 @@ constexpr int32_t NO_SCORE = INT32_MIN;
 // What a block works on: a chunk of a unit, for a kv head
 struct Work {
   bool few;   // the row has at most 16 query rows
-  bool bad;   // the row's slots or tokens are past the launch's bounds
+  bool bad;   // the row's slots are past the launch's bound
   int b, tile, unit, kvh, c;
   int tok0, T, past;  // the row's first token row, its tokens and filled slots
   int len;            // slots that its tokens see (past + T, bounded)
@@ -83,10 +83,10 @@ struct Rows {
     past = a.past[bc];
     const int c0 = ::min(::max(a.cu[bc], 0), a.N), c1 = ::min(::max(a.cu[bc + 1], c0), a.N);
     tok0 = c0;
-    over = c1 - c0 > a.max_new;
+    over = b < a.B && c1 - c0 > a.max_new;
     T = b < a.B ? ::min(c1 - c0, a.max_new) : 0;
     const i64 R = (i64)T << a.lg;
-    units = R <= 16 ? (T > 0 ? 1 : 0) : (int)((R + 63) >> 6);
+    units = R <= 16 ? (T > 0 ? 1 : 0) : ::min((int)((R + 63) >> 6), a.units);
     nc = (row_limit(a, past, T - 1) + a.chunk) / a.chunk;
     items = units * nc;
     units_to = wave_scan(units);
@@ -97,6 +97,8 @@ struct Rows {
 // Items from the last row's last unit on (the tiles of a prompt that see most go
 // first), kv heads fastest (with 8 of them a head's blocks share an XCD, so its L2
 // holds their K and V). A block takes item j, j + a.step, ...
+// Rows that overlap (a cu that is not ascending) can ask for more than a.units: items
+// past a.units nch are dropped (so no sum passes 2^31), and units past a.units (outside()).
 struct Finder {
   int total;  // items
   int ntok;   // token rows of all rows
@@ -104,12 +106,18 @@ struct Finder {
   __device__ __forceinline__ Finder(const PackedArgs& a, Rows& r) {
     ntok = ::min(::max(a.cu[a.B], 0), a.N);
     r.load(a, 0);
-    total = __builtin_amdgcn_readlane(r.items_to, 63);
+    const int most = a.units * a.nch;  // at most 2^24
+    total = ::min(__builtin_amdgcn_readlane(r.items_to, 63), most);
+    u64 over = __ballot(r.over != 0);
     for (int b0 = 64; b0 < a.B; b0 += 64) {
       Rows x;
       x.load(a, b0);
-      total += __builtin_amdgcn_readlane(x.items_to, 63);
+      total = ::min(total + __builtin_amdgcn_readlane(x.items_to, 63), most);
+      over |= __ballot(x.over != 0);
     }
+    // rows of more tokens than the bound (which may have no item)
+    if (DI_UNLIKELY(over != 0) && blockIdx.x == 0 && threadIdx.x == 0 && a.err)
+      atomicOr(a.err, DI_ERR_SLOTS);
   }
   // item j of kv head kvh; x: the first 64 rows
   __device__ __forceinline__ Work find(const PackedArgs& a, Rows x, int kvh, int j) const {
@@ -135,7 +143,7 @@ struct Finder {
     w.tok0 = of(x.tok0);
     w.T = of(x.T);
     const int past = of(x.past);
-    w.bad = of(x.over) != 0 || past < 0 || (i64)past + w.T > (i64)a.S;
+    w.bad = past < 0 || (i64)past + w.T > (i64)a.S;
     w.past = ::max(past, 0);
     w.len = row_limit(a, w.past, w.T - 1) + 1;
     w.few = (w.T << a.lg) <= 16;
@@ -147,6 +155,13 @@ struct Finder {
 __device__ __forceinline__ void report_row(const PackedArgs& a, const Work& w) {
   if (w.bad && w.tile == 0 && w.kvh == 0 && w.c == 0 && threadIdx.x == 0 && a.err)
     atomicOr(a.err, DI_ERR_SLOTS);
+}
+
+// A unit that the launch has no room for (rows that overlap)
+__device__ __forceinline__ bool outside(const PackedArgs& a, const Work& w) {
+  if (DI_LIKELY(w.unit < a.units)) return false;
+  if (threadIdx.x == 0 && a.err) atomicOr(a.err, DI_ERR_SLOTS);
+  return true;
 }
 
 // Token rows behind the last row's: zeros, shared among the blocks

@@ -66,6 +66,7 @@ __global__ __launch_bounds__(256, FEW == 0 || PH == PH_PV ? 3 : 4) void k_packed
       __syncthreads();  // the item before is done with LDS
     }
     const Work w = f.find(a, rows, kvh, j);
+    if (outside(a, w)) continue;
     if (PH == PH_MAX) report_row(a, w);
     if constexpr (FEW != 0) {
       __shared__ FewLds<4> lds;
@@ -193,6 +194,8 @@ int detllm_attn_packed(const int8_t* q8, const int64_t* tpos, const int8_t* kpoo
   if (!q8 || !tpos || !kv_ok(kpool, vpool, table, width) || n_pages < 1 || !cu || !past || !out ||
       S > (i64)width * DI_PAGE)
     return DI_EINVAL;
+  // (16-byte loads)
+  if ((((uintptr_t)q8 | (uintptr_t)kpool | (uintptr_t)vpool) & 15) != 0) return DI_EINVAL;
   const Plan p = packed_plan(N, B, S, max_new, n_q, n_kv);
   if (p.bytes > 0 && (!work || ((uintptr_t)work & 15))) return DI_EINVAL;
   if (work_bytes < p.bytes) return DI_ERANGE;

@@ -723,12 +723,19 @@ void check_is(const char* op, const char* name, const Tensor& t, at::ScalarType 
            " as contiguous ", dt, " ", sizes, ", got ", t.scalar_type(), " ", t.sizes());
   DI_CHECK(t.device() == like.device(), op, "operands on ", like.device(), " and ", t.device());
 }
+bool on16(const Tensor& t) { return (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0; }
+// (the kernels load 16 bytes at a time)
+Tensor aligned(const Tensor& t) {
+  const Tensor c = t.contiguous();
+  return on16(c) ? c : c.clone();
+}
 void check_pools(const char* op, const Tensor& kpool, const Tensor& vpool, int64_t n_kv,
                  const Tensor& like) {
   rank(kpool, 4, op);
   DI_CHECK(kpool.size(0) > 0 && kpool.size(0) <= INT32_MAX / 128, op, "no pages, or too many");
   check_is(op, "the K pool", kpool, at::kChar, {kpool.size(0), n_kv, 128, 128}, like);
   check_is(op, "the V pool", vpool, at::kChar, {kpool.size(0), n_kv, 128, 128}, like);
+  DI_CHECK(on16(kpool) && on16(vpool), op, "pools that do not start on 16 bytes");
 }
 
 std::tuple<Tensor, Tensor, Tensor, Tensor> op_packed_plan(const Tensor& table, const Tensor& free,
@@ -829,7 +836,7 @@ Tensor op_attn_packed(const Tensor& q8, const Tensor& tpos, const Tensor& kpool,
   DI_CHECK(N * n_q <= (1 << 24) && B >= 1 && B <= 65536, op, N, " token rows of ", B, " rows");
   DI_CHECK(S >= 1 && S <= 131071 && S <= table.size(1) * 128 && max_new >= 0, op, S,
            " slots over a table of ", table.size(1), " pages, ", max_new, " new tokens");
-  const Tensor qc = q8.contiguous(), tc = tpos.contiguous();
+  const Tensor qc = aligned(q8), tc = tpos.contiguous();
   check_is(op, "tpos", tc, at::kLong, {N, n_q}, q8);
   check_pools(op, kpool, vpool, n_kv, q8);
   check_is(op, "the table", table, at::kInt, {B, table.size(1)}, q8);
@@ -863,10 +870,6 @@ Tensor op_lora_gemm(const Tensor& x8, const Tensor& w, const Tensor& a8, const T
            "K of ", K, " (a multiple of 16 up to 65536), rank ", r, " (one up to 128)");
   DI_CHECK(N <= (1 << 20) && C >= 1 && C <= (1 << 24) && n_ad >= 1 && n_ad <= INT32_MAX, op, N,
            " token rows, ", C, " columns, ", n_ad, " adapters");
-  auto aligned = [](const Tensor& t) {   // (the kernels load 16 bytes at a time)
-    const Tensor c = t.contiguous();
-    return (reinterpret_cast<uintptr_t>(c.data_ptr()) & 15) == 0 ? c : c.clone();
-  };
   const Tensor xc = aligned(x8), wc = aligned(w), ac = aligned(a8), bc = aligned(b8);
   check_is(op, "x8", xc, at::kChar, {N, K}, x8);
   check_is(op, "w", wc, at::kChar, {C, K}, x8);
