@@ -7,13 +7,16 @@
 // product's column c gets rshift_round(v[c] bm_a[c], bk_a - h) (a left shift by
 // h - bk_a where that is positive; int64, then added as int32).
 //
-// A block takes up to 16 consecutive token rows and 256 columns. Its adapters are
+// A block takes up to 16 consecutive token rows and up to four times 256 columns. Its
+// adapters are
 // the distinct ones of those rows, one after another: u on i8 MFMA with K split over
 // the four waves, the other adapters' rows dropped as the sums meet in LDS; then w as two
 // int8 operands (w = 256 H + L - 128, bytes H and L ^ 0x80), rows of other adapters
 // zero, so the adapters' products add up in one accumulator. What bounds it: at
 // few rows one chain of loads (adapters, x and A, B, then the product's own
-// columns), at many the product's columns read and written once more.
+// columns; 8 rows of K 1024, 4096 columns and rank 16: 6 us), at many the product's
+// columns read and written once more (2000 rows of K 1024, 4096 columns and rank 32:
+// 27 us, 65 MB in 14 us of them).
 #include "attn_tiles.h"
 
 #include "../../include/detllm_hip.h"
@@ -32,7 +35,8 @@ struct LoraArgs {
   const int64_t* bk;  // [n_ad]
   const int32_t* adapter;  // [N]
   int N, K, C, rank, n_ad;
-  int tm;  // token rows a block, at most 16
+  int tm;      // token rows a block, at most 16
+  int groups;  // of 256 columns a block
 };
 
 template <int NR>  // 16-wide steps of the rank, at least rank / 16
@@ -112,62 +116,82 @@ __global__ __launch_bounds__(256) void k_lora(LoraArgs a) {
     if (j == 0) h_lds[row] = h;
   }
   __syncthreads();
-  // v of the wave's 64 columns
-  const int c0 = blockIdx.x * LR_COLS + wave * 64;
-  if (c0 >= a.C) return;
-  // the product's own values load first
-  int p[4][4];
-  i64 m[4][4];
+  // rows 4 grp + r of the lane
   int h[4], ar[4];
   i64 bk[4];
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
-    const int row = 4 * grp + r;
-    ar[r] = __shfl(ad, row);
-    h[r] = h_lds[row];
+    ar[r] = __shfl(ad, 4 * grp + r);
+    h[r] = h_lds[4 * grp + r];
     bk[r] = a.bk[::max(ar[r], 0)];
-#pragma unroll
-    for (int n = 0; n < 4; ++n) {
-      const int c = ::min(c0 + 16 * n + l16, a.C - 1);
-      p[r][n] = a.P[(i64)(r0 + (row < rows ? row : 0)) * a.C + c];
-      m[r][n] = a.bm[(i64)::max(ar[r], 0) * a.C + c];
-    }
   }
-  v4i hi[4], lo[4];
+  // (most tiles of a prompt have one adapter: its scales are loaded once)
+  const u64 with = __ballot(ad >= 0 && grp == 0);
+  const int first = __builtin_amdgcn_readlane(ad, __ffsll((unsigned long long)with) - 1);
+  const bool single = __ballot(ad >= 0 && ad != first) == 0;
+  for (int cg = 0; cg < a.groups; ++cg) {
+    // v of the wave's 64 columns
+    const int c0 = (blockIdx.x * a.groups + cg) * LR_COLS + wave * 64;
+    if (c0 >= a.C) return;
+    auto col = [&](int n) { return ::min(c0 + 16 * n + l16, a.C - 1); };
+    // the product's own values load first
+    int p[4][4];
+    i64 m[4][4];
 #pragma unroll
-  for (int n = 0; n < 4; ++n) hi[n] = lo[n] = z;
-  for (u64 left = __ballot(ad >= 0 && grp == 0); left != 0;) {
-    const int cur = __builtin_amdgcn_readlane(ad, __ffsll((unsigned long long)left) - 1);
-    left &= ~__ballot(ad == cur);
+    for (int n = 0; n < 4; ++n)
 #pragma unroll
-    for (int k = 0; k < RP; k += 64) {
-      const int at = k + 16 * grp;
-      const bool in = at < a.rank;
-      v4i wh = z, wl = z;
-      if (ad == cur && in) {
-        wh = *(const v4i*)&w_lds[0][l16][at];
-        wl = *(const v4i*)&w_lds[1][l16][at];
+      for (int r = 0; r < 4; ++r) {
+        const int row = 4 * grp + r;
+        p[r][n] = a.P[(i64)(r0 + (row < rows ? row : 0)) * a.C + col(n)];
       }
+#pragma unroll
+    for (int n = 0; n < 4; ++n) m[0][n] = a.bm[(i64)(single ? first : ::max(ar[0], 0)) * a.C + col(n)];
+    if (single) {
+#pragma unroll
+      for (int r = 1; r < 4; ++r)
+#pragma unroll
+        for (int n = 0; n < 4; ++n) m[r][n] = m[0][n];
+    } else {
+#pragma unroll
+      for (int r = 1; r < 4; ++r)
+#pragma unroll
+        for (int n = 0; n < 4; ++n) m[r][n] = a.bm[(i64)::max(ar[r], 0) * a.C + col(n)];
+    }
+    v4i hi[4], lo[4];
+#pragma unroll
+    for (int n = 0; n < 4; ++n) hi[n] = lo[n] = z;
+    for (u64 left = with; left != 0;) {
+      const int cur = __builtin_amdgcn_readlane(ad, __ffsll((unsigned long long)left) - 1);
+      left &= ~__ballot(ad == cur);
+#pragma unroll
+      for (int k = 0; k < RP; k += 64) {
+        const int at = k + 16 * grp;
+        const bool in = at < a.rank;
+        v4i wh = z, wl = z;
+        if (ad == cur && in) {
+          wh = *(const v4i*)&w_lds[0][l16][at];
+          wl = *(const v4i*)&w_lds[1][l16][at];
+        }
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+          const v4i b = *(const v4i*)(a.b8 + ((i64)cur * a.C + col(n)) * a.rank + (in ? at : 0));
+          hi[n] = mfma16(wh, b, hi[n]);
+          lo[n] = mfma16(wl, b, lo[n]);
+        }
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int row = 4 * grp + r;
+      const i64 s = wsub(bk[r], h[r]);
 #pragma unroll
       for (int n = 0; n < 4; ++n) {
-        const int c = ::min(c0 + 16 * n + l16, a.C - 1);
-        const v4i b = *(const v4i*)(a.b8 + ((i64)cur * a.C + c) * a.rank + (in ? at : 0));
-        hi[n] = mfma16(wh, b, hi[n]);
-        lo[n] = mfma16(wl, b, lo[n]);
+        const int c = c0 + 16 * n + l16;
+        const i64 t = wmul((i64)hi[n][r] * 256 + lo[n][r], m[r][n]);
+        const i64 d = s > 0 ? rshift_round(t, s) : shl(t, wneg(s));
+        if (row < rows && ar[r] >= 0 && c < a.C)
+          a.P[(i64)(r0 + row) * a.C + c] = (int32_t)((uint32_t)p[r][n] + (uint32_t)(u64)d);
       }
-    }
-  }
-#pragma unroll
-  for (int r = 0; r < 4; ++r) {
-    const int row = 4 * grp + r;
-    const i64 s = wsub(bk[r], h[r]);
-#pragma unroll
-    for (int n = 0; n < 4; ++n) {
-      const int c = c0 + 16 * n + l16;
-      const i64 t = wmul((i64)hi[n][r] * 256 + lo[n][r], m[r][n]);
-      const i64 d = s > 0 ? rshift_round(t, s) : shl(t, wneg(s));
-      if (row < rows && ar[r] >= 0 && c < a.C)
-        a.P[(i64)(r0 + row) * a.C + c] = (int32_t)((uint32_t)p[r][n] + (uint32_t)(u64)d);
     }
   }
 }
@@ -185,11 +209,14 @@ int detllm_lora_add(int32_t* P, const int8_t* x8, const int8_t* a8, const int8_t
   if (!P || !x8 || !a8 || !b8 || !bm || !bk || !adapter) return DI_EINVAL;
   // (16-byte loads)
   if ((((uintptr_t)x8 | (uintptr_t)a8 | (uintptr_t)b8) & 15) != 0) return DI_EINVAL;
-  LoraArgs a{P, x8, a8, b8, bm, bk, adapter, N, K, C, rank, n_ad, 16};
+  LoraArgs a{P, x8, a8, b8, bm, bk, adapter, N, K, C, rank, n_ad, 16, 1};
   const int cb = (C + LR_COLS - 1) / LR_COLS;
   // fewer rows a block while the blocks are few: a block's adapters run one after another
   while (a.tm > 1 && (i64)cb * ((N + a.tm - 1) / a.tm) < 256) a.tm /= 2;
-  const dim3 grid(cb, (N + a.tm - 1) / a.tm);
+  // and more columns while they are many: u is made again by every block of the same
+  // rows (the 2000 rows above: 34 us at 1 group, 15 of them for u, 29.5 at 2, 27 at 4)
+  while (a.groups < 4 && (i64)cb * ((N + a.tm - 1) / a.tm) > 512 * a.groups) a.groups *= 2;
+  const dim3 grid((cb + a.groups - 1) / a.groups, (N + a.tm - 1) / a.tm);
   if (grid.y > 65535) return DI_ERANGE;
   switch ((rank + 15) / 16) {
     case 1: hipLaunchKernelGGL(k_lora<1>, grid, dim3(256), 0, s, a); break;
