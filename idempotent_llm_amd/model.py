@@ -38,8 +38,8 @@ import torch
 
 from . import dyadic as dy
 from . import ops
-from ._lib import (attn_acc_work, attn_shared_work, attn_split_plan, call, gemv_plan, pro_fits,
-                   raise_for_error_word)
+from ._lib import (attn_acc_work, attn_shared_work, attn_split_plan, call, gemv_plan, packed_work,
+                   pro_fits, raise_for_error_word)
 from .backends import canonical_backend, gemm_nt, int_gemm, int_gemm_u16i8
 from .guard import NoFloatMode
 from .kvcache import PAGE, KVCache  # noqa: F401  (KVCache is part of this module's API)
@@ -413,6 +413,83 @@ class IntQwen3:
         logits = self._lm_head(x8.view(B, T, H), xm.view(B, T, 1), xk.view(B, T, 1))
         return logits, xm.view(B, T, 1), xk.view(B, T, 1), cache
 
+    # -- packed steps (no counterpart in the reference; packed.py) -------------------
+    @torch.no_grad()
+    def forward_packed(self, ids: torch.Tensor, new, cache, adapters=None, adapter_of=None):
+        """One step of a PackedCache: ids int64 [N], row b's new[b] tokens (a
+        sequence of host ints, N in all) after those of the rows before it.
+        adapters: an AdapterBank, adapter_of: each row's adapter in it (-1:
+        none). Returns int32 logits [rows with new tokens, vocab] of each such
+        row's last token."""
+        dev = self.device
+        new = [int(n) for n in new]
+        cache.check(new)
+        cache.check_model(self)
+        N = sum(new)
+        if ids.dim() != 1 or ids.numel() != N:
+            raise ValueError(f"packed step: {N} token ids in a row, got {tuple(ids.shape)}")
+        if self._seams_overridden():
+            raise NotImplementedError("a packed step and overridden attention seams: it does not "
+                                      "run through them")
+        S = max(n + have for n, have in zip(new, cache.lens))
+        if S > self.max_pos:
+            raise IndexError(f"position {S - 1} is outside the RoPE tables (size {self.max_pos})")
+        if adapters is not None:
+            adapters.check_model(self)
+            if adapter_of is None or len(adapter_of) != cache.rows or any(
+                    not -1 <= a < adapters.n for a in adapter_of):
+                raise ValueError(f"packed step: an adapter in [-1, {adapters.n}) for each of "
+                                 f"{cache.rows} rows")
+            adapters = None if max(adapter_of) < 0 else adapters
+        self._check_host_indices(ids, torch.zeros(1, dtype=I64))
+        counts = torch.tensor(new, dtype=torch.int32).to(dev)
+        plan = torch.ops.detllm_rocm.packed_plan
+        cu, row, pos, slot = plan(cache.table, cache.free, cache.n_free, cache.past, counts, N,
+                                  self._err)
+        if N == 0:
+            return torch.empty(0, self.vocab, dtype=torch.int32, device=dev)
+        ids = ids.to(device=dev, dtype=I64).contiguous()
+        lora = None
+        if adapters is not None:
+            of = torch.tensor(list(adapter_of), dtype=torch.int32).to(dev)
+            lora = (adapters, of[row.long()].contiguous())
+        H, nq, nkv, hd = self.hidden, self.n_q, self.n_kv, self.hd
+        h = torch.empty(N, H, dtype=torch.int32, device=dev)
+        k_res, xm, xk = (torch.empty(N, dtype=I64, device=dev) for _ in range(3))
+        x8 = torch.empty(N, H, dtype=torch.int8, device=dev)
+        L0 = self.layers[0]
+        call("detllm_embed_normq", ids, N, H, self.vocab, self.embed_e8, self.embed_m, self.embed_k,
+             h, k_res, L0.as_m, L0.as_k, x8, xm, xk, self._err)
+        ws = _Workspace(dev)
+        most = max(new)
+        work = packed_work(N, cache.rows, S, most, nq, nkv)
+        for li, L in enumerate(self.layers):
+            nxt = self.layers[li + 1] if li + 1 < self.n_layers else None
+            P, ns, st = self._gemm(x8, L.wqkv, (L.pf_attn,), ws=ws, name="P_qkv")
+            if lora is not None:
+                lora[0].add(li, "qkv", P, x8, lora[1])
+            q8 = ws.buf("q8", (N, nq * hd), torch.int8)
+            tpos = ws.buf("tpos", (N, nq), I64)
+            kp, vp = cache.k_pools[li], cache.v_pools[li]
+            call("detllm_qkv_epilogue_packed", P, ns, st, N, nq, nkv, xm, xk, pos, slot, *L.epi,
+                 self.rope_cos, self.rope_sin, self.max_pos, q8, tpos, kp, vp, cache.pages,
+                 L.kq_est, self._err)
+            attn = ws.buf("attn", (N, nq * hd), I64)
+            call("detllm_attn_packed", q8, tpos, kp, vp, cache.pages, cache.table,
+                 cache.table.shape[1], cu, cache.past, N, cache.rows, S, most, nq, nkv,
+                 ws.buf("work", (work,), torch.uint8), work, attn, self._err)
+            self._after_attention(ws, L, nxt, N, 1, (attn, 1, 0, None), h, k_res, x8, xm, xk, lora)
+        ws.clear()
+        cache.past += counts
+        cache.lens = [n + have for n, have in zip(new, cache.lens)]
+        ends, at = [], 0
+        for n in new:
+            at += n
+            if n > 0:
+                ends.append(at - 1)
+        sel = torch.tensor(ends).to(dev)
+        return self._lm_head(x8[sel], xm[sel], xk[sel])
+
     # -- seams (model.py:430-432, :469-478): override points for diagnostics --------
     def _lm_head(self, x8: torch.Tensor, xm: torch.Tensor, xk: torch.Tensor) -> torch.Tensor:
         """Seam: the LM head GEMM, x8 [..., H] int8 -> int32 [..., vocab]
@@ -737,8 +814,10 @@ class IntQwen3:
         a = torch.cat(parts, dim=2) if len(parts) > 1 else parts[0]
         attn.copy_(a.permute(0, 2, 1, 3).reshape(B * T, nq * hd))
 
-    def _after_attention(self, ws: _Workspace, L, nxt, B, T, attn, h, k_res, x8, xm, xk):
-        """attn: (context partials, nsplit, split_stride) as _attend returns."""
+    def _after_attention(self, ws: _Workspace, L, nxt, B, T, attn, h, k_res, x8, xm, xk,
+                         lora=None):
+        """attn: (context partials, nsplit, split_stride) as _attend returns.
+        lora: None or (AdapterBank, each row's adapter), added to the products."""
         R, H, nq, hd, I_ = B * T, self.hidden, self.n_q, self.hd, self.inter
         # (prefill: the layer's footprint matters; the queries are read, and the
         # o product is, before what takes their buffers here is written)
@@ -756,14 +835,20 @@ class IntQwen3:
             call("detllm_merge_rowcol", *attn[:3], R, nq * hd, L.os_m, L.os_k,
                  L.attn_out_col_m, L.attn_out_col_k, a8, am, ak, *self._next_gemm(L.wo, R), dfit)
         P, ns, st = self._gemm(a8, L.wo, (L.pf_o,), ws=ws, name="P_o")
+        if lora is not None:
+            lora[0].add(L.idx, "o", P, a8, lora[1])
         call("detllm_residual_normq", P, ns, st, R, H, am, ak, L.o_m, L.o_k, 20, h, k_res,
              L.ms_m, L.ms_k, x8, xm, xk, *self._next_gemm(L.wgu, R), dfit)
         P, ns, st = self._gemm(x8, L.wgu, (L.pf_mlp,), ws=ws, name="P_gu")
+        if lora is not None:
+            lora[0].add(L.idx, "gu", P, x8, lora[1])
         y8 = ws.buf("y8", (R, I_), torch.int8)
         call("detllm_swiglu_quant", P, ns, st, R, I_, xm, xk, L.gate_m, L.gate_k, L.up_m,
              L.up_k, L.ds_m, L.ds_k, y8, ym, yk, *self._next_gemm(L.wd, R), dfit)
         P, ns, st = self._gemm(y8, L.wd, (L.down_m,) if nxt is None else (L.down_m, nxt.as_m),
                                ws=ws, name="P_o" if R > 64 else "P_d")
+        if lora is not None:
+            lora[0].add(L.idx, "d", P, y8, lora[1])
         sm_m, sm_k = (nxt.as_m, nxt.as_k) if nxt is not None else (None, 0)
         call("detllm_residual_normq", P, ns, st, R, H, ym, yk, L.down_m, L.down_k, 20, h, k_res,
              sm_m, sm_k, x8, xm, xk, *self._next_gemm(None if nxt is None else nxt.wqkv, R), dfit)
