@@ -11,8 +11,8 @@
 //
 // DI-Exp is not multiplicative: the row maximum comes before the first
 // exponential, the whole denominator before the first probability. One launch
-// makes all three passes (k_packed_one: short rows, or enough units to fill the
-// chip); else each pass is a launch over chunks of the slots (k_packed_phase),
+// makes all three passes (k_packed_few, k_packed_one: short rows, or enough units to
+// fill the chip); else each pass is a launch over chunks of the slots (k_packed_phase),
 // whose maxima, denominators and int32 contexts meet in scratch.
 #include "attn_packed.h"
 
@@ -126,8 +126,8 @@ struct Plan {
   i64 scores_at, max_at, den_at, part_at, bytes;
 };
 
-// us a call, one launch against chunks, stand beside the rules (16 query heads,
-// 8 kv heads).
+// The figures beside the rules: us a call, one launch / chunks, 16 query heads over 8
+// kv heads.
 inline Plan packed_plan(int N, int B, int S, int max_new, int n_q, int n_kv) {
   Plan p{};
   const int G = n_q / n_kv;
@@ -137,17 +137,34 @@ inline Plan packed_plan(int N, int B, int S, int max_new, int n_q, int n_kv) {
   const i64 units = p.few ? rows : imin((i64)N * G / 64 + rows, N);
   p.units = (int)imax(1, units);
   p.rows = (int)imin(16, most * G);
-  const i64 pairs = units * n_kv;
-  p.one = p.few ? S <= FEW_SLOTS : S <= FEW_ONE_SLOTS || pairs >= 384;
+  const i64 pairs = imax(1, units) * n_kv;
+  if (p.few) {
+    // one-token rows x slots: 1 x 1024 13 / 16, 1 x 1500 18 / 14, 8 x 1500 19 / 19, 16 x
+    // 2048 23 / 25, 48 x 1024 25 / 34, 48 x 2048 53 / 61
+    p.one = S <= (pairs >= 128 ? FEW_SLOTS : FEW_SLOTS / 2);
+  } else {
+    // a tile's chain over its slots, against three launches that fill the chip and
+    // parts that are written and added up: tokens behind filled slots 700 + 0 24 / 34,
+    // 1500 + 0 44 / 55, 64 + 500 20 / 25, 64 + 1000 31 / 26, 512 + 2000 64 / 50, 1024 +
+    // 2000 78 / 70, 1200 + 8000 243 / 213, 1600 + 8000 257 / 315, 4 x 512 + 1000 53 / 67
+    const i64 tiles = ((i64)N * G + 63) / 64 * n_kv;
+    p.one = S <= FEW_ONE_SLOTS || S * (420 - tiles) <= 300000;
+  }
   p.chunk = S;
   if (!p.one) {
-    // few-row units: chunks of 512 slots; 64 query rows: chunks for about 1024 blocks
-    const i64 want = p.few ? (S + 511) / 512 : imax(1, imin((S + 511) / 512, 1024 / imax(1, pairs)));
+    // few-row units: about 512 blocks of 256 to 1024 slots (256 / 512 / 1024 / 2048: 1 x
+    // 4000 14 / 16 / 21 / 32, 8 x 4000 30 / 25 / 27 / 39, 48 x 4000 146 / 109 / 99 / 95, 16 rows
+    // of 100 to 7500 57 / 46 / 46 / 61); 64 query rows: about 1024 blocks (a prompt's 512
+    // tokens beside 24 rows: 512, 1024, 2048 blocks 67, 56, 58)
+    const i64 want = p.few ? imin((S + 255) / 256, imax((S + 1023) / 1024, 512 / pairs))
+                           : imax(1, imin((S + 511) / 512, 1024 / pairs));
     p.chunk = (int)(((S + want - 1) / want + DI_PAGE - 1) / DI_PAGE * DI_PAGE);
   }
   p.chunk = ::max(p.chunk, 1);
   p.nch = ::max(1, (S + p.chunk - 1) / p.chunk);
   p.step = p.units * p.nch;
+  // blocks that share the items out (48 rows of 8000 slots: 1024, 2048, 4096 blocks
+  // 207, 187, 184 us)
   if (!p.one) p.step = (int)imin(p.step, imax(1, 2048 / n_kv));
   if (p.one) return p;
   auto room = [&](i64 n) {
@@ -203,8 +220,9 @@ int detllm_attn_packed(const int8_t* q8, const int64_t* tpos, const int8_t* kpoo
   a.q8 = q8; a.tpos = tpos;
   a.kv = KVPages{(int8_t*)kpool, (int8_t*)vpool, table, width, n_kv};
   a.n_pages = n_pages; a.cu = cu; a.past = past; a.N = N; a.B = B; a.S = S;
-  a.n_q = n_q; a.n_kv = n_kv; a.lg = n_q / n_kv == 1 ? 0 : n_q / n_kv == 2 ? 1 : n_q / n_kv == 4 ? 2 : 3;
-  a.max_new = max_new; a.few_rows = p.rows; a.units = p.units; a.step = p.step; a.chunk = p.chunk; a.nch = p.nch; a.out = out; a.err = err;
+  a.n_q = n_q; a.n_kv = n_kv; a.lg = __builtin_ctz((unsigned)(n_q / n_kv));
+  a.max_new = max_new; a.few_rows = p.rows; a.units = p.units; a.step = p.step;
+  a.chunk = p.chunk; a.nch = p.nch; a.out = out; a.err = err;
   char* const w = (char*)work;
   a.scores = (int32_t*)(w + p.scores_at);
   a.smax = (int32_t*)(w + p.max_at);

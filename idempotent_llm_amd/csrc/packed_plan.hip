@@ -20,8 +20,9 @@ constexpr int PLAN_NT = 1024;
 constexpr int PLAN_MAX_ROWS = 2048;   // 16 bytes of LDS each
 constexpr int PLAN_MAX_WIDTH = 1024;  // 131072 slots
 constexpr int PLAN_MAX_SLOTS = 131071;
-// Token rows that the one block writes itself. us, one launch / two: see detllm_packed_plan
-constexpr int PLAN_ONE = 4096;
+// Token rows that the one block writes itself (64 rows; us, one launch / two: 8 tokens
+// 3.3 / 4.7, 1024 5.5 / 7.1, 2048 6.4 / 7.1, 4096 8.0 / 7.1, 16384 18 / 7.2)
+constexpr int PLAN_ONE = 2048;
 
 struct PlanArgs {
   int32_t* table;  // [B][width]

@@ -86,6 +86,9 @@ ATTENTION = {
     "mixed_few_long": ([1500, 0], [2, 40], 2, 1, {}),
     "mixed_chunks": ([3000, 0, 4001, 700], [70, 130, 1, 0], 4, 2, dict(tail=5)),
     "mixed_chunks_group_8": ([1300, 2000], [20, 2], 8, 1, {}),
+    "few_one_launch_2048": ([2047, 1500, 3, 900], [1, 1, 1, 1], 32, 32, {}),
+    "prompt_behind_one_launch": ([400, 3], [300, 1], 8, 8, {}),
+    "prompts_one_launch": ([700, 0, 1300, 90], [300, 260, 200, 1], 8, 8, {}),
     "mixed_one_launch": (_spread(60, 900, 1), [1] * 55 + [40, 30, 20, 90, 0], 8, 8, {}),
     "many_rows": (_spread(300, 400, 2), _spread(300, 3, 3), 2, 1, {}),
     "many_rows_idle": (_spread(200, 300, 4), [0] * 130 + [1] + [0] * 60 + [25] + [0] * 8, 2, 1, {}),
@@ -276,7 +279,7 @@ def test_plan_steps(B, width, cap, top):
     assert seen in (0, 8)
 
 
-@pytest.mark.parametrize("N", [4095, 4096, 4097, 20000])
+@pytest.mark.parametrize("N", [2047, 2048, 2049, 20000])
 def test_plan_many_tokens(N):
     """Token rows of one launch and of two, some behind the last row's."""
     print(f"[plan N={N}]", flush=True)

@@ -233,7 +233,7 @@ def test_scratch_sizes():
     at most as their product does."""
     work = ctypes.c_int64(0)
     lib = _lib.load()
-    for B, N, want in ((1, 0, 0), (2048, 4096, 0), (2048, 4097, 2049 * 16), (3, 1 << 30, 64)):
+    for B, N, want in ((1, 0, 0), (2048, 2048, 0), (2048, 2049, 2049 * 16), (3, 1 << 30, 64)):
         assert lib.detllm_packed_plan_work(B, N, ctypes.byref(work)) == 0 and work.value == want
     for B, N, rc in ((0, 1, -22), (2049, 1, -34), (1, -1, -22)):
         assert lib.detllm_packed_plan_work(B, N, ctypes.byref(work)) == rc
