@@ -152,13 +152,18 @@ inline Plan packed_plan(int N, int B, int S, int max_new, int n_q, int n_kv) {
   }
   p.chunk = S;
   if (!p.one) {
-    // few-row units: about 512 blocks of 256 to 1024 slots (256 / 512 / 1024 / 2048: 1 x
-    // 4000 14 / 16 / 21 / 32, 8 x 4000 30 / 25 / 27 / 39, 48 x 4000 146 / 109 / 99 / 95, 16 rows
-    // of 100 to 7500 57 / 46 / 46 / 61); 64 query rows: about 1024 blocks (a prompt's 512
-    // tokens beside 24 rows: 512, 1024, 2048 blocks 67, 56, 58)
-    const i64 want = p.few ? imin((S + 255) / 256, imax((S + 1023) / 1024, 512 / pairs))
-                           : imax(1, imin((S + 511) / 512, 1024 / pairs));
-    p.chunk = (int)(((S + want - 1) / want + DI_PAGE - 1) / DI_PAGE * DI_PAGE);
+    // few-row units: 256, 512 or 1024 slots (whole steps of a block's waves), the most
+    // that make 512 blocks (256 / 512 / 768 / 1024: 1 x 4000 14 / 16 / - / 21, 8 x 4000 30 / 25
+    // / - / 27, 48 x 4000 146 / 109 / - / 99, 16 rows of 200 to 3000 29 / 24 / 29 / 29, 16 of
+    // 100 to 7500 57 / 46 / - / 46); 64 query rows: about 1024 blocks (512 tokens beside 24
+    // rows of 200 to 5800: 512, 1024, 2048 blocks 180, 107, 116)
+    if (p.few) {
+      p.chunk = 256;
+      while (p.chunk < 1024 && pairs * ((S + 2 * p.chunk - 1) / (2 * p.chunk)) >= 512) p.chunk *= 2;
+    } else {
+      const i64 want = imax(1, imin((S + 511) / 512, 1024 / pairs));
+      p.chunk = (int)(((S + want - 1) / want + DI_PAGE - 1) / DI_PAGE * DI_PAGE);
+    }
   }
   p.chunk = ::max(p.chunk, 1);
   p.nch = ::max(1, (S + p.chunk - 1) / p.chunk);
