@@ -48,6 +48,22 @@ def quantize(A, B, col_m, col_k: int, in_scale=None, scale: float = 1.0):
     return a8, b8, torch.round(ratio * 2.0 ** bk).to(I64), bk
 
 
+def in_scales(model, attn_gains, mlp_gains) -> dict:
+    """What one unit of each product's int8 input stands for, per channel and
+    (layer, site), for adapters trained beside the float model: the artifact's
+    inputs are normalised rows without the norms' gains (attn_gains and mlp_gains,
+    float, one vector per layer) times the smoothing factors 1 / s; its weights have
+    both folded in (prepare.py)."""
+    out = {}
+    for li, L in enumerate(model.layers):
+        s = lambda m, k: 2.0 ** k / m.detach().to("cpu", F64)
+        out[li, "qkv"] = s(L.as_m, L.as_k) * attn_gains[li].detach().to("cpu", F64)
+        out[li, "o"] = s(L.os_m, L.os_k)
+        out[li, "gu"] = s(L.ms_m, L.ms_k) * mlp_gains[li].detach().to("cpu", F64)
+        out[li, "d"] = s(L.ds_m, L.ds_k)
+    return out
+
+
 class AdapterBank:
     """``n`` adapters of rank up to ``rank`` per module for ``model``."""
 
@@ -87,7 +103,7 @@ class AdapterBank:
     def set(self, i: int, weights: dict, scale: float = 1.0, in_scales: dict | None = None) -> None:
         """Adapter i from float weights {(layer, module): (A, B)}, module one of q,
         k, v, o, gate, up, down; modules that are not there add nothing.
-        in_scales {(layer, site): in_scale} as quantize takes it."""
+        in_scales {(layer, site): in_scale} as quantize takes it (in_scales())."""
         if not 0 <= i < self.n:
             raise ValueError(f"adapter {i} of a bank of {self.n}")
         known = {(li, m) for li in range(self.n_layers) for m in self.cols}

@@ -3,6 +3,7 @@ checks on host tensors, before any launch), the entry points' error codes, the
 planners, the fakes, the cache's and the adapters' host side."""
 
 import ctypes
+import json
 from types import SimpleNamespace
 
 import numpy as np
@@ -495,6 +496,38 @@ def test_bank_stacks_the_modules_of_a_product():
             pc.lora(P, x, a8, b8, bm, bk, [2, -1, 2, 0])
     bank.set(2, {})
     assert all(not t.any() for site in bank.sites for v in site.values() for t in v)
+
+
+def test_in_scales_are_what_the_weights_have_folded_in(tmp_path):
+    """Every int8 weight of a quantised model, times its column's scale, is the float
+    weight times in_scales within half a step (and the scales' 16 bits)."""
+    from floatmodel import small_float_model
+    from safetensors.torch import load_file
+
+    from idempotent_llm_amd import prepare as P
+    fm = small_float_model(seed=0)
+    ids = torch.randint(0, 1000, (2, 16), generator=torch.Generator().manual_seed(0))
+    P.prepare(str(tmp_path), fm, ids, device="cpu", model_id="test")
+    t = load_file(tmp_path / "model.safetensors")
+    cfg = json.loads((tmp_path / "config.json").read_text())
+    layers = []
+    for i, Lc in enumerate(cfg["layers"]):
+        layers.append(SimpleNamespace(**{f"{n}_m": t[f"layers.{i}.{n}_m"] for n in ("as", "os", "ms", "ds")},
+                                      **{f"{n}_k": Lc[f"{n}_k"] for n in ("as", "os", "ms", "ds")}))
+    got = lora.in_scales(SimpleNamespace(layers=layers),
+                         [x.input_layernorm.weight for x in fm.model.layers],
+                         [x.post_attention_layernorm.weight for x in fm.model.layers])
+    for i, x in enumerate(fm.model.layers):
+        mods = dict(q=x.self_attn.q_proj, k=x.self_attn.k_proj, v=x.self_attn.v_proj,
+                    o=x.self_attn.o_proj, gate=x.mlp.gate_proj, up=x.mlp.up_proj,
+                    down=x.mlp.down_proj)
+        for site, ms in lora.SITES.items():
+            for m in ms:
+                step = (t[f"layers.{i}.{m}.m"].double() / 2.0 ** cfg["layers"][i][m]["k"])[:, None]
+                w8 = t[f"layers.{i}.{m}.w8t"].double().t()
+                want = mods[m].weight.detach().double() * got[i, site]
+                # half a step, and 127 steps of a 16-bit mantissa's half unit (2^-16)
+                assert ((w8 * step - want).abs() <= step * (0.5 + 127 * 2.0 ** -15)).all()
 
 
 def test_bank_refusals():
