@@ -22,10 +22,12 @@ struct PackedArgs {
   const int32_t* past;  // [B]
   int N, B, S, max_new, n_q, n_kv;
   int lg;        // log2 of the query heads per kv head
-  int few_rows;  // query rows of a few-row unit at most (its rows of scores)
+  // A few-row unit's rows of scores start at row b few_rows, or, where all token rows
+  // have fewer (few_rows 0), at its first token's
+  int few_rows, score_rows;
   int units, chunk, nch;
   int step;      // blocks per kv head
-  int32_t* scores;  // few-row units: [B][n_kv][few_rows][nch * chunk]
+  int32_t* scores;  // few-row units: [n_kv][score_rows][nch * chunk]
   int32_t* smax;    // [units][n_kv][nch][64]: maxima of the visible scores
   int64_t* sden;    // the same of partial denominators
   int32_t* part;    // [nch][N][n_q * 128] contexts (null: one chunk, straight to out)
@@ -652,7 +654,8 @@ __device__ __forceinline__ void few_phase(const PackedArgs& a, const Work& w, Fe
   if (lo_s >= hi_s) return;
   const int R = w.T << a.lg, nc = (w.len + a.chunk - 1) / a.chunk;
   const i64 pitch = (i64)a.nch * a.chunk;
-  int32_t* const sc = a.scores + (((i64)w.b * a.n_kv + w.kvh) * a.few_rows) * pitch;
+  const i64 row0 = a.few_rows ? (i64)w.b * a.few_rows : (i64)w.tok0 << a.lg;
+  int32_t* const sc = a.scores + ((i64)w.kvh * a.score_rows + row0) * pitch;
   const int t0 = lo_s / 64, t1 = (hi_s + 63) / 64;
   if constexpr (PH == PH_MAX) {
     if (w.c == 0 && !a.part && a.nch > 1)

@@ -122,6 +122,7 @@ struct Plan {
   int units;   // units that the rows can make
   int step;    // blocks per kv head
   int rows;    // query rows of a few-row unit
+  i64 score_rows;  // rows of scores per kv head: B times that, or the token rows'
   int chunk, nch;
   i64 scores_at, max_at, den_at, part_at, bytes;
 };
@@ -137,6 +138,7 @@ inline Plan packed_plan(int N, int B, int S, int max_new, int n_q, int n_kv) {
   const i64 units = p.few ? rows : imin((i64)N * G / 64 + rows, N);
   p.units = (int)imax(1, units);
   p.rows = (int)imin(16, most * G);
+  p.score_rows = imin((i64)B * p.rows, (i64)N * G);
   const i64 pairs = imax(1, units) * n_kv;
   if (p.few) {
     // one-token rows x slots: 1 x 1024 13 / 16, 1 x 1500 18 / 14, 8 x 1500 19 / 19, 16 x
@@ -177,7 +179,7 @@ inline Plan packed_plan(int N, int B, int S, int max_new, int n_q, int n_kv) {
     p.bytes += (n + 15) / 16 * 16;
     return at;
   };
-  p.scores_at = room((i64)B * n_kv * p.rows * p.nch * p.chunk * 4);
+  p.scores_at = room(p.score_rows * n_kv * p.nch * p.chunk * 4);
   const i64 cells = (i64)p.units * n_kv * p.nch * 64;
   p.max_at = room(cells * 4);
   p.den_at = room(cells * 8);
@@ -226,8 +228,9 @@ int detllm_attn_packed(const int8_t* q8, const int64_t* tpos, const int8_t* kpoo
   a.kv = KVPages{(int8_t*)kpool, (int8_t*)vpool, table, width, n_kv};
   a.n_pages = n_pages; a.cu = cu; a.past = past; a.N = N; a.B = B; a.S = S;
   a.n_q = n_q; a.n_kv = n_kv; a.lg = __builtin_ctz((unsigned)(n_q / n_kv));
-  a.max_new = max_new; a.few_rows = p.rows; a.units = p.units; a.step = p.step;
+  a.max_new = max_new; a.score_rows = (int)p.score_rows; a.units = p.units; a.step = p.step;
   a.chunk = p.chunk; a.nch = p.nch; a.out = out; a.err = err;
+  a.few_rows = p.score_rows < (i64)B * p.rows ? 0 : p.rows;
   char* const w = (char*)work;
   a.scores = (int32_t*)(w + p.scores_at);
   a.smax = (int32_t*)(w + p.max_at);

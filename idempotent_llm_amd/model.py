@@ -442,6 +442,8 @@ class IntQwen3:
                                  f"{cache.rows} rows")
             adapters = None if max(adapter_of) < 0 else adapters
         self._check_host_indices(ids, torch.zeros(1, dtype=I64))
+        most = max(new)
+        work = packed_work(N, cache.rows, max(S, 1), most, self.n_q, self.n_kv)
         counts = torch.tensor(new, dtype=torch.int32).to(dev)
         plan = torch.ops.detllm_rocm.packed_plan
         cu, row, pos, slot = plan(cache.table, cache.free, cache.n_free, cache.past, counts, N,
@@ -461,8 +463,6 @@ class IntQwen3:
         call("detllm_embed_normq", ids, N, H, self.vocab, self.embed_e8, self.embed_m, self.embed_k,
              h, k_res, L0.as_m, L0.as_k, x8, xm, xk, self._err)
         ws = _Workspace(dev)
-        most = max(new)
-        work = packed_work(N, cache.rows, S, most, nq, nkv)
         for li, L in enumerate(self.layers):
             nxt = self.layers[li + 1] if li + 1 < self.n_layers else None
             P, ns, st = self._gemm(x8, L.wqkv, (L.pf_attn,), ws=ws, name="P_qkv")

@@ -115,6 +115,10 @@ def generate_packed(model, prompts, max_new, rows: int = 32, step_tokens: int = 
         return [torch.empty(0, dtype=torch.int64) for _ in range(n)]
     # (the last token of a reply is not fed back)
     total = [prompts[i].numel() + most[i] - 1 for i in range(n)]
+    for i in todo:
+        if total[i] > model.max_pos:
+            raise IndexError(f"generate_packed: request {i} reaches position {total[i] - 1}, outside "
+                             f"the RoPE tables (size {model.max_pos})")
     rows = min(rows, len(todo))
     cache = PackedCache(model, rows, max(total[i] for i in todo), pages)
     for i in todo:

@@ -608,6 +608,25 @@ def test_captured_step(lens, news):
         assert torch.equal(st[0], st_w[0]) and int(st[2]) == int(st_w[2])
 
 
+def test_opcheck():
+    """The fakes agree with the kernels, and only what is declared changes."""
+    print("[opcheck]", flush=True)
+    tests = ("test_schema", "test_faketensor")
+    check = lambda op, *args: torch.library.opcheck(op.default, args, test_utils=tests)
+    m, epi = _together()
+    P, xm, xk = _step_inputs(m, 6, 1)
+    pools = [torch.zeros(4, m["n_kv"], 128, 128, dtype=I8, device="cuda") for _ in range(2)]
+    arange = torch.arange(6, device="cuda")
+    check(_ops().qkv_epilogue_packed, P, m["n_q"], m["n_kv"], xm, xk, arange, arange, *epi, *pools,
+          _err())
+    c = pc.make([300, 20], [1, 30], 4, 2, seed=10)
+    check(_ops().attn_packed, *(_cuda(c[k]) for k in ORDER), c["S"], 30, _err())
+    st = _state(2, 3, 6, 1)
+    check(_ops().packed_plan, *st[:3], _cuda(np.array([0, 0], np.int32)),
+          _cuda(np.array([200, 3], np.int32)), 205, _err())
+    check(_ops().lora_gemm, *(_cuda(t) for t in _lora_case(5, 64, 30, 16, 2, 1)))
+
+
 def test_side_stream():
     """Two calls at once on streams of their own."""
     print("[side streams]", flush=True)

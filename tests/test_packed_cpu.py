@@ -324,7 +324,7 @@ def test_cache_checks_a_step():
 class _Echo:
     """A model whose reply to a request is its tokens' running sum (and
     whose step notes what it was given)."""
-    n_layers, n_kv, hd, device = 1, 1, 128, torch.device("cpu")
+    n_layers, n_kv, hd, max_pos, device = 1, 1, 128, 500, torch.device("cpu")
     cfg = {"eos_token_id": 40}
 
     def __init__(self):
@@ -394,6 +394,11 @@ def test_generate_packed_stops_and_refuses():
             packed.generate_packed(m, p, 3, **kw)
     with pytest.raises(packed.OutOfPages):
         packed.generate_packed(m, [torch.ones(200, dtype=I64)], 3, pages=1)
+    with pytest.raises(IndexError):
+        packed.generate_packed(m, [torch.ones(498, dtype=I64)], 4)
+    m.steps.clear()
+    packed.generate_packed(m, [torch.ones(498, dtype=I64)], 3)
+    assert sum(map(sum, m.steps)) == 500
 
 
 # ---------------------------------------------------------------- adapters
