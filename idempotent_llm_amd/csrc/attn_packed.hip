@@ -140,6 +140,7 @@ inline Plan packed_plan(int N, int B, int S, int max_new, int n_q, int n_kv) {
   p.rows = (int)imin(16, most * G);
   p.score_rows = imin((i64)B * p.rows, (i64)N * G);
   const i64 pairs = imax(1, units) * n_kv;
+  const i64 tiles = ((i64)N * G + 63) / 64 * n_kv;  // of 64 query rows, were all in one row
   if (p.few) {
     // one-token rows x slots: 1 x 1024 13 / 16, 1 x 1500 18 / 14, 8 x 1500 19 / 19, 16 x
     // 2048 23 / 25, 48 x 1024 25 / 34, 48 x 2048 53 / 61
@@ -148,8 +149,8 @@ inline Plan packed_plan(int N, int B, int S, int max_new, int n_q, int n_kv) {
     // a tile's chain over its slots, against three launches that fill the chip and
     // parts that are written and added up: tokens behind filled slots 700 + 0 24 / 34,
     // 1500 + 0 44 / 55, 64 + 500 20 / 25, 64 + 1000 31 / 26, 512 + 2000 64 / 50, 1024 +
-    // 2000 78 / 70, 1200 + 8000 243 / 213, 1600 + 8000 257 / 315, 4 x 512 + 1000 53 / 67
-    const i64 tiles = ((i64)N * G + 63) / 64 * n_kv;
+    // 2000 78 / 68, 1200 + 8000 243 / 186, 1600 + 8000 256 / 253, 2048 + 8000 271 / 302, 4 x
+    // 512 + 1000 53 / 67
     p.one = S <= FEW_ONE_SLOTS || S * (420 - tiles) <= 300000;
   }
   p.chunk = S;
@@ -157,13 +158,21 @@ inline Plan packed_plan(int N, int B, int S, int max_new, int n_q, int n_kv) {
     // few-row units: 256, 512 or 1024 slots (whole steps of a block's waves), the most
     // that make 512 blocks (256 / 512 / 768 / 1024: 1 x 4000 14 / 16 / - / 21, 8 x 4000 30 / 25
     // / - / 27, 48 x 4000 146 / 109 / - / 99, 16 rows of 200 to 3000 29 / 24 / 29 / 29, 16 of
-    // 100 to 7500 57 / 46 / - / 46); 64 query rows: about 1024 blocks (512 tokens beside 24
-    // rows of 200 to 5800: 512, 1024, 2048 blocks 180, 107, 116)
+    // 100 to 7500 57 / 46 / - / 46). 64 query rows:
+    // three tiles a CU at once, or twice that where their chunks would pass 2048 slots, since
+    // a tile takes its chunk's time however few are left (512 tokens behind 8000 slots in
+    // 7, 6, 5 chunks: 896, 768, 640 items, 110, 86, 102 us; 256 behind 8000 in 13, 11, 9: 68,
+    // 56, 65); a short row beside them counts 5 / 8 of a tile (300 tokens beside 60 rows of 0
+    // to 2950 in 1, 2, 3, 6 chunks 75, 70, 72, 78). At least 384 slots (128 tokens behind 2000:
+    // 384, 512, 1024 28, 31, 42), 512 beside short rows (whole steps of their waves).
     if (p.few) {
       p.chunk = 256;
       while (p.chunk < 1024 && pairs * ((S + 2 * p.chunk - 1) / (2 * p.chunk)) >= 512) p.chunk *= 2;
     } else {
-      const i64 want = imax(1, imin((S + 511) / 512, 1024 / pairs));
+      const i64 load = (imax(1, N - rows) * G + 63) / 64 * n_kv + imax(0, rows - 2) * n_kv * 5 / 8;
+      const i64 rounds = S * load > 2048 * 768 ? 2 : 1, least = rows > 2 ? 512 : 384;
+      const i64 top = imin((S + least - 1) / least, imax(32, S / 2048));
+      const i64 want = imax(1, imin(top, 768 * rounds / load));
       p.chunk = (int)(((S + want - 1) / want + DI_PAGE - 1) / DI_PAGE * DI_PAGE);
     }
   }
