@@ -434,13 +434,9 @@ class IntQwen3:
         S = max(n + have for n, have in zip(new, cache.lens))
         if S > self.max_pos:
             raise IndexError(f"position {S - 1} is outside the RoPE tables (size {self.max_pos})")
-        if adapters is not None:
-            adapters.check_model(self)
-            if adapter_of is None or len(adapter_of) != cache.rows or any(
-                    not -1 <= a < adapters.n for a in adapter_of):
-                raise ValueError(f"packed step: an adapter in [-1, {adapters.n}) for each of "
-                                 f"{cache.rows} rows")
-            adapters = None if max(adapter_of) < 0 else adapters
+        self._check_adapters(adapters, adapter_of, cache.rows)
+        if adapters is not None and max(adapter_of) < 0:
+            adapters = None
         self._check_host_indices(ids, torch.zeros(1, dtype=I64))
         most = max(new)
         work = packed_work(N, cache.rows, max(S, 1), most, self.n_q, self.n_kv)
@@ -489,6 +485,20 @@ class IntQwen3:
                 ends.append(at - 1)
         sel = torch.tensor(ends).to(dev)
         return self._lm_head(x8[sel], xm[sel], xk[sel])
+
+    def _check_adapters(self, adapters, adapter_of, rows: int) -> None:
+        """ValueError unless adapter_of names an adapter of the bank, or none (-1),
+        for each of the rows (without a bank it may be left out, and names none)."""
+        n = 0
+        if adapters is not None:
+            adapters.check_model(self)
+            n = adapters.n
+        elif adapter_of is None:
+            return
+        if adapter_of is None or len(adapter_of) != rows or any(
+                not -1 <= a < n for a in adapter_of):
+            raise ValueError(f"packed step: an adapter in [-1, {n}) for each of {rows} rows"
+                             + ("" if adapters is not None else ", as there is no bank"))
 
     # -- seams (model.py:430-432, :469-478): override points for diagnostics --------
     def _lm_head(self, x8: torch.Tensor, xm: torch.Tensor, xk: torch.Tensor) -> torch.Tensor:

@@ -548,3 +548,49 @@ def test_bank_refusals():
                  (0, {(0, "q"): (torch.zeros(4, 64), torch.zeros(255, 4))})):
         with pytest.raises(ValueError):
             bank.set(i, w)
+
+
+# ---------------------------------------------------------------- the model's step
+
+def _step_model():
+    """An IntQwen3 of sizes alone: what forward_packed checks before it launches."""
+    from idempotent_llm_amd.model import IntQwen3
+    m = object.__new__(IntQwen3)
+    vars(m).update(vars(_bank_model()), max_pos=4000, vocab=50, _err=torch.zeros(1, dtype=I32))
+    return m
+
+
+class _Launched(Exception):
+    pass
+
+
+@pytest.fixture
+def step_bounds(monkeypatch):
+    """The bounds that forward_packed sizes its launches by; it goes no further."""
+    from idempotent_llm_amd import model
+    seen = []
+
+    def work(N, B, S, max_new, n_q, n_kv):
+        seen.append(dict(N=N, B=B, S=S, max_new=max_new))
+        raise _Launched
+
+    monkeypatch.setattr(model, "packed_work", work)
+    return seen
+
+
+def test_step_refuses_adapters_without_a_bank(step_bounds):
+    """Adapters that a call names are in a bank, or the call is refused: it does not
+    answer with the plain model."""
+    m = _step_model()
+    cache, ids = packed.PackedCache(m, 2, 100), torch.zeros(3, dtype=I64)
+    for of in ((0, -1), (-1, 5), (-2, -1), (-1,), (-1, -1, -1)):
+        with pytest.raises(ValueError, match="packed step"):
+            m.forward_packed(ids, (1, 2), cache, None, of)
+    bank = lora.AdapterBank(m, 2, 4)
+    for of in (None, (0,), (0, 2), (-2, 0)):
+        with pytest.raises(ValueError, match="packed step"):
+            m.forward_packed(ids, (1, 2), cache, bank, of)
+    assert not step_bounds
+    for bk, of in ((None, None), (None, (-1, -1)), (bank, (-1, -1)), (bank, (1, -1))):
+        with pytest.raises(_Launched):
+            m.forward_packed(ids, (1, 2), cache, bk, of)
