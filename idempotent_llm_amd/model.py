@@ -488,7 +488,7 @@ class IntQwen3:
 
     def _check_adapters(self, adapters, adapter_of, rows: int) -> None:
         """ValueError unless adapter_of names an adapter of the bank, or none (-1),
-        for each of the rows (without a bank it may be left out, and names none)."""
+        for each of the requests (without a bank it may be left out, and names none)."""
         n = 0
         if adapters is not None:
             adapters.check_model(self)
@@ -497,8 +497,16 @@ class IntQwen3:
             return
         if adapter_of is None or len(adapter_of) != rows or any(
                 not -1 <= a < n for a in adapter_of):
-            raise ValueError(f"packed step: an adapter in [-1, {n}) for each of {rows} rows"
+            raise ValueError(f"packed step: an adapter in [-1, {n}) for each of {rows} requests"
                              + ("" if adapters is not None else ", as there is no bank"))
+
+    def check_requests(self, prompts, adapters=None, adapter_of=None) -> None:
+        """What forward_packed refuses in a request, for all of them before the first
+        step: IndexError for token ids outside the vocabulary (host tensors),
+        ValueError for adapters that the bank does not hold."""
+        for p in prompts:
+            self._check_host_indices(p, torch.zeros(1, dtype=I64))
+        self._check_adapters(adapters, adapter_of, len(prompts))
 
     # -- seams (model.py:430-432, :469-478): override points for diagnostics --------
     def _lm_head(self, x8: torch.Tensor, xm: torch.Tensor, xk: torch.Tensor) -> torch.Tensor:

@@ -103,8 +103,9 @@ def generate_packed(model, prompts, max_new, rows: int = 32, step_tokens: int = 
     n = len(prompts)
     prompts = [p.reshape(-1).to("cpu", torch.int64) for p in prompts]
     most = [int(max_new)] * n if not hasattr(max_new, "__len__") else [int(m) for m in max_new]
-    which = [-1 if adapter_of is None or adapter_of[i] is None else int(adapter_of[i])
-             for i in range(n)]
+    which = [-1 if a is None else int(a) for a in ([None] * n if adapter_of is None else adapter_of)]
+    if len(which) != n:
+        raise ValueError(f"generate_packed: {len(which)} adapters of {n} prompts")
     if len(most) != n or any(m < 0 for m in most) or any(p.numel() < 1 for p in prompts):
         raise ValueError("generate_packed: prompts of at least one token, as many reply lengths")
     if step_tokens < 1 or rows < 1:
@@ -119,6 +120,11 @@ def generate_packed(model, prompts, max_new, rows: int = 32, step_tokens: int = 
         if total[i] > model.max_pos:
             raise IndexError(f"generate_packed: request {i} reaches position {total[i] - 1}, outside "
                              f"the RoPE tables (size {model.max_pos})")
+    # every request before the first step: one that the model refuses would end the
+    # run with the replies of the others (a stand-in for a model may take any)
+    check = getattr(model, "check_requests", None)
+    if check is not None:
+        check(prompts, adapters, which)
     rows = min(rows, len(todo))
     cache = PackedCache(model, rows, max(total[i] for i in todo), pages)
     for i in todo:

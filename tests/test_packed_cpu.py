@@ -594,3 +594,32 @@ def test_step_refuses_adapters_without_a_bank(step_bounds):
     for bk, of in ((None, None), (None, (-1, -1)), (bank, (-1, -1)), (bank, (1, -1))):
         with pytest.raises(_Launched):
             m.forward_packed(ids, (1, 2), cache, bk, of)
+
+
+def test_generate_packed_checks_every_request_first(monkeypatch):
+    """A request that the model refuses is refused before the first step, however late
+    it would be admitted: the others' replies are not lost with it."""
+    m = _step_model()
+    steps = []
+
+    def forward_packed(ids, new, cache, adapters=None, adapter_of=None):
+        steps.append(list(new))
+        raise _Launched
+
+    monkeypatch.setattr(m, "forward_packed", forward_packed, raising=False)
+    good, bank = [torch.tensor([1, 2])] * 3, lora.AdapterBank(m, 2, 4)
+    for bad in (torch.tensor([50]), torch.tensor([3, -51, 3])):
+        with pytest.raises(IndexError, match="token id"):
+            packed.generate_packed(m, good + [bad], 2, rows=1)
+    for bk, of in ((None, (-1, -1, 0)), (None, (0, None, None)), (bank, (0, 1, 2)),
+                   (bank, (0, 1, -2)), (bank, (0, 1)), (None, (-1,) * 4), (bank, ())):
+        with pytest.raises(ValueError, match="packed"):
+            packed.generate_packed(m, good, 2, rows=1, adapters=bk, adapter_of=of)
+    bank.cols = dict(bank.cols, q=384)
+    with pytest.raises(ValueError, match="adapters of a model"):
+        packed.generate_packed(m, good, 2, rows=1, adapters=bank, adapter_of=(0, None, 1))
+    assert not steps
+    with pytest.raises(_Launched):
+        packed.generate_packed(m, good, 2, rows=1, adapters=lora.AdapterBank(m, 2, 4),
+                               adapter_of=(0, None, 1))
+    assert steps == [[2]]
