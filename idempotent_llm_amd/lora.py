@@ -109,9 +109,11 @@ class AdapterBank:
         known = {(li, m) for li in range(self.n_layers) for m in self.cols}
         if set(weights) - known:
             raise ValueError(f"no such module: {sorted(set(weights) - known)[0]}")
+        # (all modules before anything is written: one that is refused leaves the
+        # adapter as it was)
+        made = {}       # (layer, site): its exponent, [(place, first column, module, ...)]
         for li in range(self.n_layers):
             for s, ms in SITES.items():
-                a8, b8, bm, bk = self.sites[li][s]
                 parts, at = [], 0
                 for j, m in enumerate(ms):
                     if (li, m) in weights:
@@ -124,17 +126,19 @@ class AdapterBank:
                         parts.append((j, at, m, *quantize(A, B, cm, ck, sc, scale)))
                     at += self.cols[m]
                 # one exponent per site: the smallest, so that no mantissa passes 16 bits
-                k = min((p[-1] for p in parts if int(p[-2].max()) > 0), default=0)
-                for t in (a8, b8, bm):
-                    t[i].zero_()
-                bk[i] = k
-                for j, c, m, qa, qb, qm, qk in parts:
-                    r = qa.shape[0]
-                    a8[i, j * self.pad:j * self.pad + r] = qa.to(self.device)
-                    b8[i, c:c + self.cols[m], j * self.pad:j * self.pad + r] = qb.to(self.device)
-                    down = max(0, qk - k)
-                    qm = (qm + (1 << (down - 1)) >> down) if down else qm
-                    bm[i, c:c + self.cols[m]] = qm.to(self.device)
+                made[li, s] = min((p[-1] for p in parts if int(p[-2].max()) > 0), default=0), parts
+        for (li, s), (k, parts) in made.items():
+            a8, b8, bm, bk = self.sites[li][s]
+            for t in (a8, b8, bm):
+                t[i].zero_()
+            bk[i] = k
+            for j, c, m, qa, qb, qm, qk in parts:
+                r = qa.shape[0]
+                a8[i, j * self.pad:j * self.pad + r] = qa.to(self.device)
+                b8[i, c:c + self.cols[m], j * self.pad:j * self.pad + r] = qb.to(self.device)
+                down = max(0, qk - k)
+                qm = (qm + (1 << (down - 1)) >> down) if down else qm
+                bm[i, c:c + self.cols[m]] = qm.to(self.device)
 
     def add(self, li: int, site: str, P, x8, adapter) -> None:
         """The adapters' part of layer li's product P ([.., N, C], its first

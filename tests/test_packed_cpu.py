@@ -623,3 +623,22 @@ def test_generate_packed_checks_every_request_first(monkeypatch):
         packed.generate_packed(m, good, 2, rows=1, adapters=lora.AdapterBank(m, 2, 4),
                                adapter_of=(0, None, 1))
     assert steps == [[2]]
+
+
+def test_bank_keeps_an_adapter_that_cannot_be_replaced():
+    """A set that is refused, in whichever layer, leaves every adapter as it was."""
+    bank = lora.AdapterBank(_bank_model(), 2, 4)
+    g = torch.Generator().manual_seed(3)
+    r = lambda *s: torch.randn(*s, generator=g)
+    bank.set(1, {(0, "q"): (r(4, 64), r(256, 4)), (1, "down"): (r(4, 96), r(64, 4))})
+    before = [{s: [t.clone() for t in v] for s, v in site.items()} for site in bank.sites]
+    first = {(0, "q"): (r(4, 64), r(256, 4)), (0, "o"): (r(4, 256), r(64, 4))}
+    nan = r(64, 4)
+    nan[3, 1] = float("nan")
+    for bad in ((r(5, 96), r(64, 5)), (r(4, 95), r(64, 4)), (r(4, 96), r(63, 4)),
+                (r(4, 96), r(64, 3)), (r(4, 96), nan)):
+        with pytest.raises(ValueError):
+            bank.set(1, {**first, (1, "down"): bad})
+        for site, was in zip(bank.sites, before):
+            for s, v in site.items():
+                assert all(torch.equal(a, b) for a, b in zip(v, was[s]))
