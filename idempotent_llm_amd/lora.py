@@ -136,7 +136,7 @@ class AdapterBank:
                 r = qa.shape[0]
                 a8[i, j * self.pad:j * self.pad + r] = qa.to(self.device)
                 b8[i, c:c + self.cols[m], j * self.pad:j * self.pad + r] = qb.to(self.device)
-                down = max(0, qk - k)
+                down = min(max(0, qk - k), 62)      # (62: nothing of 17 bits is left)
                 qm = (qm + (1 << (down - 1)) >> down) if down else qm
                 bm[i, c:c + self.cols[m]] = qm.to(self.device)
 

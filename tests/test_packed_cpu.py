@@ -642,3 +642,22 @@ def test_bank_keeps_an_adapter_that_cannot_be_replaced():
         for site, was in zip(bank.sites, before):
             for s, v in site.items():
                 assert all(torch.equal(a, b) for a, b in zip(v, was[s]))
+
+
+@pytest.mark.parametrize("small", [1e-14, 1e-19, 1e-22, 1e-38])
+def test_bank_takes_modules_of_far_scales(small):
+    """Modules of one product whose scales are any factor apart: the larger one's
+    integers are those of the module alone, the smaller one's are what is left of
+    it at the larger one's exponent."""
+    m = _bank_model()
+    bank = lora.AdapterBank(m, 1, 4)
+    g = torch.Generator().manual_seed(5)
+    r = lambda *s: torch.randn(*s, generator=g)
+    q, k = (r(4, 64), r(256, 4)), (r(4, 64), r(128, 4) * small)
+    bank.set(0, {(0, "q"): q, (0, "k"): k})
+    _, _, bm, bk = bank.sites[0]["qkv"]
+    _, _, qm, qk = lora.quantize(*q, m.layers[0].q_m, m.layers[0].q_k)
+    _, _, km, kk = lora.quantize(*k, m.layers[0].k_m, m.layers[0].k_k)
+    assert int(bk[0]) == qk and torch.equal(bm[0, :256], qm)
+    exact = km.double() * 2.0 ** (qk - kk)
+    assert ((bm[0, 256:384] - exact).abs() <= 0.5).all()
