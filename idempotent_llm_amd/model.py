@@ -431,7 +431,8 @@ class IntQwen3:
         if self._seams_overridden():
             raise NotImplementedError("a packed step and overridden attention seams: it does not "
                                       "run through them")
-        S = max(n + have for n, have in zip(new, cache.lens))
+        # (idle rows, however long, size nothing)
+        S = max((n + have for n, have in zip(new, cache.lens) if n > 0), default=1)
         if S > self.max_pos:
             raise IndexError(f"position {S - 1} is outside the RoPE tables (size {self.max_pos})")
         self._check_adapters(adapters, adapter_of, cache.rows)
@@ -439,7 +440,7 @@ class IntQwen3:
             adapters = None
         self._check_host_indices(ids, torch.zeros(1, dtype=I64))
         most = max(new)
-        work = packed_work(N, cache.rows, max(S, 1), most, self.n_q, self.n_kv)
+        work = packed_work(N, cache.rows, S, most, self.n_q, self.n_kv)
         counts = torch.tensor(new, dtype=torch.int32).to(dev)
         plan = torch.ops.detllm_rocm.packed_plan
         cu, row, pos, slot = plan(cache.table, cache.free, cache.n_free, cache.past, counts, N,

@@ -290,8 +290,8 @@ def qkv_epilogue_packed(P, n_q, n_kv, *rest):
      "Tensor past, SymInt S, SymInt max_new, Tensor(a9!) err) -> Tensor")
 def attn_packed(q8, tpos, kpool, vpool, table, cu, past, S, max_new, err):
     """Attention of packed token rows over the cache: q8 [N, n_q, 128], tpos
-    [N, n_q], cu [B + 1] and past [B] int32; no row has more than S slots (its new
-    ones counted) or max_new tokens. Slots of pages that are not mapped are not
+    [N, n_q], cu [B + 1] and past [B] int32; no row with new tokens has more than S
+    slots (those counted) or max_new tokens. Slots of pages that are not mapped are not
     seen. -> exact int64 contexts [N, n_q * 128], 0 behind the last row's tokens."""
     return q8.new_empty(q8.shape[0], q8.shape[1] * 128, dtype=I64)
 

@@ -466,9 +466,10 @@ int detllm_attn_decode_shared(const int8_t* q8, const int64_t* tpos, const int8_
  * step without padding: row b has past[b] filled slots and new tokens, the token
  * rows of all follow each other (row b's at cu[b] .. cu[b + 1] - 1, int32), and
  * token t of row b has position and slot past[b] + t. The integers are those of
- * the padded forms. Lengths stay on the device; N (token rows), S (slots of a row)
- * and max_new (new tokens of a row) are bounds that size a launch. Values outside
- * them set bit 4 of *err; nothing is read or written out of range. */
+ * the padded forms. Lengths stay on the device; N (token rows), S (slots of a row
+ * that has new tokens) and max_new (new tokens of a row) are bounds that size a
+ * launch. Values outside them set bit 4 of *err; nothing is read or written out of
+ * range. */
 
 /* The step's bookkeeping: cu [B + 1] from fresh [B] (new tokens), and of each of
  * the N token rows its row, position and slot (page * 128 + position % 128; behind

@@ -643,3 +643,15 @@ def test_side_stream():
     wants = [pc.attend(c) for c in cases]
     for i, (out, _) in enumerate(outs):
         _eq(out, wants[i % 2])
+
+
+@pytest.mark.parametrize("new", [[0, 1, 0, 1], [0, 20, 0, 1], [0, 1, 70, 0]])
+def test_attention_idle_rows_past_the_bound(new):
+    """S bounds the rows that have new tokens: idle rows of more slots are neither
+    reported nor read, and the others are exact."""
+    print(f"[attention idle rows past the bound {new}]", flush=True)
+    c = pc.make([4000, 300, 1500 if new[2] == 0 else 30, 5], new, 4, 2, seed=11)
+    busy = [p + n for p, n in zip(c["past"], new) if n]
+    out, err = _attend(c, int(max(busy)))
+    assert err == 0
+    _eq(out, pc.attend(c))

@@ -661,3 +661,16 @@ def test_bank_takes_modules_of_far_scales(small):
     assert int(bk[0]) == qk and torch.equal(bm[0, :256], qm)
     exact = km.double() * 2.0 ** (qk - kk)
     assert ((bm[0, 256:384] - exact).abs() <= 0.5).all()
+
+
+def test_step_is_sized_by_the_rows_in_it(step_bounds):
+    """Rows without new tokens, however long, do not size a step's launches and
+    scratch."""
+    m = _step_model()
+    cache = packed.PackedCache(m, 3, 3000)
+    for lens, new, S in (([2900, 5, 0], (0, 1, 0), 6), ([2900, 5, 0], (1, 1, 0), 2901),
+                         ([0, 0, 2999], (7, 0, 0), 7), ([130, 0, 2999], (2, 64, 0), 132)):
+        cache.lens = lens
+        with pytest.raises(_Launched):
+            m.forward_packed(torch.zeros(sum(new), dtype=I64), new, cache)
+        assert step_bounds[-1] == dict(N=sum(new), B=3, S=S, max_new=max(new))
