@@ -25,6 +25,7 @@ namespace {
 
 constexpr int LR_MAX_RANK = 128;
 constexpr int LR_COLS = 256;
+constexpr int LR_MAX_ROWS = 65535 * 16;  // blocks of a grid's second dimension
 
 struct LoraArgs {
   int32_t* P;         // [N][C]
@@ -204,7 +205,7 @@ int detllm_lora_add(int32_t* P, const int8_t* x8, const int8_t* a8, const int8_t
                     const int64_t* bm, const int64_t* bk, const int32_t* adapter, int N, int K,
                     int C, int rank, int n_ad, hipStream_t s) {
   if (N < 0 || K < 16 || K % 16 || C < 1 || rank < 16 || rank % 16 || n_ad < 1) return DI_EINVAL;
-  if (K > 65536 || rank > LR_MAX_RANK || C > (1 << 24) || N > (1 << 20)) return DI_ERANGE;
+  if (K > 65536 || rank > LR_MAX_RANK || C > (1 << 24) || N > LR_MAX_ROWS) return DI_ERANGE;
   if (N == 0) return DI_OK;
   if (!P || !x8 || !a8 || !b8 || !bm || !bk || !adapter) return DI_EINVAL;
   // (16-byte loads)
@@ -219,7 +220,6 @@ int detllm_lora_add(int32_t* P, const int8_t* x8, const int8_t* a8, const int8_t
   // rows (the 2000 rows above: 34 us at 1 group, 15 of them for u, 29.5 at 2, 27 at 4)
   while (a.groups < 4 && (i64)cb * ((N + a.tm - 1) / a.tm) > 512 * a.groups) a.groups *= 2;
   const dim3 grid((cb + a.groups - 1) / a.groups, (N + a.tm - 1) / a.tm);
-  if (grid.y > 65535) return DI_ERANGE;
   switch ((rank + 15) / 16) {
     case 1: hipLaunchKernelGGL(k_lora<1>, grid, dim3(256), 0, s, a); break;
     case 2: hipLaunchKernelGGL(k_lora<2>, grid, dim3(256), 0, s, a); break;

@@ -868,8 +868,8 @@ Tensor op_lora_gemm(const Tensor& x8, const Tensor& w, const Tensor& a8, const T
   const int64_t N = x8.size(0), K = x8.size(1), C = w.size(0), n_ad = a8.size(0), r = a8.size(1);
   DI_CHECK(K >= 16 && K % 16 == 0 && K <= 65536 && r >= 16 && r % 16 == 0 && r <= 128, op,
            "K of ", K, " (a multiple of 16 up to 65536), rank ", r, " (one up to 128)");
-  DI_CHECK(N <= (1 << 20) && C >= 1 && C <= (1 << 24) && n_ad >= 1 && n_ad <= INT32_MAX, op, N,
-           " token rows, ", C, " columns, ", n_ad, " adapters");
+  DI_CHECK(N <= 65535 * 16 && C >= 1 && C <= (1 << 24) && n_ad >= 1 && n_ad <= INT32_MAX, op, N,
+           " token rows (at most 1048560), ", C, " columns, ", n_ad, " adapters");
   const Tensor xc = aligned(x8), wc = aligned(w), ac = aligned(a8), bc = aligned(b8);
   check_is(op, "x8", xc, at::kChar, {N, K}, x8);
   check_is(op, "w", wc, at::kChar, {C, K}, x8);

@@ -674,3 +674,11 @@ def test_step_is_sized_by_the_rows_in_it(step_bounds):
         with pytest.raises(_Launched):
             m.forward_packed(torch.zeros(sum(new), dtype=I64), new, cache)
         assert step_bounds[-1] == dict(N=sum(new), B=3, S=S, max_new=max(new))
+
+
+def test_lora_refuses_more_rows_than_a_launch_takes():
+    """Before the product is launched, by name."""
+    _refused("lora_gemm", _lora(), {"rows": lambda c: _lora(N=1 << 20, K=16)})
+    t = torch.zeros(64, dtype=I64)
+    with pytest.raises(RuntimeError, match=r"detllm_lora_add failed \(code -34\)"):
+        _lib.native().entries()["detllm_lora_add"](0, t, t, t, t, t, t, t, 1 << 20, 64, 10, 16, 2)
