@@ -655,3 +655,39 @@ def test_attention_idle_rows_past_the_bound(new):
     out, err = _attend(c, int(max(busy)))
     assert err == 0
     _eq(out, pc.attend(c))
+
+
+# past, new, n_q, n_kv, whether the call is one launch (no scratch), extras
+PATHS = {
+    "few_one": ([2047, 1500, 3], [1, 1, 1], 64, 64, True, {}),
+    "few_chunks": ([2048, 3], [1, 1], 64, 64, False, {}),
+    "short_row_past_512": ([650, 10], [1, 40], 8, 8, True, dict(holes=((0, 3, -1),))),
+    "short_rows_past_512": ([700, 513, 690, 511, 0, 30], [1, 2, 1, 1, 0, 40], 8, 8, True, {}),
+    "prompts": ([560, 0, 400, 300], [300, 260, 100, 1], 8, 8, True, {}),
+    "prompts_group_4": ([300, 0, 37], [90, 120, 1], 16, 4, True, {}),
+    "tile_chunks": ([700, 3], [300, 1], 8, 8, False, {}),
+    # from 420 tiles on one launch takes any length: rows of more than 64 pages, whose
+    # ids a wave holds in two lots, with holes on both sides of the 64th
+    "long_rows_beside_many_tiles": (
+        [9000, 8300, 0, 100, 0, 0, 5, 0, 2047], [1, 70, 128, 128, 128, 128, 128, 128, 1], 32, 32,
+        True, dict(holes=((0, 3, -1), (0, 64, -1), (0, 66, 2**31 - 1), (1, 1, -1), (1, 63, -1),
+                          (1, 64, -5)))),
+    "long_few_rows_beside_many_tiles": (
+        [8191, 8192, 8320, 0, 3], [1, 4, 1, 700, 200], 32, 32, True,
+        dict(holes=((1, 64, -1), (2, 0, -1)), tpos=(30, 40))),
+}
+
+
+@pytest.mark.parametrize("name", list(PATHS))
+def test_attention_paths(name):
+    """Cases of each launch, which the scratch tells apart (a rule that moves them
+    elsewhere fails here)."""
+    from idempotent_llm_amd import _lib
+    print(f"[attention path {name}]", flush=True)
+    past, new, n_q, n_kv, one, extra = PATHS[name]
+    c = pc.make(past, new, n_q, n_kv, seed=len(name), **extra)
+    work = _lib.packed_work(int(sum(new)), len(past), c["S"], c["max_new"], n_q, n_kv)
+    assert (work == 0) == one
+    out, err = _attend(c)
+    assert err == 0
+    _eq(out, pc.attend(c))
