@@ -691,3 +691,119 @@ def test_attention_paths(name):
     out, err = _attend(c)
     assert err == 0
     _eq(out, pc.attend(c))
+
+
+class _Guarded:
+    """Buffers of exact sizes between marks that no launch may change."""
+    MARK = 0x5A
+
+    def __init__(self):
+        self.made = []
+
+    def __call__(self, shape, dtype):
+        n = int(np.prod(shape)) * torch.empty(0, dtype=dtype).element_size()
+        whole = torch.full((n + 8192 - n % 4096,), self.MARK, dtype=torch.uint8, device="cuda")
+        self.made.append((whole, n))
+        return whole[2048:2048 + n].view(dtype).view(shape)
+
+    def check(self):
+        for whole, n in self.made:
+            assert bool((whole[:2048] == self.MARK).all()), "written before a buffer"
+            assert bool((whole[2048 + n:] == self.MARK).all()), "written behind a buffer"
+
+
+def _args(c, work, out, err, S, max_new):
+    dev = [_cuda(c[k]) for k in ORDER]
+    q8, tpos, kp, vp, table, cu, past = dev
+    N, n_q = q8.shape[:2]
+    return dev, ["detllm_attn_packed", q8, tpos, kp, vp, kp.shape[0], table, table.shape[1], cu,
+                 past, N, past.shape[0], S, max_new, n_q, kp.shape[1], work,
+                 work.numel() if work is not None else 0, out, err]
+
+
+# a call's scratch is used up to its last byte in some of these, the outputs in all
+GUARDED = {
+    "few": ([300, 20, 5], [1, 2, 0], 4, 2, 321, 2, 0),
+    "few_chunks": ([6000, 10, 2300, 0], [1, 1, 1, 1], 4, 2, None, 1, 3),
+    "few_chunks_16": ([5000, 10, 2300], [8, 3, 8], 4, 2, None, 8, 0),
+    "few_by_token": ([3000, 40, 2999, 0, 7, 1], [8, 1, 1, 0, 1, 1], 4, 2, None, 8, 0),
+    "tiles": ([560, 0, 40], [300, 26, 1], 4, 2, None, 300, 2),
+    "tile_chunks": ([3000, 0, 4001, 700], [70, 130, 1, 0], 4, 2, None, 130, 5),
+    "tile_chunks_8": ([2900, 17], [33, 2], 8, 1, None, 33, 0),
+    "tile_chunks_wider": ([900, 40, 5], [40, 1, 1], 4, 2, 10240, 500, 0),
+}
+
+
+def _attend_guarded(c, S, max_new, cus):
+    """Calls with each of the offsets; the last is the case's own. -> its contexts."""
+    from idempotent_llm_amd import _lib
+    buf = _Guarded()
+    N, n_q = c["q8"].shape[:2]
+    B, n_kv = len(c["past"]), c["kpool"].shape[1]
+    work = buf((_lib.packed_work(N, B, S, max_new, n_q, n_kv),), torch.uint8)
+    out, err = buf((N, n_q * 128), I64), buf((1,), I32)
+    for cu in [*cus, c["cu"]]:
+        err.zero_()
+        dev, args = _args(dict(c, cu=np.asarray(cu, np.int32)), work, out, err, S, max_new)
+        before = [t.clone() for t in dev]
+        _lib.call(*args)
+        torch.cuda.synchronize()
+        buf.check()
+        assert all(torch.equal(a, b) for a, b in zip(dev, before)), "an operand changed"
+    assert int(err) == 0
+    return out
+
+
+@pytest.mark.parametrize("name", list(GUARDED))
+def test_attention_stays_in_its_buffers(name):
+    """Scratch of exactly the stated size, outputs and the error word: nothing
+    beside them is written, no operand changes, and the size suffices."""
+    print(f"[attention buffers {name}]", flush=True)
+    past, new, n_q, n_kv, S, max_new, tail = GUARDED[name]
+    c = pc.make(past, new, n_q, n_kv, seed=len(name), tail=tail,
+                width=80 if S == 10240 else None)
+    _eq(_attend_guarded(c, S or c["S"], max_new, ()), pc.attend(c))
+
+
+@pytest.mark.parametrize("S,n_kv", [(300, 2), (700, 2), (700, 8), (3000, 1)])
+@pytest.mark.parametrize("max_new", [1, 8, 40])
+def test_attention_of_odd_offsets_stays_in_its_buffers(S, n_kv, max_new):
+    """Token offsets that overlap, decrease or leave the rows: the same."""
+    print(f"[attention odd offsets {S} {n_kv} {max_new}]", flush=True)
+    c = pc.make([5, 70, 290, 0, 130], [8] * 5, 8, n_kv, seed=8, width=24)
+    odd = ([0, 10, 0, 10, 0, 10], [40] * 6, [-5, 3, 2, 1, 0, 60], [0, 90, 90, 90, -1, 2**31 - 1],
+           [0, 40, 0, 40, 0, 40], [9, 8, 7, 6, 5, 4], [0, 0, 0, 0, 0, 2**31 - 1],
+           [-2**31, 2**31 - 1, -2**31, 2**31 - 1, -2**31, 2**31 - 1])
+    if max_new < 8:                       # the good call behind them needs its bound
+        c = pc.make([5, 70, 290, 0, 130], [1] * 5, 8, n_kv, seed=8, width=24, tail=35)
+    _eq(_attend_guarded(c, S, max_new, odd), pc.attend(c))
+
+
+@pytest.mark.parametrize("N", [5, 700, 2049, 5000])
+def test_plan_stays_in_its_buffers(N):
+    """A plan's table, free list, outputs and scratch of exact sizes, and fewer token
+    rows than tokens."""
+    from idempotent_llm_amd import _lib
+    print(f"[plan buffers {N}]", flush=True)
+    B, width, cap = 5, 30, 120
+    buf = _Guarded()
+    table, free, n_free = buf((B, width), I32), buf((cap,), I32), buf((1,), I32)
+    past, new = _cuda(np.zeros(B, np.int32)), _cuda(np.array([N, 0, 129, 7, 2000], np.int32))
+    cu, row, pos, slot = buf((B + 1,), I32), buf((N,), I32), buf((N,), I64), buf((N,), I64)
+    work, err = buf(((B + 1) * 16 if N > 2048 else 0,), torch.uint8), buf((1,), I32)
+    if N > 3840:
+        new[0] = 3840                     # the row's own slots
+    table.fill_(-1)
+    free.copy_(torch.arange(cap, dtype=I32))
+    n_free.fill_(cap)
+    err.zero_()
+    before = [table.cpu().numpy(), free.cpu().numpy(), cap]
+    _lib.call("detllm_packed_plan", table, width, free, cap, n_free, past, new, B, N, cu, row, pos,
+              slot, work, work.numel(), err)
+    torch.cuda.synchronize()
+    buf.check()
+    want = pc.plan(*before, past.cpu().numpy(), new.cpu().numpy(), N)
+    assert int(n_free) == want[2] and int(err) == want[7]
+    for g, w in zip((table, free[:want[2]], cu, row, pos, slot),
+                    (want[0], want[1][:want[2]], *want[3:7])):
+        _eq(g, w)
