@@ -185,9 +185,11 @@ __device__ __forceinline__ int packed_page(const PackedArgs& a, int b, int j) {
 //
 // For tpos < 2^17 (a wave's rows decide together; else the integer forms):
 // with n = m - s >= 0, t = tpos, sp = t - n, the exponential is
-// e = ((q + 1) t - n) >> (q + 1), q = n div t (intops.h, dexp_est). The scores'
-// accumulators start from 0x4B400000 + t - m, so that they arrive as the bits of
-// the float 1.5 2^23 + sp (|sp| < 2^22: |n| <= 2^22). Then
+// e = ((q + 1) t + sp) >> (q + 1) = ((q + 2) t - n) >> (q + 1), q = n div t
+// (intops.h, dexp_est): what is shifted is 2 t - n mod t, above t and at most
+// 2 t < 2^18. The scores' accumulators start from 0x4B400000 + t - m, so that they
+// arrive as the bits of the float 1.5 2^23 + sp (|sp| < 2^22: |n| <= 2^22), whose
+// low 22 bits the multiply-add and the AND leave. Then
 //   x = clamp01(b - sp a), a = fl(1 / 31 t), b = fl((1.5 + 0.5 / t) / 31):
 //     31 x is (n + 0.5) / t + 0.5 within 2^-18.3 where that is below 31 (a, b and
 //     the fma are off by at most half a step, on values up to 32 / 31), and a
@@ -792,7 +794,7 @@ __device__ __forceinline__ void few_phase(const PackedArgs& a, const Work& w, Fe
 //
 // What bounds it is issue. Alone on a SIMD a wave takes some 240, 670 and 1520
 // cycles for a half page's three passes, two side by side 170, 460 and 1050, so a
-// prompt of 2500 tokens (632 tiles of up to 40 half pages, 75 us) is bound by its last
+// prompt of 2500 tokens (632 tiles of up to 40 half pages, 68 us) is bound by its last
 // tiles' own chains; its loads alone take 30 us. Three blocks a CU (168 registers a lane,
 // none spilled: scratch memory cost a launch 8 us by itself, and two waves more a
 // SIMD at 128 registers did not make up for it).

@@ -128,7 +128,7 @@ struct Plan {
 };
 
 // The figures beside the rules: us a call, one launch / chunks, 16 query heads over 8
-// kv heads.
+// kv heads unless they say otherwise.
 inline Plan packed_plan(int N, int B, int S, int max_new, int n_q, int n_kv) {
   Plan p{};
   const int G = n_q / n_kv;
@@ -150,7 +150,13 @@ inline Plan packed_plan(int N, int B, int S, int max_new, int n_q, int n_kv) {
     // parts that are written and added up: tokens behind filled slots 700 + 0 24 / 34,
     // 1500 + 0 44 / 55, 64 + 500 20 / 25, 64 + 1000 31 / 26, 512 + 2000 64 / 50, 1024 +
     // 2000 78 / 68, 1200 + 8000 243 / 186, 1600 + 8000 256 / 253, 2048 + 8000 271 / 302, 4 x
-    // 512 + 1000 53 / 67
+    // 512 + 1000 53 / 67. From 420 tiles on whatever S is: 2048 + 16000 496 /
+    // 494, + 64000 1862 / 1713, 4 x 512 + 16000 479 / 511, + 64000 1852 / 1878, 32 heads over 8
+    // 4 x 256 + 32000 927 / 955. The bounds do not tell whose S it is: one long row beside
+    // tiles that are prompts of 100 tokens lasts as long as its own chain (42 of them + a row
+    // of 4000 100 / 71, 16000 368 / 208, 131000 2943 / 1968; 16 rows up to 16000 371 / 274). Chunks
+    // would take scratch there, 16 words for each row, kv head and slot (64 rows over
+    // 131000 slots 4.3 GB): a call that now needs none could run out of memory.
     p.one = S <= FEW_ONE_SLOTS || S * (420 - tiles) <= 300000;
   }
   p.chunk = S;

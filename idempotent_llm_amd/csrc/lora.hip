@@ -8,11 +8,11 @@
 // h - bk_a where that is positive; int64, then added as int32).
 //
 // A block takes up to 16 consecutive token rows and up to four times 256 columns. Its
-// adapters are
-// the distinct ones of those rows, one after another: u on i8 MFMA with K split over
-// the four waves, the other adapters' rows dropped as the sums meet in LDS; then w as two
-// int8 operands (w = 256 H + L - 128, bytes H and L ^ 0x80), rows of other adapters
-// zero, so the adapters' products add up in one accumulator. What bounds it: at
+// adapters are the distinct ones of those rows, one after another: u on i8 MFMA with
+// K split over the four waves, the other adapters' rows dropped as the sums meet in
+// LDS; then w as two int8 operands (w = 256 H + L - 128, bytes H and L ^ 0x80), rows
+// of other adapters zero, so the adapters' products add up in one accumulator. Each
+// group of column blocks makes u for itself. What bounds it: at
 // few rows one chain of loads (adapters, x and A, B, then the product's own
 // columns; 8 rows of K 1024, 4096 columns and rank 16: 6 us), at many the product's
 // columns read and written once more (2000 rows of K 1024, 4096 columns and rank 32:
