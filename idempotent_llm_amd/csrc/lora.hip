@@ -5,7 +5,7 @@
 // h = max(ilog2(max |u|) - 12, 0), w = rshift_round(u, h), |w| <= 2^13 (the rule of
 // requant_i32_common at 13 bits), v = B_a w (int32, |v| <= rank 2^20), and the
 // product's column c gets rshift_round(v[c] bm_a[c], bk_a - h) (a left shift by
-// h - bk_a where that is positive; int64, then added as int32).
+// h - bk_a where that is positive, 0 from shifts of 64 on; int64, then added as int32).
 //
 // A block takes up to 16 consecutive token rows and up to four times 256 columns. Its
 // adapters are the distinct ones of those rows, one after another: u on i8 MFMA with
@@ -185,12 +185,14 @@ __global__ __launch_bounds__(256) void k_lora(LoraArgs a) {
     for (int r = 0; r < 4; ++r) {
       const int row = 4 * grp + r;
       const i64 s = wsub(bk[r], h[r]);
+      // (shifts from 64 on leave nothing; rshift_round's half would wrap)
+      const bool adds = row < rows && ar[r] >= 0 && s < 64;
 #pragma unroll
       for (int n = 0; n < 4; ++n) {
         const int c = c0 + 16 * n + l16;
         const i64 t = wmul((i64)hi[n][r] * 256 + lo[n][r], m[r][n]);
         const i64 d = s > 0 ? rshift_round(t, s) : shl(t, wneg(s));
-        if (row < rows && ar[r] >= 0 && c < a.C)
+        if (adds && c < a.C)
           a.P[(i64)(r0 + row) * a.C + c] = (int32_t)((uint32_t)p[r][n] + (uint32_t)(u64)d);
       }
     }

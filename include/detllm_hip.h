@@ -519,9 +519,10 @@ int detllm_attn_packed(const int8_t* q8, const int64_t* tpos, const int8_t* kpoo
  * value none (its row of P is left as it is). Per row, with a8 [n_ad][rank][K], b8
  * [n_ad][C][rank], bm [n_ad][C], bk [n_ad]: u = a8 x8; h = max(ilog2(max(|u|, 1)) - 12,
  * 0); w = rshift_round(u, h) (dyadic.py:108-120 at 13 bits); v = b8 w; P[c] +=
- * rshift_round(v[c] bm[c], bk - h), a left shift where bk < h, int64 and then int32
- * (wrapping). rank a multiple of 16 up to 128 (zeros fill it up), K one up to 65536,
- * N up to 1048560, C to 2^24; x8, a8 and b8 16-byte aligned. */
+ * rshift_round(v[c] bm[c], bk - h), a left shift where bk < h, 0 where the shift is 64
+ * or more, int64 and then int32 (wrapping). rank a multiple of 16 up to 128 (zeros
+ * fill it up), K one up to 65536, N up to 1048560, C to 2^24; x8, a8 and b8 16-byte
+ * aligned. */
 int detllm_lora_add(int32_t* P, const int8_t* x8, const int8_t* a8, const int8_t* b8,
                     const int64_t* bm, const int64_t* bk, const int32_t* adapter, int N, int K,
                     int C, int rank, int n_ad, hipStream_t s);

@@ -807,3 +807,37 @@ def test_plan_stays_in_its_buffers(N):
     for g, w in zip((table, free[:want[2]], cu, row, pos, slot),
                     (want[0], want[1][:want[2]], *want[3:7])):
         _eq(g, w)
+
+
+@pytest.mark.parametrize("bk", [-70, -64, -63, 0, 61, 62, 63, 64, 65, 70, 77, 116, 2**40])
+def test_lora_shifts_of_any_size(bk):
+    """Adapters whose scale is far from the product's: a shift that nothing survives
+    adds nothing (quantize gives exponents past 64 for very small adapters)."""
+    print(f"[lora shift {bk}]", flush=True)
+    rng = np.random.default_rng(3)
+    N, K, C, rank = 20, 64, 300, 16
+    x8, w, a8, b8 = (rng.integers(-128, 128, s, dtype=np.int8)
+                     for s in ((N, K), (C, K), (2, rank, K), (2, C, rank)))
+    x8[0], b8[:, 5] = 0, 0                     # u = 0, and a column of zeros
+    bm = rng.integers(1, 1 << 16, (2, C), dtype=np.int64)
+    ad = rng.integers(-1, 2, N).astype(np.int32)
+    ad[0] = 0
+    P = (x8.astype(np.int64) @ w.astype(np.int64).T).astype(np.int32)
+    want = P.astype(np.int64)
+    for i in range(N):
+        if ad[i] < 0:
+            continue
+        u = a8[ad[i]].astype(np.int64) @ x8[i].astype(np.int64)
+        h = max(max(int(np.abs(u).max()), 1).bit_length() - 13, 0)
+        v = b8[ad[i]].astype(np.int64) @ ((u + (1 << h >> 1)) >> h)
+        s = bk - h
+        for c in range(C):
+            t = int(v[c]) * int(bm[ad[i], c])          # below 2^43
+            if s >= 64:
+                d = 0
+            else:
+                d = (t + (1 << s >> 1)) >> s if s > 0 else (t << -s if -s < 64 else 0)
+            want[i, c] += (d + 2**31) % 2**32 - 2**31
+    want = ((want + 2**31) % 2**32 - 2**31).astype(np.int32)
+    got = _ops().lora_gemm(*(_cuda(t) for t in (x8, w, a8, b8, bm, np.full(2, bk, np.int64), ad)))
+    _eq(got, want)
