@@ -7,7 +7,8 @@ at one slot).
   ``packed_plan`` maps and gives back pages there, so a step needs nothing from
   the device.
 * ``IntQwen3.forward_packed`` runs one step of it: each row's new tokens (none,
-  one, a draft, a chunk of its prompt) follow each other in ``ids``.
+  one, a chunk of its prompt) follow each other in ``ids``, and each row's last
+  one gets logits.
 * ``generate_packed`` is a scheduler on top: prompts are admitted as rows and
   pages allow, fed in chunks beside the running replies, and leave when done.
 
