@@ -104,9 +104,10 @@ def generate_packed(model, prompts, max_new, rows: int = 32, step_tokens: int = 
     n = len(prompts)
     prompts = [p.reshape(-1).to("cpu", torch.int64) for p in prompts]
     most = [int(max_new)] * n if not hasattr(max_new, "__len__") else [int(m) for m in max_new]
-    which = [-1 if a is None else int(a) for a in ([None] * n if adapter_of is None else adapter_of)]
-    if len(which) != n:
-        raise ValueError(f"generate_packed: {len(which)} adapters of {n} prompts")
+    if adapter_of is not None and len(adapter_of) != n:
+        raise ValueError(f"generate_packed: {len(adapter_of)} adapters of {n} prompts")
+    which = [-1 if adapter_of is None or adapter_of[i] is None else int(adapter_of[i])
+             for i in range(n)]
     if len(most) != n or any(m < 0 for m in most) or any(p.numel() < 1 for p in prompts):
         raise ValueError("generate_packed: prompts of at least one token, as many reply lengths")
     if step_tokens < 1 or rows < 1:
